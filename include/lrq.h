@@ -350,6 +350,86 @@ int lrq_threshold_split(const void* x, int64_t n, float threshold, void* outlier
 int lrq_gather_rows_zero(void* x, int64_t B, int64_t M, int64_t N, const int32_t* idx, int32_t k, void* out,
                          void* stream);
 
+/* ------------------------------------------------------------------ layer norm and dropout
+ * Operators around a compressed layer (no counterpart in the reference).  Element types: */
+#define LRQ_BF16 0
+#define LRQ_F16 1
+#define LRQ_F32 2
+
+/* Dropout whose mask is drawn again wherever it is needed (Philox4x32-10, counter-based).  Element
+ * (row, col) of a tensor of n columns takes the 16-bit number col % 8 (the low half of word 0 first) of the
+ * block with counter (row * ceil(n / 8) + col / 8, offset) and key seed; it is kept where that number is
+ * below keep (0 .. 65536) and multiplied by 65536 / keep, else 0.  `state`, if not NULL, points to two
+ * device words: the seed (in place of `seed`) and a number added to `offset`, read when the kernel runs, so
+ * that a captured graph draws new masks by changing them between replays. */
+typedef struct lrq_dropout {
+  uint32_t keep;
+  uint64_t seed, offset;
+  const uint64_t* state;
+} lrq_dropout;
+
+/* out = residual + drop(x) over [rows, n] (residual may be NULL: 0), in fp32, rounded once.  The same call
+ * on the gradient of out is the backward pass for x.  out may be x or residual (same row stride). */
+int lrq_dropout_add(const lrq_dropout* drop, const void* x, int64_t ldx, const void* residual, int64_t ld_residual,
+                    int32_t dtype, int64_t rows, int64_t n, void* out, int64_t ldo, void* stream);
+
+/* y = (h - mean) * rstd * w + b per row of n columns; mean and rstd (fp32 [rows]) are kept for the backward
+ * pass.  h == NULL: the rows are x's (drop and residual NULL).  Otherwise h = residual + drop(x) (either may be
+ * NULL), rounded to dtype, is written and normalised as stored.  w, b (of w_dtype) may be NULL: 1 and 0.
+ * Sums are fp32, the variance is that of deviations from the mean. */
+int lrq_layer_norm_fwd(const lrq_dropout* drop, const void* x, int64_t ldx, const void* residual, int64_t ld_residual,
+                       int32_t dtype, const void* w, const void* b, int32_t w_dtype, int64_t rows, int64_t n, float eps,
+                       void* h, int64_t ldh, void* y, int64_t ldy, float* mean, float* rstd, void* stream);
+
+/* Gradients of lrq_layer_norm_fwd from dy and, if not NULL, dh (the gradient of h from its other uses):
+ * d = dh + (gradient through the norm); dresidual = d (may be NULL), dx = drop(d) (may be NULL where dresidual
+ * is given).  h: the rows that were normalised (x of the plain call).  dw, db (w_dtype, both or neither):
+ * summed over the rows in a fixed order through `workspace` (4-byte aligned, lrq_layer_norm_bwd_workspace(rows,
+ * n) bytes; unused without dw); rows == 0 writes zeros to them. */
+int lrq_layer_norm_bwd(const lrq_dropout* drop, const void* dy, int64_t lddy, const void* dh, int64_t lddh,
+                       const void* h, int64_t ldh, int32_t dtype, const void* w, int32_t w_dtype, const float* mean,
+                       const float* rstd, int64_t rows, int64_t n, void* dx, int64_t lddx, void* dresidual,
+                       int64_t ld_dresidual, void* dw, void* db, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Workspace bytes of lrq_layer_norm_bwd with weight gradients (>= 0), or a negative LRQ_ERR_*.  Host only. */
+int64_t lrq_layer_norm_bwd_workspace(int64_t rows, int64_t n);
+
+/* ------------------------------------------------------------------ MXFP4
+ * OCP Microscaling 4-bit floating point.  A matrix [rows, cols]: codes, ld_codes bytes a row (16-byte aligned
+ * rows), hold e2m1 elements, the even column in a byte's low nibble; scales, ld_scales bytes a row (4-byte
+ * aligned rows), hold one E8M0 exponent for 32 columns.  Rows are padded to 128 columns: ld_codes >=
+ * 64 * ceil(cols / 128), ld_scales >= 4 * ceil(cols / 128), padding columns have code 0 and a scale below 255
+ * (lrq_mxfp4_quantize writes both). */
+typedef struct lrq_mxfp4 {
+  void* codes;
+  int64_t ld_codes;
+  void* scales;
+  int64_t ld_scales;
+  int64_t rows, cols;
+} lrq_mxfp4;
+
+/* Quantise x[rows, cols]: a block's scale is 2^(floor(log2(largest magnitude)) - 2) (the smallest, 2^-127, for
+ * a block below 2^-124), elements round to the nearest code, ties to the even code, and saturate at 6.  A block
+ * with an infinity or a NaN becomes NaN (scale 255, codes 0). */
+int lrq_mxfp4_quantize(const void* x, int64_t ldx, int32_t dtype, const lrq_mxfp4* t, void* stream);
+
+/* out[rows, cols] = the values of t, rounded to dtype (exact in bf16 and fp32). */
+int lrq_mxfp4_dequantize(const lrq_mxfp4* t, void* out, int64_t ldo, int32_t dtype, void* stream);
+
+/* out[a.rows, b.rows] = a b^T, both MXFP4 with the same cols; fp32 accumulation, out fp32 when out_fp32 != 0,
+ * else bf16. */
+int lrq_mxfp4_gemm(const lrq_mxfp4* a, const lrq_mxfp4* b, void* out, int64_t ldo, int32_t out_fp32, void* stream);
+
+/* out[rows, w.rows] = x w^T with x bf16 [rows, w.cols]: each row of x holds cols rounded up to 8 elements, those
+ * past cols finite (their products are with code 0). */
+int lrq_mxfp4_linear(const void* x, int64_t ldx, int64_t rows, const lrq_mxfp4* w, void* out, int64_t ldo,
+                     int32_t out_fp32, void* stream);
+
+/* out[rows, w.cols] = y w with y bf16 [rows, w.rows], the gradient of lrq_mxfp4_linear for x: each row of y holds
+ * w.rows rounded up to 8 elements, those past w.rows zero. */
+int lrq_mxfp4_linear_t(const void* y, int64_t ldy, int64_t rows, const lrq_mxfp4* w, void* out, int64_t ldo,
+                       int32_t out_fp32, void* stream);
+
 /* ------------------------------------------------------------------ misc */
 const char* lrq_status_string(int status);
 int32_t lrq_abi_version(void);

@@ -1,0 +1,383 @@
+"""Layer norm, dropout and dropout + add + layer norm on the HIP kernels against 64-bit forms, within bounds
+counted from the roundings the kernels make (opref.py)."""
+
+import importlib
+
+import pytest
+import torch
+
+import opref as R
+
+pytestmark = pytest.mark.gpu
+DT = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+EPS = 1e-5
+SEED, OFFSET = 0x1234_5678_9ABC_DEF1, 0x2_0000_0003
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _x(shape, dtype, dev, seed, offset=0.3):
+    g = _gen(seed)
+    x = torch.randn(shape, generator=g) + offset
+    x[..., ::64] *= 10
+    return x.to(dtype).to(dev)
+
+
+def _w(n, dtype, dev, seed):
+    g = _gen(seed)
+    return (1 + 0.2 * torch.randn(n, generator=g)).to(dtype).to(dev), (0.2 * torch.randn(n, generator=g)).to(dtype).to(dev)
+
+
+def _bits(t):
+    return t.view(torch.int16 if t.element_size() == 2 else torch.int32)
+
+
+# row widths: one element, inside a chunk, one chunk, the limits of each register geometry (16, 64, 256 and 1024
+# threads, one to three chunks each) and past the last one; odd widths start rows off every alignment
+WIDTHS = [1, 3, 8, 77, 128, 129, 512, 1000, 1024, 1025, 2048, 2050, 4096, 4099, 5120, 6144, 6145, 8192, 8200, 16384,
+          16385, 20011]
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("n", WIDTHS)
+def test_layer_norm(pkg, dev, n, dtype):
+    dt = DT[dtype]
+    for rows in (1, 37):
+        print(f"[norm] rows={rows} n={n} {dtype}", flush=True)
+        x = _x((rows, n), dt, dev, n)
+        w, b = _w(n, dt, dev, n + 1)
+        dy = _x((rows, n), dt, dev, n + 2, 0.0)
+        y, mean, rstd = pkg.layer_norm_forward(x, w, b, EPS)
+        dx, dw, db = pkg.layer_norm_backward(dy, x, w, mean, rstd)
+        dx2, none_w, none_b = pkg.layer_norm_backward(dy, x, w, mean, rstd, weight_grad=False)
+        torch.cuda.synchronize()
+        ref = R.Norm64(x, w, b, EPS)
+        R.assert_within(y, ref.y, ref.bound_y(dt), "y")
+        R.assert_within(mean, ref.mean[:, 0], (ref.e_mean + R.U * ref.mean.abs())[:, 0], "mean")
+        R.assert_within(rstd, ref.rstd[:, 0], ref.e_rstd[:, 0], "rstd")
+        (rdx, rdw, rdb), (bx, bw, bb), _ = ref.grads(dy, dt, dt)
+        R.assert_within(dx, rdx, bx, "dx")
+        R.assert_within(dw, rdw, bw, "dw")
+        R.assert_within(db, rdb, bb, "db")
+        assert torch.equal(_bits(dx2), _bits(dx)) and none_w is None and none_b is None
+
+
+@pytest.mark.parametrize("rows,n", [(5000, 64), (3000, 512), (2111, 1024), (1500, 4096), (1100, 8192), (300, 17000)])
+def test_layer_norm_many_rows(pkg, dev, rows, n):
+    """More rows than row groups run at once: each group walks several; the weight gradients' parts add up, and
+    twice the same call gives the same bits."""
+    x = _x((rows, n), torch.bfloat16, dev, 5)
+    w, b = _w(n, torch.float32, dev, 6)
+    dy = _x((rows, n), torch.bfloat16, dev, 7, 0.01)
+    y, mean, rstd = pkg.layer_norm_forward(x, w, b, EPS)
+    first = pkg.layer_norm_backward(dy, x, w, mean, rstd)
+    again = pkg.layer_norm_backward(dy, x, w, mean, rstd)
+    torch.cuda.synchronize()
+    ref = R.Norm64(x, w, b, EPS)
+    R.assert_within(y, ref.y, ref.bound_y(torch.bfloat16), "y")
+    refs, bounds, _ = ref.grads(dy, torch.bfloat16, torch.float32)
+    for got, g2, r, bound, name in zip(first, again, refs, bounds, ("dx", "dw", "db")):
+        R.assert_within(got, r, bound, name)
+        assert torch.equal(_bits(got), _bits(g2)), name
+
+
+def test_layer_norm_without_weights_and_mixed_types(pkg, dev):
+    x = _x((9, 300), torch.float16, dev, 11)
+    dy = _x((9, 300), torch.float16, dev, 12, 0.0)
+    w, b = _w(300, torch.bfloat16, dev, 13)
+    for ww, bb in ((None, None), (w, None), (None, b), (w, b)):
+        y, mean, rstd = pkg.layer_norm_forward(x, ww, bb, EPS)
+        dx, dw, db = pkg.layer_norm_backward(dy, x, ww, mean, rstd)
+        ref = R.Norm64(x, ww, bb, EPS)
+        R.assert_within(y, ref.y, ref.bound_y(torch.float16), "y")
+        wt = torch.float32 if ww is None else torch.bfloat16
+        assert dw.dtype == wt and db.dtype == wt
+        refs, bounds, _ = ref.grads(dy, torch.float16, wt)
+        for got, r, bound in zip((dx, dw, db), refs, bounds):
+            R.assert_within(got, r, bound, "grad")
+
+
+def test_layer_norm_variance_of_a_large_offset(pkg, dev):
+    """Rows of 1000 + noise in fp32: a variance from the difference of squared sums would lose all digits."""
+    x = (1000 + torch.randn(7, 4096, generator=_gen(1))).to(dev)
+    y, mean, rstd = pkg.layer_norm_forward(x, None, None, EPS)
+    ref = R.Norm64(x, None, None, EPS)
+    R.assert_within(y, ref.y, ref.bound_y(torch.float32), "y")
+    # a constant row: deviations are zero or the mean's rounding, y is at most that over sqrt(eps)
+    y, _, rstd = pkg.layer_norm_forward(torch.full((3, 1000), 7.0, device=dev), None, None, EPS)
+    assert float(y.abs().max()) <= 64 * R.U * 7 / EPS ** 0.5
+    assert torch.isfinite(rstd).all()
+
+
+def test_layer_norm_not_finite_rows_stay_apart(pkg, dev):
+    x = _x((6, 500), torch.float32, dev, 3)
+    clean, _, _ = pkg.layer_norm_forward(x, None, None, EPS)
+    x[1, 7] = float("nan")
+    x[4, 499] = float("inf")
+    y, _, _ = pkg.layer_norm_forward(x, None, None, EPS)
+    assert torch.isnan(y[1]).all() and torch.isnan(y[4]).all()
+    keep = [0, 2, 3, 5]
+    assert torch.equal(y[keep], clean[keep])
+
+
+def test_layer_norm_strides_and_empty(pkg, dev):
+    base = _x((40, 1000), torch.bfloat16, dev, 21)
+    w, b = _w(333, torch.bfloat16, dev, 22)
+    x = base[3:, 5:338]  # rows 1000 apart, starting off alignment
+    y, mean, rstd = pkg.layer_norm_forward(x, w, b, EPS)
+    y2, mean2, rstd2 = pkg.layer_norm_forward(x.contiguous(), w, b, EPS)
+    assert torch.equal(_bits(y), _bits(y2)) and torch.equal(mean, mean2)
+    # a broadcast gradient (stride 0 over the rows, over everything) and a transposed one
+    for dy in (base[0, 5:338].expand(37, 333), torch.ones((), dtype=torch.bfloat16, device=dev).expand(37, 333),
+               base[:333, :37].T if base.shape[0] >= 333 else _x((333, 37), torch.bfloat16, dev, 23).T):
+        got = pkg.layer_norm_backward(dy, x, w, mean, rstd)
+        exp = pkg.layer_norm_backward(dy.contiguous(), x.contiguous(), w, mean, rstd)
+        for g, e in zip(got, exp):
+            assert torch.equal(_bits(g), _bits(e))
+    # 3-D, and the neighbours of a strided view stay as they are
+    x3 = _x((4, 5, 96), torch.float32, dev, 24)
+    y3, m3, r3 = pkg.layer_norm_forward(x3.transpose(0, 1), None, None, EPS)
+    assert y3.shape == (5, 4, 96) and m3.shape == (5, 4) and y3.is_contiguous()
+    R.assert_within(y3, R.Norm64(x3.transpose(0, 1), None, None, EPS).y,
+                    R.Norm64(x3.transpose(0, 1), None, None, EPS).bound_y(torch.float32), "y3")
+    e = torch.empty(0, 333, dtype=torch.bfloat16, device=dev)
+    y, mean, rstd = pkg.layer_norm_forward(e, w, b, EPS)
+    dx, dw, db = pkg.layer_norm_backward(e, e, w, mean, rstd)
+    assert y.shape == (0, 333) and dx.shape == (0, 333) and not dw.any() and not db.any()
+
+
+# ---------------------------------------------------------------- dropout
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("shape", [(1, 1), (1, 7), (5, 8), (3, 9), (33, 1001), (2, 3, 77), (7, 4096), (2, 20000)])
+def test_dropout(pkg, dev, shape, dtype):
+    dt = DT[dtype]
+    x, res = _x(shape, dt, dev, 31), _x(shape, dt, dev, 32)
+    for p in (0.0, 0.1, 0.5, 1.0):
+        y = pkg.dropout(x, p, (SEED, OFFSET))
+        yr = pkg.dropout(x, p, (SEED, OFFSET), residual=res)
+        ref, _ = R.drop64(x, p, SEED, OFFSET)
+        # one rounding of the product in fp32, one of the scale, the output's
+        e = 2 * R.U * ref.abs()
+        R.assert_within(y, ref, R.half_step(dt) * ref.abs() * (1 + 2 * R.U) + e + R.smallest(dt), f"p={p}")
+        assert torch.equal(y.cpu() == 0, (ref == 0)), "mask"
+        r64 = res.double().cpu() + ref
+        e = e + R.U * (ref.abs() + res.double().cpu().abs())
+        R.assert_within(yr, r64, R.half_step(dt) * (r64.abs() + e) + e + R.smallest(dt), f"p={p} residual")
+
+
+def test_dropout_generator_is_the_published_one():
+    """The oracle's generator gives the published known answers of Philox4x32-10 (counter and key all zeros, all ones)."""
+    zero = R.philox([[0]] * 4, (0, 0))
+    assert [int(w[0]) for w in zero] == [0x6627E8D5, 0xE169C58D, 0xBC57AC4C, 0x9B00DBD8]
+    ones = R.philox([[0xFFFFFFFF]] * 4, (0xFFFFFFFF, 0xFFFFFFFF))
+    assert [int(w[0]) for w in ones] == [0x408F276D, 0x41C83B0E, 0xA20BC7C6, 0x6D5451FD]
+
+
+def test_dropout_rate_and_independence(pkg, dev):
+    """The kept share of 2^22 draws is within 6 standard deviations; other seeds and offsets give other masks, which
+    agree as often as independent ones do."""
+    x = torch.ones(1024, 4096, device=dev)
+    n = x.numel()
+    keep = 1 - round(65536 * 0.1) / 65536
+    masks = [pkg.dropout(x, 0.1, s) != 0 for s in (1, 2, (1, 1), (1, 1 << 32), 1 << 32)]
+    for m in masks:
+        assert abs(float(m.double().mean()) - keep) <= 6 * (keep * (1 - keep) / n) ** 0.5
+    agree = keep * keep + (1 - keep) ** 2
+    for i in range(len(masks)):
+        for j in range(i):
+            share = float((masks[i] == masks[j]).double().mean())
+            assert abs(share - agree) <= 6 * (agree * (1 - agree) / n) ** 0.5, (i, j, share)
+
+
+def test_dropout_drops_what_is_not_finite(pkg, dev):
+    x = torch.full((64, 64), float("nan"), device=dev)
+    x[::2] = float("inf")
+    y = pkg.dropout(x, 0.5, SEED)
+    k = R.kept(64, 64, 32768, SEED, 0).to(dev)
+    assert not y[~k].any() and not torch.isfinite(y[k]).any()
+    assert not pkg.dropout(x, 1.0, SEED).any()
+
+
+def test_dropout_strides_offsets_and_tensor_seed(pkg, dev):
+    base = _x((20, 700), torch.bfloat16, dev, 41)
+    x = base[1:18, 3:500]
+    want = pkg.dropout(x.contiguous(), 0.2, (SEED, 5))
+    assert torch.equal(_bits(pkg.dropout(x, 0.2, (SEED, 5))), _bits(want))
+    state = torch.tensor([SEED, 2], dtype=torch.int64, device=dev)
+    assert torch.equal(_bits(pkg.dropout(x, 0.2, (state, 3))), _bits(want))
+    state[1] = 5
+    assert torch.equal(_bits(pkg.dropout(x, 0.2, state)), _bits(want))
+    # negative seeds are the same 64 bits
+    assert torch.equal(pkg.dropout(x, 0.2, -1), pkg.dropout(x, 0.2, (1 << 64) - 1))
+    assert pkg.dropout(x[:0], 0.2, 1).shape == (0, 497)
+    assert pkg.dropout(x[:, :0], 0.2, 1).shape == (17, 0)
+
+
+def test_dropout_past_32_bits(pkg, dev):
+    """2^31 + elements (offsets past 2^32 bytes): the last rows against the oracle."""
+    rows, n = 524300, 4104
+    x = torch.ones(rows, n, dtype=torch.bfloat16, device=dev)
+    y = pkg.dropout(x, 0.5, (SEED, OFFSET))
+    for first in (0, rows // 2, rows - 3):
+        k = R.kept(3, n, 32768, SEED, OFFSET, first)
+        assert torch.equal(y[first:first + 3].cpu() != 0, k)
+    del x, y
+
+
+# ---------------------------------------------------------------- dropout + add + norm
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("rows,n", [(1, 1), (3, 13), (65, 1000), (130, 1024), (19, 4096), (40, 5120), (6, 9001), (3, 18000)])
+def test_dropout_add_layer_norm(pkg, dev, rows, n, dtype):
+    dt = DT[dtype]
+    p = 0.1
+    print(f"[add_norm] rows={rows} n={n} {dtype}", flush=True)
+    x, res = _x((rows, n), dt, dev, 51), _x((rows, n), dt, dev, 52)
+    w, b = _w(n, dt, dev, 53)
+    dy, dh = _x((rows, n), dt, dev, 54, 0.0), _x((rows, n), dt, dev, 55, 0.0)
+    y, h, mean, rstd = pkg.dropout_add_layer_norm_forward(x, res, w, b, p, (SEED, OFFSET), EPS)
+    dx, dres, dw, db = pkg.dropout_add_layer_norm_backward(dy, dh, h, w, mean, rstd, p, (SEED, OFFSET))
+    torch.cuda.synchronize()
+    d64, mask = R.drop64(x, p, SEED, OFFSET)
+    h64 = res.double().cpu() + d64
+    e = 3 * R.U * (d64.abs() + res.double().cpu().abs())
+    R.assert_within(h, h64, R.half_step(dt) * (h64.abs() + e) + e + R.smallest(dt), "h")
+    ref = R.Norm64(h, w, b, EPS)  # the norm is that of h as stored
+    R.assert_within(y, ref.y, ref.bound_y(dt), "y")
+    (rd, rdw, rdb), (bd, bw, bb), e_d = ref.grads(dy, dt, dt, dh=dh)
+    R.assert_within(dres, rd, bd, "dresidual")
+    rdx = rd * mask
+    e = e_d * mask + 2 * R.U * rdx.abs()
+    R.assert_within(dx, rdx, R.half_step(dt) * (rdx.abs() + e) + e + R.smallest(dt), "dx")
+    assert torch.equal((dx.cpu() == 0) | (rdx == 0), dx.cpu() == 0), "dropped gradients are zero"
+    R.assert_within(dw, rdw, bw, "dw")
+    R.assert_within(db, rdb, bb, "db")
+    # without dh, without dropout, without a residual
+    dx0, dres0, _, _ = pkg.dropout_add_layer_norm_backward(dy, None, h, w, mean, rstd, 0.0, 0)
+    plain, _, _ = pkg.layer_norm_backward(dy, h, w, mean, rstd)
+    assert dx0 is dres0 and torch.equal(_bits(dx0), _bits(plain))
+    y1, h1, _, _ = pkg.dropout_add_layer_norm_forward(x, None, w, b, 0.0, 0, EPS)
+    yp, _, _ = pkg.layer_norm_forward(x, w, b, EPS)
+    assert torch.equal(_bits(h1), _bits(x)) and torch.equal(_bits(y1), _bits(yp))
+
+
+def test_gradients_against_differences(pkg, dev):
+    """The gradient of sum(dy y + dh h) along random directions, against central differences of the oracle's 64-bit
+    forward pass (the mask fixed): truncation is O(step^2), the rest is the fp32 kernel's."""
+    AG = importlib.import_module("triton-kernel-test_amd.autograd")
+    g = _gen(61)
+    rows, n, p = 5, 40, 0.25
+    x, res = (torch.randn(rows, n, generator=g).to(dev).requires_grad_() for _ in range(2))
+    w, b = (t.requires_grad_() for t in _w(n, torch.float32, dev, 62))
+    cy, ch = torch.randn(rows, n, generator=g).double(), torch.randn(rows, n, generator=g).double()
+    y, h = AG.dropout_add_layer_norm(x, res, w, b, p, 77, EPS)
+    (y * cy.float().to(dev) + h * ch.float().to(dev)).sum().backward()
+
+    def loss(x_, r_, w_, b_):
+        d, _ = R.drop64(x_, p, 77)
+        h_ = r_ + d
+        m = h_.mean(-1, keepdim=True)
+        z = (h_ - m) / torch.sqrt(((h_ - m) ** 2).mean(-1, keepdim=True) + EPS)
+        return float(((z * w_ + b_) * cy + h_ * ch).sum())
+
+    at = [t.detach().double().cpu() for t in (x, res, w, b)]
+    for i, t in enumerate((x, res, w, b)):
+        for _ in range(3):
+            v = torch.randn(at[i].shape, generator=g).double()
+            step = 1e-5
+            up = [a + (step * v if k == i else 0) for k, a in enumerate(at)]
+            dn = [a - (step * v if k == i else 0) for k, a in enumerate(at)]
+            diff = (loss(*up) - loss(*dn)) / (2 * step)
+            got = float((t.grad.double().cpu() * v).sum())
+            scale = float((t.grad.double().cpu().abs() * v.abs()).sum())
+            # 1e-5 of the terms: fp32 gradients (about 200 U), differences (1e-16 * loss / 1e-5, and step^2)
+            assert abs(got - diff) <= 2e-5 * scale, (i, got, diff)
+
+
+# ---------------------------------------------------------------- autograd, streams, graphs
+def test_autograd_layer_norm_and_dropout(pkg, dev):
+    AG = importlib.import_module("triton-kernel-test_amd.autograd")
+    x = _x((4, 6, 256), torch.bfloat16, dev, 71).requires_grad_()
+    w, b = (t.requires_grad_() for t in _w(256, torch.bfloat16, dev, 72))
+    y = AG.layer_norm(x, w, b)
+    z = AG.dropout(y, 0.3, (9, 1), residual=x)
+    z.float().sum().backward()  # a broadcast gradient
+    dz = torch.ones_like(z)
+    dyd = pkg.dropout(dz, 0.3, (9, 1))
+    _, mean, rstd = pkg.layer_norm_forward(x.detach(), w.detach(), b.detach())
+    dx, dw, db = pkg.layer_norm_backward(dyd, x.detach(), w.detach(), mean, rstd)
+    assert torch.equal(w.grad, dw) and torch.equal(b.grad, db)
+    assert torch.equal(x.grad, dx + dz)
+    # frozen weights, no bias
+    x2 = x.detach().requires_grad_()
+    AG.layer_norm(x2, w.detach(), None).backward(torch.ones_like(x2))
+    assert x2.grad is not None
+    # evaluation: dropout is the identity plus the residual
+    assert AG.dropout(y, 0.3, 9, training=False) is y
+    with pytest.raises(RuntimeError):
+        gx, = torch.autograd.grad(AG.layer_norm(x2, None, None).sum(), x2, create_graph=True)
+        gx.sum().backward()
+
+
+def test_autograd_state_changed_before_backward_is_refused(pkg, dev):
+    AG = importlib.import_module("triton-kernel-test_amd.autograd")
+    state = torch.tensor([3, 0], dtype=torch.int64, device=dev)
+    x = _x((8, 64), torch.float32, dev, 73).requires_grad_()
+    y = AG.dropout(x, 0.5, state)
+    state[1] += 1
+    with pytest.raises(RuntimeError):
+        y.sum().backward()
+
+
+def test_side_stream(pkg, dev):
+    x = _x((300, 1024), torch.bfloat16, dev, 81)
+    w, b = _w(1024, torch.bfloat16, dev, 82)
+    want = pkg.layer_norm_forward(x, w, b)
+    grads = pkg.layer_norm_backward(x, x, w, want[1], want[2])
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = pkg.layer_norm_forward(x, w, b)
+        g2 = pkg.layer_norm_backward(x, x, w, got[1], got[2])
+        d = pkg.dropout(x, 0.5, 4)
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    for a, e in zip((*got, *g2, d), (*want, *grads, pkg.dropout(x, 0.5, 4))):
+        assert torch.equal(a, e)
+
+
+def test_captured_graphs_draw_new_masks(pkg, dev):
+    """Two captured graphs of the fused pass over one seed tensor, replayed in turn with eager work between: every
+    replay equals the eager call at the tensor's value."""
+    x, res = _x((70, 1000), torch.bfloat16, dev, 91), _x((70, 1000), torch.bfloat16, dev, 92)
+    w, b = _w(1000, torch.bfloat16, dev, 93)
+    state = torch.tensor([11, 0], dtype=torch.int64, device=dev)
+
+    def step(offset):
+        y, h, mean, rstd = pkg.dropout_add_layer_norm_forward(x, res, w, b, 0.2, (state, offset))
+        return (y, h, *pkg.dropout_add_layer_norm_backward(x, res, h, w, mean, rstd, 0.2, (state, offset)))
+
+    step(0)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for offset in (0, 100):
+        g = torch.cuda.CUDAGraph()
+        print("[norm] capture", flush=True)
+        with torch.cuda.graph(g):
+            outs.append(step(offset))
+        graphs.append(g)
+    seen = []
+    for i in range(3):
+        state[1] = i
+        for k, offset in enumerate((0, 100)):
+            graphs[k].replay()
+        torch.cuda.synchronize()
+        for k, offset in enumerate((0, 100)):
+            for got, want in zip(outs[k], step(offset)):
+                assert torch.equal(_bits(got), _bits(want)), (i, k)
+            seen.append(outs[k][1].clone())
+    for i in range(len(seen)):
+        for j in range(i):
+            assert not torch.equal(seen[i], seen[j])

@@ -5,8 +5,10 @@ not a Python identifier).  The HIP library liblrq.so must be built first; nothin
 falls back to a CPU implementation.
 """
 
-from . import _lib, api, autograd, inputs, offload  # noqa: F401
+from . import _lib, api, autograd, inputs, mxfp4, norm, offload  # noqa: F401
 from .api import *  # noqa: F401,F403
 from .legacy import *  # noqa: F401,F403
+from .mxfp4 import *  # noqa: F401,F403
+from .norm import *  # noqa: F401,F403
 
 __version__ = "0.1.0"

@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, c_float, c_int32, c_int64, c_size_t, c_void_p
+from ctypes import POINTER, c_float, c_int32, c_int64, c_size_t, c_uint32, c_uint64, c_void_p
 from pathlib import Path
 
 LIB_PATH = Path(os.environ.get("LRQ_LIBRARY", Path(__file__).resolve().parent / "liblrq.so"))
@@ -22,6 +22,9 @@ LRQ_ERR_ALIGN = -4
 LRQ_ERR_WORKSPACE = -5
 LRQ_FLAG_HADAMARD = 1
 LRQ_GEMM_T_SCRATCH_BYTES = 16 * 1024 * 1024  # include/lrq.h
+LRQ_BF16 = 0
+LRQ_F16 = 1
+LRQ_F32 = 2
 
 
 class LrqTensors(ctypes.Structure):
@@ -39,7 +42,22 @@ class LrqTensors(ctypes.Structure):
     ]
 
 
+class LrqDropout(ctypes.Structure):
+    """Mirror of ``lrq_dropout`` in include/lrq.h."""
+
+    _fields_ = [("keep", c_uint32), ("seed", c_uint64), ("offset", c_uint64), ("state", c_void_p)]
+
+
+class LrqMxfp4(ctypes.Structure):
+    """Mirror of ``lrq_mxfp4`` in include/lrq.h."""
+
+    _fields_ = [("codes", c_void_p), ("ld_codes", c_int64), ("scales", c_void_p), ("ld_scales", c_int64),
+                ("rows", c_int64), ("cols", c_int64)]
+
+
 _T = POINTER(LrqTensors)
+_D = POINTER(LrqDropout)
+_M = POINTER(LrqMxfp4)
 
 # name -> (restype, argtypes); must cover every function declared in include/*.h (the drop-in
 # ABI in lrq.h and the test hooks in lrq_test_hooks.h)
@@ -98,6 +116,20 @@ SIGNATURES = {
     "lrq_threshold_split": (c_int32, [c_void_p, c_int64, c_float, c_void_p, c_void_p, c_void_p]),
     "lrq_gather_rows_zero": (c_int32, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int32, c_void_p,
                                        c_void_p]),
+    "lrq_dropout_add": (c_int32, [_D, c_void_p, c_int64, c_void_p, c_int64, c_int32, c_int64, c_int64, c_void_p,
+                                  c_int64, c_void_p]),
+    "lrq_layer_norm_fwd": (c_int32, [_D, c_void_p, c_int64, c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_int32,
+                                     c_int64, c_int64, c_float, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
+                                     c_void_p, c_void_p]),
+    "lrq_layer_norm_bwd": (c_int32, [_D, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int32, c_void_p,
+                                     c_int32, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p,
+                                     c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
+    "lrq_layer_norm_bwd_workspace": (c_int64, [c_int64, c_int64]),
+    "lrq_mxfp4_quantize": (c_int32, [c_void_p, c_int64, c_int32, _M, c_void_p]),
+    "lrq_mxfp4_dequantize": (c_int32, [_M, c_void_p, c_int64, c_int32, c_void_p]),
+    "lrq_mxfp4_gemm": (c_int32, [_M, _M, c_void_p, c_int64, c_int32, c_void_p]),
+    "lrq_mxfp4_linear": (c_int32, [c_void_p, c_int64, c_int64, _M, c_void_p, c_int64, c_int32, c_void_p]),
+    "lrq_mxfp4_linear_t": (c_int32, [c_void_p, c_int64, c_int64, _M, c_void_p, c_int64, c_int32, c_void_p]),
     "lrq_status_string": (ctypes.c_char_p, [c_int32]),
     "lrq_abi_version": (c_int32, []),
 }
@@ -167,5 +199,5 @@ def call(name: str, *args) -> None:
         check(st, name)
 
 
-__all__ = ["LrqTensors", "load", "call", "call_raw", "check", "status_string", "missing_symbols", "SIGNATURES",
+__all__ = ["LrqTensors", "LrqDropout", "LrqMxfp4", "load", "call", "call_raw", "check", "status_string", "missing_symbols", "SIGNATURES",
            "LIB_PATH", "LRQ_FLAG_HADAMARD", "c_size_t"]

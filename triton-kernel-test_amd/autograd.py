@@ -18,6 +18,9 @@ round trip part of autograd:
 * ``compressed_saved_tensors`` is a ``torch.autograd.graph.saved_tensors_hooks`` context that
   stores every saved bf16 activation with a suitable last dimension in the compressed format
   and decodes it when backward asks for it, for any model.
+* ``layer_norm``, ``dropout``, ``dropout_add_layer_norm`` and ``mxfp4_linear`` are the operators of
+  ``norm.py`` and ``mxfp4.py`` with their gradients; ``lora_linear_compressed`` takes an MXFP4 base
+  weight and LoRA dropout.
 * ``fit_basis`` builds the rank-r basis V from a sample of activation rows (top right singular
   vectors), the counterpart of the reference's low-rank factors of x.
 
@@ -29,11 +32,14 @@ from __future__ import annotations
 from typing import Callable, Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
+from . import mxfp4 as _mx
+from . import norm as _norm
 from .api import CompressedActivation, LowRankBasis, decode, encode, lora_grads
 
 __all__ = ["compute_lora", "compute_lora_gradient", "LoRALinearCompressed", "lora_linear_compressed",
-           "compressed_saved_tensors", "fit_basis"]
+           "compressed_saved_tensors", "fit_basis", "layer_norm", "dropout", "dropout_add_layer_norm", "mxfp4_linear"]
 
 
 def compute_lora(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
@@ -62,30 +68,58 @@ class LoRALinearCompressed(torch.autograd.Function):
     """y = compute_lora(x, W, A, B); x is saved compressed (bits, group, optional basis).
 
     Gradients: dx, dA, dB of compute_lora_gradient on the decoded x; W gets none.  ``fused``
-    reads the codes directly for dA and x A (no decoded x), see the module docstring."""
+    reads the codes directly for dA and x A (no decoded x), see the module docstring.  W may be an
+    ``MXFP4Tensor`` [out, in].  With ``dropout_p`` the LoRA branch reads dropout(x): y = x W^T + (dropout(x) A) B, its
+    mask drawn again from ``seed`` in the backward pass, where x is decoded for it."""
 
     @staticmethod
-    def forward(ctx, x, w, a, b, basis: Optional[LowRankBasis], bits: int, group: int, fused: bool = True):
-        y = compute_lora(x, w, a, b)
+    def forward(ctx, x, w, a, b, basis: Optional[LowRankBasis], bits: int, group: int, fused: bool = True,
+                dropout_p: float = 0.0, seed=None):
+        ctx.p, ctx.seed, state = _seeded(dropout_p, seed)
+        ctx.mx = w if isinstance(w, _mx.MXFP4Tensor) else None
+        if ctx.p == 0.0 and ctx.mx is None:
+            y = compute_lora(x, w, a, b)
+        else:
+            x2 = _flat(x)
+            xd = _norm.dropout(x2, ctx.p, seed) if ctx.p > 0.0 else x2
+            base = _mx.mxfp4_linear(x2, w) if ctx.mx is not None else x2 @ w.mT
+            y = torch.addmm(base, xd @ a, b).reshape(x.shape[:-1] + (w.shape[0],))
         ctx.c = encode(x.detach(), basis, bits=bits, group_size=group)
         ctx.fused = fused
-        ctx.save_for_backward(w, a, b)
+        ctx.save_for_backward(None if ctx.mx is not None else w, a, b, state)
         return y
 
     @staticmethod
     def backward(ctx, dy):
-        w, a, b = ctx.saved_tensors
+        w, a, b, state = ctx.saved_tensors
         c, ctx.c = ctx.c, None
         dy2 = _flat(dy)
-        if ctx.fused and _codes_gemm_ok(c, a, dy2):
-            dx = dy2 @ (w + b.mT @ a.mT)
+        codes = ctx.fused and ctx.p == 0.0 and _codes_gemm_ok(c, a, dy2)
+        if ctx.p == 0.0 and ctx.mx is None:
+            if codes:
+                dx = dy2 @ (w + b.mT @ a.mT)
+                g = dy2 @ b.mT
+            else:
+                dx, da, db = compute_lora_gradient(dy2, _flat(decode(c)), w, a, b)
+        else:
+            g = dy2 @ b.mT
+            dx = _mx.mxfp4_linear_backward(dy2, ctx.mx) if ctx.mx is not None else dy2 @ w
+            if ctx.p > 0.0:
+                dx = _norm.dropout(g @ a.mT, ctx.p, _with_state(ctx.seed, state), residual=dx)
+            else:
+                dx = torch.addmm(dx, g, a.mT)
+            if not codes:
+                xh = _flat(decode(c))
+                if ctx.p > 0.0:
+                    xh = _norm.dropout(xh, ctx.p, _with_state(ctx.seed, state))
+                da, db = xh.mT @ g, (xh @ a).mT @ dy2
+        if codes:
             # x A and x^T (dy B^T) from one pass over the codes where the format allows it
-            xa, da = lora_grads(c, a, dy2 @ b.mT, xa_dtype=a.dtype, da_dtype=torch.float32)
+            xa, da = lora_grads(c, a, g, xa_dtype=a.dtype, da_dtype=torch.float32)
             da = da.to(a.dtype)
             db = xa.mT @ dy2  # (x A)^T dy
-        else:
-            dx, da, db = compute_lora_gradient(dy2, _flat(decode(c)), w, a, b)
-        return dx.reshape(dy.shape[:-1] + (w.shape[1],)), None, da, db, None, None, None, None
+        dx = dx.reshape(dy.shape[:-1] + (a.shape[0],))
+        return dx, None, da, db, None, None, None, None, None, None
 
 
 def _codes_gemm_ok(c: CompressedActivation, a: torch.Tensor, dy2: torch.Tensor) -> bool:
@@ -96,8 +130,127 @@ def _codes_gemm_ok(c: CompressedActivation, a: torch.Tensor, dy2: torch.Tensor) 
 
 
 def lora_linear_compressed(x, w, a, b, basis: Optional[LowRankBasis] = None, bits: int = 4, group: int = 64,
-                           fused: bool = True):
-    return LoRALinearCompressed.apply(x, w, a, b, basis, bits, group, fused)
+                           fused: bool = True, dropout_p: float = 0.0, seed=None):
+    """The LoRA layer that saves x compressed (``LoRALinearCompressed``).  w: dense [out, in] or an
+    ``MXFP4Tensor``; ``dropout_p`` > 0 needs a ``seed`` (``norm.dropout``'s), a new one for every step and layer."""
+    return LoRALinearCompressed.apply(x, w, a, b, basis, bits, group, fused, dropout_p, seed)
+
+
+def _seeded(p: float, seed):
+    """(p, seed without its tensor, the tensor or None): a seed tensor is saved for the backward pass, which then
+    refuses one that was changed in between (it would draw another mask)."""
+    p = float(p)
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"dropout probability must lie in [0, 1], got {p}")
+    if p > 0.0 and seed is None:
+        raise ValueError("dropout needs a seed")
+    if isinstance(seed, torch.Tensor):
+        return p, (None, 0), seed
+    if isinstance(seed, (tuple, list)) and len(seed) == 2 and isinstance(seed[0], torch.Tensor):
+        return p, (None, seed[1]), seed[0]
+    return p, seed, None
+
+
+def _with_state(seed, state):
+    return seed if state is None else (state, seed[1])
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, mean, rstd = _norm.layer_norm_forward(x, weight, bias, eps)
+        ctx.save_for_backward(x, weight, mean, rstd)
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, mean, rstd = ctx.saved_tensors
+        need_w, need_b = ctx.needs_input_grad[1], ctx.needs_input_grad[2]
+        dx, dw, db = _norm.layer_norm_backward(dy, x, weight, mean, rstd, weight_grad=need_w or need_b)
+        return dx, dw if need_w else None, db.to(ctx.bias_dtype) if need_b else None, None
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+               eps: float = 1e-5) -> torch.Tensor:
+    """Layer norm over the last axis (``norm.layer_norm_forward``) with gradients for x, weight and bias; the sums of
+    the weights' gradients are skipped where neither needs one."""
+    return _LayerNorm.apply(x, weight, bias, eps)
+
+
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, p, seed):
+        ctx.p, ctx.seed, state = _seeded(p, seed)
+        ctx.save_for_backward(state)
+        return _norm.dropout(x, p, seed, residual)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        state, = ctx.saved_tensors
+        dx = _norm.dropout(dy, ctx.p, _with_state(ctx.seed, state)) if ctx.needs_input_grad[0] else None
+        return dx, dy if ctx.needs_input_grad[1] else None, None, None
+
+
+def dropout(x: torch.Tensor, p: float, seed, residual: Optional[torch.Tensor] = None,
+            training: bool = True) -> torch.Tensor:
+    """residual + dropout(x) (``norm.dropout``); the mask is drawn again for the gradient, not stored.  With
+    ``training=False`` x itself (plus the residual)."""
+    if not training:
+        return x if residual is None else x + residual
+    return _Dropout.apply(x, residual, p, seed)
+
+
+class _DropoutAddLayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, weight, bias, p, seed, eps):
+        ctx.p, ctx.seed, state = _seeded(p, seed)
+        y, h, mean, rstd = _norm.dropout_add_layer_norm_forward(x, residual, weight, bias, p, 0 if seed is None else seed,
+                                                                eps)
+        ctx.save_for_backward(h, weight, mean, rstd, state)
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        ctx.set_materialize_grads(False)
+        return y, h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dh):
+        h, weight, mean, rstd, state = ctx.saved_tensors
+        if dy is None and dh is None:
+            return (None,) * 7
+        dy = torch.zeros_like(h) if dy is None else dy
+        seed = 0 if ctx.p == 0.0 else _with_state(ctx.seed, state)
+        _, need_r, need_w, need_b = ctx.needs_input_grad[:4]
+        dx, dres, dw, db = _norm.dropout_add_layer_norm_backward(dy, dh, h, weight, mean, rstd, ctx.p, seed,
+                                                                 weight_grad=need_w or need_b)
+        return (dx, dres if need_r else None, dw if need_w else None, db.to(ctx.bias_dtype) if need_b else None, None,
+                None, None)
+
+
+def dropout_add_layer_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: Optional[torch.Tensor],
+                           bias: Optional[torch.Tensor], p: float, seed, eps: float = 1e-5):
+    """(y, h) of h = residual + dropout(x), y = layer_norm(h), in one kernel each way; h is the residual stream that
+    the next block adds to."""
+    return _DropoutAddLayerNorm.apply(x, residual, weight, bias, p, seed, eps)
+
+
+class _MXFP4Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, out_dtype):
+        ctx.w = w
+        return _mx.mxfp4_linear(x, w, out_dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        return _mx.mxfp4_linear_backward(dy.to(torch.bfloat16), ctx.w), None, None
+
+
+def mxfp4_linear(x: torch.Tensor, w: "_mx.MXFP4Tensor", out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """x w^T for a frozen MXFP4 weight (``mxfp4.mxfp4_linear``), with the gradient for x (taken from dy in bf16)."""
+    return _MXFP4Linear.apply(x, w, out_dtype)
 
 
 class compressed_saved_tensors(torch.autograd.graph.saved_tensors_hooks):

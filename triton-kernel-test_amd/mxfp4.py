@@ -1,0 +1,158 @@
+"""Microscaled 4-bit floating point (OCP MXFP4): quantisation, and products with operands held in it.
+
+A weight in MXFP4 takes 17/32 of a byte an element.  ``mxfp4_linear`` multiplies bf16 activations by it
+(a frozen base weight: the reference's profiles keep theirs in another 4-bit format through a closed
+library) and ``mxfp4_linear_backward`` is the gradient for the activations; ``mxfp4_gemm`` multiplies two
+MXFP4 operands on the scaled matrix instructions.  ``autograd.mxfp4_linear`` and
+``autograd.lora_linear_compressed`` (an ``MXFP4Tensor`` as its base weight) call them.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass
+
+import torch
+
+from ._lib import LrqMxfp4, call
+from .api import _on, _p, _require_device, _stream
+from .norm import _dtype, _rows
+
+__all__ = ["MXFP4Tensor", "mxfp4_quantize", "mxfp4_dequantize", "mxfp4_gemm", "mxfp4_linear", "mxfp4_linear_backward"]
+
+
+@dataclass(frozen=True)
+class MXFP4Tensor:
+    """A tensor [..., cols] in MXFP4; rows are its leading dimensions flattened.
+
+    ``codes`` uint8 [rows, >= 64 ceil(cols / 128)]: e2m1 elements, the even column in a byte's low nibble.
+    ``scales`` uint8 [rows, >= 4 ceil(cols / 128)]: one E8M0 exponent for 32 columns.  Columns past ``cols``
+    have code 0 and a scale below 255."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+    shape: tuple
+
+    @property
+    def rows(self) -> int:
+        return self.codes.shape[0]
+
+    @property
+    def cols(self) -> int:
+        return self.shape[-1]
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    def nbytes(self) -> int:
+        return self.codes.numel() + self.scales.numel()
+
+    def to(self, device) -> "MXFP4Tensor":
+        return MXFP4Tensor(self.codes.to(device), self.scales.to(device), self.shape)
+
+    def descriptor(self) -> LrqMxfp4:
+        c, s = self.codes, self.scales
+        _require_device(c, s)
+        rows = 1
+        for d in self.shape[:-1]:
+            rows *= d
+        if len(self.shape) < 1 or self.shape[-1] <= 0:
+            raise ValueError("an MXFP4 tensor needs rows of at least one element")
+        steps = (self.shape[-1] + 127) // 128
+        for t, name, width in ((c, "codes", 64 * steps), (s, "scales", 4 * steps)):
+            if t.dtype != torch.uint8 or t.dim() != 2 or t.shape[0] != rows or t.shape[1] < width or t.device != c.device:
+                raise ValueError(f"{name} must be uint8 [{rows}, >= {width}] on one device, got {t.dtype} {tuple(t.shape)}")
+            if t.stride(1) != 1:
+                raise ValueError(f"{name} must have unit inner stride")
+        # the stride of a single row means nothing
+        return LrqMxfp4(c.data_ptr(), c.stride(0) if rows > 1 else 64 * steps, s.data_ptr(),
+                        s.stride(0) if rows > 1 else 4 * steps, rows, self.shape[-1])
+
+
+def mxfp4_quantize(x: torch.Tensor) -> MXFP4Tensor:
+    """x[..., n] (bf16, fp16 or fp32) in MXFP4: per 32 columns of a row the scale 2^(floor(log2 max|x|) - 2),
+    elements rounded to the nearest code (ties to the even one) and saturated.  A block with an infinity
+    or a NaN becomes NaN."""
+    _require_device(x)
+    dt = _dtype(x, "x")
+    x2, rows, n, ldx = _rows(x, "x")
+    steps = (n + 127) // 128
+    q = MXFP4Tensor(torch.empty((rows, 64 * steps), dtype=torch.uint8, device=x.device),
+                    torch.empty((rows, 4 * steps), dtype=torch.uint8, device=x.device), tuple(x.shape))
+    with _on(x.device):
+        call("lrq_mxfp4_quantize", _p(x2), ldx, dt, ctypes.byref(q.descriptor()), _stream(x.device))
+    return q
+
+
+def mxfp4_dequantize(q: MXFP4Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values of q (exact in bf16 and fp32)."""
+    t = q.descriptor()
+    out = torch.empty(q.shape, dtype=dtype, device=q.device)
+    with _on(q.device):
+        call("lrq_mxfp4_dequantize", ctypes.byref(t), _p(out), q.cols, _dtype(out, "the output"), _stream(q.device))
+    return out
+
+
+def _out_fp32(out_dtype) -> int:
+    if out_dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError("out_dtype must be float32 or bfloat16")
+    return 1 if out_dtype == torch.float32 else 0
+
+
+def _matrix(w: MXFP4Tensor, device: torch.device) -> LrqMxfp4:
+    if len(w.shape) != 2:
+        raise ValueError(f"an MXFP4 weight must be a matrix, got {tuple(w.shape)}")
+    if w.device != device:
+        raise ValueError(f"the weight is on {w.device}, the operand on {device}")
+    return w.descriptor()
+
+
+def mxfp4_gemm(a: MXFP4Tensor, b: MXFP4Tensor, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """a @ b^T for a [..., K] and b [N, K], both MXFP4: [..., N], fp32 accumulate."""
+    f32 = _out_fp32(out_dtype)
+    tb = _matrix(b, a.device)
+    ta = a.descriptor()
+    if a.cols != b.cols:
+        raise ValueError(f"operands have {a.cols} and {b.cols} columns")
+    out = torch.empty(tuple(a.shape[:-1]) + (b.rows,), dtype=out_dtype, device=a.device)
+    with _on(a.device):
+        call("lrq_mxfp4_gemm", ctypes.byref(ta), ctypes.byref(tb), _p(out), b.rows, f32, _stream(a.device))
+    return out
+
+
+def _operand(x: torch.Tensor, cols: int, name: str):
+    """x as rows of whole 16-byte pieces (zeros appended where the width is no multiple of 8)."""
+    _require_device(x)
+    if x.dtype != torch.bfloat16 or x.dim() < 1 or x.shape[-1] != cols:
+        raise ValueError(f"{name} must be bf16 [..., {cols}], got {x.dtype} {tuple(x.shape)}")
+    if cols == 0:
+        return x, x.numel(), 0
+    if cols % 8:
+        x = torch.nn.functional.pad(x, (0, -cols % 8))
+    x2, rows, _, ld = _rows(x, name)
+    return x2, rows, ld
+
+
+def mxfp4_linear(x: torch.Tensor, w: MXFP4Tensor, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """x @ w^T for bf16 x [..., K] and an MXFP4 weight [N, K]: [..., N], fp32 accumulate."""
+    f32 = _out_fp32(out_dtype)
+    t = _matrix(w, x.device)
+    x2, rows, ldx = _operand(x, w.cols, "x")
+    out = torch.empty(tuple(x.shape[:-1]) + (w.rows,), dtype=out_dtype, device=x.device)
+    with _on(x.device):
+        call("lrq_mxfp4_linear", _p(x2), ldx, rows, ctypes.byref(t), _p(out), w.rows, f32, _stream(x.device))
+    return out
+
+
+def mxfp4_linear_backward(dy: torch.Tensor, w: MXFP4Tensor, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """dy @ w for bf16 dy [..., N] and an MXFP4 weight [N, K]: the gradient of ``mxfp4_linear`` for x."""
+    f32 = _out_fp32(out_dtype)
+    t = _matrix(w, dy.device)
+    dy2, rows, ld = _operand(dy, w.rows, "dy")
+    out = torch.empty(tuple(dy.shape[:-1]) + (w.cols,), dtype=out_dtype, device=dy.device)
+    if w.rows == 0:
+        return out.zero_()
+    with _on(dy.device):
+        call("lrq_mxfp4_linear_t", _p(dy2), ld, rows, ctypes.byref(t), _p(out), w.cols, f32, _stream(dy.device))
+    return out
