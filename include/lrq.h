@@ -420,15 +420,22 @@ int lrq_mxfp4_dequantize(const lrq_mxfp4* t, void* out, int64_t ldo, int32_t dty
  * else bf16. */
 int lrq_mxfp4_gemm(const lrq_mxfp4* a, const lrq_mxfp4* b, void* out, int64_t ldo, int32_t out_fp32, void* stream);
 
-/* out[rows, w.rows] = x w^T with x bf16 [rows, w.cols]: each row of x holds cols rounded up to 8 elements, those
- * past cols finite (their products are with code 0). */
+/* out[rows, w.rows] = x w^T with x bf16 [rows, w.cols] (16-byte aligned rows): each row of x holds cols rounded up to
+ * 8 elements, those past cols finite (their products are with code 0).  The contraction may be split over
+ * workgroups: `workspace` (16-byte aligned, lrq_mxfp4_linear_workspace(rows, w, 0) bytes) takes their fp32 sums, which
+ * are added in a fixed order. */
 int lrq_mxfp4_linear(const void* x, int64_t ldx, int64_t rows, const lrq_mxfp4* w, void* out, int64_t ldo,
-                     int32_t out_fp32, void* stream);
+                     int32_t out_fp32, void* workspace, int64_t workspace_bytes, void* stream);
 
-/* out[rows, w.cols] = y w with y bf16 [rows, w.rows], the gradient of lrq_mxfp4_linear for x: each row of y holds
- * w.rows rounded up to 8 elements, those past w.rows zero. */
+/* out[rows, w.cols] = y w with y bf16 [rows, w.rows] (16-byte aligned rows), the gradient of lrq_mxfp4_linear for x:
+ * each row of y holds w.rows rounded up to 8 elements, those past w.rows zero; w.rows > 0.  `workspace`:
+ * lrq_mxfp4_linear_workspace(rows, w, 1) bytes. */
 int lrq_mxfp4_linear_t(const void* y, int64_t ldy, int64_t rows, const lrq_mxfp4* w, void* out, int64_t ldo,
-                       int32_t out_fp32, void* stream);
+                       int32_t out_fp32, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Workspace bytes (>= 0) of lrq_mxfp4_linear (transposed == 0) or lrq_mxfp4_linear_t on `rows` rows, or a negative
+ * LRQ_ERR_*.  Host only. */
+int64_t lrq_mxfp4_linear_workspace(int64_t rows, const lrq_mxfp4* w, int32_t transposed);
 
 /* ------------------------------------------------------------------ misc */
 const char* lrq_status_string(int status);

@@ -108,8 +108,9 @@ def test_mxfp4_descriptors(L, change, code):
     assert L.call_raw("lrq_mxfp4_dequantize", b, P, 256, 0, None) == want
     assert L.call_raw("lrq_mxfp4_gemm", b, g, P, 16, 0, None) == want
     assert L.call_raw("lrq_mxfp4_gemm", g, b, P, 16, 0, None) == want
-    assert L.call_raw("lrq_mxfp4_linear", P, 256, 4, b, Q, 16, 0, None) == want
-    assert L.call_raw("lrq_mxfp4_linear_t", P, 16, 4, b, Q, 256, 0, None) == want
+    assert L.call_raw("lrq_mxfp4_linear", P, 256, 4, b, Q, 16, 0, None, 0, None) == want
+    assert L.call_raw("lrq_mxfp4_linear_t", P, 16, 4, b, Q, 256, 0, None, 0, None) == want
+    assert L.call_raw("lrq_mxfp4_linear_workspace", 4, b, 0) == want
 
 
 def test_mxfp4_arguments(L):
@@ -119,13 +120,27 @@ def test_mxfp4_arguments(L):
     assert L.call_raw("lrq_mxfp4_gemm", g, g, None, 16, 0, None) == L.LRQ_ERR_NULL
     assert L.call_raw("lrq_mxfp4_gemm", g, g, P, 15, 0, None) == L.LRQ_ERR_SHAPE
     assert L.call_raw("lrq_mxfp4_gemm", g, g, ctypes.c_void_p(0x10002), 16, 1, None) == L.LRQ_ERR_ALIGN
-    assert L.call_raw("lrq_mxfp4_linear", None, 256, 4, g, Q, 16, 0, None) == L.LRQ_ERR_NULL
-    assert L.call_raw("lrq_mxfp4_linear", P, 255, 4, g, Q, 16, 0, None) == L.LRQ_ERR_SHAPE
-    assert L.call_raw("lrq_mxfp4_linear", P, 256, -4, g, Q, 16, 0, None) == L.LRQ_ERR_SHAPE
-    assert L.call_raw("lrq_mxfp4_linear", ctypes.c_void_p(0x10001), 256, 4, g, Q, 16, 0, None) == L.LRQ_ERR_ALIGN
-    assert L.call_raw("lrq_mxfp4_linear", P, 256, 4, g, Q, 15, 0, None) == L.LRQ_ERR_SHAPE
-    assert L.call_raw("lrq_mxfp4_linear_t", P, 8, 4, g, Q, 256, 0, None) == L.LRQ_ERR_SHAPE
-    assert L.call_raw("lrq_mxfp4_linear_t", P, 16, 4, g, Q, 255, 0, None) == L.LRQ_ERR_SHAPE
+    assert L.call_raw("lrq_mxfp4_linear", None, 256, 4, g, Q, 16, 0, None, 0, None) == L.LRQ_ERR_NULL
+    assert L.call_raw("lrq_mxfp4_linear", P, 255, 4, g, Q, 16, 0, None, 0, None) == L.LRQ_ERR_SHAPE
+    assert L.call_raw("lrq_mxfp4_linear", P, 256, -4, g, Q, 16, 0, None, 0, None) == L.LRQ_ERR_SHAPE
+    assert L.call_raw("lrq_mxfp4_linear", ctypes.c_void_p(0x10001), 256, 4, g, Q, 16, 0, None, 0, None) == L.LRQ_ERR_ALIGN
+    assert L.call_raw("lrq_mxfp4_linear", P, 256, 4, g, Q, 15, 0, None, 0, None) == L.LRQ_ERR_SHAPE
+    assert L.call_raw("lrq_mxfp4_linear_t", P, 8, 4, g, Q, 256, 0, None, 0, None) == L.LRQ_ERR_SHAPE
+    assert L.call_raw("lrq_mxfp4_linear_t", P, 16, 4, g, Q, 255, 0, None, 0, None) == L.LRQ_ERR_SHAPE
+    assert L.call_raw("lrq_mxfp4_linear", ctypes.c_void_p(0x10008), 256, 4, g, Q, 16, 0, None, 0, None) == L.LRQ_ERR_ALIGN
+    assert L.call_raw("lrq_mxfp4_linear", P, 260, 4, g, Q, 16, 0, None, 0, None) == L.LRQ_ERR_ALIGN
+    # a product split over workgroups needs its workspace
+    big = ctypes.byref(_mx(L, rows=1024, cols=8192, ld_codes=4096, ld_scales=256))
+    need = L.call_raw("lrq_mxfp4_linear_workspace", 256, big, 0)
+    assert need > 0 and need % (256 * 1024 * 4) == 0
+    args = (P, 8192, 256, big, Q, 1024, 0)
+    assert L.call_raw("lrq_mxfp4_linear", *args, None, need, None) == L.LRQ_ERR_NULL
+    assert L.call_raw("lrq_mxfp4_linear", *args, R_, need - 1, None) == L.LRQ_ERR_WORKSPACE
+    assert L.call_raw("lrq_mxfp4_linear", *args, ctypes.c_void_p(0x30004), need, None) == L.LRQ_ERR_ALIGN
+    assert L.call_raw("lrq_mxfp4_linear_workspace", 1, big, 0) == 0
+    assert L.call_raw("lrq_mxfp4_linear_workspace", -1, big, 0) == L.LRQ_ERR_SHAPE
+    empty = ctypes.byref(_mx(L, rows=0))
+    assert L.call_raw("lrq_mxfp4_linear_t", P, 8, 4, empty, Q, 256, 0, None, 0, None) == L.LRQ_ERR_SHAPE
     assert L.call_raw("lrq_mxfp4_quantize", P, 255, 0, g, None) == L.LRQ_ERR_SHAPE
     assert L.call_raw("lrq_mxfp4_quantize", P, 256, 5, g, None) == L.LRQ_ERR_UNSUPPORTED
     assert L.call_raw("lrq_mxfp4_dequantize", g, P, 256, 5, None) == L.LRQ_ERR_UNSUPPORTED

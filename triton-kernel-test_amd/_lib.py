@@ -128,8 +128,11 @@ SIGNATURES = {
     "lrq_mxfp4_quantize": (c_int32, [c_void_p, c_int64, c_int32, _M, c_void_p]),
     "lrq_mxfp4_dequantize": (c_int32, [_M, c_void_p, c_int64, c_int32, c_void_p]),
     "lrq_mxfp4_gemm": (c_int32, [_M, _M, c_void_p, c_int64, c_int32, c_void_p]),
-    "lrq_mxfp4_linear": (c_int32, [c_void_p, c_int64, c_int64, _M, c_void_p, c_int64, c_int32, c_void_p]),
-    "lrq_mxfp4_linear_t": (c_int32, [c_void_p, c_int64, c_int64, _M, c_void_p, c_int64, c_int32, c_void_p]),
+    "lrq_mxfp4_linear": (c_int32, [c_void_p, c_int64, c_int64, _M, c_void_p, c_int64, c_int32, c_void_p, c_int64,
+                                   c_void_p]),
+    "lrq_mxfp4_linear_t": (c_int32, [c_void_p, c_int64, c_int64, _M, c_void_p, c_int64, c_int32, c_void_p, c_int64,
+                                     c_void_p]),
+    "lrq_mxfp4_linear_workspace": (c_int64, [c_int64, _M, c_int32]),
     "lrq_status_string": (ctypes.c_char_p, [c_int32]),
     "lrq_abi_version": (c_int32, []),
 }

@@ -69,104 +69,371 @@ __global__ __launch_bounds__(256) void k_mx_gemm(Mx a, Mx b, void* out, int64_t 
       }
 }
 
-// Workgroup: 16 MT rows of X by 16 rows of W; its 8 waves take every eighth K step of 32 and join in LDS.
-template <int MT, bool F32>
+// ---------------------------------------------------------------- bf16 rows, few of them
+// Workgroup: 16 MT rows of X (all of them) by 16 NT rows of W; its 8 waves take every eighth K step of 128 and join in
+// LDS.  Lane (j, g) reads the 16 code bytes and the scale of block g of W row j: its k are 32g .. 32g + 31, 8 of them
+// for each of the step's four matrix instructions, and X is read in the same order.  Bound by the codes' bytes as long
+// as X is read seldom enough: NT grows with the rows of X.  Lanes without a row of X load nothing of it.
+template <int MT, int NT, bool F32>
 __global__ __launch_bounds__(512) void k_mx_linear(const uint16_t* x, int64_t ldx, int64_t rows, Mx w, void* out,
                                                    int64_t ldo) {
-  __shared__ float red[8][MT][64][4];
+  constexpr int U = MT * NT >= 8 ? 1 : MT * NT >= 4 ? 2 : 4;
+  __shared__ f32x4 red[8][NT][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 15, g = lane >> 4;
-  const int64_t m0 = (int64_t)blockIdx.y * 16 * MT, n0 = (int64_t)blockIdx.x * 16;
-  const int64_t rw = min(n0 + j, w.rows - 1);
-  const uint8_t* codes = w.codes + rw * w.ldc + 4 * g;
-  const uint8_t* scales = w.scales + rw * w.lds;
+  const int64_t n0 = (int64_t)blockIdx.x * 16 * NT;
+  const uint8_t *codes[NT], *scales[NT];
   const uint16_t* px[MT];
-  f32x4 acc[MT];
+  bool in[MT];
+  f32x4 acc[MT][NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int64_t rw = min(n0 + 16 * t + j, w.rows - 1);
+    codes[t] = w.codes + rw * w.ldc + 16 * g;
+    scales[t] = w.scales + rw * w.lds + g;
+  }
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
-    px[i] = x + min(m0 + 16 * i + j, rows - 1) * ldx + 8 * g;
-    acc[i] = zero4();
-  }
-  const int steps = (w.cols + 31) / 32;
-  for (int s = wave; s < steps; s += 8) {
-    const u32x4 b = fp4x8_to_bf16(ld4(codes + 16 * (int64_t)s), e8m0_operand(scales[s]));
-    const bool in = 32 * s + 8 * g < w.cols;
+    in[i] = 16 * i + j < rows;
+    px[i] = x + min((int64_t)(16 * i + j), rows - 1) * ldx + 32 * g;
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      u32x4 a = u32x4{0u, 0u, 0u, 0u};
-      if (in) a = *reinterpret_cast<const u32x4_any*>(px[i] + 32 * (int64_t)s);
-      acc[i] = mfma_16x16x32(a, b, acc[i]);
+    for (int t = 0; t < NT; ++t) acc[i][t] = zero4();
+  }
+  for (int s0 = wave; s0 < w.steps; s0 += 8 * U) {
+    u32x4 c[U][NT], a[U][MT][4];
+    uint32_t sc[U][NT];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int s = s0 + 8 * u, sl = min(s, w.steps - 1);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        c[u][t] = ld16_stream(codes[t] + 64 * (int64_t)sl);
+        sc[u][t] = scales[t][4 * (int64_t)sl];
+      }
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          a[u][i][q] = u32x4{0u, 0u, 0u, 0u};
+          if (in[i] && 128 * s + 32 * g + 8 * q < w.cols) a[u][i][q] = ld16(px[i] + 128 * (int64_t)s + 8 * q);
+        }
     }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const u32x4 b = fp4x8_to_bf16(c[u][t][q], e8m0_operand(sc[u][t]));
+#pragma unroll
+          for (int i = 0; i < MT; ++i) acc[i][t] = mfma_16x16x32(a[u][i][q], b, acc[i][t]);
+        }
   }
 #pragma unroll
-  for (int i = 0; i < MT; ++i)
+  for (int i = 0; i < MT; ++i) {
+    if (i > 0) __syncthreads();
 #pragma unroll
-    for (int v = 0; v < 4; ++v) red[wave][i][lane][v] = acc[i][v];
-  __syncthreads();
-  for (int o = threadIdx.x; o < MT * 256; o += 512) {
-    const int i = o >> 8, l = (o >> 2) & 63, v = o & 3;
-    float sum = 0.f;
+    for (int t = 0; t < NT; ++t) red[wave][t][lane] = acc[i][t];
+    __syncthreads();
+    for (int o = threadIdx.x; o < NT * 256; o += 512) {
+      const int t = o >> 8, l = (o & 15) + (o >> 2 & 48), v = o >> 4 & 3;  // 16 columns of an output row to 16 threads
+      float sum = 0.f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) sum += red[k][i][l][v];
-    const int64_t m = m0 + 16 * i + 4 * (l >> 4) + v, n = n0 + (l & 15);
-    if (m < rows && n < w.rows) st_out<F32>(out, m * ldo + n, sum);
+      for (int k = 0; k < 8; ++k) sum += red[k][t][l][v];
+      const int64_t m = 16 * i + 4 * (l >> 4) + v, n = n0 + 16 * t + (l & 15);
+      if (m < rows && n < w.rows) st_out<F32>(out, m * ldo + n, sum);
+    }
   }
 }
 
-// Wave: 16 MT rows of Y by 128 columns of W, summed over the rows of W.  Lane (j, g) widens the 8 x 8 block of
-// columns 8j .. 8j + 7 and rows 8g .. 8g + 7 and transposes it in registers: operand c holds column 8j + c, so the
-// output of operand c is column 8j + c of the wave's 128.
-template <int MT, bool F32>
-__global__ __launch_bounds__(256) void k_mx_linear_t(const uint16_t* y, int64_t ldy, int64_t rows, Mx w, void* out,
-                                                     int64_t ldo) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 15, g = lane >> 4;
-  const int64_t m0 = ((int64_t)blockIdx.y * 4 + wave) * 16 * MT;
-  if (m0 >= rows) return;
-  const int k0 = blockIdx.x * 128;
-  const uint8_t* codes = w.codes + k0 / 2 + 4 * j;
-  const uint8_t* scales = w.scales + k0 / 32 + j / 4;
-  const uint16_t* py[MT];
-  f32x4 acc[MT][8];
+// ---------------------------------------------------------------- bf16 rows, many of them
+// 16 zero bytes, read in place of a row's chunks past its end.
+__device__ const u32x4 kZeroChunk = u32x4{0u, 0u, 0u, 0u};
+
+template <int BYTES>
+__device__ __forceinline__ void ld_to_lds(const void* g, char* lds) {
+  const auto l = (__attribute__((address_space(3))) void*)lds;
+  if constexpr (BYTES == 16) __builtin_amdgcn_global_load_lds(g, l, 16, 0, 0);
+  else __builtin_amdgcn_global_load_lds(g, l, 4, 0, 0);
+}
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ f32x16 mfma_32x32x16(u32x4 a, u32x4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+struct TileArgs {
+  const uint16_t* x;  // [rows, contraction]
+  int64_t ldx;
+  int64_t rows;
+  Mx w;
+  void* out;          // [splits][rows][ldo] fp32 parts where splits > 1
+  int64_t ldo;
+  int64_t cols;       // columns of the output
+  int tiles_m, tiles_n, splits;
+  int steps;          // contraction steps of 128
+  int chunks;         // 8-element chunks of a row of x
+};
+
+// out = x w^T (TRANS false: the contraction runs along w's columns) or x w (true: along w's rows).
+//
+// Workgroup: 128 rows of x by 256 output columns, 8 waves.  Waves 4 gq .. 4 gq + 3 take the half gq of each contraction
+// step of 128, wave 4 gq + wn all 128 rows and columns 64 wn .. + 63 of it: so W's codes are widened once in a
+// workgroup, and two waves a SIMD cover each other's waits.  The halves are added through LDS at the end.  Every
+// operand goes straight to LDS, three steps deep, with counted waits: one barrier a step.
+//
+// 32x32x16 instructions.  Lane (c, h) (c = lane % 32, h = lane / 32) of instruction s < 4 holds contraction indices
+// 64 gq + 32 h + 8 s .. + 7 of the step (any order serves that both operands share), and column tile t is columns
+// 64 wn + 2 c + t: neighbouring columns end in one lane.
+//   TRANS false: those are 32 consecutive k of one W row, so the lane reads 16 code bytes and one scale a step.
+//   TRANS true: the lane's two columns are one code byte of each W row.  The transposing LDS read gives it that byte
+//   of 8 rows at once; each is widened with its own row's scale and the halves of two rows are paired by v_perm_b32.
+template <bool TRANS, bool F32>
+__global__ __launch_bounds__(512) void k_mx_tile(TileArgs a) {
+  constexpr int kA = 128 * 256, kB = 16384, kS = TRANS ? 2048 : 1024, kStage = kA + kB + kS;
+  constexpr int kLoads = 4 + 2 + 1;  // of a stage, a wave
+  extern __shared__ char sm[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int gq = wave >> 2, wn = wave & 3, c = lane & 31, h = lane >> 5;
+  const uint32_t tiles = a.tiles_m * a.tiles_n, id = xcd_tile(blockIdx.x, gridDim.x);
+  const uint32_t z = __builtin_amdgcn_readfirstlane(id / tiles), tile = id - z * tiles;
+  const uint32_t tn = __builtin_amdgcn_readfirstlane(tile / a.tiles_m), tm = tile - tn * a.tiles_m;
+  const int64_t m0 = (int64_t)tm * 128, n0 = (int64_t)tn * 256;
+  const int first = __builtin_amdgcn_readfirstlane((uint32_t)a.steps * z / (uint32_t)a.splits);
+  const int last = __builtin_amdgcn_readfirstlane((uint32_t)a.steps * (z + 1) / (uint32_t)a.splits);
+
+  // x: instruction i of wave w fills rows 4 (4 w + i) .. + 3 of the tile; chunk q of row r sits in slot q ^ (r % 16)
+  const char* px[4];
+  int qx[4];
 #pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    py[i] = y + min(m0 + 16 * i + j, rows - 1) * ldy + 8 * g;
-#pragma unroll
-    for (int c = 0; c < 8; ++c) acc[i][c] = zero4();
+  for (int i = 0; i < 4; ++i) {
+    const int r = 4 * (4 * wave + i) + (lane >> 4);
+    qx[i] = (lane & 15) ^ (r & 15);
+    px[i] = (const char*)(a.x + min(m0 + r, a.rows - 1) * a.ldx + 8 * qx[i]);
   }
-  for (int64_t n = 0; n < w.rows; n += 32) {
-    u32x4 r[8];  // row 8g + i, columns 8j .. 8j + 7
+  // codes: TRANS false: 256 rows of 64 bytes, 16-byte piece q of row r in slot q ^ (r / 4 % 4); TRANS true: 128 rows
+  // of 128 bytes, piece q of row r in slot q ^ (r / 2 % 4).  Both spread a wave's reads over the banks.
+  const uint8_t* pb[2];
+  int rb[2];
+  const uint8_t* ps;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int64_t rw = min(n + 8 * g + i, w.rows - 1);
-      r[i] = fp4x8_to_bf16(ld4(codes + rw * w.ldc), e8m0_operand(scales[rw * w.lds]));
-    }
-    u32x4 a[MT];
-    const bool in = n + 8 * g < w.rows;
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      a[i] = u32x4{0u, 0u, 0u, 0u};
-      if (in) a[i] = *reinterpret_cast<const u32x4_any*>(py[i] + n);
-    }
-#pragma unroll
-    for (int c = 0; c < 8; ++c) {
-      u32x4 b;
-#pragma unroll
-      for (int p = 0; p < 4; ++p)
-        b[p] = __builtin_amdgcn_perm(r[2 * p + 1][c / 2], r[2 * p][c / 2], (c & 1) ? 0x07060302u : 0x05040100u);
-#pragma unroll
-      for (int i = 0; i < MT; ++i) acc[i][c] = mfma_16x16x32(a[i], b, acc[i][c]);
+  for (int i = 0; i < 2; ++i) {
+    const int in = 2 * wave + i;
+    if constexpr (!TRANS) {
+      const int r = 16 * in + (lane >> 2);
+      pb[i] = a.w.codes + min(n0 + r, a.w.rows - 1) * a.w.ldc + 16 * ((lane & 3) ^ (r >> 2 & 3));
+    } else {
+      rb[i] = 8 * in + (lane >> 3);
+      pb[i] = a.w.codes + rb[i] * a.w.ldc + min(n0 / 2 + 16 * ((lane & 7) ^ (rb[i] >> 1 & 3)), 64 * (int64_t)a.w.steps - 16);
     }
   }
+  const int rs = TRANS ? (threadIdx.x & 255) >> 1 : 64 * (wave & 3) + lane;  // (waves 4 .. 7 load the same again)
+  if constexpr (!TRANS) ps = a.w.scales + min(n0 + rs, a.w.rows - 1) * a.w.lds;
+  else ps = a.w.scales + rs * a.w.lds + min(n0 / 32 + 4 * (lane & 1), 4 * (int64_t)a.w.steps - 4);
+
+  const auto issue = [&](int step, int buf) {
+    char* st = sm + buf * kStage;
+    if (16 * step + 16 <= a.chunks) {
 #pragma unroll
-  for (int i = 0; i < MT; ++i)
+      for (int i = 0; i < 4; ++i) ld_to_lds<16>(px[i] + 256 * (int64_t)step, st + 1024 * (4 * wave + i));
+    } else {
 #pragma unroll
-    for (int v = 0; v < 4; ++v) {
-      const int64_t m = m0 + 16 * i + 4 * g + v;
-      const int k = k0 + 8 * j;
-      if (m >= rows) continue;
-#pragma unroll
-      for (int c = 0; c < 8; ++c)
-        if (k + c < w.cols) st_out<F32>(out, m * ldo + k + c, acc[i][c][v]);
+      for (int i = 0; i < 4; ++i) {
+        const char* g = 16 * step + qx[i] < a.chunks ? px[i] + 256 * (int64_t)step : (const char*)&kZeroChunk;
+        ld_to_lds<16>(g, st + 1024 * (4 * wave + i));
+      }
     }
+    if constexpr (!TRANS) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) ld_to_lds<16>(pb[i] + 64 * (int64_t)step, st + kA + 1024 * (2 * wave + i));
+      ld_to_lds<4>(ps + 4 * (int64_t)step, st + kA + kB + 256 * (wave & 3));
+    } else if (128 * (int64_t)step + 128 <= a.w.rows) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) ld_to_lds<16>(pb[i] + step * (128 * a.w.ldc), st + kA + 1024 * (2 * wave + i));
+      ld_to_lds<4>(ps + step * (128 * a.w.lds), st + kA + kB + 256 * (wave & 3));
+    } else {  // rows past W's last: its last row (their x is zero)
+      const int64_t r0 = 128 * (int64_t)step, most = a.w.rows - 1 - r0;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        ld_to_lds<16>(pb[i] + (r0 + min((int64_t)rb[i], most) - rb[i]) * a.w.ldc, st + kA + 1024 * (2 * wave + i));
+      ld_to_lds<4>(ps + (r0 + min((int64_t)rs, most) - rs) * a.w.lds, st + kA + kB + 256 * (wave & 3));
+    }
+  };
+
+  f32x16 acc[4][2];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) acc[i][t][v] = 0.f;
+
+  issue(first, 0);
+  issue(min(first + 1, last - 1), 1);
+  int buf = 0;
+  for (int step = first; step < last; ++step) {
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(kLoads));  // this step's loads (the next step's are still out)
+    char* st = sm + buf * kStage;
+    if constexpr (TRANS) {
+      // the scales arrive as [row][8]; this thread's dword goes to [block][row]
+      const uint32_t s4 = ld4(st + kA + kB + 4 * (threadIdx.x & 255));
+#pragma unroll
+      for (int k = 0; k < 4; ++k) st[kA + kB + 1024 + (4 * (lane & 1) + k) * 128 + rs] = (char)(s4 >> (8 * k));
+    }
+    lds_barrier();  // every wave's loads are in, and the buffer of the step before is free
+    issue(min(step + 2, last - 1), buf == 0 ? 2 : buf - 1);
+    u32x4 code[2];
+    float scale[2];
+    u32x2 cols[4], rows8[4];  // TRANS: this lane's code byte and scale byte of 8 rows, for each instruction
+    if constexpr (TRANS) {
+      const int r0 = 64 * gq + 32 * h, blk = 2 * wn + (lane >> 4 & 1), r = r0 + (lane >> 1 & 7);
+      // by hand, with its wait: for the builtin the compiler first drains the loads to LDS just issued
+      const uint32_t p = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)(
+          st + kA + 128 * r + 16 * (blk ^ (r >> 1 & 3)) + 8 * (lane & 1));
+      asm volatile("ds_read_b64_tr_b8 %0, %4\n\tds_read_b64_tr_b8 %1, %4 offset:1024\n\t"
+                   "ds_read_b64_tr_b8 %2, %4 offset:2048\n\tds_read_b64_tr_b8 %3, %4 offset:3072\n\t"
+                   "s_waitcnt lgkmcnt(0)"
+                   : "=&v"(cols[0]), "=&v"(cols[1]), "=&v"(cols[2]), "=&v"(cols[3])
+                   : "v"(p)
+                   : "memory");
+#pragma unroll
+      for (int s = 0; s < 4; ++s) rows8[s] = ld8(st + kA + kB + 1024 + 128 * blk + r0 + 8 * s);
+    }
+    if constexpr (!TRANS) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int r = 64 * wn + 2 * c + t;
+        code[t] = ld16(st + kA + 64 * r + 16 * ((2 * gq + h) ^ (r >> 2 & 3)));
+        scale[t] = e8m0_operand((uint8_t)st[kA + kB + 4 * r + 2 * gq + h]);
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      u32x4 b[2];
+      if constexpr (!TRANS) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) b[t] = fp4x8_to_bf16(code[t][s], scale[t]);
+      } else {
+        uint32_t e[8];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {  // the conversion reads the exponent field alone
+          const uint32_t cw = cols[s][i], sw = rows8[s][i];
+          e[4 * i + 0] = fp4_to_bf16x2<0>(cw, __uint_as_float(sw << 23));
+          e[4 * i + 1] = fp4_to_bf16x2<1>(cw, __uint_as_float(sw << 15));
+          e[4 * i + 2] = fp4_to_bf16x2<2>(cw, __uint_as_float(sw << 7));
+          e[4 * i + 3] = fp4_to_bf16x2<3>(cw, __uint_as_float(sw >> 1));
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          b[0][i] = __builtin_amdgcn_perm(e[2 * i + 1], e[2 * i], 0x05040100u);
+          b[1][i] = __builtin_amdgcn_perm(e[2 * i + 1], e[2 * i], 0x07060302u);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = 32 * i + c;
+        const u32x4 x = ld16(st + 256 * r + 16 * ((8 * gq + 4 * h + s) ^ (r & 15)));
+#pragma unroll
+        for (int t = 0; t < 2; ++t) acc[i][t] = mfma_32x32x16(x, b[t], acc[i][t]);
+      }
+    }
+    buf = buf == 2 ? 0 : buf + 1;
+  }
+
+  // Half gq finishes rows 64 gq .. + 63: each wave passes the other half's sums through LDS.
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+  __syncthreads();
+  f32x4* ex = (f32x4*)sm;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f32x16& v = gq ? acc[i][t] : acc[2 + i][t];
+        ex[((wave * 16) + 8 * i + 4 * t + q) * 64 + lane] = f32x4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+      }
+  __syncthreads();
+  char* out = (char*)a.out + (a.splits > 1 ? (int64_t)z * a.rows * a.ldo * 4 : 0);
+  const int64_t n = n0 + 64 * wn + 2 * c;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      f32x4 v[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const f32x4 o = ex[(((wave ^ 4) * 16) + 8 * i + 4 * t + q) * 64 + lane];
+        const f32x16& w = gq ? acc[2 + i][t] : acc[i][t];
+        v[t] = f32x4{w[4 * q] + o[0], w[4 * q + 1] + o[1], w[4 * q + 2] + o[2], w[4 * q + 3] + o[3]};
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int64_t m = m0 + 64 * gq + 32 * i + 8 * q + 4 * h + k;
+        if (m >= a.rows || n >= a.cols) continue;
+        if (n + 1 < a.cols) {
+          if constexpr (F32) {
+            typedef f32x2_t f32x2_any __attribute__((aligned(4)));
+            *(f32x2_any*)(out + (m * a.ldo + n) * 4) = f32x2_t{v[0][k], v[1][k]};
+          } else {
+            typedef uint32_t u32_any __attribute__((aligned(2)));
+            *(u32_any*)(out + (m * a.ldo + n) * 2) = pack_bf16x2(v[0][k], v[1][k]);
+          }
+        } else {
+          st_out<F32>(out, m * a.ldo + n, v[0][k]);
+        }
+      }
+    }
+}
+
+// out[rows, cols] = the splits' sums, in their order; 4 columns a thread.
+template <bool F32>
+__global__ __launch_bounds__(256) void k_mx_join(const float* part, int splits, int64_t rows, int64_t cols, int64_t ldp,
+                                                 void* out, int64_t ldo) {
+  const int64_t quads = ldp / 4, total = rows * quads;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t m = i / quads, n = 4 * (i - m * quads);
+    f32x4 s = *(const f32x4*)(part + m * ldp + n);
+    for (int z = 1; z < splits; ++z) {
+      const f32x4 v = *(const f32x4*)(part + ((int64_t)z * rows + m) * ldp + n);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s[k] += v[k];
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (n + k < cols) st_out<F32>(out, m * ldo + n + k, s[k]);
+  }
+}
+
+// Rows of x that the few-row kernel takes (one 16-row tile of matrix instructions, or up to four).
+static constexpr int64_t kFewRows = 64;
+// Workgroups that give every CU work.
+static constexpr int64_t kWideRows = 200;
+
+struct SplitPlan {
+  int64_t tiles_m, tiles_n;
+  int splits, steps;
+};
+
+// How often the contraction is split over workgroups: one workgroup runs on a CU at a time, so a grid takes
+// ceil(workgroups / CUs) rounds of its steps; every split writes and re-reads fp32 parts.  Times in us.
+static SplitPlan split_plan(int64_t rows, const lrq_mxfp4* t, bool trans) {
+  const int64_t cols = trans ? t->cols : t->rows, depth = trans ? t->rows : t->cols;
+  SplitPlan p{(rows + 127) / 128, (cols + 255) / 256, 1, (int)((depth + 127) / 128)};
+  if (!trans && rows <= kFewRows) return p;
+  constexpr double kStep = 1.1, kJoin = 4.0, kPerByte = 2.0 / 4.0e6;
+  const int64_t tiles = p.tiles_m * p.tiles_n;
+  double best = 0.;
+  for (int s = 1; s <= 16 && s <= std::max(1, p.steps / 2); ++s) {
+    const double rounds = (double)((tiles * s + 255) / 256);
+    const double cost = rounds * ((p.steps + s - 1) / s + 2) * kStep + (s > 1 ? kJoin + kPerByte * 4. * s * rows * cols : 0.);
+    if (s == 1 || cost < best) best = cost, p.splits = s;
+  }
+  return p;
+}
+
+static int64_t split_bytes(const SplitPlan& p, int64_t rows, int64_t cols) {
+  return p.splits > 1 ? (int64_t)p.splits * rows * ((cols + 3) / 4 * 4) * 4 : 0;
 }
 
 static int validate_out(const void* out, int64_t ldo, int64_t cols, int32_t f32) {
@@ -195,43 +462,80 @@ extern "C" int lrq_mxfp4_gemm(const lrq_mxfp4* ta, const lrq_mxfp4* tb, void* ou
                   : launch(k_mx_gemm<false>, grid, dim3(256), 0, s, a, b, out, ldo);
 }
 
-extern "C" int lrq_mxfp4_linear(const void* x, int64_t ldx, int64_t rows, const lrq_mxfp4* t, void* out, int64_t ldo,
-                                int32_t out_fp32, void* stream) {
+extern "C" int64_t lrq_mxfp4_linear_workspace(int64_t rows, const lrq_mxfp4* t, int32_t transposed) {
   LRQ_TRY(validate_mx(t));
   if (rows < 0 || rows > INT32_MAX) return LRQ_ERR_SHAPE;
-  if (rows == 0 || t->rows == 0) return LRQ_OK;
-  if (x == nullptr) return LRQ_ERR_NULL;
-  if (ldx < (t->cols + 7) / 8 * 8) return LRQ_ERR_SHAPE;
-  if (!aligned(x, 2)) return LRQ_ERR_ALIGN;
-  LRQ_TRY(validate_out(out, ldo, t->rows, out_fp32));
-  const Mx w = make_mx(t);
-  hipStream_t s = (hipStream_t)stream;
-  const int mt = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-  const dim3 grid((unsigned)((w.rows + 15) / 16), (unsigned)((rows + 16 * mt - 1) / (16 * mt)));
-  const uint16_t* px = (const uint16_t*)x;
-#define LRQ_GO(MT) return out_fp32 ? launch(k_mx_linear<MT, true>, grid, dim3(512), 0, s, px, ldx, rows, w, out, ldo) \
-                                   : launch(k_mx_linear<MT, false>, grid, dim3(512), 0, s, px, ldx, rows, w, out, ldo)
-  if (mt == 1) LRQ_GO(1);
-  if (mt == 2) LRQ_GO(2);
-  LRQ_GO(4);
-#undef LRQ_GO
+  return split_bytes(split_plan(rows, t, transposed != 0), rows, transposed ? t->cols : t->rows);
 }
 
-extern "C" int lrq_mxfp4_linear_t(const void* y, int64_t ldy, int64_t rows, const lrq_mxfp4* t, void* out, int64_t ldo,
-                                  int32_t out_fp32, void* stream) {
+static int mx_linear(const void* x, int64_t ldx, int64_t rows, const lrq_mxfp4* t, bool trans, void* out, int64_t ldo,
+                     int32_t out_fp32, void* workspace, int64_t workspace_bytes, void* stream) {
   LRQ_TRY(validate_mx(t));
   if (rows < 0 || rows > INT32_MAX) return LRQ_ERR_SHAPE;
-  if (rows == 0) return LRQ_OK;
-  if (t->rows > 0) {
-    if (y == nullptr) return LRQ_ERR_NULL;
-    if (ldy < (t->rows + 7) / 8 * 8) return LRQ_ERR_SHAPE;
-    if (!aligned(y, 2)) return LRQ_ERR_ALIGN;
+  const int64_t depth = trans ? t->rows : t->cols, cols = trans ? t->cols : t->rows;
+  if (rows == 0 || cols == 0) return LRQ_OK;
+  if (depth > 0) {
+    if (x == nullptr) return LRQ_ERR_NULL;
+    if (ldx < (depth + 7) / 8 * 8) return LRQ_ERR_SHAPE;
+    if (!aligned(x, 16) || (ldx % 8) != 0) return LRQ_ERR_ALIGN;
   }
-  LRQ_TRY(validate_out(out, ldo, t->cols, out_fp32));
+  LRQ_TRY(validate_out(out, ldo, cols, out_fp32));
+  if (depth == 0) return LRQ_ERR_SHAPE;  // (a sum over no rows: the caller's zeros)
   const Mx w = make_mx(t);
   hipStream_t s = (hipStream_t)stream;
-  const dim3 grid((unsigned)w.steps, (unsigned)((rows + 127) / 128));
-  const uint16_t* py = (const uint16_t*)y;
-  return out_fp32 ? launch(k_mx_linear_t<2, true>, grid, dim3(256), 0, s, py, ldy, rows, w, out, ldo)
-                  : launch(k_mx_linear_t<2, false>, grid, dim3(256), 0, s, py, ldy, rows, w, out, ldo);
+  const uint16_t* px = (const uint16_t*)x;
+  if (!trans && rows <= kFewRows) {
+    // as many W rows a workgroup as still give each CU one
+    const auto go = [&](auto mt, auto nt) {
+      const dim3 grid((unsigned)((w.rows + 16 * nt() - 1) / (16 * nt())));
+      return out_fp32 ? launch(k_mx_linear<mt(), nt(), true>, grid, dim3(512), 0, s, px, ldx, rows, w, out, ldo)
+                      : launch(k_mx_linear<mt(), nt(), false>, grid, dim3(512), 0, s, px, ldx, rows, w, out, ldo);
+    };
+    using std::integral_constant;
+    const int most = w.rows >= 64 * kWideRows ? 4 : w.rows >= 32 * kWideRows ? 2 : 1;
+#define LRQ_GO(MT)                                                                          \
+  {                                                                                         \
+    if (most == 4) return go(integral_constant<int, MT>{}, integral_constant<int, 4>{});    \
+    if (most == 2) return go(integral_constant<int, MT>{}, integral_constant<int, 2>{});    \
+    return go(integral_constant<int, MT>{}, integral_constant<int, 1>{});                   \
+  }
+    if (rows <= 4) return go(integral_constant<int, 1>{}, integral_constant<int, 1>{});
+    if (rows <= 16) LRQ_GO(1)
+    if (rows <= 32) LRQ_GO(2)
+    LRQ_GO(4)
+#undef LRQ_GO
+  }
+  const SplitPlan p = split_plan(rows, t, trans);
+  const int64_t need = split_bytes(p, rows, cols);
+  if (need > 0 && workspace == nullptr) return LRQ_ERR_NULL;
+  if (need > 0 && !aligned(workspace, 16)) return LRQ_ERR_ALIGN;
+  if (workspace_bytes < need) return LRQ_ERR_WORKSPACE;
+  const int64_t ldp = (cols + 3) / 4 * 4;
+  const int64_t wgs = p.tiles_m * p.tiles_n * p.splits;
+  if (wgs > INT32_MAX) return LRQ_ERR_SHAPE;
+  const TileArgs a{px, ldx, rows, w, need ? workspace : out, need ? ldp : ldo, cols, (int)p.tiles_m, (int)p.tiles_n,
+                   p.splits, p.steps, (int)((depth + 7) / 8)};
+  const bool f32 = need > 0 || out_fp32;
+  const auto go = [&](auto kern, int lds) {
+    const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (e != hipSuccess) return (int)e;
+    return launch(kern, dim3((unsigned)wgs), dim3(512), (size_t)lds, s, a);
+  };
+  constexpr int kLds = 3 * (128 * 256 + 16384 + 1024), kLdsT = kLds + 3 * 1024;
+  if (trans) LRQ_TRY(f32 ? go(k_mx_tile<true, true>, kLdsT) : go(k_mx_tile<true, false>, kLdsT));
+  else LRQ_TRY(f32 ? go(k_mx_tile<false, true>, kLds) : go(k_mx_tile<false, false>, kLds));
+  if (need == 0) return LRQ_OK;
+  const dim3 grid((unsigned)std::min<int64_t>((rows * (ldp / 4) + 255) / 256, (int64_t)cu_count() * 32));
+  return out_fp32 ? launch(k_mx_join<true>, grid, dim3(256), 0, s, (const float*)workspace, p.splits, rows, cols, ldp, out, ldo)
+                  : launch(k_mx_join<false>, grid, dim3(256), 0, s, (const float*)workspace, p.splits, rows, cols, ldp, out, ldo);
+}
+
+extern "C" int lrq_mxfp4_linear(const void* x, int64_t ldx, int64_t rows, const lrq_mxfp4* w, void* out, int64_t ldo,
+                                int32_t out_fp32, void* workspace, int64_t workspace_bytes, void* stream) {
+  return mx_linear(x, ldx, rows, w, false, out, ldo, out_fp32, workspace, workspace_bytes, stream);
+}
+
+extern "C" int lrq_mxfp4_linear_t(const void* y, int64_t ldy, int64_t rows, const lrq_mxfp4* w, void* out, int64_t ldo,
+                                  int32_t out_fp32, void* workspace, int64_t workspace_bytes, void* stream) {
+  return mx_linear(y, ldy, rows, w, true, out, ldo, out_fp32, workspace, workspace_bytes, stream);
 }

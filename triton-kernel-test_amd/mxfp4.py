@@ -14,7 +14,7 @@ from dataclasses import dataclass
 
 import torch
 
-from ._lib import LrqMxfp4, call
+from ._lib import LrqMxfp4, call, call_raw, check
 from .api import _on, _p, _require_device, _stream
 from .norm import _dtype, _rows
 
@@ -131,28 +131,35 @@ def _operand(x: torch.Tensor, cols: int, name: str):
     if cols % 8:
         x = torch.nn.functional.pad(x, (0, -cols % 8))
     x2, rows, _, ld = _rows(x, name)
+    if ld % 8 or x2.data_ptr() % 16:
+        x2 = x2.clone(memory_format=torch.contiguous_format)
+        ld = x2.shape[1]
     return x2, rows, ld
+
+
+def _product(name: str, x: torch.Tensor, w: MXFP4Tensor, out_dtype, transposed: int) -> torch.Tensor:
+    f32 = _out_fp32(out_dtype)
+    t = _matrix(w, x.device)
+    depth, cols = (w.rows, w.cols) if transposed else (w.cols, w.rows)
+    x2, rows, ld = _operand(x, depth, "dy" if transposed else "x")
+    out = torch.empty(tuple(x.shape[:-1]) + (cols,), dtype=out_dtype, device=x.device)
+    if depth == 0:
+        return out.zero_()
+    ws, ws_bytes = None, call_raw("lrq_mxfp4_linear_workspace", rows, ctypes.byref(t), transposed)
+    if ws_bytes < 0:
+        check(ws_bytes, "lrq_mxfp4_linear_workspace")
+    if ws_bytes:
+        ws = torch.empty(ws_bytes // 4, dtype=torch.float32, device=x.device)
+    with _on(x.device):
+        call(name, _p(x2), ld, rows, ctypes.byref(t), _p(out), cols, f32, _p(ws), ws_bytes, _stream(x.device))
+    return out
 
 
 def mxfp4_linear(x: torch.Tensor, w: MXFP4Tensor, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """x @ w^T for bf16 x [..., K] and an MXFP4 weight [N, K]: [..., N], fp32 accumulate."""
-    f32 = _out_fp32(out_dtype)
-    t = _matrix(w, x.device)
-    x2, rows, ldx = _operand(x, w.cols, "x")
-    out = torch.empty(tuple(x.shape[:-1]) + (w.rows,), dtype=out_dtype, device=x.device)
-    with _on(x.device):
-        call("lrq_mxfp4_linear", _p(x2), ldx, rows, ctypes.byref(t), _p(out), w.rows, f32, _stream(x.device))
-    return out
+    return _product("lrq_mxfp4_linear", x, w, out_dtype, 0)
 
 
 def mxfp4_linear_backward(dy: torch.Tensor, w: MXFP4Tensor, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """dy @ w for bf16 dy [..., N] and an MXFP4 weight [N, K]: the gradient of ``mxfp4_linear`` for x."""
-    f32 = _out_fp32(out_dtype)
-    t = _matrix(w, dy.device)
-    dy2, rows, ld = _operand(dy, w.rows, "dy")
-    out = torch.empty(tuple(dy.shape[:-1]) + (w.cols,), dtype=out_dtype, device=dy.device)
-    if w.rows == 0:
-        return out.zero_()
-    with _on(dy.device):
-        call("lrq_mxfp4_linear_t", _p(dy2), ld, rows, ctypes.byref(t), _p(out), w.cols, f32, _stream(dy.device))
-    return out
+    return _product("lrq_mxfp4_linear_t", dy, w, out_dtype, 1)
