@@ -417,8 +417,13 @@ int lrq_mxfp4_quantize(const void* x, int64_t ldx, int32_t dtype, const lrq_mxfp
 int lrq_mxfp4_dequantize(const lrq_mxfp4* t, void* out, int64_t ldo, int32_t dtype, void* stream);
 
 /* out[a.rows, b.rows] = a b^T, both MXFP4 with the same cols; fp32 accumulation, out fp32 when out_fp32 != 0,
- * else bf16. */
-int lrq_mxfp4_gemm(const lrq_mxfp4* a, const lrq_mxfp4* b, void* out, int64_t ldo, int32_t out_fp32, void* stream);
+ * else bf16.  The contraction may be split over workgroups: `workspace` (16-byte aligned,
+ * lrq_mxfp4_gemm_workspace(a, b) bytes) takes their fp32 sums, which are added in a fixed order. */
+int lrq_mxfp4_gemm(const lrq_mxfp4* a, const lrq_mxfp4* b, void* out, int64_t ldo, int32_t out_fp32, void* workspace,
+                   int64_t workspace_bytes, void* stream);
+
+/* Workspace bytes of lrq_mxfp4_gemm (>= 0), or a negative LRQ_ERR_*.  Host only. */
+int64_t lrq_mxfp4_gemm_workspace(const lrq_mxfp4* a, const lrq_mxfp4* b);
 
 /* out[rows, w.rows] = x w^T with x bf16 [rows, w.cols] (16-byte aligned rows): each row of x holds cols rounded up to
  * 8 elements, those past cols finite (their products are with code 0).  The contraction may be split over

@@ -169,7 +169,9 @@ def mx_nibbles(packed):
 
 def product_bound(a, b, dtype, extra=0):
     """a [M, K] times b [K, N] in fp32 in any order: K roundings of sums at most, and the output's."""
-    mag = a.abs() @ b.abs()
+    if torch.cuda.is_available():
+        a, b = a.cuda(), b.contiguous().cuda()
+    mag = (a.abs() @ b.abs()).cpu()
     e = (a.shape[1] + extra) * U * mag
-    ref = a @ b
+    ref = (a @ b).cpu()
     return ref, half_step(dtype) * (ref.abs() + e) + e + smallest(dtype)

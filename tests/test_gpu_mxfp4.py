@@ -92,7 +92,7 @@ def _operands(pkg, dev, m, n, k, seed):
 # one row to several tiles; widths that end inside a block, a step and a tile
 SIZES = [(1, 1, 1), (1, 16, 32), (2, 17, 33), (1, 300, 4096), (5, 129, 1000), (16, 256, 128), (17, 100, 520), (33, 64, 96),
          (64, 512, 2048), (65, 257, 136), (130, 1, 257), (128, 128, 128), (129, 260, 640), (300, 513, 1111),
-         (512, 768, 1024), (1, 5000, 8), (700, 40, 72)]
+         (512, 768, 1024), (1, 5000, 8), (700, 40, 72), (4096, 4096, 160), (200, 13000, 288), (40, 13000, 264), (300, 500, 6000)]
 
 
 @pytest.mark.parametrize("m,n,k", SIZES)

@@ -106,8 +106,8 @@ def test_mxfp4_descriptors(L, change, code):
     b, g = ctypes.byref(bad), ctypes.byref(good)
     assert L.call_raw("lrq_mxfp4_quantize", P, 256, 0, b, None) == want
     assert L.call_raw("lrq_mxfp4_dequantize", b, P, 256, 0, None) == want
-    assert L.call_raw("lrq_mxfp4_gemm", b, g, P, 16, 0, None) == want
-    assert L.call_raw("lrq_mxfp4_gemm", g, b, P, 16, 0, None) == want
+    assert L.call_raw("lrq_mxfp4_gemm", b, g, P, 16, 0, None, 0, None) == want
+    assert L.call_raw("lrq_mxfp4_gemm", g, b, P, 16, 0, None, 0, None) == want
     assert L.call_raw("lrq_mxfp4_linear", P, 256, 4, b, Q, 16, 0, None, 0, None) == want
     assert L.call_raw("lrq_mxfp4_linear_t", P, 16, 4, b, Q, 256, 0, None, 0, None) == want
     assert L.call_raw("lrq_mxfp4_linear_workspace", 4, b, 0) == want
@@ -116,10 +116,10 @@ def test_mxfp4_descriptors(L, change, code):
 def test_mxfp4_arguments(L):
     g = ctypes.byref(_mx(L))
     other = ctypes.byref(_mx(L, cols=255))
-    assert L.call_raw("lrq_mxfp4_gemm", g, other, P, 16, 0, None) == L.LRQ_ERR_SHAPE
-    assert L.call_raw("lrq_mxfp4_gemm", g, g, None, 16, 0, None) == L.LRQ_ERR_NULL
-    assert L.call_raw("lrq_mxfp4_gemm", g, g, P, 15, 0, None) == L.LRQ_ERR_SHAPE
-    assert L.call_raw("lrq_mxfp4_gemm", g, g, ctypes.c_void_p(0x10002), 16, 1, None) == L.LRQ_ERR_ALIGN
+    assert L.call_raw("lrq_mxfp4_gemm", g, other, P, 16, 0, None, 0, None) == L.LRQ_ERR_SHAPE
+    assert L.call_raw("lrq_mxfp4_gemm", g, g, None, 16, 0, None, 0, None) == L.LRQ_ERR_NULL
+    assert L.call_raw("lrq_mxfp4_gemm", g, g, P, 15, 0, None, 0, None) == L.LRQ_ERR_SHAPE
+    assert L.call_raw("lrq_mxfp4_gemm", g, g, ctypes.c_void_p(0x10002), 16, 1, None, 0, None) == L.LRQ_ERR_ALIGN
     assert L.call_raw("lrq_mxfp4_linear", None, 256, 4, g, Q, 16, 0, None, 0, None) == L.LRQ_ERR_NULL
     assert L.call_raw("lrq_mxfp4_linear", P, 255, 4, g, Q, 16, 0, None, 0, None) == L.LRQ_ERR_SHAPE
     assert L.call_raw("lrq_mxfp4_linear", P, 256, -4, g, Q, 16, 0, None, 0, None) == L.LRQ_ERR_SHAPE
@@ -138,6 +138,11 @@ def test_mxfp4_arguments(L):
     assert L.call_raw("lrq_mxfp4_linear", *args, R_, need - 1, None) == L.LRQ_ERR_WORKSPACE
     assert L.call_raw("lrq_mxfp4_linear", *args, ctypes.c_void_p(0x30004), need, None) == L.LRQ_ERR_ALIGN
     assert L.call_raw("lrq_mxfp4_linear_workspace", 1, big, 0) == 0
+    need = L.call_raw("lrq_mxfp4_gemm_workspace", big, big)
+    assert need > 0 and need % (1024 * 1024 * 4) == 0
+    assert L.call_raw("lrq_mxfp4_gemm", big, big, P, 1024, 0, None, need, None) == L.LRQ_ERR_NULL
+    assert L.call_raw("lrq_mxfp4_gemm", big, big, P, 1024, 0, Q, need - 4, None) == L.LRQ_ERR_WORKSPACE
+    assert L.call_raw("lrq_mxfp4_gemm_workspace", big, g) == L.LRQ_ERR_SHAPE
     assert L.call_raw("lrq_mxfp4_linear_workspace", -1, big, 0) == L.LRQ_ERR_SHAPE
     empty = ctypes.byref(_mx(L, rows=0))
     assert L.call_raw("lrq_mxfp4_linear_t", P, 8, 4, empty, Q, 256, 0, None, 0, None) == L.LRQ_ERR_SHAPE

@@ -127,7 +127,8 @@ SIGNATURES = {
     "lrq_layer_norm_bwd_workspace": (c_int64, [c_int64, c_int64]),
     "lrq_mxfp4_quantize": (c_int32, [c_void_p, c_int64, c_int32, _M, c_void_p]),
     "lrq_mxfp4_dequantize": (c_int32, [_M, c_void_p, c_int64, c_int32, c_void_p]),
-    "lrq_mxfp4_gemm": (c_int32, [_M, _M, c_void_p, c_int64, c_int32, c_void_p]),
+    "lrq_mxfp4_gemm": (c_int32, [_M, _M, c_void_p, c_int64, c_int32, c_void_p, c_int64, c_void_p]),
+    "lrq_mxfp4_gemm_workspace": (c_int64, [_M, _M]),
     "lrq_mxfp4_linear": (c_int32, [c_void_p, c_int64, c_int64, _M, c_void_p, c_int64, c_int32, c_void_p, c_int64,
                                    c_void_p]),
     "lrq_mxfp4_linear_t": (c_int32, [c_void_p, c_int64, c_int64, _M, c_void_p, c_int64, c_int32, c_void_p, c_int64,

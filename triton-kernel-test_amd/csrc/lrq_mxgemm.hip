@@ -7,66 +7,167 @@
 
 namespace lrq {
 
-typedef int i32x8 __attribute__((ext_vector_type(8)));
-
-// D(16x16) += A(16x128) B(128x16), both e2m1 with E8M0 block scales.  Lane l holds row (column) l % 16, k = 32 (l / 16)
-// .. + 31, and its block's scale in the low byte of its scale operand.
-__device__ __forceinline__ f32x4 mfma_mx(u32x4 a, u32x4 b, f32x4 c, uint32_t sa, uint32_t sb) {
-  const i32x8 a8 = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0};
-  const i32x8 b8 = {(int)b[0], (int)b[1], (int)b[2], (int)b[3], 0, 0, 0, 0};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a8, b8, c, 4, 4, 0, (int)sa, 0, (int)sb);
-}
-
 template <bool F32>
 __device__ __forceinline__ void st_out(void* out, int64_t at, float v) {
   if constexpr (F32) reinterpret_cast<float*>(out)[at] = v;
   else reinterpret_cast<uint16_t*>(out)[at] = (uint16_t)pack_bf16x2(v, 0.f);
 }
 
-// Wave: 64 x 64 of the output, operands straight from global memory.  Rows past the operands are read from their last row
-// and not stored.
+// Columns n and n + 1 of row m (n + 1 only where the output has it).
 template <bool F32>
-__global__ __launch_bounds__(256) void k_mx_gemm(Mx a, Mx b, void* out, int64_t ldo) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 15, g = lane >> 4;
-  const int64_t m0 = (int64_t)blockIdx.y * 128 + 64 * (wave >> 1), n0 = (int64_t)blockIdx.x * 128 + 64 * (wave & 1);
-  f32x4 acc[4][4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int k = 0; k < 4; ++k) acc[i][k] = zero4();
-  const uint8_t *ca[4], *cb[4], *pa[4], *pb[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t ra = min(m0 + 16 * i + j, a.rows - 1), rb = min(n0 + 16 * i + j, b.rows - 1);
-    ca[i] = a.codes + ra * a.ldc + 16 * g;
-    pa[i] = a.scales + ra * a.lds + g;
-    cb[i] = b.codes + rb * b.ldc + 16 * g;
-    pb[i] = b.scales + rb * b.lds + g;
-  }
-  for (int s = 0; s < a.steps; ++s) {
-    u32x4 va[4], vb[4];
-    uint32_t sa[4], sb[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      va[i] = ld16(ca[i] + 64 * (int64_t)s);
-      vb[i] = ld16(cb[i] + 64 * (int64_t)s);
-      sa[i] = pa[i][4 * (int64_t)s];
-      sb[i] = pb[i][4 * (int64_t)s];
+__device__ __forceinline__ void st_pair(char* out, int64_t m, int64_t n, int64_t ldo, int64_t cols, float v0, float v1) {
+  if (n + 1 < cols) {
+    if constexpr (F32) {
+      typedef f32x2_t f32x2_any __attribute__((aligned(4)));
+      *(f32x2_any*)(out + (m * ldo + n) * 4) = f32x2_t{v0, v1};
+    } else {
+      typedef uint32_t u32_any __attribute__((aligned(2)));
+      *(u32_any*)(out + (m * ldo + n) * 2) = pack_bf16x2(v0, v1);
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) acc[i][k] = mfma_mx(va[i], vb[k], acc[i][k], sa[i], sb[k]);
+  } else if (n < cols) {
+    st_out<F32>(out, m * ldo + n, v0);
   }
+}
+
+// 16 zero bytes, read in place of a row's chunks past its end.
+__device__ const u32x4 kZeroChunk = u32x4{0u, 0u, 0u, 0u};
+
+template <int BYTES>
+__device__ __forceinline__ void ld_to_lds(const void* g, char* lds) {
+  const auto l = (__attribute__((address_space(3))) void*)lds;
+  if constexpr (BYTES == 16) __builtin_amdgcn_global_load_lds(g, l, 16, 0, 0);
+  else __builtin_amdgcn_global_load_lds(g, l, 4, 0, 0);
+}
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ f32x16 mfma_32x32x16(u32x4 a, u32x4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// D(32x32) += A(32x64) B(64x32), both e2m1 with E8M0 block scales.  Lane l holds row (column) l % 32, k = 32 (l / 32)
+// .. + 31, and its block's scale in byte SEL of its scale operand.
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+template <int SEL>
+__device__ __forceinline__ f32x16 mfma_mx(u32x4 a, u32x4 b, f32x16 c, uint32_t sa, uint32_t sb) {
+  const i32x8 a8 = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0};
+  const i32x8 b8 = {(int)b[0], (int)b[1], (int)b[2], (int)b[3], 0, 0, 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a8, b8, c, 4, 4, SEL, (int)sa, SEL, (int)sb);
+}
+
+// Workgroup tiles of a product whose contraction may be split: this workgroup's tile and steps.
+struct Place {
+  int z;
+  int64_t m0, n0;
+  int first, last;
+};
+__device__ __forceinline__ Place place(int tiles_m, int tiles_n, int splits, int steps, int bm, int bn) {
+  const uint32_t tiles = tiles_m * tiles_n, id = xcd_tile(blockIdx.x, gridDim.x);
+  const uint32_t z = __builtin_amdgcn_readfirstlane(id / tiles), tile = id - z * tiles;
+  const uint32_t tn = __builtin_amdgcn_readfirstlane(tile / tiles_m), tm = tile - tn * tiles_m;
+  return Place{(int)z, (int64_t)tm * bm, (int64_t)tn * bn,
+               (int)__builtin_amdgcn_readfirstlane((uint32_t)steps * z / (uint32_t)splits),
+               (int)__builtin_amdgcn_readfirstlane((uint32_t)steps * (z + 1) / (uint32_t)splits)};
+}
+
+// ---------------------------------------------------------------- both operands in MXFP4
+struct GemmArgs {
+  Mx a, b;
+  void* out;  // [splits][a.rows][ldo] fp32 parts where splits > 1
+  int64_t ldo;
+  int tiles_m, tiles_n, splits;
+};
+
+// Workgroup: 64 MT rows of A by 256 rows of B, 8 waves in two rows of four, each 32 MT x 64 of it in 32x32x64 scaled
+// instructions, whose operands are the stored codes and scale bytes as they are.  A K step of 128 columns is one scale
+// dword a row and 64 code bytes; both go straight to LDS, four steps deep, one barrier a step.  Row r's 16-byte piece q
+// sits in slot q ^ (r / 4 % 4): 16 lanes of a read cover all banks.  LDS row 64 wn + 32 t + c of B holds row 64 wn +
+// 2 c + t, so that a lane's two columns are neighbours in the output.
+template <int MT, bool F32>
+__global__ __launch_bounds__(512) void k_mx_gemm(GemmArgs p) {
+  constexpr int kA = 64 * MT * 64, kB = 16384, kSA = 64 * MT * 4, kSB = 1024, kStage = kA + kB + kSA + kSB, kDeep = 4;
+  constexpr int kLa = MT >= 2 ? MT / 2 : 1;  // 1 KB loads of A a wave (MT 1: the upper four waves load the same again)
+  constexpr int kLoads = kLa + 2 + 2;
+  extern __shared__ char sm[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave >> 2, wn = wave & 3, c = lane & 31, h = lane >> 5;
+  const Place at = place(p.tiles_m, p.tiles_n, p.splits, p.a.steps, 64 * MT, 256);
+
+  const uint8_t *pa[kLa], *pb[2];
+  char *la[kLa], *lb[2];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < kLa; ++i) {
+    const int in = MT >= 2 ? kLa * wave + i : wave & 3, r = 16 * in + (lane >> 2);
+    pa[i] = p.a.codes + min(at.m0 + r, p.a.rows - 1) * p.a.ldc + 16 * ((lane & 3) ^ (r >> 2 & 3));
+    la[i] = sm + 1024 * in;
+  }
+  const auto b_row = [&](int r) { return min(at.n0 + (r & ~63) + 2 * (r & 31) + (r >> 5 & 1), p.b.rows - 1); };
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
+  for (int i = 0; i < 2; ++i) {
+    const int r = 16 * (2 * wave + i) + (lane >> 2);
+    pb[i] = p.b.codes + b_row(r) * p.b.ldc + 16 * ((lane & 3) ^ (r >> 2 & 3));
+    lb[i] = sm + kA + 1024 * (2 * wave + i);
+  }
+  const int ia = MT == 4 ? wave & 3 : MT == 2 ? wave & 1 : 0;  // 64 rows' scale dwords a load
+  const uint8_t* psa = p.a.scales + min(at.m0 + 64 * ia + lane, p.a.rows - 1) * p.a.lds;
+  const uint8_t* psb = p.b.scales + b_row(64 * (wave & 3) + lane) * p.b.lds;
+  char *lsa = sm + kA + kB + 256 * ia, *lsb = sm + kA + kB + kSA + 256 * (wave & 3);
+
+  const auto issue = [&](int step, int buf) {
+    const int o = buf * kStage;
 #pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        const int64_t m = m0 + 16 * i + 4 * g + v, n = n0 + 16 * k + j;
-        if (m < a.rows && n < b.rows) st_out<F32>(out, m * ldo + n, acc[i][k][v]);
-      }
+    for (int i = 0; i < kLa; ++i) ld_to_lds<16>(pa[i] + 64 * (int64_t)step, la[i] + o);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) ld_to_lds<16>(pb[i] + 64 * (int64_t)step, lb[i] + o);
+    ld_to_lds<4>(psa + 4 * (int64_t)step, lsa + o);
+    ld_to_lds<4>(psb + 4 * (int64_t)step, lsb + o);
+  };
+
+  f32x16 acc[MT][2];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) acc[i][t][v] = 0.f;
+
+#pragma unroll
+  for (int d = 0; d < kDeep - 1; ++d) issue(min(at.first + d, at.last - 1), d);
+  const int ra = 32 * MT * wm + c, rb = 64 * wn + c;
+  int buf = 0;
+  for (int step = at.first; step < at.last; ++step) {
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(kLoads * (kDeep - 2)));
+    lds_barrier();  // this step's loads are in (every wave's), and the buffer of the step before is free
+    issue(min(step + kDeep - 1, at.last - 1), (buf + kDeep - 1) & (kDeep - 1));
+    const char* st = sm + buf * kStage;
+    uint32_t sa[MT], sb[2];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) sa[i] = ld4(st + kA + kB + 4 * (ra + 32 * i)) >> (8 * h);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) sb[t] = ld4(st + kA + kB + kSA + 4 * (rb + 32 * t)) >> (8 * h);
+    static_for<0, 2>([&](auto q) {
+      u32x4 va[MT], vb[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) vb[t] = ld16(st + kA + 64 * (rb + 32 * t) + 16 * ((2 * q() + h) ^ (c >> 2 & 3)));
+#pragma unroll
+      for (int i = 0; i < MT; ++i) va[i] = ld16(st + 64 * (ra + 32 * i) + 16 * ((2 * q() + h) ^ (c >> 2 & 3)));
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) acc[i][t] = mfma_mx<2 * q()>(va[i], vb[t], acc[i][t], sa[i], sb[t]);
+    });
+    buf = (buf + 1) & (kDeep - 1);
+  }
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // the last loads write LDS: let them end before the workgroup does
+  char* out = (char*)p.out + (p.splits > 1 ? (int64_t)at.z * p.a.rows * p.ldo * 4 : 0);
+  const int64_t n = at.n0 + 64 * wn + 2 * c;
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+      const int64_t m = at.m0 + 32 * MT * wm + 32 * i + 8 * (v >> 2) + 4 * h + (v & 3);
+      if (m < p.a.rows) st_pair<F32>(out, m, n, p.ldo, p.b.rows, acc[i][0][v], acc[i][1][v]);
+    }
 }
 
 // ---------------------------------------------------------------- bf16 rows, few of them
@@ -146,22 +247,6 @@ __global__ __launch_bounds__(512) void k_mx_linear(const uint16_t* x, int64_t ld
 }
 
 // ---------------------------------------------------------------- bf16 rows, many of them
-// 16 zero bytes, read in place of a row's chunks past its end.
-__device__ const u32x4 kZeroChunk = u32x4{0u, 0u, 0u, 0u};
-
-template <int BYTES>
-__device__ __forceinline__ void ld_to_lds(const void* g, char* lds) {
-  const auto l = (__attribute__((address_space(3))) void*)lds;
-  if constexpr (BYTES == 16) __builtin_amdgcn_global_load_lds(g, l, 16, 0, 0);
-  else __builtin_amdgcn_global_load_lds(g, l, 4, 0, 0);
-}
-
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-
-__device__ __forceinline__ f32x16 mfma_32x32x16(u32x4 a, u32x4 b, f32x16 c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-
 struct TileArgs {
   const uint16_t* x;  // [rows, contraction]
   int64_t ldx;
@@ -195,12 +280,9 @@ __global__ __launch_bounds__(512) void k_mx_tile(TileArgs a) {
   extern __shared__ char sm[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int gq = wave >> 2, wn = wave & 3, c = lane & 31, h = lane >> 5;
-  const uint32_t tiles = a.tiles_m * a.tiles_n, id = xcd_tile(blockIdx.x, gridDim.x);
-  const uint32_t z = __builtin_amdgcn_readfirstlane(id / tiles), tile = id - z * tiles;
-  const uint32_t tn = __builtin_amdgcn_readfirstlane(tile / a.tiles_m), tm = tile - tn * a.tiles_m;
-  const int64_t m0 = (int64_t)tm * 128, n0 = (int64_t)tn * 256;
-  const int first = __builtin_amdgcn_readfirstlane((uint32_t)a.steps * z / (uint32_t)a.splits);
-  const int last = __builtin_amdgcn_readfirstlane((uint32_t)a.steps * (z + 1) / (uint32_t)a.splits);
+  const Place at = place(a.tiles_m, a.tiles_n, a.splits, a.steps, 128, 256);
+  const int64_t m0 = at.m0, n0 = at.n0;
+  const int first = at.first, last = at.last;
 
   // x: instruction i of wave w fills rows 4 (4 w + i) .. + 3 of the tile; chunk q of row r sits in slot q ^ (r % 16)
   const char* px[4];
@@ -211,8 +293,10 @@ __global__ __launch_bounds__(512) void k_mx_tile(TileArgs a) {
     qx[i] = (lane & 15) ^ (r & 15);
     px[i] = (const char*)(a.x + min(m0 + r, a.rows - 1) * a.ldx + 8 * qx[i]);
   }
-  // codes: TRANS false: 256 rows of 64 bytes, 16-byte piece q of row r in slot q ^ (r / 4 % 4); TRANS true: 128 rows
-  // of 128 bytes, piece q of row r in slot q ^ (r / 2 % 4).  Both spread a wave's reads over the banks.
+  // codes: TRANS false: 256 rows of 64 bytes, 16-byte piece q of row r in slot q ^ (r / 4 % 4), LDS row 64 wn + 32 t + c
+  // holding W row 64 wn + 2 c + t; TRANS true: 128 rows of 128 bytes, piece q of row r in slot q ^ (r / 2 % 4).  Both
+  // spread a wave's reads over the banks.
+  const auto w_row = [&](int r) { return min(n0 + (r & ~63) + 2 * (r & 31) + (r >> 5 & 1), a.w.rows - 1); };
   const uint8_t* pb[2];
   int rb[2];
   const uint8_t* ps;
@@ -221,14 +305,14 @@ __global__ __launch_bounds__(512) void k_mx_tile(TileArgs a) {
     const int in = 2 * wave + i;
     if constexpr (!TRANS) {
       const int r = 16 * in + (lane >> 2);
-      pb[i] = a.w.codes + min(n0 + r, a.w.rows - 1) * a.w.ldc + 16 * ((lane & 3) ^ (r >> 2 & 3));
+      pb[i] = a.w.codes + w_row(r) * a.w.ldc + 16 * ((lane & 3) ^ (r >> 2 & 3));
     } else {
       rb[i] = 8 * in + (lane >> 3);
       pb[i] = a.w.codes + rb[i] * a.w.ldc + min(n0 / 2 + 16 * ((lane & 7) ^ (rb[i] >> 1 & 3)), 64 * (int64_t)a.w.steps - 16);
     }
   }
   const int rs = TRANS ? (threadIdx.x & 255) >> 1 : 64 * (wave & 3) + lane;  // (waves 4 .. 7 load the same again)
-  if constexpr (!TRANS) ps = a.w.scales + min(n0 + rs, a.w.rows - 1) * a.w.lds;
+  if constexpr (!TRANS) ps = a.w.scales + w_row(rs) * a.w.lds;
   else ps = a.w.scales + rs * a.w.lds + min(n0 / 32 + 4 * (lane & 1), 4 * (int64_t)a.w.steps - 4);
 
   const auto issue = [&](int step, int buf) {
@@ -302,7 +386,7 @@ __global__ __launch_bounds__(512) void k_mx_tile(TileArgs a) {
     if constexpr (!TRANS) {
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const int r = 64 * wn + 2 * c + t;
+        const int r = 64 * wn + 32 * t + c;
         code[t] = ld16(st + kA + 64 * r + 16 * ((2 * gq + h) ^ (r >> 2 & 3)));
         scale[t] = e8m0_operand((uint8_t)st[kA + kB + 4 * r + 2 * gq + h]);
       }
@@ -354,7 +438,7 @@ __global__ __launch_bounds__(512) void k_mx_tile(TileArgs a) {
         ex[((wave * 16) + 8 * i + 4 * t + q) * 64 + lane] = f32x4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
       }
   __syncthreads();
-  char* out = (char*)a.out + (a.splits > 1 ? (int64_t)z * a.rows * a.ldo * 4 : 0);
+  char* out = (char*)a.out + (a.splits > 1 ? (int64_t)at.z * a.rows * a.ldo * 4 : 0);
   const int64_t n = n0 + 64 * wn + 2 * c;
 #pragma unroll
   for (int i = 0; i < 2; ++i)
@@ -370,18 +454,7 @@ __global__ __launch_bounds__(512) void k_mx_tile(TileArgs a) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int64_t m = m0 + 64 * gq + 32 * i + 8 * q + 4 * h + k;
-        if (m >= a.rows || n >= a.cols) continue;
-        if (n + 1 < a.cols) {
-          if constexpr (F32) {
-            typedef f32x2_t f32x2_any __attribute__((aligned(4)));
-            *(f32x2_any*)(out + (m * a.ldo + n) * 4) = f32x2_t{v[0][k], v[1][k]};
-          } else {
-            typedef uint32_t u32_any __attribute__((aligned(2)));
-            *(u32_any*)(out + (m * a.ldo + n) * 2) = pack_bf16x2(v[0][k], v[1][k]);
-          }
-        } else {
-          st_out<F32>(out, m * a.ldo + n, v[0][k]);
-        }
+        if (m < a.rows) st_pair<F32>(out, m, n, a.ldo, a.cols, v[0][k], v[1][k]);
       }
     }
 }
@@ -432,8 +505,47 @@ static SplitPlan split_plan(int64_t rows, const lrq_mxfp4* t, bool trans) {
   return p;
 }
 
-static int64_t split_bytes(const SplitPlan& p, int64_t rows, int64_t cols) {
-  return p.splits > 1 ? (int64_t)p.splits * rows * ((cols + 3) / 4 * 4) * 4 : 0;
+struct GemmPlan {
+  int mt;  // 64 mt rows a workgroup
+  int64_t tiles_m, tiles_n;
+  int splits;
+};
+
+// As split_plan, over the kernel's three tile heights too: us a step of each.
+static GemmPlan gemm_plan(const lrq_mxfp4* a, const lrq_mxfp4* b) {
+  constexpr double kStep[3] = {0.35, 0.4, 0.6}, kJoin = 4.0, kPerByte = 2.0 / 4.0e6;
+  const int steps = (int)((a->cols + 127) / 128);
+  GemmPlan best{};
+  double least = 0.;
+  for (int i = 0; i < 3; ++i) {
+    GemmPlan p{1 << i, 0, (b->rows + 255) / 256, 1};
+    p.tiles_m = (a->rows + 64 * p.mt - 1) / (64 * p.mt);
+    for (p.splits = 1; p.splits <= 16 && p.splits <= std::max(1, steps / 4); ++p.splits) {
+      const double rounds = (double)((p.tiles_m * p.tiles_n * p.splits + 255) / 256);
+      const double cost = rounds * ((steps + p.splits - 1) / p.splits + 3) * kStep[i] +
+                          (p.splits > 1 ? kJoin + kPerByte * 4. * p.splits * a->rows * b->rows : 0.);
+      if (best.mt == 0 || cost < least) best = p, least = cost;
+    }
+  }
+  return best;
+}
+
+static int64_t split_bytes(int splits, int64_t rows, int64_t cols) {
+  return splits > 1 ? (int64_t)splits * rows * ((cols + 3) / 4 * 4) * 4 : 0;
+}
+
+static int validate_workspace(const void* p, int64_t bytes, int64_t need) {
+  if (need == 0) return LRQ_OK;
+  if (p == nullptr) return LRQ_ERR_NULL;
+  if (!aligned(p, 16)) return LRQ_ERR_ALIGN;
+  return bytes < need ? LRQ_ERR_WORKSPACE : LRQ_OK;
+}
+
+static int join(const float* part, int splits, int64_t rows, int64_t cols, int64_t ldp, void* out, int64_t ldo,
+                int32_t out_fp32, hipStream_t s) {
+  const dim3 grid((unsigned)std::min<int64_t>((rows * (ldp / 4) + 255) / 256, (int64_t)cu_count() * 32));
+  return out_fp32 ? launch(k_mx_join<true>, grid, dim3(256), 0, s, part, splits, rows, cols, ldp, out, ldo)
+                  : launch(k_mx_join<false>, grid, dim3(256), 0, s, part, splits, rows, cols, ldp, out, ldo);
 }
 
 static int validate_out(const void* out, int64_t ldo, int64_t cols, int32_t f32) {
@@ -446,26 +558,45 @@ static int validate_out(const void* out, int64_t ldo, int64_t cols, int32_t f32)
 
 using namespace lrq;
 
+extern "C" int64_t lrq_mxfp4_gemm_workspace(const lrq_mxfp4* ta, const lrq_mxfp4* tb) {
+  LRQ_TRY(validate_mx(ta));
+  LRQ_TRY(validate_mx(tb));
+  if (ta->cols != tb->cols) return LRQ_ERR_SHAPE;
+  return split_bytes(gemm_plan(ta, tb).splits, ta->rows, tb->rows);
+}
+
 extern "C" int lrq_mxfp4_gemm(const lrq_mxfp4* ta, const lrq_mxfp4* tb, void* out, int64_t ldo, int32_t out_fp32,
-                              void* stream) {
+                              void* workspace, int64_t workspace_bytes, void* stream) {
   LRQ_TRY(validate_mx(ta));
   LRQ_TRY(validate_mx(tb));
   if (ta->cols != tb->cols) return LRQ_ERR_SHAPE;
   if (ta->rows == 0 || tb->rows == 0) return LRQ_OK;
   LRQ_TRY(validate_out(out, ldo, tb->rows, out_fp32));
-  const Mx a = make_mx(ta), b = make_mx(tb);
-  const int64_t gx = (b.rows + 127) / 128, gy = (a.rows + 127) / 128;
-  if (gy > 65535) return LRQ_ERR_SHAPE;
-  const dim3 grid((unsigned)gx, (unsigned)gy);
+  const GemmPlan p = gemm_plan(ta, tb);
+  const int64_t need = split_bytes(p.splits, ta->rows, tb->rows), ldp = (tb->rows + 3) / 4 * 4;
+  LRQ_TRY(validate_workspace(workspace, workspace_bytes, need));
+  const int64_t wgs = p.tiles_m * p.tiles_n * p.splits;
+  if (wgs > INT32_MAX) return LRQ_ERR_SHAPE;
+  const GemmArgs a{make_mx(ta), make_mx(tb), need ? workspace : out, need ? ldp : ldo, (int)p.tiles_m, (int)p.tiles_n,
+                   p.splits};
   hipStream_t s = (hipStream_t)stream;
-  return out_fp32 ? launch(k_mx_gemm<true>, grid, dim3(256), 0, s, a, b, out, ldo)
-                  : launch(k_mx_gemm<false>, grid, dim3(256), 0, s, a, b, out, ldo);
+  const auto go = [&](auto kern) {
+    const int lds = 4 * (p.mt * 64 * 68 + 16384 + 1024);
+    const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (e != hipSuccess) return (int)e;
+    return launch(kern, dim3((unsigned)wgs), dim3(512), (size_t)lds, s, a);
+  };
+  const bool f32 = need > 0 || out_fp32;
+  if (p.mt == 4) LRQ_TRY(f32 ? go(k_mx_gemm<4, true>) : go(k_mx_gemm<4, false>));
+  else if (p.mt == 2) LRQ_TRY(f32 ? go(k_mx_gemm<2, true>) : go(k_mx_gemm<2, false>));
+  else LRQ_TRY(f32 ? go(k_mx_gemm<1, true>) : go(k_mx_gemm<1, false>));
+  return need ? join((const float*)workspace, p.splits, ta->rows, tb->rows, ldp, out, ldo, out_fp32, s) : LRQ_OK;
 }
 
 extern "C" int64_t lrq_mxfp4_linear_workspace(int64_t rows, const lrq_mxfp4* t, int32_t transposed) {
   LRQ_TRY(validate_mx(t));
   if (rows < 0 || rows > INT32_MAX) return LRQ_ERR_SHAPE;
-  return split_bytes(split_plan(rows, t, transposed != 0), rows, transposed ? t->cols : t->rows);
+  return split_bytes(split_plan(rows, t, transposed != 0).splits, rows, transposed ? t->cols : t->rows);
 }
 
 static int mx_linear(const void* x, int64_t ldx, int64_t rows, const lrq_mxfp4* t, bool trans, void* out, int64_t ldo,
@@ -506,10 +637,8 @@ static int mx_linear(const void* x, int64_t ldx, int64_t rows, const lrq_mxfp4* 
 #undef LRQ_GO
   }
   const SplitPlan p = split_plan(rows, t, trans);
-  const int64_t need = split_bytes(p, rows, cols);
-  if (need > 0 && workspace == nullptr) return LRQ_ERR_NULL;
-  if (need > 0 && !aligned(workspace, 16)) return LRQ_ERR_ALIGN;
-  if (workspace_bytes < need) return LRQ_ERR_WORKSPACE;
+  const int64_t need = split_bytes(p.splits, rows, cols);
+  LRQ_TRY(validate_workspace(workspace, workspace_bytes, need));
   const int64_t ldp = (cols + 3) / 4 * 4;
   const int64_t wgs = p.tiles_m * p.tiles_n * p.splits;
   if (wgs > INT32_MAX) return LRQ_ERR_SHAPE;
@@ -524,10 +653,7 @@ static int mx_linear(const void* x, int64_t ldx, int64_t rows, const lrq_mxfp4* 
   constexpr int kLds = 3 * (128 * 256 + 16384 + 1024), kLdsT = kLds + 3 * 1024;
   if (trans) LRQ_TRY(f32 ? go(k_mx_tile<true, true>, kLdsT) : go(k_mx_tile<true, false>, kLdsT));
   else LRQ_TRY(f32 ? go(k_mx_tile<false, true>, kLds) : go(k_mx_tile<false, false>, kLds));
-  if (need == 0) return LRQ_OK;
-  const dim3 grid((unsigned)std::min<int64_t>((rows * (ldp / 4) + 255) / 256, (int64_t)cu_count() * 32));
-  return out_fp32 ? launch(k_mx_join<true>, grid, dim3(256), 0, s, (const float*)workspace, p.splits, rows, cols, ldp, out, ldo)
-                  : launch(k_mx_join<false>, grid, dim3(256), 0, s, (const float*)workspace, p.splits, rows, cols, ldp, out, ldo);
+  return need ? join((const float*)workspace, p.splits, rows, cols, ldp, out, ldo, out_fp32, s) : LRQ_OK;
 }
 
 extern "C" int lrq_mxfp4_linear(const void* x, int64_t ldx, int64_t rows, const lrq_mxfp4* w, void* out, int64_t ldo,

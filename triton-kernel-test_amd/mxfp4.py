@@ -116,9 +116,18 @@ def mxfp4_gemm(a: MXFP4Tensor, b: MXFP4Tensor, out_dtype: torch.dtype = torch.bf
     if a.cols != b.cols:
         raise ValueError(f"operands have {a.cols} and {b.cols} columns")
     out = torch.empty(tuple(a.shape[:-1]) + (b.rows,), dtype=out_dtype, device=a.device)
+    ws, ws_bytes = _workspace(a.device, "lrq_mxfp4_gemm_workspace", ctypes.byref(ta), ctypes.byref(tb))
     with _on(a.device):
-        call("lrq_mxfp4_gemm", ctypes.byref(ta), ctypes.byref(tb), _p(out), b.rows, f32, _stream(a.device))
+        call("lrq_mxfp4_gemm", ctypes.byref(ta), ctypes.byref(tb), _p(out), b.rows, f32, _p(ws), ws_bytes,
+             _stream(a.device))
     return out
+
+
+def _workspace(device, query: str, *args):
+    n = call_raw(query, *args)
+    if n < 0:
+        check(n, query)
+    return (torch.empty(n // 4, dtype=torch.float32, device=device) if n else None), n
 
 
 def _operand(x: torch.Tensor, cols: int, name: str):
@@ -145,11 +154,7 @@ def _product(name: str, x: torch.Tensor, w: MXFP4Tensor, out_dtype, transposed: 
     out = torch.empty(tuple(x.shape[:-1]) + (cols,), dtype=out_dtype, device=x.device)
     if depth == 0:
         return out.zero_()
-    ws, ws_bytes = None, call_raw("lrq_mxfp4_linear_workspace", rows, ctypes.byref(t), transposed)
-    if ws_bytes < 0:
-        check(ws_bytes, "lrq_mxfp4_linear_workspace")
-    if ws_bytes:
-        ws = torch.empty(ws_bytes // 4, dtype=torch.float32, device=x.device)
+    ws, ws_bytes = _workspace(x.device, "lrq_mxfp4_linear_workspace", rows, ctypes.byref(t), transposed)
     with _on(x.device):
         call(name, _p(x2), ld, rows, ctypes.byref(t), _p(out), cols, f32, _p(ws), ws_bytes, _stream(x.device))
     return out
