@@ -78,20 +78,38 @@ struct GemmArgs {
   int tiles_m, tiles_n, splits;
 };
 
+// Scale bytes come to LDS four steps at a time, 16 bytes a row (one dword a step: a load of a dword a row for each step
+// kept the address unit busier than all codes did, 228 against 150 us on [4096, 4096] x [14336, 4096]).  A row holds
+// 4 bytes a step, so the last group starts early enough to end with the row; a matrix of fewer than four steps is
+// copied by the threads instead.
+__device__ __forceinline__ int scale_base(int step, int steps) { return max(0, min(step, steps - 4)); }
+
+__device__ __forceinline__ void short_scales(const uint8_t* row, int steps, char* lds) {
+  for (int k = 0; k < steps; ++k) st4(lds + 4 * k, ld4(row + 4 * k));
+}
+
 // Workgroup: 64 MT rows of A by 256 rows of B, 8 waves in two rows of four, each 32 MT x 64 of it in 32x32x64 scaled
 // instructions, whose operands are the stored codes and scale bytes as they are.  A K step of 128 columns is one scale
-// dword a row and 64 code bytes; both go straight to LDS, four steps deep, one barrier a step.  Row r's 16-byte piece q
+// dword a row and 64 code bytes; the codes go straight to LDS, four steps deep, one barrier a step, their loads spread
+// between the step's instructions (issued at once they queue up before the first of them).  Row r's 16-byte piece q
 // sits in slot q ^ (r / 4 % 4): 16 lanes of a read cover all banks.  LDS row 64 wn + 32 t + c of B holds row 64 wn +
 // 2 c + t, so that a lane's two columns are neighbours in the output.
+template <int MT>
+struct GemmLds {
+  static constexpr int kA = 64 * MT * 64, kB = 16384, kStage = kA + kB, kDeep = 4;
+  static constexpr int kScales = (64 * MT + 256) * 16, kBytes = kDeep * kStage + 2 * kScales;
+};
 template <int MT, bool F32>
 __global__ __launch_bounds__(512) void k_mx_gemm(GemmArgs p) {
-  constexpr int kA = 64 * MT * 64, kB = 16384, kSA = 64 * MT * 4, kSB = 1024, kStage = kA + kB + kSA + kSB, kDeep = 4;
+  using G = GemmLds<MT>;
+  constexpr int kA = G::kA, kStage = G::kStage, kDeep = G::kDeep, kRing = kDeep * kStage;
   constexpr int kLa = MT >= 2 ? MT / 2 : 1;  // 1 KB loads of A a wave (MT 1: the upper four waves load the same again)
-  constexpr int kLoads = kLa + 2 + 2;
+  constexpr int kLoads = kLa + 2;
   extern __shared__ char sm[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave >> 2, wn = wave & 3, c = lane & 31, h = lane >> 5;
-  const Place at = place(p.tiles_m, p.tiles_n, p.splits, p.a.steps, 64 * MT, 256);
+  const int steps = p.a.steps;
+  const Place at = place(p.tiles_m, p.tiles_n, p.splits, steps, 64 * MT, 256);
 
   const uint8_t *pa[kLa], *pb[2];
   char *la[kLa], *lb[2];
@@ -108,19 +126,19 @@ __global__ __launch_bounds__(512) void k_mx_gemm(GemmArgs p) {
     pb[i] = p.b.codes + b_row(r) * p.b.ldc + 16 * ((lane & 3) ^ (r >> 2 & 3));
     lb[i] = sm + kA + 1024 * (2 * wave + i);
   }
-  const int ia = MT == 4 ? wave & 3 : MT == 2 ? wave & 1 : 0;  // 64 rows' scale dwords a load
-  const uint8_t* psa = p.a.scales + min(at.m0 + 64 * ia + lane, p.a.rows - 1) * p.a.lds;
-  const uint8_t* psb = p.b.scales + b_row(64 * (wave & 3) + lane) * p.b.lds;
-  char *lsa = sm + kA + kB + 256 * ia, *lsb = sm + kA + kB + kSA + 256 * (wave & 3);
+  // 64 rows' scales a load: A's rows, then B's (waves past them load the last again)
+  const int is = min(wave, MT + 3);
+  const uint8_t* ps = is < MT ? p.a.scales + min(at.m0 + 64 * is + lane, p.a.rows - 1) * p.a.lds
+                              : p.b.scales + b_row(64 * (is - MT) + lane) * p.b.lds;
+  char* ls = sm + kRing + 1024 * is;
 
-  const auto issue = [&](int step, int buf) {
+  const auto issue_codes = [&](int step, int buf, int i) {
     const int o = buf * kStage;
-#pragma unroll
-    for (int i = 0; i < kLa; ++i) ld_to_lds<16>(pa[i] + 64 * (int64_t)step, la[i] + o);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) ld_to_lds<16>(pb[i] + 64 * (int64_t)step, lb[i] + o);
-    ld_to_lds<4>(psa + 4 * (int64_t)step, lsa + o);
-    ld_to_lds<4>(psb + 4 * (int64_t)step, lsb + o);
+    if (i < kLa) ld_to_lds<16>(pa[i < kLa ? i : 0] + 64 * (int64_t)step, la[i < kLa ? i : 0] + o);
+    else ld_to_lds<16>(pb[i - kLa] + 64 * (int64_t)step, lb[i - kLa] + o);
+  };
+  const auto issue_scales = [&](int step, int ring) {
+    ld_to_lds<16>(ps + 4 * (int64_t)scale_base(step, steps), ls + ring * G::kScales);
   };
 
   f32x16 acc[MT][2];
@@ -131,20 +149,30 @@ __global__ __launch_bounds__(512) void k_mx_gemm(GemmArgs p) {
 #pragma unroll
       for (int v = 0; v < 16; ++v) acc[i][t][v] = 0.f;
 
+  if (steps >= 4) issue_scales(at.first, 0);
+  else short_scales(ps, steps, ls + 16 * lane);
 #pragma unroll
-  for (int d = 0; d < kDeep - 1; ++d) issue(min(at.first + d, at.last - 1), d);
+  for (int d = 0; d < kDeep - 1; ++d)
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) issue_codes(min(at.first + d, at.last - 1), d, i);
   const int ra = 32 * MT * wm + c, rb = 64 * wn + c;
-  int buf = 0;
+  int buf = 0, ring = 0;
   for (int step = at.first; step < at.last; ++step) {
-    __builtin_amdgcn_s_waitcnt(vmcnt_imm(kLoads * (kDeep - 2)));
-    lds_barrier();  // this step's loads are in (every wave's), and the buffer of the step before is free
-    issue(min(step + kDeep - 1, at.last - 1), (buf + kDeep - 1) & (kDeep - 1));
+    // this step's loads, and its scales' (loaded with the step before at the latest), not those of the two steps after
+    const int phase = (step - at.first) & 3;
+    if (phase == 1 || phase == 2) __builtin_amdgcn_s_waitcnt(vmcnt_imm(kLoads * (kDeep - 2) + 1));
+    else __builtin_amdgcn_s_waitcnt(vmcnt_imm(kLoads * (kDeep - 2)));
+    lds_barrier();  // every wave's loads are in, and the buffer of the step before is free
+    const int ahead = min(step + kDeep - 1, at.last - 1), to = (buf + kDeep - 1) & (kDeep - 1);
+    if (phase == 0 && steps >= 4) issue_scales(step + 4, ring ^ 1);
+    else if (phase == 0) ld_to_lds<16>(pa[0] + 64 * (int64_t)ahead, la[0] + to * kStage);  // (keeps the counts)
     const char* st = sm + buf * kStage;
+    const char* sc = sm + kRing + ring * G::kScales + 4 * (step - scale_base(step - phase, steps));
     uint32_t sa[MT], sb[2];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) sa[i] = ld4(st + kA + kB + 4 * (ra + 32 * i)) >> (8 * h);
+    for (int i = 0; i < MT; ++i) sa[i] = ld4(sc + 16 * (ra + 32 * i)) >> (8 * h);
 #pragma unroll
-    for (int t = 0; t < 2; ++t) sb[t] = ld4(st + kA + kB + kSA + 4 * (rb + 32 * t)) >> (8 * h);
+    for (int t = 0; t < 2; ++t) sb[t] = ld4(sc + 1024 * MT + 16 * (rb + 32 * t)) >> (8 * h);
     static_for<0, 2>([&](auto q) {
       u32x4 va[MT], vb[2];
 #pragma unroll
@@ -152,10 +180,16 @@ __global__ __launch_bounds__(512) void k_mx_gemm(GemmArgs p) {
 #pragma unroll
       for (int i = 0; i < MT; ++i) va[i] = ld16(st + 64 * (ra + 32 * i) + 16 * ((2 * q() + h) ^ (c >> 2 & 3)));
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
+      for (int i = 0; i < MT; ++i) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) acc[i][t] = mfma_mx<2 * q()>(va[i], vb[t], acc[i][t], sa[i], sb[t]);
+        // a load after every second row of instructions
+        const int n = (MT * q() + i) * kLoads / (2 * MT), n1 = (MT * q() + i + 1) * kLoads / (2 * MT);
+#pragma unroll
+        for (int k = n; k < n1; ++k) issue_codes(ahead, to, k);
+      }
     });
+    if (phase == 3) ring ^= 1;
     buf = (buf + 1) & (kDeep - 1);
   }
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // the last loads write LDS: let them end before the workgroup does
@@ -273,10 +307,15 @@ struct TileArgs {
 //   TRANS false: those are 32 consecutive k of one W row, so the lane reads 16 code bytes and one scale a step.
 //   TRANS true: the lane's two columns are one code byte of each W row.  The transposing LDS read gives it that byte
 //   of 8 rows at once; each is widened with its own row's scale and the halves of two rows are paired by v_perm_b32.
+template <bool TRANS>
+struct TileLds {
+  static constexpr int kA = 128 * 256, kB = 16384, kS = TRANS ? 2048 : 0, kStage = kA + kB + kS, kDeep = 3;
+  static constexpr int kScales = TRANS ? 0 : 4096, kBytes = kDeep * kStage + 2 * kScales;
+};
 template <bool TRANS, bool F32>
 __global__ __launch_bounds__(512) void k_mx_tile(TileArgs a) {
-  constexpr int kA = 128 * 256, kB = 16384, kS = TRANS ? 2048 : 1024, kStage = kA + kB + kS;
-  constexpr int kLoads = 4 + 2 + 1;  // of a stage, a wave
+  using T = TileLds<TRANS>;
+  constexpr int kA = T::kA, kB = T::kB, kStage = T::kStage, kRing = T::kDeep * kStage;
   extern __shared__ char sm[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int gq = wave >> 2, wn = wave & 3, c = lane & 31, h = lane >> 5;
@@ -311,37 +350,34 @@ __global__ __launch_bounds__(512) void k_mx_tile(TileArgs a) {
       pb[i] = a.w.codes + rb[i] * a.w.ldc + min(n0 / 2 + 16 * ((lane & 7) ^ (rb[i] >> 1 & 3)), 64 * (int64_t)a.w.steps - 16);
     }
   }
-  const int rs = TRANS ? (threadIdx.x & 255) >> 1 : 64 * (wave & 3) + lane;  // (waves 4 .. 7 load the same again)
+  const int rs = TRANS ? (threadIdx.x & 255) >> 1 : 64 * (wave & 3) + lane;
   if constexpr (!TRANS) ps = a.w.scales + w_row(rs) * a.w.lds;
   else ps = a.w.scales + rs * a.w.lds + min(n0 / 32 + 4 * (lane & 1), 4 * (int64_t)a.w.steps - 4);
 
-  const auto issue = [&](int step, int buf) {
+  // part i < 4 of a step's loads
+  const auto issue = [&](int step, int buf, int i) {
     char* st = sm + buf * kStage;
-    if (16 * step + 16 <= a.chunks) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) ld_to_lds<16>(px[i] + 256 * (int64_t)step, st + 1024 * (4 * wave + i));
+    const char* g = px[i] + 256 * (int64_t)step;
+    if (16 * step + 16 > a.chunks && 16 * step + qx[i] >= a.chunks) g = (const char*)&kZeroChunk;
+    ld_to_lds<16>(g, st + 1024 * (4 * wave + i));
+    if constexpr (!TRANS) {
+      if (i < 2) ld_to_lds<16>(pb[i & 1] + 64 * (int64_t)step, st + kA + 1024 * (2 * wave + i));
     } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const char* g = 16 * step + qx[i] < a.chunks ? px[i] + 256 * (int64_t)step : (const char*)&kZeroChunk;
-        ld_to_lds<16>(g, st + 1024 * (4 * wave + i));
+      const int64_t r0 = 128 * (int64_t)step, most = a.w.rows - 1 - r0;  // rows past W's last: that one (their x is zero)
+      const bool whole = most >= 127;
+      if (i < 2) {
+        const int64_t r = whole ? r0 : r0 + min((int64_t)rb[i & 1], most) - rb[i & 1];
+        ld_to_lds<16>(pb[i & 1] + r * a.w.ldc, st + kA + 1024 * (2 * wave + i));
+      }
+      if (i == 2 && wave < 4) {
+        const int64_t r = whole ? r0 : r0 + min((int64_t)rs, most) - rs;
+        ld_to_lds<4>(ps + r * a.w.lds, st + kA + kB + 256 * wave);
       }
     }
-    if constexpr (!TRANS) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) ld_to_lds<16>(pb[i] + 64 * (int64_t)step, st + kA + 1024 * (2 * wave + i));
-      ld_to_lds<4>(ps + 4 * (int64_t)step, st + kA + kB + 256 * (wave & 3));
-    } else if (128 * (int64_t)step + 128 <= a.w.rows) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) ld_to_lds<16>(pb[i] + step * (128 * a.w.ldc), st + kA + 1024 * (2 * wave + i));
-      ld_to_lds<4>(ps + step * (128 * a.w.lds), st + kA + kB + 256 * (wave & 3));
-    } else {  // rows past W's last: its last row (their x is zero)
-      const int64_t r0 = 128 * (int64_t)step, most = a.w.rows - 1 - r0;
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        ld_to_lds<16>(pb[i] + (r0 + min((int64_t)rb[i], most) - rb[i]) * a.w.ldc, st + kA + 1024 * (2 * wave + i));
-      ld_to_lds<4>(ps + (r0 + min((int64_t)rs, most) - rs) * a.w.lds, st + kA + kB + 256 * (wave & 3));
-    }
+  };
+  // TRANS false: W's scales, four steps at a time (waves 4 .. 7 load the same again)
+  const auto issue_scales = [&](int step, int ring) {
+    ld_to_lds<16>(ps + 4 * (int64_t)scale_base(step, a.steps), sm + kRing + ring * T::kScales + 1024 * (wave & 3));
   };
 
   f32x16 acc[4][2];
@@ -352,20 +388,38 @@ __global__ __launch_bounds__(512) void k_mx_tile(TileArgs a) {
 #pragma unroll
       for (int v = 0; v < 16; ++v) acc[i][t][v] = 0.f;
 
-  issue(first, 0);
-  issue(min(first + 1, last - 1), 1);
-  int buf = 0;
+  if constexpr (!TRANS) {
+    if (a.steps >= 4) issue_scales(first, 0);
+    else short_scales(ps, a.steps, sm + kRing + 16 * rs);
+  }
+#pragma unroll
+  for (int d = 0; d < 2; ++d)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) issue(min(first + d, last - 1), d, i);
+  int buf = 0, ring = 0;
   for (int step = first; step < last; ++step) {
-    __builtin_amdgcn_s_waitcnt(vmcnt_imm(kLoads));  // this step's loads (the next step's are still out)
+    // this step's loads, and its scales' (issued ahead of the codes of the step before), not those of the step after
+    const int phase = (step - first) & 3;
+    if constexpr (TRANS) {
+      if (wave < 4) __builtin_amdgcn_s_waitcnt(vmcnt_imm(7));
+      else __builtin_amdgcn_s_waitcnt(vmcnt_imm(6));
+    } else {
+      __builtin_amdgcn_s_waitcnt(vmcnt_imm(6));
+    }
     char* st = sm + buf * kStage;
     if constexpr (TRANS) {
       // the scales arrive as [row][8]; this thread's dword goes to [block][row]
-      const uint32_t s4 = ld4(st + kA + kB + 4 * (threadIdx.x & 255));
+      if (wave < 4) {
+        const uint32_t s4 = ld4(st + kA + kB + 4 * threadIdx.x);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) st[kA + kB + 1024 + (4 * (lane & 1) + k) * 128 + rs] = (char)(s4 >> (8 * k));
+        for (int k = 0; k < 4; ++k) st[kA + kB + 1024 + (4 * (lane & 1) + k) * 128 + rs] = (char)(s4 >> (8 * k));
+      }
     }
     lds_barrier();  // every wave's loads are in, and the buffer of the step before is free
-    issue(min(step + 2, last - 1), buf == 0 ? 2 : buf - 1);
+    const int ahead = min(step + 2, last - 1), to = buf == 0 ? 2 : buf - 1;
+    if constexpr (!TRANS) {
+      if (phase == 2 && a.steps >= 4) issue_scales(step + 2, ring ^ 1);
+    }
     u32x4 code[2];
     float scale[2];
     u32x2 cols[4], rows8[4];  // TRANS: this lane's code byte and scale byte of 8 rows, for each instruction
@@ -388,7 +442,8 @@ __global__ __launch_bounds__(512) void k_mx_tile(TileArgs a) {
       for (int t = 0; t < 2; ++t) {
         const int r = 64 * wn + 32 * t + c;
         code[t] = ld16(st + kA + 64 * r + 16 * ((2 * gq + h) ^ (r >> 2 & 3)));
-        scale[t] = e8m0_operand((uint8_t)st[kA + kB + 4 * r + 2 * gq + h]);
+        scale[t] = e8m0_operand((uint8_t)sm[kRing + ring * T::kScales + 16 * r + 4 * (step - scale_base(step - phase, a.steps)) +
+                                            2 * gq + h]);
       }
     }
 #pragma unroll
@@ -420,7 +475,9 @@ __global__ __launch_bounds__(512) void k_mx_tile(TileArgs a) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) acc[i][t] = mfma_32x32x16(x, b[t], acc[i][t]);
       }
+      issue(ahead, to, s);  // spread over the step: issued at once the loads queue up before its first instruction
     }
+    if (phase == 3) ring ^= 1;
     buf = buf == 2 ? 0 : buf + 1;
   }
 
@@ -581,7 +638,7 @@ extern "C" int lrq_mxfp4_gemm(const lrq_mxfp4* ta, const lrq_mxfp4* tb, void* ou
                    p.splits};
   hipStream_t s = (hipStream_t)stream;
   const auto go = [&](auto kern) {
-    const int lds = 4 * (p.mt * 64 * 68 + 16384 + 1024);
+    const int lds = p.mt == 4 ? GemmLds<4>::kBytes : p.mt == 2 ? GemmLds<2>::kBytes : GemmLds<1>::kBytes;
     const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (e != hipSuccess) return (int)e;
     return launch(kern, dim3((unsigned)wgs), dim3(512), (size_t)lds, s, a);
@@ -650,7 +707,7 @@ static int mx_linear(const void* x, int64_t ldx, int64_t rows, const lrq_mxfp4* 
     if (e != hipSuccess) return (int)e;
     return launch(kern, dim3((unsigned)wgs), dim3(512), (size_t)lds, s, a);
   };
-  constexpr int kLds = 3 * (128 * 256 + 16384 + 1024), kLdsT = kLds + 3 * 1024;
+  constexpr int kLds = TileLds<false>::kBytes, kLdsT = TileLds<true>::kBytes;
   if (trans) LRQ_TRY(f32 ? go(k_mx_tile<true, true>, kLdsT) : go(k_mx_tile<true, false>, kLdsT));
   else LRQ_TRY(f32 ? go(k_mx_tile<false, true>, kLds) : go(k_mx_tile<false, false>, kLds));
   return need ? join((const float*)workspace, p.splits, rows, cols, ldp, out, ldo, out_fp32, s) : LRQ_OK;
