@@ -155,42 +155,61 @@ __global__ __launch_bounds__(512) void k_mx_gemm(GemmArgs p) {
   for (int d = 0; d < kDeep - 1; ++d)
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) issue_codes(min(at.first + d, at.last - 1), d, i);
-  const int ra = 32 * MT * wm + c, rb = 64 * wn + c;
+  // The operands of instruction column q of a step, read from LDS while the column before runs: that of a step's
+  // first column is the last of the step before, so the step's loads are waited for, and the workgroup meets, in the
+  // middle of the step before.
+  const int ra = 32 * MT * wm + c, rb = 64 * wn + c, slot = c >> 2 & 3;
+  u32x4 va[2][MT], vb[2][2];
+  uint32_t sa[MT], sb[2], na[MT], nb[2];
+  const auto read = [&](int q, int buf) {
+    const char* st = sm + buf * kStage;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) vb[q][t] = ld16(st + kA + 64 * (rb + 32 * t) + 16 * ((2 * q + h) ^ slot));
+#pragma unroll
+    for (int i = 0; i < MT; ++i) va[q][i] = ld16(st + 64 * (ra + 32 * i) + 16 * ((2 * q + h) ^ slot));
+  };
+  const auto read_scales = [&](int step, int phase, int ring) {
+    const char* sc = sm + kRing + ring * G::kScales + 4 * min(step - scale_base(step - phase, steps), 3);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) na[i] = ld4(sc + 16 * (ra + 32 * i)) >> (8 * h);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) nb[t] = ld4(sc + 1024 * MT + 16 * (rb + 32 * t)) >> (8 * h);
+  };
+  // the scales' loads are ahead of the codes of the step before theirs
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(kLoads * 2));
+  lds_barrier();
+  read(0, 0);
+  read_scales(at.first, 0, 0);
   int buf = 0, ring = 0;
   for (int step = at.first; step < at.last; ++step) {
-    // this step's loads, and its scales' (loaded with the step before at the latest), not those of the two steps after
-    const int phase = (step - at.first) & 3;
-    if (phase == 1 || phase == 2) __builtin_amdgcn_s_waitcnt(vmcnt_imm(kLoads * (kDeep - 2) + 1));
-    else __builtin_amdgcn_s_waitcnt(vmcnt_imm(kLoads * (kDeep - 2)));
-    lds_barrier();  // every wave's loads are in, and the buffer of the step before is free
-    const int ahead = min(step + kDeep - 1, at.last - 1), to = (buf + kDeep - 1) & (kDeep - 1);
+    const int phase = (step - at.first) & 3, ahead = min(step + kDeep - 1, at.last - 1), to = (buf + kDeep - 1) & (kDeep - 1);
+    read(1, buf);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) sa[i] = na[i];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) sb[t] = nb[t];
+    __builtin_amdgcn_sched_barrier(0);
     if (phase == 0 && steps >= 4) issue_scales(step + 4, ring ^ 1);
-    else if (phase == 0) ld_to_lds<16>(pa[0] + 64 * (int64_t)ahead, la[0] + to * kStage);  // (keeps the counts)
-    const char* st = sm + buf * kStage;
-    const char* sc = sm + kRing + ring * G::kScales + 4 * (step - scale_base(step - phase, steps));
-    uint32_t sa[MT], sb[2];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) sa[i] = ld4(sc + 16 * (ra + 32 * i)) >> (8 * h);
+    for (int i = 0; i < MT; ++i) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t) sb[t] = ld4(sc + 1024 * MT + 16 * (rb + 32 * t)) >> (8 * h);
-    static_for<0, 2>([&](auto q) {
-      u32x4 va[MT], vb[2];
+      for (int t = 0; t < 2; ++t) acc[i][t] = mfma_mx<0>(va[0][i], vb[0][t], acc[i][t], sa[i], sb[t]);
 #pragma unroll
-      for (int t = 0; t < 2; ++t) vb[t] = ld16(st + kA + 64 * (rb + 32 * t) + 16 * ((2 * q() + h) ^ (c >> 2 & 3)));
-#pragma unroll
-      for (int i = 0; i < MT; ++i) va[i] = ld16(st + 64 * (ra + 32 * i) + 16 * ((2 * q() + h) ^ (c >> 2 & 3)));
-#pragma unroll
-      for (int i = 0; i < MT; ++i) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t) acc[i][t] = mfma_mx<2 * q()>(va[i], vb[t], acc[i][t], sa[i], sb[t]);
-        // a load after every second row of instructions
-        const int n = (MT * q() + i) * kLoads / (2 * MT), n1 = (MT * q() + i + 1) * kLoads / (2 * MT);
-#pragma unroll
-        for (int k = n; k < n1; ++k) issue_codes(ahead, to, k);
-      }
-    });
+      for (int k = i * kLoads / MT; k < (i + 1) * kLoads / MT; ++k) issue_codes(ahead, to, k);
+    }
+    // the next step's loads, not those of the two steps after it (nor the scales among them)
+    if (phase < 2 && steps >= 4) __builtin_amdgcn_s_waitcnt(vmcnt_imm(kLoads * (kDeep - 2) + 1));
+    else __builtin_amdgcn_s_waitcnt(vmcnt_imm(kLoads * (kDeep - 2)));
+    lds_barrier();  // every wave's are in, and every wave has read all of this step's buffer
     if (phase == 3) ring ^= 1;
     buf = (buf + 1) & (kDeep - 1);
+    read(0, buf);
+    read_scales(step + 1, (phase + 1) & 3, ring);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) acc[i][t] = mfma_mx<2>(va[1][i], vb[1][t], acc[i][t], sa[i], sb[t]);
   }
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // the last loads write LDS: let them end before the workgroup does
   char* out = (char*)p.out + (p.splits > 1 ? (int64_t)at.z * p.a.rows * p.ldo * 4 : 0);
