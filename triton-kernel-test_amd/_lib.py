@@ -186,19 +186,21 @@ def check(code: int, what: str) -> None:
 _bound: dict = {}  # name -> the library's function, bound on its first call
 
 
+def _bind(name: str):
+    lib = load()
+    if name in _missing:
+        raise RuntimeError(f"{name} is not exported by {LIB_PATH}")
+    fn = _bound[name] = getattr(lib, name)
+    return fn
+
+
 def call_raw(name: str, *args) -> int:
     """Call an entry point and return its status without raising."""
-    fn = _bound.get(name)
-    if fn is None:
-        lib = load()
-        if name in _missing:
-            raise RuntimeError(f"{name} is not exported by {LIB_PATH}")
-        fn = _bound[name] = getattr(lib, name)
-    return fn(*args)
+    return (_bound.get(name) or _bind(name))(*args)
 
 
 def call(name: str, *args) -> None:
-    st = call_raw(name, *args)
+    st = (_bound.get(name) or _bind(name))(*args)
     if st:
         check(st, name)
 

@@ -46,6 +46,8 @@ def _p(t: Optional[torch.Tensor]) -> int:
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+# (the checks of torch.cuda.current_device() without its initialisation: a device tensor is at hand)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _stream(device: torch.device) -> int:
@@ -68,7 +70,7 @@ _no_guard = _NoGuard()
 
 def _on(device: torch.device):
     """``torch.cuda.device(device)``, or nothing to enter where it is the current one already."""
-    return _no_guard if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _no_guard if device.index == _current_device() else torch.cuda.device(device)
 
 
 def _require_device(*ts):

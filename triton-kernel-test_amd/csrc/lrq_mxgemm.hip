@@ -224,79 +224,63 @@ __global__ __launch_bounds__(512) void k_mx_gemm(GemmArgs p) {
 }
 
 // ---------------------------------------------------------------- bf16 rows, few of them
-// Workgroup: 16 MT rows of X (all of them) by 16 NT rows of W; its 8 waves take every eighth K step of 128 and join in
-// LDS.  Lane (j, g) reads the 16 code bytes and the scale of block g of W row j: its k are 32g .. 32g + 31, 8 of them
-// for each of the step's four matrix instructions, and X is read in the same order.  Bound by the codes' bytes as long
-// as X is read seldom enough: NT grows with the rows of X.  Lanes without a row of X load nothing of it.
-template <int MT, int NT, bool F32>
-__global__ __launch_bounds__(512) void k_mx_linear(const uint16_t* x, int64_t ldx, int64_t rows, Mx w, void* out,
-                                                   int64_t ldo) {
-  constexpr int U = MT * NT >= 8 ? 1 : MT * NT >= 4 ? 2 : 4;
-  __shared__ f32x4 red[8][NT][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 15, g = lane >> 4;
-  const int64_t n0 = (int64_t)blockIdx.x * 16 * NT;
-  const uint8_t *codes[NT], *scales[NT];
-  const uint16_t* px[MT];
-  bool in[MT];
-  f32x4 acc[MT][NT];
+// Up to ROWS rows of X (a decoding step) by 16 rows of W a workgroup; each of its WAVES waves takes a run of the K steps
+// of 128 and they join in LDS.  Lane (j, g) reads the 16 code bytes of block g of W row j: its k are 32g .. 32g + 31, 8
+// of them for each of the step's four matrix instructions, and X is read in the same order.  Everything a wave needs
+// for its next D steps is in flight at once: X's columns go to the wave's own part of LDS (16-byte piece i of row r in
+// slot i ^ r, so that the 16 rows' reads fall in different banks), the codes and scales to registers.  The time is the
+// codes' arrival after a fixed 5 us.
+template <int ROWS, int WAVES, bool F32>
+__global__ __launch_bounds__(64 * WAVES) void k_mx_token(const uint16_t* x, int64_t ldx, int rows, Mx w, void* out,
+                                                         int64_t ldo) {
+  constexpr int D = ROWS > 4 ? 4 : 8, kRow = 256 * D;
+  __shared__ __attribute__((aligned(16))) char xs[WAVES][ROWS][kRow];
+  __shared__ f32x4 red[WAVES][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 15, g = lane >> 4;
+  const int64_t n0 = (int64_t)blockIdx.x * 16, rw = min(n0 + j, w.rows - 1);
+  const int per = (w.steps + WAVES - 1) / WAVES, first = min(wave * per, w.steps), last = min(first + per, w.steps);
+  const uint8_t* codes = w.codes + rw * w.ldc + 16 * g;
+  const uint8_t* scales = w.scales + rw * w.lds;
+  const int row = min(j, rows - 1);  // (lanes past X's rows repeat its last: their rows of the product are not stored)
+  f32x4 acc = zero4();
+  for (int s0 = first; s0 < last; s0 += D) {
+    u32x4 c[D];
+    uint32_t sc[D];
+    for (int r = 0; r < rows; ++r)
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const int64_t rw = min(n0 + 16 * t + j, w.rows - 1);
-    codes[t] = w.codes + rw * w.ldc + 16 * g;
-    scales[t] = w.scales + rw * w.lds + g;
-  }
-#pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    in[i] = 16 * i + j < rows;
-    px[i] = x + min((int64_t)(16 * i + j), rows - 1) * ldx + 32 * g;
-#pragma unroll
-    for (int t = 0; t < NT; ++t) acc[i][t] = zero4();
-  }
-  for (int s0 = wave; s0 < w.steps; s0 += 8 * U) {
-    u32x4 c[U][NT], a[U][MT][4];
-    uint32_t sc[U][NT];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int s = s0 + 8 * u, sl = min(s, w.steps - 1);
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        c[u][t] = ld16_stream(codes[t] + 64 * (int64_t)sl);
-        sc[u][t] = scales[t][4 * (int64_t)sl];
+      for (int i = 0; i < kRow / 1024; ++i) {
+        const int k = 128 * s0 + 512 * i + 8 * (lane ^ r);
+        ld_to_lds<16>(k < w.cols ? (const void*)(x + r * ldx + k) : &kZeroChunk, &xs[wave][r][1024 * i]);
       }
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          a[u][i][q] = u32x4{0u, 0u, 0u, 0u};
-          if (in[i] && 128 * s + 32 * g + 8 * q < w.cols) a[u][i][q] = ld16(px[i] + 128 * (int64_t)s + 8 * q);
-        }
+    for (int u = 0; u < D; ++u) {
+      const int s = min(s0 + u, last - 1);
+      c[u] = ld16_stream(codes + 64 * (int64_t)s);
+      sc[u] = ld4(scales + 4 * (int64_t)s);
     }
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+    asm volatile("" ::: "memory");
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int u = 0; u < D; ++u) {
+      if (s0 + u >= last) break;
+      const float sf = e8m0_operand(sc[u] >> (8 * g));
 #pragma unroll
       for (int q = 0; q < 4; ++q)
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const u32x4 b = fp4x8_to_bf16(c[u][t][q], e8m0_operand(sc[u][t]));
-#pragma unroll
-          for (int i = 0; i < MT; ++i) acc[i][t] = mfma_16x16x32(a[u][i][q], b, acc[i][t]);
-        }
-  }
-#pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    if (i > 0) __syncthreads();
-#pragma unroll
-    for (int t = 0; t < NT; ++t) red[wave][t][lane] = acc[i][t];
-    __syncthreads();
-    for (int o = threadIdx.x; o < NT * 256; o += 512) {
-      const int t = o >> 8, l = (o & 15) + (o >> 2 & 48), v = o >> 4 & 3;  // 16 columns of an output row to 16 threads
-      float sum = 0.f;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) sum += red[k][t][l][v];
-      const int64_t m = 16 * i + 4 * (l >> 4) + v, n = n0 + 16 * t + (l & 15);
-      if (m < rows && n < w.rows) st_out<F32>(out, m * ldo + n, sum);
+        acc = mfma_16x16x32(ld16(&xs[wave][row][16 * ((16 * u + 4 * g + q) ^ row)]), fp4x8_to_bf16(c[u][q], sf), acc);
     }
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the reads are done before the next steps' X lands
   }
+  red[wave][lane] = acc;
+  __syncthreads();
+  if (threadIdx.x >= 256) return;
+  // 16 columns of an output row to 16 threads
+  const int l = (threadIdx.x & 15) + (threadIdx.x >> 2 & 48), v = threadIdx.x >> 4 & 3;
+  float sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < WAVES; ++k) sum += red[k][l][v];
+  const int m = 4 * (l >> 4) + v;
+  const int64_t n = n0 + (l & 15);
+  if (m < rows && n < w.rows) st_out<F32>(out, m * ldo + n, sum);
 }
 
 // ---------------------------------------------------------------- bf16 rows, many of them
@@ -315,8 +299,8 @@ struct TileArgs {
 
 // out = x w^T (TRANS false: the contraction runs along w's columns) or x w (true: along w's rows).
 //
-// Workgroup: 128 rows of x by 256 output columns, 8 waves.  Waves 4 gq .. 4 gq + 3 take the half gq of each contraction
-// step of 128, wave 4 gq + wn all 128 rows and columns 64 wn .. + 63 of it: so W's codes are widened once in a
+// Workgroup: 32 MT rows of x by 256 output columns, 8 waves.  Waves 4 gq .. 4 gq + 3 take the half gq of each contraction
+// step of 128, wave 4 gq + wn all its rows and columns 64 wn .. + 63 of it: so W's codes are widened once in a
 // workgroup, and two waves a SIMD cover each other's waits.  The halves are added through LDS at the end.  Every
 // operand goes straight to LDS, three steps deep, with counted waits: one barrier a step.
 //
@@ -326,28 +310,29 @@ struct TileArgs {
 //   TRANS false: those are 32 consecutive k of one W row, so the lane reads 16 code bytes and one scale a step.
 //   TRANS true: the lane's two columns are one code byte of each W row.  The transposing LDS read gives it that byte
 //   of 8 rows at once; each is widened with its own row's scale and the halves of two rows are paired by v_perm_b32.
-template <bool TRANS>
+template <bool TRANS, int MT>
 struct TileLds {
-  static constexpr int kA = 128 * 256, kB = 16384, kS = TRANS ? 2048 : 0, kStage = kA + kB + kS, kDeep = 3;
-  static constexpr int kScales = TRANS ? 0 : 4096, kBytes = kDeep * kStage + 2 * kScales;
+  static constexpr int kA = 32 * MT * 256, kB = 16384, kS = TRANS ? 2048 : 0, kStage = kA + kB + kS, kDeep = 3;
+  static constexpr int kScales = TRANS ? 0 : 4096, kLoop = kDeep * kStage + 2 * kScales;
+  static constexpr int kJoin = (MT >= 2 ? 8 * MT / 2 : 4) * 8192, kBytes = kLoop > kJoin ? kLoop : kJoin;
 };
-template <bool TRANS, bool F32>
+template <bool TRANS, int MT, bool F32>
 __global__ __launch_bounds__(512) void k_mx_tile(TileArgs a) {
-  using T = TileLds<TRANS>;
+  using T = TileLds<TRANS, MT>;
   constexpr int kA = T::kA, kB = T::kB, kStage = T::kStage, kRing = T::kDeep * kStage;
   extern __shared__ char sm[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int gq = wave >> 2, wn = wave & 3, c = lane & 31, h = lane >> 5;
-  const Place at = place(a.tiles_m, a.tiles_n, a.splits, a.steps, 128, 256);
+  const Place at = place(a.tiles_m, a.tiles_n, a.splits, a.steps, 32 * MT, 256);
   const int64_t m0 = at.m0, n0 = at.n0;
   const int first = at.first, last = at.last;
 
-  // x: instruction i of wave w fills rows 4 (4 w + i) .. + 3 of the tile; chunk q of row r sits in slot q ^ (r % 16)
-  const char* px[4];
-  int qx[4];
+  // x: instruction i of wave w fills rows 4 (MT w + i) .. + 3 of the tile; chunk q of row r sits in slot q ^ (r % 16)
+  const char* px[MT];
+  int qx[MT];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = 4 * (4 * wave + i) + (lane >> 4);
+  for (int i = 0; i < MT; ++i) {
+    const int r = 4 * (MT * wave + i) + (lane >> 4);
     qx[i] = (lane & 15) ^ (r & 15);
     px[i] = (const char*)(a.x + min(m0 + r, a.rows - 1) * a.ldx + 8 * qx[i]);
   }
@@ -376,9 +361,12 @@ __global__ __launch_bounds__(512) void k_mx_tile(TileArgs a) {
   // part i < 4 of a step's loads
   const auto issue = [&](int step, int buf, int i) {
     char* st = sm + buf * kStage;
-    const char* g = px[i] + 256 * (int64_t)step;
-    if (16 * step + 16 > a.chunks && 16 * step + qx[i] >= a.chunks) g = (const char*)&kZeroChunk;
-    ld_to_lds<16>(g, st + 1024 * (4 * wave + i));
+    if (i < MT) {
+      const int k = i < MT ? i : 0;
+      const char* g = px[k] + 256 * (int64_t)step;
+      if (16 * step + 16 > a.chunks && 16 * step + qx[k] >= a.chunks) g = (const char*)&kZeroChunk;
+      ld_to_lds<16>(g, st + 1024 * (MT * wave + i));
+    }
     if constexpr (!TRANS) {
       if (i < 2) ld_to_lds<16>(pb[i & 1] + 64 * (int64_t)step, st + kA + 1024 * (2 * wave + i));
     } else {
@@ -399,9 +387,9 @@ __global__ __launch_bounds__(512) void k_mx_tile(TileArgs a) {
     ld_to_lds<16>(ps + 4 * (int64_t)scale_base(step, a.steps), sm + kRing + ring * T::kScales + 1024 * (wave & 3));
   };
 
-  f32x16 acc[4][2];
+  f32x16 acc[MT][2];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < MT; ++i)
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -420,10 +408,10 @@ __global__ __launch_bounds__(512) void k_mx_tile(TileArgs a) {
     // this step's loads, and its scales' (issued ahead of the codes of the step before), not those of the step after
     const int phase = (step - first) & 3;
     if constexpr (TRANS) {
-      if (wave < 4) __builtin_amdgcn_s_waitcnt(vmcnt_imm(7));
-      else __builtin_amdgcn_s_waitcnt(vmcnt_imm(6));
+      if (wave < 4) __builtin_amdgcn_s_waitcnt(vmcnt_imm(MT + 3));
+      else __builtin_amdgcn_s_waitcnt(vmcnt_imm(MT + 2));
     } else {
-      __builtin_amdgcn_s_waitcnt(vmcnt_imm(6));
+      __builtin_amdgcn_s_waitcnt(vmcnt_imm(MT + 2));
     }
     char* st = sm + buf * kStage;
     if constexpr (TRANS) {
@@ -488,7 +476,7 @@ __global__ __launch_bounds__(512) void k_mx_tile(TileArgs a) {
         }
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < MT; ++i) {
         const int r = 32 * i + c;
         const u32x4 x = ld16(st + 256 * r + 16 * ((8 * gq + 4 * h + s) ^ (r & 15)));
 #pragma unroll
@@ -500,36 +488,41 @@ __global__ __launch_bounds__(512) void k_mx_tile(TileArgs a) {
     buf = buf == 2 ? 0 : buf + 1;
   }
 
-  // Half gq finishes rows 64 gq .. + 63: each wave passes the other half's sums through LDS.
+  // The two halves' sums meet through LDS: half gq finishes half of the rows (MT 1: half 0 all of them).
+  constexpr int kOwn = MT >= 2 ? MT / 2 : 1;
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
   __syncthreads();
   f32x4* ex = (f32x4*)sm;
+  if (MT >= 2 || gq == 1) {
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < kOwn; ++i)
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const f32x16& v = gq ? acc[i][t] : acc[2 + i][t];
-        ex[((wave * 16) + 8 * i + 4 * t + q) * 64 + lane] = f32x4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
-      }
+        for (int q = 0; q < 4; ++q) {
+          const f32x16& v = gq ? acc[i][t] : acc[MT - kOwn + i][t];
+          ex[(((MT >= 2 ? wave : wn) * kOwn + i) * 8 + 4 * t + q) * 64 + lane] =
+              f32x4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+        }
+  }
   __syncthreads();
+  if (MT == 1 && gq == 1) return;
   char* out = (char*)a.out + (a.splits > 1 ? (int64_t)at.z * a.rows * a.ldo * 4 : 0);
   const int64_t n = n0 + 64 * wn + 2 * c;
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < kOwn; ++i)
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       f32x4 v[2];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const f32x4 o = ex[(((wave ^ 4) * 16) + 8 * i + 4 * t + q) * 64 + lane];
-        const f32x16& w = gq ? acc[2 + i][t] : acc[i][t];
+        const f32x4 o = ex[(((MT >= 2 ? wave ^ 4 : wn) * kOwn + i) * 8 + 4 * t + q) * 64 + lane];
+        const f32x16& w = gq ? acc[MT - kOwn + i][t] : acc[i][t];
         v[t] = f32x4{w[4 * q] + o[0], w[4 * q + 1] + o[1], w[4 * q + 2] + o[2], w[4 * q + 3] + o[3]};
       }
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int64_t m = m0 + 64 * gq + 32 * i + 8 * q + 4 * h + k;
+        const int64_t m = m0 + 32 * (gq * kOwn + i) + 8 * q + 4 * h + k;
         if (m < a.rows) st_pair<F32>(out, m, n, a.ldo, a.cols, v[0][k], v[1][k]);
       }
     }
@@ -543,6 +536,7 @@ __global__ __launch_bounds__(256) void k_mx_join(const float* part, int splits, 
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
     const int64_t m = i / quads, n = 4 * (i - m * quads);
     f32x4 s = *(const f32x4*)(part + m * ldp + n);
+#pragma unroll 4
     for (int z = 1; z < splits; ++z) {
       const f32x4 v = *(const f32x4*)(part + ((int64_t)z * rows + m) * ldp + n);
 #pragma unroll
@@ -554,31 +548,33 @@ __global__ __launch_bounds__(256) void k_mx_join(const float* part, int splits, 
   }
 }
 
-// Rows of x that the few-row kernel takes (one 16-row tile of matrix instructions, or up to four).
-static constexpr int64_t kFewRows = 64;
-// Workgroups that give every CU work.
-static constexpr int64_t kWideRows = 200;
-
 struct SplitPlan {
+  int mt;  // 32 mt rows a workgroup; 0: the few-row kernel
   int64_t tiles_m, tiles_n;
   int splits, steps;
 };
 
-// How often the contraction is split over workgroups: one workgroup runs on a CU at a time, so a grid takes
-// ceil(workgroups / CUs) rounds of its steps; every split writes and re-reads fp32 parts.  Times in us.
+// The tile's height and how often the contraction is split over workgroups: one workgroup runs on a CU at a time, so a
+// grid takes ceil(workgroups / CUs) rounds of its steps; every split writes and re-reads fp32 parts.  Times in us, as
+// measured (a step of each height; a workgroup's start and end; the join's launch; its bytes at 4 TB/s).
 static SplitPlan split_plan(int64_t rows, const lrq_mxfp4* t, bool trans) {
+  constexpr double kSteps[2][3] = {{0.53, 0.72, 1.4}, {0.6, 1.0, 1.6}}, kFixed = 9.0, kJoin = 4.0, kPerByte = 2.0 / 4.0e6;
   const int64_t cols = trans ? t->cols : t->rows, depth = trans ? t->rows : t->cols;
-  SplitPlan p{(rows + 127) / 128, (cols + 255) / 256, 1, (int)((depth + 127) / 128)};
-  if (!trans && rows <= kFewRows) return p;
-  constexpr double kStep = 1.1, kJoin = 4.0, kPerByte = 2.0 / 4.0e6;
-  const int64_t tiles = p.tiles_m * p.tiles_n;
-  double best = 0.;
-  for (int s = 1; s <= 16 && s <= std::max(1, p.steps / 2); ++s) {
-    const double rounds = (double)((tiles * s + 255) / 256);
-    const double cost = rounds * ((p.steps + s - 1) / s + 2) * kStep + (s > 1 ? kJoin + kPerByte * 4. * s * rows * cols : 0.);
-    if (s == 1 || cost < best) best = cost, p.splits = s;
+  const int steps = (int)((depth + 127) / 128);
+  if (!trans && rows <= 16) return SplitPlan{0, 0, 0, 1, steps};
+  SplitPlan best{};
+  double least = 0.;
+  for (int i = 0; i < 3; ++i) {
+    SplitPlan p{1 << i, 0, (cols + 255) / 256, 1, steps};
+    p.tiles_m = (rows + 32 * p.mt - 1) / (32 * p.mt);
+    for (; p.splits <= 16 && p.splits <= std::max(1, steps / 2); ++p.splits) {
+      const double rounds = (double)((p.tiles_m * p.tiles_n * p.splits + 255) / 256);
+      const double cost = rounds * ((steps + p.splits - 1) / p.splits * kSteps[trans][i] + kFixed) +
+                          (p.splits > 1 ? kJoin + kPerByte * 4. * p.splits * rows * cols : 0.);
+      if (best.mt == 0 || cost < least) best = p, least = cost;
+    }
   }
-  return p;
+  return best;
 }
 
 struct GemmPlan {
@@ -691,25 +687,22 @@ static int mx_linear(const void* x, int64_t ldx, int64_t rows, const lrq_mxfp4* 
   const Mx w = make_mx(t);
   hipStream_t s = (hipStream_t)stream;
   const uint16_t* px = (const uint16_t*)x;
-  if (!trans && rows <= kFewRows) {
-    // as many W rows a workgroup as still give each CU one
-    const auto go = [&](auto mt, auto nt) {
-      const dim3 grid((unsigned)((w.rows + 16 * nt() - 1) / (16 * nt())));
-      return out_fp32 ? launch(k_mx_linear<mt(), nt(), true>, grid, dim3(512), 0, s, px, ldx, rows, w, out, ldo)
-                      : launch(k_mx_linear<mt(), nt(), false>, grid, dim3(512), 0, s, px, ldx, rows, w, out, ldo);
-    };
+  if (!trans && rows <= 16) {
     using std::integral_constant;
-    const int most = w.rows >= 64 * kWideRows ? 4 : w.rows >= 32 * kWideRows ? 2 : 1;
-#define LRQ_GO(MT)                                                                          \
-  {                                                                                         \
-    if (most == 4) return go(integral_constant<int, MT>{}, integral_constant<int, 4>{});    \
-    if (most == 2) return go(integral_constant<int, MT>{}, integral_constant<int, 2>{});    \
-    return go(integral_constant<int, MT>{}, integral_constant<int, 1>{});                   \
-  }
-    if (rows <= 4) return go(integral_constant<int, 1>{}, integral_constant<int, 1>{});
-    if (rows <= 16) LRQ_GO(1)
-    if (rows <= 32) LRQ_GO(2)
-    LRQ_GO(4)
+    const dim3 grid((unsigned)((w.rows + 15) / 16));
+    const auto go = [&](auto r, auto waves) {
+      return out_fp32 ? launch((k_mx_token<r(), waves(), true>), grid, dim3(64 * waves()), 0, s, px, ldx, (int)rows, w, out, ldo)
+                      : launch((k_mx_token<r(), waves(), false>), grid, dim3(64 * waves()), 0, s, px, ldx, (int)rows, w, out, ldo);
+    };
+    // four waves a workgroup (8 steps each of 4096 columns: one round of loads); eight where workgroups are few and the
+    // runs long, 11.6 against 12.4 us on 4096 rows of 14336 columns (but 6.6 against 5.2 us on 4096 of 4096)
+#define LRQ_GO(R, W) return go(integral_constant<int, R>{}, integral_constant<int, W>{})
+    if (rows <= 4) {
+      if (grid.x >= 512 || w.steps <= 64) LRQ_GO(4, 4);
+      LRQ_GO(4, 8);
+    }
+    if (grid.x >= 512) LRQ_GO(16, 4);
+    LRQ_GO(16, 8);
 #undef LRQ_GO
   }
   const SplitPlan p = split_plan(rows, t, trans);
@@ -726,9 +719,14 @@ static int mx_linear(const void* x, int64_t ldx, int64_t rows, const lrq_mxfp4* 
     if (e != hipSuccess) return (int)e;
     return launch(kern, dim3((unsigned)wgs), dim3(512), (size_t)lds, s, a);
   };
-  constexpr int kLds = TileLds<false>::kBytes, kLdsT = TileLds<true>::kBytes;
-  if (trans) LRQ_TRY(f32 ? go(k_mx_tile<true, true>, kLdsT) : go(k_mx_tile<true, false>, kLdsT));
-  else LRQ_TRY(f32 ? go(k_mx_tile<false, true>, kLds) : go(k_mx_tile<false, false>, kLds));
+  const auto with = [&](auto mt) {
+    constexpr int kLds = TileLds<false, mt()>::kBytes, kLdsT = TileLds<true, mt()>::kBytes;
+    if (trans) return f32 ? go(k_mx_tile<true, mt(), true>, kLdsT) : go(k_mx_tile<true, mt(), false>, kLdsT);
+    return f32 ? go(k_mx_tile<false, mt(), true>, kLds) : go(k_mx_tile<false, mt(), false>, kLds);
+  };
+  if (p.mt == 4) LRQ_TRY(with(std::integral_constant<int, 4>{}));
+  else if (p.mt == 2) LRQ_TRY(with(std::integral_constant<int, 2>{}));
+  else LRQ_TRY(with(std::integral_constant<int, 1>{}));
   return need ? join((const float*)workspace, p.splits, rows, cols, ldp, out, ldo, out_fp32, s) : LRQ_OK;
 }
 

@@ -10,6 +10,7 @@ MXFP4 operands on the scaled matrix instructions.  ``autograd.mxfp4_linear`` and
 from __future__ import annotations
 
 import ctypes
+import math
 from dataclasses import dataclass
 
 import torch
@@ -21,7 +22,7 @@ from .norm import _dtype, _rows
 __all__ = ["MXFP4Tensor", "mxfp4_quantize", "mxfp4_dequantize", "mxfp4_gemm", "mxfp4_linear", "mxfp4_linear_backward"]
 
 
-@dataclass(frozen=True)
+@dataclass(eq=False)
 class MXFP4Tensor:
     """A tensor [..., cols] in MXFP4; rows are its leading dimensions flattened.
 
@@ -52,22 +53,22 @@ class MXFP4Tensor:
         return MXFP4Tensor(self.codes.to(device), self.scales.to(device), self.shape)
 
     def descriptor(self) -> LrqMxfp4:
-        c, s = self.codes, self.scales
+        c, s, shape = self.codes, self.scales, self.shape
         _require_device(c, s)
-        rows = 1
-        for d in self.shape[:-1]:
-            rows *= d
-        if len(self.shape) < 1 or self.shape[-1] <= 0:
+        cols = shape[-1] if len(shape) else 0
+        if cols <= 0:
             raise ValueError("an MXFP4 tensor needs rows of at least one element")
-        steps = (self.shape[-1] + 127) // 128
+        rows = shape[0] if len(shape) == 2 else math.prod(shape[:-1])
+        steps = (cols + 127) // 128
         for t, name, width in ((c, "codes", 64 * steps), (s, "scales", 4 * steps)):
-            if t.dtype != torch.uint8 or t.dim() != 2 or t.shape[0] != rows or t.shape[1] < width or t.device != c.device:
+            if t.dtype is not torch.uint8 or t.dim() != 2 or t.shape[0] != rows or t.shape[1] < width or t.device != c.device:
                 raise ValueError(f"{name} must be uint8 [{rows}, >= {width}] on one device, got {t.dtype} {tuple(t.shape)}")
             if t.stride(1) != 1:
                 raise ValueError(f"{name} must have unit inner stride")
         # the stride of a single row means nothing
-        return LrqMxfp4(c.data_ptr(), c.stride(0) if rows > 1 else 64 * steps, s.data_ptr(),
-                        s.stride(0) if rows > 1 else 4 * steps, rows, self.shape[-1])
+        if rows > 1:
+            return LrqMxfp4(c.data_ptr(), c.stride(0), s.data_ptr(), s.stride(0), rows, cols)
+        return LrqMxfp4(c.data_ptr(), 64 * steps, s.data_ptr(), 4 * steps, rows, cols)
 
 
 def mxfp4_quantize(x: torch.Tensor) -> MXFP4Tensor:
@@ -142,7 +143,7 @@ def _operand(x: torch.Tensor, cols: int, name: str):
     x2, rows, _, ld = _rows(x, name)
     if ld % 8 or x2.data_ptr() % 16:
         x2 = x2.clone(memory_format=torch.contiguous_format)
-        ld = x2.shape[1]
+        ld = x2.shape[-1]
     return x2, rows, ld
 
 
