@@ -116,6 +116,11 @@ __device__ __forceinline__ void ld_weight(const void* p, int dt, int64_t at, int
   else widen<kF32>(ld_chunk<kF32>(q, valid), f);
 }
 
+// ---------------------------------------------------------------- workgroup barrier
+// Waits for this wave's LDS traffic and meets the workgroup; loads from memory stay in flight.  One statement that no
+// memory access moves across in either direction.
+__device__ __forceinline__ void lds_meet() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
 // ---------------------------------------------------------------- sums over lanes
 // Sum over each group of LANES (16 or 64) consecutive lanes, in every lane: quad and mirror moves of the
 // DPP network, then the row swaps, so no LDS round trip.

@@ -177,7 +177,7 @@ __global__ __launch_bounds__(512) void k_mx_gemm(GemmArgs p) {
   };
   // the scales' loads are ahead of the codes of the step before theirs
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(kLoads * 2));
-  lds_barrier();
+  lds_meet();
   read(0, 0);
   read_scales(at.first, 0, 0);
   int buf = 0, ring = 0;
@@ -200,7 +200,7 @@ __global__ __launch_bounds__(512) void k_mx_gemm(GemmArgs p) {
     // the next step's loads, not those of the two steps after it (nor the scales among them)
     if (phase < 2 && steps >= 4) __builtin_amdgcn_s_waitcnt(vmcnt_imm(kLoads * (kDeep - 2) + 1));
     else __builtin_amdgcn_s_waitcnt(vmcnt_imm(kLoads * (kDeep - 2)));
-    lds_barrier();  // every wave's are in, and every wave has read all of this step's buffer
+    lds_meet();  // every wave's are in, and every wave has read all of this step's buffer
     if (phase == 3) ring ^= 1;
     buf = (buf + 1) & (kDeep - 1);
     read(0, buf);
@@ -422,7 +422,7 @@ __global__ __launch_bounds__(512) void k_mx_tile(TileArgs a) {
         for (int k = 0; k < 4; ++k) st[kA + kB + 1024 + (4 * (lane & 1) + k) * 128 + rs] = (char)(s4 >> (8 * k));
       }
     }
-    lds_barrier();  // every wave's loads are in, and the buffer of the step before is free
+    lds_meet();  // every wave's loads are in, and the buffer of the step before is free
     const int ahead = min(step + 2, last - 1), to = buf == 0 ? 2 : buf - 1;
     if constexpr (!TRANS) {
       if (phase == 2 && a.steps >= 4) issue_scales(step + 2, ring ^ 1);

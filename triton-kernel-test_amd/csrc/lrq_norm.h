@@ -5,8 +5,8 @@
 //   g = dy w,  dn = r (g - mean(g) - z mean(g z)),  dw = sum_rows dy z,  db = sum_rows dy
 //   dresidual = dh + dn,  dx = drop(dresidual)
 //
-// TPR consecutive threads own a row, each with C chunks of 8 columns (chunk t + j TPR), which stay
-// in registers between the statistics and the output: one read of the row.  All sums are fp32.
+// The threads of a row own C chunks of 8 columns each (thread t chunks t + j * threads), which stay in registers between
+// the statistics and the output: one read of the row.  All sums are fp32.
 #pragma once
 
 #include "lrq_dropout.h"
@@ -15,16 +15,38 @@
 
 namespace lrq {
 
-// A workgroup's row groups walk rows g, g + G, ... (G = groups in the grid).
-template <int TPR, int C>
-struct RowGeom {
-  static constexpr int kThreads = TPR > 256 ? TPR : 256;
-  static constexpr int kGroups = kThreads / TPR;          // row groups a workgroup
-  static constexpr int kWaves = TPR > 64 ? TPR / 64 : 1;  // waves a row
+// Rows of up to 16 chunks take 16 threads, up to 64 chunks a wave, wider ones as many whole waves as they need (LANES 0,
+// waves at run time): 5120 columns are five waves of two chunks a thread with nothing idle.  A workgroup's row groups
+// walk rows g, g + G, ... (G = groups in the grid).
+struct RowShape {
+  int lanes;   // 16, 64, or 0: several waves
+  int chunks;  // a thread
+  int waves;   // a row
 };
+// `one`: up to how many chunks a row has one a thread, `more`: how many a thread above that.
+static inline RowShape row_shape(int64_t n, int64_t one, int more) {
+  const int64_t nc = (n + 7) / 8;
+  if (nc <= 16) return RowShape{16, 1, 1};
+  if (nc <= 64) return RowShape{64, 1, 1};
+  const int c = nc <= one ? 1 : more;
+  return RowShape{nc <= 64 * c ? 64 : 0, c, (int)((nc + 64 * c - 1) / (64 * c))};
+}
+
+// Row groups of a workgroup of up to `waves` waves: one where the rows are too few for every CU, so that they spread.
+static inline int row_groups(const RowShape& r, int64_t rows, int waves) {
+  const int64_t most = r.lanes ? 64 * waves / r.lanes : std::max(1, waves / r.waves);
+  return (int)std::min<int64_t>(most, std::max<int64_t>(1, r.lanes == 16 ? 4 * ((rows + 1023) / 1024) : (rows + 255) / 256));
+}
+
+// The row group of a thread, known to be the wave's where a wave holds one row: its addresses then need one register a
+// chunk beside scalar bases.
+template <int LANES>
+__device__ __forceinline__ int wave_row(int grp) {
+  return LANES == 16 ? grp : (int)__builtin_amdgcn_readfirstlane(grp);
+}
 
 // The widest row of the register-resident kernels; wider rows sweep the row again.
-static constexpr int64_t kNormMaxWidth = 1024 * 2 * 8;
+static constexpr int64_t kNormMaxWidth = 16384;
 
 struct NormFwd {
   const char* x;
@@ -42,6 +64,7 @@ struct NormFwd {
   int wdt;
   int64_t rows;
   int n;
+  int waves, groups;  // of a row, of a workgroup
   float eps;
   Drop drop;
 };
@@ -64,24 +87,8 @@ struct NormBwd {
   float* part;     // [workgroups][2][n] sums of dy z and dy, or NULL (no weight gradients)
   int64_t rows;
   int n;
+  int waves, groups;  // of a row, of a workgroup
   Drop drop;
 };
-
-// Picks <TPR, C> for a row of nc chunks: the fewest threads that keep a thread at 4 chunks or fewer;
-// f(TPR, C) receives them as integral constants.
-template <class F>
-static inline int with_row_geom(int nc, F&& f) {
-  using std::integral_constant;
-#define LRQ_GEOM(T, CC) return f(integral_constant<int, T>{}, integral_constant<int, CC>{})
-  if (nc <= 16) LRQ_GEOM(16, 1);
-  if (nc <= 64) LRQ_GEOM(64, 1);
-  if (nc <= 128) LRQ_GEOM(64, 2);
-  if (nc <= 256) LRQ_GEOM(256, 1);
-  if (nc <= 512) LRQ_GEOM(256, 2);
-  if (nc <= 768) LRQ_GEOM(256, 3);
-  if (nc <= 1024) LRQ_GEOM(1024, 1);
-  LRQ_GEOM(1024, 2);
-#undef LRQ_GEOM
-}
 
 }  // namespace lrq

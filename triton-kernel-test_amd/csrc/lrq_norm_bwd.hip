@@ -12,35 +12,36 @@ __device__ __forceinline__ void norm_outputs(const NormBwd& a, const DropKey& ke
   if constexpr (FUSED) {
     if (a.dh != nullptr) {
       float q[8];
-      widen<DT>(ld_chunk<DT>(a.dh + (row * a.lddh + 8 * (int64_t)c) * ES, k), q);
+      widen<DT>(ld_chunk<DT>(a.dh + row * a.lddh * ES + 8u * ES * (uint32_t)c, k), q);
 #pragma unroll
       for (int e = 0; e < 8; ++e) d[e] = q[e] + d[e];
     }
-    if (a.dres != nullptr) st_chunk<DT>(a.dres + (row * a.lddr + 8 * (int64_t)c) * ES, narrow<DT>(d), k);
+    if (a.dres != nullptr) st_chunk<DT>(a.dres + row * a.lddr * ES + 8u * ES * (uint32_t)c, narrow<DT>(d), k);
     if (a.drop.keep < 65536u) drop_chunk(a.drop, key, (uint64_t)row * nc + c, d);
   }
-  if (!FUSED || a.dx != nullptr) st_chunk<DT>(a.dx + (row * a.lddx + 8 * (int64_t)c) * ES, narrow<DT>(d), k);
+  if (!FUSED || a.dx != nullptr) st_chunk<DT>(a.dx + row * a.lddx * ES + 8u * ES * (uint32_t)c, narrow<DT>(d), k);
 }
 
 // One pass over dy and h.  A thread owns the same columns in every row of its group, so dy z and dy of the
 // weight gradients add up in its registers; the workgroup's groups join them in LDS at the end, and
-// k_norm_wgrad adds the workgroups' sums in a fixed order.
-template <int DT, int TPR, int C, bool FUSED>
-__global__ __launch_bounds__((RowGeom<TPR, C>::kThreads)) void k_norm_bwd(NormBwd a) {
-  using G = RowGeom<TPR, C>;
-  constexpr int ES = Elem<DT>::kBytes;
-  constexpr int L = TPR < 64 ? TPR : 64;
-  constexpr int kCols = TPR * 8 * C;
-  __shared__ float red[2][G::kGroups][G::kWaves][2];
-  extern __shared__ float sums[];  // [groups][kCols], with weight gradients only
-  const int t = threadIdx.x % TPR, grp = threadIdx.x / TPR, wave = t / 64;
+// k_norm_wgrad adds the workgroups' sums in a fixed order.  Rows are held as stored between the two uses, with the next
+// row's already on the way: sixteen waves a CU in 128 registers, and few workgroups, whose sums are few.
+template <int DT, int LANES, int C, bool FUSED>
+__global__ __launch_bounds__(C > 1 ? 512 : 1024) void k_norm_bwd(NormBwd a) {
+  constexpr int ES = Elem<DT>::kBytes, L = LANES == 16 ? 16 : 64;
+  constexpr bool kPrefetch = C == 1;  // (four chunks a thread leave no registers for a second row)
+  __shared__ float red[2][16][2];
+  extern __shared__ float sums[];  // [groups][threads of a row * 8 C], with weight gradients only
+  const int tpr = LANES ? LANES : 64 * a.waves, kCols = tpr * 8 * C;
+  const int grp = wave_row<LANES>(threadIdx.x / tpr), t = threadIdx.x - grp * tpr;
+  const int wv = threadIdx.x >> 6, w0 = LANES ? 0 : grp * a.waves;
   const int n = a.n, nc = (n + 7) / 8;
   const float rn = 1.f / (float)n;
   int valid[C];
   float wt[C][8], gw[C][8], gb[C][8];
 #pragma unroll
   for (int j = 0; j < C; ++j) {
-    const int c = t + j * TPR;
+    const int c = t + j * tpr;
     valid[j] = c < nc ? min(8, n - 8 * c) : 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) wt[j][e] = 1.f, gw[j][e] = 0.f, gb[j][e] = 0.f;
@@ -48,55 +49,84 @@ __global__ __launch_bounds__((RowGeom<TPR, C>::kThreads)) void k_norm_bwd(NormBw
   }
   DropKey key{};
   if constexpr (FUSED) key = drop_key(a.drop);
-  int slot = 0;
-  for (int64_t r0 = (int64_t)blockIdx.x * G::kGroups; r0 < a.rows; r0 += (int64_t)gridDim.x * G::kGroups) {
-    const int64_t row = r0 + grp;
+  struct Row {
+    Chunk<DT> dy[C], h[C];
+    float mean, rstd;
+  };
+  // a group past the last row works on zeros; elements past the row are zero in dy, so they add nothing to any sum (z is
+  // finite there for finite statistics; a row whose statistics are not finite is lost anyway)
+  const auto load = [&](int64_t row) {
+    Row r;
     const bool on = row < a.rows;
-    const float mean = on ? a.mean[row] : 0.f, rstd = on ? a.rstd[row] : 0.f;
-    float g[C][8], z[C][8];
+    r.mean = on ? a.mean[row] : 0.f;
+    r.rstd = on ? a.rstd[row] : 0.f;
+#pragma unroll
+    for (int j = 0; j < C; ++j) {
+      const uint32_t at = 8u * ES * (uint32_t)(t + j * tpr);
+      r.dy[j] = ld_chunk<DT>(a.dy + row * a.lddy * ES + at, on ? valid[j] : 0);
+      r.h[j] = ld_chunk<DT>(a.h + row * a.ldh * ES + at, on ? valid[j] : 0);
+    }
+    return r;
+  };
+  int slot = 0;
+  const int64_t step = (int64_t)gridDim.x * a.groups;
+  Row cur;
+  if constexpr (kPrefetch) cur = load((int64_t)blockIdx.x * a.groups + grp);
+  for (int64_t r0 = (int64_t)blockIdx.x * a.groups; r0 < a.rows; r0 += step) {
+    const int64_t row = r0 + grp;
+    Row next;
+    if constexpr (kPrefetch) next = load(row + step);
+    else cur = load(row);
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int j = 0; j < C; ++j) {
-      const int k = on ? valid[j] : 0;
-      const int64_t c8 = 8 * (int64_t)(t + j * TPR);
-      // elements past the row are zero in dy, so they add nothing to any sum (z is finite there for
-      // finite statistics; a row whose statistics are not finite is lost anyway)
-      widen<DT>(ld_chunk<DT>(a.dy + (row * a.lddy + c8) * ES, k), g[j]);
-      widen<DT>(ld_chunk<DT>(a.h + (row * a.ldh + c8) * ES, k), z[j]);
+      float g[8], z[8];
+      widen<DT>(cur.dy[j], g);
+      widen<DT>(cur.h[j], z);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        z[j][e] = (z[j][e] - mean) * rstd;
-        gw[j][e] = __builtin_fmaf(g[j][e], z[j][e], gw[j][e]);
-        gb[j][e] += g[j][e];
-        g[j][e] *= wt[j][e];
-        s1 += g[j][e];
-        s2 = __builtin_fmaf(g[j][e], z[j][e], s2);
+        const float ze = (z[e] - cur.mean) * cur.rstd;
+        gw[j][e] = __builtin_fmaf(g[e], ze, gw[j][e]);
+        gb[j][e] += g[e];
+        const float ge = g[e] * wt[j][e];
+        s1 += ge;
+        s2 = __builtin_fmaf(ge, ze, s2);
       }
+      if constexpr (C > 1) __builtin_amdgcn_sched_barrier(0);
     }
     s1 = lanes_sum<L>(s1);
     s2 = lanes_sum<L>(s2);
-    if constexpr (G::kWaves > 1) {
-      if ((t & 63) == 0) {
-        red[slot][grp][wave][0] = s1;
-        red[slot][grp][wave][1] = s2;
+    if constexpr (LANES == 0) {
+      if ((threadIdx.x & 63) == 0) {
+        red[slot][wv][0] = s1;
+        red[slot][wv][1] = s2;
       }
-      __syncthreads();
+      lds_meet();  // (leaves the next row's loads in flight)
       s1 = 0.f, s2 = 0.f;
-#pragma unroll
-      for (int k = 0; k < G::kWaves; ++k) {
-        s1 += red[slot][grp][k][0];
-        s2 += red[slot][grp][k][1];
+      for (int k = 0; k < a.waves; ++k) {
+        s1 += red[slot][w0 + k][0];
+        s2 += red[slot][w0 + k][1];
       }
-      slot ^= 1;
+      slot ^= 1;  // this slot is written again only after the next row's barrier
     }
-    if (!on) continue;
     s1 *= rn, s2 *= rn;
+    if (row < a.rows) {
 #pragma unroll
-    for (int j = 0; j < C; ++j) {
+      for (int j = 0; j < C; ++j) {
+        float g[8], z[8];
+        // widened again: kept from above, the fp32 values would take twice the registers
 #pragma unroll
-      for (int e = 0; e < 8; ++e) g[j][e] = rstd * (g[j][e] - s1 - z[j][e] * s2);
-      norm_outputs<DT, FUSED>(a, key, row, t + j * TPR, nc, valid[j], g[j]);
+        for (int k = 0; k < Elem<DT>::kVecs; ++k) pin(cur.dy[j].v[k]), pin(cur.h[j].v[k]);
+        widen<DT>(cur.dy[j], g);
+        widen<DT>(cur.h[j], z);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          g[e] = cur.rstd * (g[e] * wt[j][e] - s1 - (z[e] - cur.mean) * cur.rstd * s2);
+        norm_outputs<DT, FUSED>(a, key, row, t + j * tpr, nc, valid[j], g);
+        if constexpr (C > 1) __builtin_amdgcn_sched_barrier(0);  // one chunk's temporaries at a time
+      }
     }
+    if constexpr (kPrefetch) cur = next;
   }
   if (a.part == nullptr) return;  // uniform
   float* part = a.part + (int64_t)blockIdx.x * 2 * n;
@@ -106,11 +136,11 @@ __global__ __launch_bounds__((RowGeom<TPR, C>::kThreads)) void k_norm_bwd(NormBw
 #pragma unroll
     for (int j = 0; j < C; ++j)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sums[grp * kCols + 8 * (t + j * TPR) + e] = half ? gb[j][e] : gw[j][e];
+      for (int e = 0; e < 8; ++e) sums[grp * kCols + 8 * (t + j * tpr) + e] = half ? gb[j][e] : gw[j][e];
     __syncthreads();
-    for (int c = threadIdx.x; c < n; c += G::kThreads) {
+    for (int c = threadIdx.x; c < n; c += blockDim.x) {
       float s = 0.f;
-      for (int k = 0; k < G::kGroups; ++k) s += sums[k * kCols + c];
+      for (int k = 0; k < a.groups; ++k) s += sums[k * kCols + c];
       part[half * (int64_t)n + c] = s;
     }
   }
@@ -218,37 +248,49 @@ __global__ __launch_bounds__(1024) void k_norm_wgrad(const float* part, int part
 }
 
 struct BwdPlan {
+  RowShape shape;
+  int groups;     // rows a workgroup takes at a time
   int64_t grid;   // workgroups of the row kernel
   int64_t parts;  // sums of the weight gradients
 };
 
 static BwdPlan bwd_plan(int64_t rows, int64_t n) {
   constexpr int kCus = 256;  // a fixed count, so that the workspace and the order of the sums depend on the shape alone
-  if (n > kNormMaxWidth) return BwdPlan{std::min<int64_t>(rows, 2 * kCus), std::min<int64_t>((rows + 3) / 4, 64)};
-  int64_t grid = 0;
-  with_row_geom((int)((n + 7) / 8), [&](auto tpr, auto c) {
-    using G = RowGeom<tpr(), c()>;
-    grid = std::min<int64_t>((rows + G::kGroups - 1) / G::kGroups, (int64_t)kCus * 1024 / G::kThreads);
-    return 0;
-  });
-  return BwdPlan{grid, grid};
+  // one chunk a thread as far as 16 waves go (each has 16 sums besides), else four in half as many waves
+  BwdPlan p{row_shape(n, 1024, 4), 1, 0, 0};
+  if (n > kNormMaxWidth) {
+    p.grid = std::min<int64_t>(rows, 2 * kCus);
+    p.parts = std::min<int64_t>((rows + 3) / 4, 64);
+    return p;
+  }
+  p.groups = row_groups(p.shape, rows, p.shape.chunks == 1 ? 16 : 8);
+  p.grid = p.parts = std::min<int64_t>((rows + p.groups - 1) / p.groups, kCus);
+  return p;
 }
 
 template <int DT, bool FUSED>
-static int norm_bwd(const NormBwd& a, hipStream_t s) {
+static int norm_bwd(NormBwd a, hipStream_t s) {
   const BwdPlan p = bwd_plan(a.rows, a.n);
   if (a.n > kNormMaxWidth) {
     if (a.part != nullptr)
       LRQ_TRY(launch((k_norm_cols<DT>), dim3((unsigned)((a.n + 511) / 512), (unsigned)p.parts), dim3(256), 0, s, a));
     return launch((k_norm_bwd_wide<DT, FUSED>), dim3((unsigned)p.grid), dim3(1024), 0, s, a);
   }
-  return with_row_geom((a.n + 7) / 8, [&](auto tpr, auto c) {
-    using G = RowGeom<tpr(), c()>;
-    const size_t lds = a.part == nullptr ? 0 : sizeof(float) * G::kThreads * 8 * c();
-    const void* kern = (const void*)k_norm_bwd<DT, tpr(), c(), FUSED>;
-    if (lds >= 64 * 1024) (void)hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    return launch((k_norm_bwd<DT, tpr(), c(), FUSED>), dim3((unsigned)p.grid), dim3(G::kThreads), lds, s, a);
-  });
+  a.waves = p.shape.waves;
+  a.groups = p.groups;
+  const int threads = std::max(64, (p.shape.lanes ? p.shape.lanes : 64 * p.shape.waves) * p.groups);
+  const size_t lds = a.part == nullptr ? 0 : sizeof(float) * threads * 8 * p.shape.chunks;
+  const auto go = [&](auto kern) {
+    if (lds >= 64 * 1024) {
+      const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+      if (e != hipSuccess) return (int)e;
+    }
+    return launch(kern, dim3((unsigned)p.grid), dim3(threads), lds, s, a);
+  };
+  if (p.shape.lanes == 16) return go(k_norm_bwd<DT, 16, 1, FUSED>);
+  if (p.shape.lanes == 64) return go(k_norm_bwd<DT, 64, 1, FUSED>);
+  if (p.shape.chunks == 1) return go(k_norm_bwd<DT, 0, 1, FUSED>);
+  return go(k_norm_bwd<DT, 0, 4, FUSED>);
 }
 
 }  // namespace lrq
@@ -292,7 +334,7 @@ extern "C" int lrq_layer_norm_bwd(const lrq_dropout* drop, const void* dy, int64
     const bool fused = drop != nullptr || dh != nullptr || dresidual != nullptr;
     const NormBwd a{(const char*)dy, lddy, (const char*)dh, lddh, (const char*)h, ldh, mean, rstd, w, w_dtype, (char*)dx,
                     lddx, (char*)dresidual, ld_dresidual, wgrad ? (float*)workspace : nullptr, rows, (int)n,
-                    make_drop(drop)};
+                    0, 0, make_drop(drop)};
     const auto go = [&] {
       switch (dtype) {
         case LRQ_BF16: return fused ? norm_bwd<kBf16, true>(a, s) : norm_bwd<kBf16, false>(a, s);

@@ -3,24 +3,41 @@
 
 namespace lrq {
 
-// One row's h chunk c (k valid elements): x, dropped, with the residual added, rounded and stored.
+// A chunk of a row's inputs as stored.
 template <int DT, bool FUSED>
-__device__ __forceinline__ void norm_input(const NormFwd& a, const DropKey& key, int64_t row, int c, int nc, int k,
-                                           float* v) {
+struct Input {
+  Chunk<DT> x, res;
+};
+template <int DT>
+struct Input<DT, false> {
+  Chunk<DT> x;
+};
+template <int DT, bool FUSED>
+__device__ __forceinline__ Input<DT, FUSED> ld_input(const NormFwd& a, int64_t row, int c, int k) {
   constexpr int ES = Elem<DT>::kBytes;
-  widen<DT>(ld_chunk<DT>(a.x + (row * a.ldx + 8 * (int64_t)c) * ES, k), v);
+  Input<DT, FUSED> in;
+  in.x = ld_chunk<DT>(a.x + row * a.ldx * ES + 8u * ES * (uint32_t)c, k);
+  if constexpr (FUSED) in.res = ld_chunk<DT>(a.res + row * a.ldr * ES + 8u * ES * (uint32_t)c, a.res != nullptr ? k : 0);
+  return in;
+}
+
+// h of chunk c (k valid elements): x, dropped, with the residual added, rounded and stored.
+template <int DT, bool FUSED>
+__device__ __forceinline__ void norm_input(const NormFwd& a, const DropKey& key, const Input<DT, FUSED>& in, int64_t row,
+                                           int c, int nc, int k, float* v) {
+  widen<DT>(in.x, v);
   if constexpr (FUSED) {
     if (k > 0) {
       if (a.drop.keep < 65536u) drop_chunk(a.drop, key, (uint64_t)row * nc + c, v);
       if (a.res != nullptr) {
         float q[8];
-        widen<DT>(ld_chunk<DT>(a.res + (row * a.ldr + 8 * (int64_t)c) * ES, k), q);
+        widen<DT>(in.res, q);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = q[e] + v[e];
       }
       // the statistics are those of h as stored
       const Chunk<DT> hc = narrow<DT>(v);
-      st_chunk<DT>(a.h + (row * a.ldh + 8 * (int64_t)c) * ES, hc, k);
+      st_chunk<DT>(a.h + row * a.ldh * Elem<DT>::kBytes + 8u * Elem<DT>::kBytes * (uint32_t)c, hc, k);
       widen<DT>(hc, v);
     }
   }
@@ -29,20 +46,20 @@ __device__ __forceinline__ void norm_input(const NormFwd& a, const DropKey& key,
 // One pass: a row's chunks are read once.  Each wave reduces its part of the row to (mean, sum of
 // squared deviations from it) and the waves' parts are merged (Chan, Golub and LeVeque's update), so a
 // row costs one barrier and the variance never comes from a difference of large sums.
-template <int DT, int TPR, int C, bool FUSED>
-__global__ __launch_bounds__((RowGeom<TPR, C>::kThreads)) void k_norm_fwd(NormFwd a) {
-  using G = RowGeom<TPR, C>;
-  constexpr int ES = Elem<DT>::kBytes;
-  constexpr int L = TPR < 64 ? TPR : 64;
-  __shared__ float red[2][G::kGroups][G::kWaves][2], cnts[G::kWaves];
-  const int t = threadIdx.x % TPR, grp = threadIdx.x / TPR, wave = t / 64;
+template <int DT, int LANES, int C, bool FUSED>
+__global__ __launch_bounds__(1024) void k_norm_fwd(NormFwd a) {
+  constexpr int ES = Elem<DT>::kBytes, L = LANES == 16 ? 16 : 64;
+  __shared__ float red[2][16][2], cnts[16];
+  const int tpr = LANES ? LANES : 64 * a.waves;
+  const int grp = wave_row<LANES>(threadIdx.x / tpr), t = threadIdx.x - grp * tpr;
+  const int wv = threadIdx.x >> 6, w0 = LANES ? 0 : grp * a.waves;  // this wave, its row's first
   const int n = a.n, nc = (n + 7) / 8;
   int valid[C];
   float wt[C][8], bs[C][8];
   float cnt = 0.f;
 #pragma unroll
   for (int j = 0; j < C; ++j) {
-    const int c = t + j * TPR;
+    const int c = t + j * tpr;
     valid[j] = c < nc ? min(8, n - 8 * c) : 0;
     cnt += (float)valid[j];
 #pragma unroll
@@ -52,21 +69,38 @@ __global__ __launch_bounds__((RowGeom<TPR, C>::kThreads)) void k_norm_fwd(NormFw
   }
   cnt = lanes_sum<L>(cnt);  // this wave's columns of a row
   const float rcnt = cnt > 0.f ? 1.f / cnt : 0.f, rn = 1.f / (float)n;
-  if constexpr (G::kWaves > 1) {
-    if (grp == 0 && (t & 63) == 0) cnts[wave] = cnt;
+  if constexpr (LANES == 0) {
+    if ((threadIdx.x & 63) == 0) cnts[wv] = cnt;
   }
   DropKey key{};
   if constexpr (FUSED) key = drop_key(a.drop);
   int slot = 0;
-  // Every thread takes every step (barriers): a group past the last row works on zeros.
-  for (int64_t r0 = (int64_t)blockIdx.x * G::kGroups; r0 < a.rows; r0 += (int64_t)gridDim.x * G::kGroups) {
+  struct Row {
+    Input<DT, FUSED> in[C];
+  };
+  const auto load = [&](int64_t row) {
+    Row r;
+#pragma unroll
+    for (int j = 0; j < C; ++j) r.in[j] = ld_input<DT, FUSED>(a, row, t + j * tpr, row < a.rows ? valid[j] : 0);
+    return r;
+  };
+  const int64_t step = (int64_t)gridDim.x * a.groups;
+  constexpr bool kPrefetch = C == 1 || !FUSED || (DT != kF32 && LANES == 0);  // (two rows of two inputs: too many registers)
+  Row cur;
+  if constexpr (kPrefetch) cur = load((int64_t)blockIdx.x * a.groups + grp);
+  // Every thread takes every step (barriers): a group past the last row works on zeros.  The next row is on its way
+  // while this one is reduced and written.
+  for (int64_t r0 = (int64_t)blockIdx.x * a.groups; r0 < a.rows; r0 += step) {
     const int64_t row = r0 + grp;
     const bool on = row < a.rows;
+    Row next;
+    if constexpr (kPrefetch) next = load(row + step);
+    else cur = load(row);
     float v[C][8];
     float s = 0.f;
 #pragma unroll
     for (int j = 0; j < C; ++j) {
-      norm_input<DT, FUSED>(a, key, row, t + j * TPR, nc, on ? valid[j] : 0, v[j]);
+      norm_input<DT, FUSED>(a, key, cur.in[j], row, t + j * tpr, nc, on ? valid[j] : 0, v[j]);
       if (valid[j] >= 8) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) s += v[j][e];
@@ -74,6 +108,7 @@ __global__ __launch_bounds__((RowGeom<TPR, C>::kThreads)) void k_norm_fwd(NormFw
 #pragma unroll
         for (int e = 0; e < 7; ++e) s += e < valid[j] ? v[j][e] : 0.f;
       }
+      if constexpr (FUSED) __builtin_amdgcn_sched_barrier(0);  // one chunk's generator state at a time
     }
     float mean = lanes_sum<L>(s) * rcnt, m2 = 0.f;
 #pragma unroll
@@ -87,25 +122,24 @@ __global__ __launch_bounds__((RowGeom<TPR, C>::kThreads)) void k_norm_fwd(NormFw
       }
     }
     m2 = lanes_sum<L>(m2);
-    if constexpr (G::kWaves > 1) {
-      if ((t & 63) == 0) {
-        red[slot][grp][wave][0] = mean;
-        red[slot][grp][wave][1] = m2;
+    if constexpr (LANES == 0) {
+      if ((threadIdx.x & 63) == 0) {
+        red[slot][wv][0] = mean;
+        red[slot][wv][1] = m2;
       }
-      __syncthreads();
+      lds_meet();  // (leaves the next row's loads in flight)
       float tm = 0.f;
-#pragma unroll
-      for (int k = 0; k < G::kWaves; ++k) tm = __builtin_fmaf(red[slot][grp][k][0], cnts[k], tm);
+      for (int k = 0; k < a.waves; ++k) tm = __builtin_fmaf(red[slot][w0 + k][0], cnts[w0 + k], tm);
       mean = tm * rn;
       m2 = 0.f;
-#pragma unroll
-      for (int k = 0; k < G::kWaves; ++k) {
-        const float d = red[slot][grp][k][0] - mean;
-        m2 += __builtin_fmaf(cnts[k] * d, d, red[slot][grp][k][1]);
+      for (int k = 0; k < a.waves; ++k) {
+        const float d = red[slot][w0 + k][0] - mean;
+        m2 += __builtin_fmaf(cnts[w0 + k] * d, d, red[slot][w0 + k][1]);
       }
       slot ^= 1;  // the next row's parts; this slot is written again only after its barrier
     }
     const float rstd = 1.f / sqrtf(__builtin_fmaf(m2, rn, a.eps));
+    if constexpr (kPrefetch) cur = next;
     if (!on) continue;
     if (t == 0) {
       a.mean[row] = mean;
@@ -116,7 +150,7 @@ __global__ __launch_bounds__((RowGeom<TPR, C>::kThreads)) void k_norm_fwd(NormFw
       float o[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) o[e] = __builtin_fmaf((v[j][e] - mean) * rstd, wt[j][e], bs[j][e]);
-      st_chunk<DT>(a.y + (row * a.ldy + 8 * (int64_t)(t + j * TPR)) * ES, narrow<DT>(o), valid[j]);
+      st_chunk<DT>(a.y + row * a.ldy * ES + 8u * ES * (uint32_t)(t + j * tpr), narrow<DT>(o), valid[j]);
     }
   }
 }
@@ -148,7 +182,7 @@ __global__ __launch_bounds__(1024) void k_norm_fwd_wide(NormFwd a) {
     float v[8], s = 0.f;
     for (int c = threadIdx.x; c < nc; c += 1024) {
       const int k = min(8, n - 8 * c);
-      norm_input<DT, FUSED>(a, key, row, c, nc, k, v);
+      norm_input<DT, FUSED>(a, key, ld_input<DT, FUSED>(a, row, c, k), row, c, nc, k, v);
 #pragma unroll
       for (int e = 0; e < 8; ++e) s += e < k ? v[e] : 0.f;
     }
@@ -181,17 +215,21 @@ __global__ __launch_bounds__(1024) void k_norm_fwd_wide(NormFwd a) {
 }
 
 template <int DT, bool FUSED>
-static int norm_fwd(const NormFwd& a, hipStream_t s) {
+static int norm_fwd(NormFwd a, hipStream_t s) {
   const int cus = cu_count();
   if (a.n > kNormMaxWidth)
     return launch((k_norm_fwd_wide<DT, FUSED>), dim3((unsigned)std::min<int64_t>(a.rows, 2 * cus)), dim3(1024), 0, s, a);
-  return with_row_geom((a.n + 7) / 8, [&](auto tpr, auto c) {
-    using G = RowGeom<tpr(), c()>;
-    // as many workgroups as run at once (8 waves per SIMD), each walking rows with the weights held
-    const int64_t most = (int64_t)cus * (2048 / G::kThreads);
-    const int64_t grid = std::min<int64_t>((a.rows + G::kGroups - 1) / G::kGroups, most);
-    return launch((k_norm_fwd<DT, tpr(), c(), FUSED>), dim3((unsigned)grid), dim3(G::kThreads), 0, s, a);
-  });
+  const RowShape r = row_shape(a.n, 64, 2);
+  a.waves = r.waves;
+  a.groups = row_groups(r, a.rows, 16);
+  const int threads = std::max(64, (r.lanes ? r.lanes : 64 * r.waves) * a.groups);
+  // as many workgroups as run at once (4 waves per SIMD), each walking rows with the weights held
+  const int64_t grid = std::min<int64_t>((a.rows + a.groups - 1) / a.groups, (int64_t)cus * (1024 / threads));
+  const auto go = [&](auto kern) { return launch(kern, dim3((unsigned)grid), dim3(threads), 0, s, a); };
+  if (r.lanes == 16) return go(k_norm_fwd<DT, 16, 1, FUSED>);
+  if (r.lanes == 64 && r.chunks == 1) return go(k_norm_fwd<DT, 64, 1, FUSED>);
+  if (r.lanes == 64) return go(k_norm_fwd<DT, 64, 2, FUSED>);
+  return go(k_norm_fwd<DT, 0, 2, FUSED>);
 }
 
 }  // namespace lrq
@@ -215,7 +253,7 @@ extern "C" int lrq_layer_norm_fwd(const lrq_dropout* drop, const void* x, int64_
       !aligned(b, ws) || !aligned(mean, 4) || !aligned(rstd, 4))
     return LRQ_ERR_ALIGN;
   const NormFwd a{(const char*)x, ldx, (const char*)residual, ld_residual, (char*)h, ldh, (char*)y, ldy, mean, rstd, w, b,
-                  w_dtype, rows, (int)n, eps, make_drop(drop)};
+                  w_dtype, rows, (int)n, 0, 0, eps, make_drop(drop)};
   hipStream_t s = (hipStream_t)stream;
   switch (dtype) {
     case LRQ_BF16: return fused ? norm_fwd<kBf16, true>(a, s) : norm_fwd<kBf16, false>(a, s);
