@@ -27,9 +27,9 @@ __device__ __forceinline__ void norm_outputs(const NormBwd& a, const DropKey& ke
 // k_norm_wgrad adds the workgroups' sums in a fixed order.  Rows are held as stored between the two uses, with the next
 // row's already on the way: sixteen waves a CU in 128 registers, and few workgroups, whose sums are few.
 template <int DT, int LANES, int C, bool FUSED>
-__global__ __launch_bounds__(C > 1 ? 512 : 1024) void k_norm_bwd(NormBwd a) {
+__global__ __launch_bounds__(C == 4 ? 512 : 1024) void k_norm_bwd(NormBwd a) {
   constexpr int ES = Elem<DT>::kBytes, L = LANES == 16 ? 16 : 64;
-  constexpr bool kPrefetch = C == 1;  // (four chunks a thread leave no registers for a second row)
+  constexpr bool kPrefetch = C == 1;  // (more leave no registers for a second row)
   __shared__ float red[2][16][2];
   extern __shared__ float sums[];  // [groups][threads of a row * 8 C], with weight gradients only
   const int tpr = LANES ? LANES : 64 * a.waves, kCols = tpr * 8 * C;
@@ -114,9 +114,11 @@ __global__ __launch_bounds__(C > 1 ? 512 : 1024) void k_norm_bwd(NormBwd a) {
 #pragma unroll
       for (int j = 0; j < C; ++j) {
         float g[8], z[8];
-        // widened again: kept from above, the fp32 values would take twice the registers
+        if constexpr (C > 1) {
+          // widened again: kept from above, the fp32 values would take twice the registers
 #pragma unroll
-        for (int k = 0; k < Elem<DT>::kVecs; ++k) pin(cur.dy[j].v[k]), pin(cur.h[j].v[k]);
+          for (int k = 0; k < Elem<DT>::kVecs; ++k) pin(cur.dy[j].v[k]), pin(cur.h[j].v[k]);
+        }
         widen<DT>(cur.dy[j], g);
         widen<DT>(cur.h[j], z);
 #pragma unroll
@@ -263,7 +265,7 @@ static BwdPlan bwd_plan(int64_t rows, int64_t n) {
     p.parts = std::min<int64_t>((rows + 3) / 4, 64);
     return p;
   }
-  p.groups = row_groups(p.shape, rows, p.shape.chunks == 1 ? 16 : 8);
+  p.groups = row_groups(p.shape, rows, p.shape.chunks == 4 ? 8 : 16);
   p.grid = p.parts = std::min<int64_t>((rows + p.groups - 1) / p.groups, kCus);
   return p;
 }
