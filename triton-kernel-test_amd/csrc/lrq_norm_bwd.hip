@@ -3,16 +3,22 @@
 
 namespace lrq {
 
-// dresidual and dx of one chunk from the norm's input gradient dn.
+// A chunk of dh (zeros without one).
+template <int DT>
+__device__ __forceinline__ Chunk<DT> ld_dh(const NormBwd& a, int64_t row, int c, int k) {
+  return ld_chunk<DT>(a.dh + row * a.lddh * Elem<DT>::kBytes + 8u * Elem<DT>::kBytes * (uint32_t)c, a.dh != nullptr ? k : 0);
+}
+
+// dresidual and dx of one chunk from the norm's input gradient dn and dh.
 template <int DT, bool FUSED>
 __device__ __forceinline__ void norm_outputs(const NormBwd& a, const DropKey& key, int64_t row, int c, int nc, int k,
-                                             float* d) {
+                                             float* d, const Chunk<DT>& dh) {
   constexpr int ES = Elem<DT>::kBytes;
   if (k <= 0) return;
   if constexpr (FUSED) {
     if (a.dh != nullptr) {
       float q[8];
-      widen<DT>(ld_chunk<DT>(a.dh + row * a.lddh * ES + 8u * ES * (uint32_t)c, k), q);
+      widen<DT>(dh, q);
 #pragma unroll
       for (int e = 0; e < 8; ++e) d[e] = q[e] + d[e];
     }
@@ -38,14 +44,26 @@ __global__ __launch_bounds__(C == 4 ? 512 : 1024) void k_norm_bwd(NormBwd a) {
   const int n = a.n, nc = (n + 7) / 8;
   const float rn = 1.f / (float)n;
   int valid[C];
-  float wt[C][8], gw[C][8], gb[C][8];
+  float gw[C][8], gb[C][8];
 #pragma unroll
   for (int j = 0; j < C; ++j) {
     const int c = t + j * tpr;
     valid[j] = c < nc ? min(8, n - 8 * c) : 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) wt[j][e] = 1.f, gw[j][e] = 0.f, gb[j][e] = 0.f;
-    if (a.w != nullptr) ld_weight(a.w, a.wdt, 8 * (int64_t)c, valid[j], wt[j]);
+    for (int e = 0; e < 8; ++e) gw[j][e] = 0.f, gb[j][e] = 0.f;
+  }
+  // the weights of a thread's columns: held over the rows, or (four chunks a thread and the generator) read again for
+  // each use
+  constexpr bool kHold = C == 1 || !FUSED;
+  const auto weights = [&](int j, float* w) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = 1.f;
+    if (a.w != nullptr) ld_weight(a.w, a.wdt, 8 * (int64_t)(t + j * tpr), valid[j], w);
+  };
+  float wt[kHold ? C : 1][8];
+  if constexpr (kHold) {
+#pragma unroll
+    for (int j = 0; j < C; ++j) weights(j, wt[j]);
   }
   DropKey key{};
   if constexpr (FUSED) key = drop_key(a.drop);
@@ -55,42 +73,51 @@ __global__ __launch_bounds__(C == 4 ? 512 : 1024) void k_norm_bwd(NormBwd a) {
   };
   // a group past the last row works on zeros; elements past the row are zero in dy, so they add nothing to any sum (z is
   // finite there for finite statistics; a row whose statistics are not finite is lost anyway)
+  int slot = 0;
+  const int64_t step = (int64_t)gridDim.x * a.groups, row0 = (int64_t)blockIdx.x * a.groups + grp;
+  // the row to load, stepped along (with four chunks a thread computed instead: no registers to spare)
+  const char *pdy = a.dy + row0 * a.lddy * ES, *ph = a.h + row0 * a.ldh * ES;
+  const int64_t idy = step * a.lddy * ES, ih = step * a.ldh * ES;
   const auto load = [&](int64_t row) {
     Row r;
     const bool on = row < a.rows;
     r.mean = on ? a.mean[row] : 0.f;
     r.rstd = on ? a.rstd[row] : 0.f;
+    if constexpr (C > 1) pdy = a.dy + row * a.lddy * ES, ph = a.h + row * a.ldh * ES;
 #pragma unroll
     for (int j = 0; j < C; ++j) {
       const uint32_t at = 8u * ES * (uint32_t)(t + j * tpr);
-      r.dy[j] = ld_chunk<DT>(a.dy + row * a.lddy * ES + at, on ? valid[j] : 0);
-      r.h[j] = ld_chunk<DT>(a.h + row * a.ldh * ES + at, on ? valid[j] : 0);
+      r.dy[j] = ld_chunk<DT>(pdy + at, on ? valid[j] : 0);
+      r.h[j] = ld_chunk<DT>(ph + at, on ? valid[j] : 0);
     }
+    if constexpr (C == 1) pdy += idy, ph += ih;
     return r;
   };
-  int slot = 0;
-  const int64_t step = (int64_t)gridDim.x * a.groups;
   Row cur;
-  if constexpr (kPrefetch) cur = load((int64_t)blockIdx.x * a.groups + grp);
+  if constexpr (kPrefetch) cur = load(row0);
   for (int64_t r0 = (int64_t)blockIdx.x * a.groups; r0 < a.rows; r0 += step) {
     const int64_t row = r0 + grp;
+    const bool on = row < a.rows;
     Row next;
     if constexpr (kPrefetch) next = load(row + step);
     else cur = load(row);
     float s1 = 0.f, s2 = 0.f;
+    float ge[C == 1 ? 8 : 1], ze[C == 1 ? 8 : 1];  // dy w and z, kept for the output where registers allow
 #pragma unroll
     for (int j = 0; j < C; ++j) {
       float g[8], z[8];
+      const int jw = kHold ? j : 0;
+      if constexpr (!kHold) weights(j, wt[0]);
       widen<DT>(cur.dy[j], g);
       widen<DT>(cur.h[j], z);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float ze = (z[e] - cur.mean) * cur.rstd;
-        gw[j][e] = __builtin_fmaf(g[e], ze, gw[j][e]);
+        const float zz = (z[e] - cur.mean) * cur.rstd, gg = g[e] * wt[jw][e];
+        gw[j][e] = __builtin_fmaf(g[e], zz, gw[j][e]);
         gb[j][e] += g[e];
-        const float ge = g[e] * wt[j][e];
-        s1 += ge;
-        s2 = __builtin_fmaf(ge, ze, s2);
+        s1 += gg;
+        s2 = __builtin_fmaf(gg, zz, s2);
+        if constexpr (C == 1) ge[e] = gg, ze[e] = zz;
       }
       if constexpr (C > 1) __builtin_amdgcn_sched_barrier(0);
     }
@@ -102,29 +129,36 @@ __global__ __launch_bounds__(C == 4 ? 512 : 1024) void k_norm_bwd(NormBwd a) {
         red[slot][wv][1] = s2;
       }
       lds_meet();  // (leaves the next row's loads in flight)
-      s1 = 0.f, s2 = 0.f;
-      for (int k = 0; k < a.waves; ++k) {
-        s1 += red[slot][w0 + k][0];
-        s2 += red[slot][w0 + k][1];
-      }
+      const int k = threadIdx.x & 15;  // each 16 lanes add the waves' sums
+      s1 = lanes_sum<16>(k < a.waves ? red[slot][w0 + k][0] : 0.f);
+      s2 = lanes_sum<16>(k < a.waves ? red[slot][w0 + k][1] : 0.f);
       slot ^= 1;  // this slot is written again only after the next row's barrier
     }
-    s1 *= rn, s2 *= rn;
-    if (row < a.rows) {
+    if (on) {
+      const float c1 = cur.rstd * (s1 * rn), c2 = -cur.rstd * (s2 * rn);
 #pragma unroll
       for (int j = 0; j < C; ++j) {
         float g[8], z[8];
-        if constexpr (C > 1) {
+        if constexpr (C == 1) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) g[e] = ge[e], z[e] = ze[e];
+        } else {
           // widened again: kept from above, the fp32 values would take twice the registers
 #pragma unroll
           for (int k = 0; k < Elem<DT>::kVecs; ++k) pin(cur.dy[j].v[k]), pin(cur.h[j].v[k]);
-        }
-        widen<DT>(cur.dy[j], g);
-        widen<DT>(cur.h[j], z);
+          const int jw = kHold ? j : 0;
+          if constexpr (!kHold) weights(j, wt[0]);
+          widen<DT>(cur.dy[j], g);
+          widen<DT>(cur.h[j], z);
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          g[e] = cur.rstd * (g[e] * wt[j][e] - s1 - (z[e] - cur.mean) * cur.rstd * s2);
-        norm_outputs<DT, FUSED>(a, key, row, t + j * tpr, nc, valid[j], g);
+          for (int e = 0; e < 8; ++e) g[e] *= wt[jw][e], z[e] = (z[e] - cur.mean) * cur.rstd;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) g[e] = __builtin_fmaf(z[e], c2, __builtin_fmaf(g[e], cur.rstd, -c1));
+        // asked for here: asked for ahead of the sums it holds up the rows in flight ([16384, 4096]: 127 against 143 us)
+        Chunk<DT> dh;
+        if constexpr (FUSED) dh = ld_dh<DT>(a, row, t + j * tpr, valid[j]);
+        norm_outputs<DT, FUSED>(a, key, row, t + j * tpr, nc, valid[j], g, dh);
         if constexpr (C > 1) __builtin_amdgcn_sched_barrier(0);  // one chunk's temporaries at a time
       }
     }
@@ -189,7 +223,9 @@ __global__ __launch_bounds__(1024) void k_norm_bwd_wide(NormBwd a) {
       load(c, k);
 #pragma unroll
       for (int e = 0; e < 8; ++e) g[e] = rstd * (g[e] - s1 - z[e] * s2);
-      norm_outputs<DT, FUSED>(a, key, row, c, nc, k, g);
+      Chunk<DT> dh;
+      if constexpr (FUSED) dh = ld_dh<DT>(a, row, c, k);
+      norm_outputs<DT, FUSED>(a, key, row, c, nc, k, g, dh);
     }
   }
 }
@@ -256,11 +292,14 @@ struct BwdPlan {
   int64_t parts;  // sums of the weight gradients
 };
 
-static BwdPlan bwd_plan(int64_t rows, int64_t n) {
+// Rows the register-resident kernel takes: four fp32 chunks a thread do not fit.
+static bool bwd_wide(int64_t n, int dt) { return n > (dt == kF32 ? 8192 : kNormMaxWidth); }
+
+static BwdPlan bwd_plan(int64_t rows, int64_t n, int dt) {
   constexpr int kCus = 256;  // a fixed count, so that the workspace and the order of the sums depend on the shape alone
   // one chunk a thread as far as 16 waves go (each has 16 sums besides), else four in half as many waves
   BwdPlan p{row_shape(n, 1024, 4), 1, 0, 0};
-  if (n > kNormMaxWidth) {
+  if (bwd_wide(n, dt)) {
     p.grid = std::min<int64_t>(rows, 2 * kCus);
     p.parts = std::min<int64_t>((rows + 3) / 4, 64);
     return p;
@@ -272,8 +311,8 @@ static BwdPlan bwd_plan(int64_t rows, int64_t n) {
 
 template <int DT, bool FUSED>
 static int norm_bwd(NormBwd a, hipStream_t s) {
-  const BwdPlan p = bwd_plan(a.rows, a.n);
-  if (a.n > kNormMaxWidth) {
+  const BwdPlan p = bwd_plan(a.rows, a.n, DT);
+  if (bwd_wide(a.n, DT)) {
     if (a.part != nullptr)
       LRQ_TRY(launch((k_norm_cols<DT>), dim3((unsigned)((a.n + 511) / 512), (unsigned)p.parts), dim3(256), 0, s, a));
     return launch((k_norm_bwd_wide<DT, FUSED>), dim3((unsigned)p.grid), dim3(1024), 0, s, a);
@@ -292,7 +331,8 @@ static int norm_bwd(NormBwd a, hipStream_t s) {
   if (p.shape.lanes == 16) return go(k_norm_bwd<DT, 16, 1, FUSED>);
   if (p.shape.lanes == 64) return go(k_norm_bwd<DT, 64, 1, FUSED>);
   if (p.shape.chunks == 1) return go(k_norm_bwd<DT, 0, 1, FUSED>);
-  return go(k_norm_bwd<DT, 0, 4, FUSED>);
+  if constexpr (DT != kF32) return go(k_norm_bwd<DT, 0, 4, FUSED>);
+  return LRQ_ERR_UNSUPPORTED;  // (not reached: wide)
 }
 
 }  // namespace lrq
@@ -301,7 +341,7 @@ using namespace lrq;
 
 extern "C" int64_t lrq_layer_norm_bwd_workspace(int64_t rows, int64_t n) {
   if (rows < 0 || rows > INT32_MAX || n <= 0 || n > INT32_MAX / 2) return LRQ_ERR_SHAPE;
-  return bwd_plan(rows, n).parts * 2 * n * (int64_t)sizeof(float);
+  return std::max(bwd_plan(rows, n, kBf16).parts, bwd_plan(rows, n, kF32).parts) * 2 * n * (int64_t)sizeof(float);
 }
 
 extern "C" int lrq_layer_norm_bwd(const lrq_dropout* drop, const void* dy, int64_t lddy, const void* dh, int64_t lddh,
@@ -347,7 +387,7 @@ extern "C" int lrq_layer_norm_bwd(const lrq_dropout* drop, const void* dy, int64
     LRQ_TRY(go());
   }
   if (!wgrad) return LRQ_OK;
-  const int parts = rows > 0 ? (int)bwd_plan(rows, n).parts : 0;  // no rows: zeros
+  const int parts = rows > 0 ? (int)bwd_plan(rows, n, dtype).parts : 0;  // no rows: zeros
   return launch(k_norm_wgrad, dim3((unsigned)((n + 63) / 64), 2), dim3(1024), 0, s, (const float*)workspace, parts, (int)n,
                 dw, db, w_dtype);
 }

@@ -46,7 +46,7 @@ __device__ __forceinline__ void norm_input(const NormFwd& a, const DropKey& key,
 // One pass: a row's chunks are read once.  Each wave reduces its part of the row to (mean, sum of
 // squared deviations from it) and the waves' parts are merged (Chan, Golub and LeVeque's update), so a
 // row costs one barrier and the variance never comes from a difference of large sums.
-template <int DT, int LANES, int C, bool FUSED>
+template <int DT, int LANES, int C, bool FUSED, bool SAME>
 __global__ __launch_bounds__(1024) void k_norm_fwd(NormFwd a) {
   constexpr int ES = Elem<DT>::kBytes, L = LANES == 16 ? 16 : 64;
   __shared__ float red[2][16][2], cnts[16];
@@ -55,17 +55,31 @@ __global__ __launch_bounds__(1024) void k_norm_fwd(NormFwd a) {
   const int wv = threadIdx.x >> 6, w0 = LANES ? 0 : grp * a.waves;  // this wave, its row's first
   const int n = a.n, nc = (n + 7) / 8;
   int valid[C];
-  float wt[C][8], bs[C][8];
   float cnt = 0.f;
 #pragma unroll
   for (int j = 0; j < C; ++j) {
     const int c = t + j * tpr;
     valid[j] = c < nc ? min(8, n - 8 * c) : 0;
     cnt += (float)valid[j];
+  }
+  // The weights of a thread's columns, held over the rows: widened, or with dropout and the residual, which leave fewer
+  // registers, as stored if both are there in x's type (SAME) and else read again for each row.
+  constexpr bool kWide = !FUSED || C == 1, kRaw = !kWide && SAME;
+  const auto weights = [&](int j, float* w, float* b) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) wt[j][e] = 1.f, bs[j][e] = 0.f;
-    if (a.w != nullptr) ld_weight(a.w, a.wdt, 8 * (int64_t)c, valid[j], wt[j]);
-    if (a.b != nullptr) ld_weight(a.b, a.wdt, 8 * (int64_t)c, valid[j], bs[j]);
+    for (int e = 0; e < 8; ++e) w[e] = 1.f, b[e] = 0.f;
+    if (a.w != nullptr) ld_weight(a.w, a.wdt, 8 * (int64_t)(t + j * tpr), valid[j], w);
+    if (a.b != nullptr) ld_weight(a.b, a.wdt, 8 * (int64_t)(t + j * tpr), valid[j], b);
+  };
+  float wt[kWide ? C : 1][8], bs[kWide ? C : 1][8];
+  Chunk<DT> wr[kRaw ? C : 1], br[kRaw ? C : 1];
+#pragma unroll
+  for (int j = 0; j < C; ++j) {
+    if constexpr (kWide) weights(j, wt[j], bs[j]);
+    if constexpr (kRaw) {
+      wr[j] = ld_chunk<DT>((const char*)a.w + 8 * ES * (t + j * tpr), valid[j]);
+      br[j] = ld_chunk<DT>((const char*)a.b + 8 * ES * (t + j * tpr), valid[j]);
+    }
   }
   cnt = lanes_sum<L>(cnt);  // this wave's columns of a row
   const float rcnt = cnt > 0.f ? 1.f / cnt : 0.f, rn = 1.f / (float)n;
@@ -85,7 +99,7 @@ __global__ __launch_bounds__(1024) void k_norm_fwd(NormFwd a) {
     return r;
   };
   const int64_t step = (int64_t)gridDim.x * a.groups;
-  constexpr bool kPrefetch = C == 1 || !FUSED || (DT != kF32 && LANES == 0);  // (two rows of two inputs: too many registers)
+  constexpr bool kPrefetch = C == 1 || !FUSED || DT != kF32;  // (two fp32 rows of two inputs: too many registers)
   Row cur;
   if constexpr (kPrefetch) cur = load((int64_t)blockIdx.x * a.groups + grp);
   // Every thread takes every step (barriers): a group past the last row works on zeros.  The next row is on its way
@@ -128,14 +142,12 @@ __global__ __launch_bounds__(1024) void k_norm_fwd(NormFwd a) {
         red[slot][wv][1] = m2;
       }
       lds_meet();  // (leaves the next row's loads in flight)
-      float tm = 0.f;
-      for (int k = 0; k < a.waves; ++k) tm = __builtin_fmaf(red[slot][w0 + k][0], cnts[w0 + k], tm);
-      mean = tm * rn;
-      m2 = 0.f;
-      for (int k = 0; k < a.waves; ++k) {
-        const float d = red[slot][w0 + k][0] - mean;
-        m2 += __builtin_fmaf(cnts[w0 + k] * d, d, red[slot][w0 + k][1]);
-      }
+      const int k = threadIdx.x & 15;  // each 16 lanes merge the waves' parts
+      const bool has = k < a.waves;
+      const float pm = has ? red[slot][w0 + k][0] : 0.f, p2 = has ? red[slot][w0 + k][1] : 0.f;
+      const float pc = has ? cnts[w0 + k] : 0.f;
+      mean = lanes_sum<16>(pm * pc) * rn;
+      m2 = lanes_sum<16>(__builtin_fmaf(pc * (pm - mean), pm - mean, p2));
       slot ^= 1;  // the next row's parts; this slot is written again only after its barrier
     }
     const float rstd = 1.f / sqrtf(__builtin_fmaf(m2, rn, a.eps));
@@ -147,9 +159,18 @@ __global__ __launch_bounds__(1024) void k_norm_fwd(NormFwd a) {
     }
 #pragma unroll
     for (int j = 0; j < C; ++j) {
+      const int k = kWide ? j : 0;
+      if constexpr (kRaw) {
+#pragma unroll
+        for (int q = 0; q < Elem<DT>::kVecs; ++q) pin(wr[j].v[q]), pin(br[j].v[q]);
+        widen<DT>(wr[j], wt[0]);
+        widen<DT>(br[j], bs[0]);
+      } else if constexpr (!kWide) {
+        weights(j, wt[0], bs[0]);
+      }
       float o[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) o[e] = __builtin_fmaf((v[j][e] - mean) * rstd, wt[j][e], bs[j][e]);
+      for (int e = 0; e < 8; ++e) o[e] = __builtin_fmaf((v[j][e] - mean) * rstd, wt[k][e], bs[k][e]);
       st_chunk<DT>(a.y + row * a.ldy * ES + 8u * ES * (uint32_t)(t + j * tpr), narrow<DT>(o), valid[j]);
     }
   }
@@ -226,10 +247,11 @@ static int norm_fwd(NormFwd a, hipStream_t s) {
   // as many workgroups as run at once (4 waves per SIMD), each walking rows with the weights held
   const int64_t grid = std::min<int64_t>((a.rows + a.groups - 1) / a.groups, (int64_t)cus * (1024 / threads));
   const auto go = [&](auto kern) { return launch(kern, dim3((unsigned)grid), dim3(threads), 0, s, a); };
-  if (r.lanes == 16) return go(k_norm_fwd<DT, 16, 1, FUSED>);
-  if (r.lanes == 64 && r.chunks == 1) return go(k_norm_fwd<DT, 64, 1, FUSED>);
-  if (r.lanes == 64) return go(k_norm_fwd<DT, 64, 2, FUSED>);
-  return go(k_norm_fwd<DT, 0, 2, FUSED>);
+  if (r.lanes == 16) return go(k_norm_fwd<DT, 16, 1, FUSED, false>);
+  if (r.lanes == 64 && r.chunks == 1) return go(k_norm_fwd<DT, 64, 1, FUSED, false>);
+  const bool same = FUSED && a.wdt == DT && a.w != nullptr && a.b != nullptr;
+  if (r.lanes == 64) return same ? go(k_norm_fwd<DT, 64, 2, FUSED, FUSED>) : go(k_norm_fwd<DT, 64, 2, FUSED, false>);
+  return same ? go(k_norm_fwd<DT, 0, 2, FUSED, FUSED>) : go(k_norm_fwd<DT, 0, 2, FUSED, false>);
 }
 
 }  // namespace lrq
