@@ -312,7 +312,7 @@ struct TileArgs {
 //   of 8 rows at once; each is widened with its own row's scale and the halves of two rows are paired by v_perm_b32.
 template <bool TRANS, int MT>
 struct TileLds {
-  static constexpr int kA = 32 * MT * 256, kB = 16384, kS = TRANS ? 2048 : 0, kStage = kA + kB + kS, kDeep = 3;
+  static constexpr int kA = 32 * MT * 256, kB = 16384, kS = TRANS ? 3072 : 0, kStage = kA + kB + kS, kDeep = 3;
   static constexpr int kScales = TRANS ? 0 : 4096, kLoop = kDeep * kStage + 2 * kScales;
   static constexpr int kJoin = (MT >= 2 ? 8 * MT / 2 : 4) * 8192, kBytes = kLoop > kJoin ? kLoop : kJoin;
 };
@@ -415,11 +415,13 @@ __global__ __launch_bounds__(512) void k_mx_tile(TileArgs a) {
     }
     char* st = sm + buf * kStage;
     if constexpr (TRANS) {
-      // the scales arrive as [row][8]; this thread's dword goes to [block][row]
+      // the scales arrive as [row][8]; this thread's four go to [block][row] as bf16, so that half of them are a
+      // conversion's scale operand as read
       if (wave < 4) {
         const uint32_t s4 = ld4(st + kA + kB + 4 * threadIdx.x);
+        uint16_t* to = (uint16_t*)(st + kA + kB + 1024) + 512 * (lane & 1) + rs;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) st[kA + kB + 1024 + (4 * (lane & 1) + k) * 128 + rs] = (char)(s4 >> (8 * k));
+        for (int k = 0; k < 4; ++k) to[128 * k] = (uint16_t)((s4 >> (8 * k) & 255u) << 7);
       }
     }
     lds_meet();  // every wave's loads are in, and the buffer of the step before is free
@@ -429,7 +431,8 @@ __global__ __launch_bounds__(512) void k_mx_tile(TileArgs a) {
     }
     u32x4 code[2];
     float scale[2];
-    u32x2 cols[4], rows8[4];  // TRANS: this lane's code byte and scale byte of 8 rows, for each instruction
+    u32x2 cols[4];            // TRANS: this lane's code byte of 8 rows, for each instruction
+    u32x4 rows8[4];           // and the rows' scales
     if constexpr (TRANS) {
       const int r0 = 64 * gq + 32 * h, blk = 2 * wn + (lane >> 4 & 1), r = r0 + (lane >> 1 & 7);
       // by hand, with its wait: for the builtin the compiler first drains the loads to LDS just issued
@@ -442,7 +445,7 @@ __global__ __launch_bounds__(512) void k_mx_tile(TileArgs a) {
                    : "v"(p)
                    : "memory");
 #pragma unroll
-      for (int s = 0; s < 4; ++s) rows8[s] = ld8(st + kA + kB + 1024 + 128 * blk + r0 + 8 * s);
+      for (int s = 0; s < 4; ++s) rows8[s] = ld16(st + kA + kB + 1024 + 2 * (128 * blk + r0 + 8 * s));
     }
     if constexpr (!TRANS) {
 #pragma unroll
@@ -463,11 +466,11 @@ __global__ __launch_bounds__(512) void k_mx_tile(TileArgs a) {
         uint32_t e[8];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {  // the conversion reads the exponent field alone
-          const uint32_t cw = cols[s][i], sw = rows8[s][i];
-          e[4 * i + 0] = fp4_to_bf16x2<0>(cw, __uint_as_float(sw << 23));
-          e[4 * i + 1] = fp4_to_bf16x2<1>(cw, __uint_as_float(sw << 15));
-          e[4 * i + 2] = fp4_to_bf16x2<2>(cw, __uint_as_float(sw << 7));
-          e[4 * i + 3] = fp4_to_bf16x2<3>(cw, __uint_as_float(sw >> 1));
+          const uint32_t cw = cols[s][i], s01 = rows8[s][2 * i], s23 = rows8[s][2 * i + 1];
+          e[4 * i + 0] = fp4_to_bf16x2<0>(cw, __uint_as_float(s01 << 16));
+          e[4 * i + 1] = fp4_to_bf16x2<1>(cw, __uint_as_float(s01));
+          e[4 * i + 2] = fp4_to_bf16x2<2>(cw, __uint_as_float(s23 << 16));
+          e[4 * i + 3] = fp4_to_bf16x2<3>(cw, __uint_as_float(s23));
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
