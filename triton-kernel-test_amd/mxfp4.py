@@ -60,15 +60,15 @@ class MXFP4Tensor:
             raise ValueError("an MXFP4 tensor needs rows of at least one element")
         rows = shape[0] if len(shape) == 2 else math.prod(shape[:-1])
         steps = (cols + 127) // 128
-        for t, name, width in ((c, "codes", 64 * steps), (s, "scales", 4 * steps)):
-            if t.dtype is not torch.uint8 or t.dim() != 2 or t.shape[0] != rows or t.shape[1] < width or t.device != c.device:
-                raise ValueError(f"{name} must be uint8 [{rows}, >= {width}] on one device, got {t.dtype} {tuple(t.shape)}")
-            if t.stride(1) != 1:
-                raise ValueError(f"{name} must have unit inner stride")
-        # the stride of a single row means nothing
-        if rows > 1:
-            return LrqMxfp4(c.data_ptr(), c.stride(0), s.data_ptr(), s.stride(0), rows, cols)
-        return LrqMxfp4(c.data_ptr(), 64 * steps, s.data_ptr(), 4 * steps, rows, cols)
+        if c.dim() == 2 and s.dim() == 2 and c.dtype is torch.uint8 and s.dtype is torch.uint8 and c.device == s.device:
+            (cr, cw), (sr, sw), (ldc, c1), (lds, s1) = c.shape, s.shape, c.stride(), s.stride()
+            if cr == rows and sr == rows and cw >= 64 * steps and sw >= 4 * steps and c1 == 1 and s1 == 1:
+                if rows <= 1:  # the stride of a single row means nothing
+                    ldc, lds = 64 * steps, 4 * steps
+                return LrqMxfp4(c.data_ptr(), ldc, s.data_ptr(), lds, rows, cols)
+        raise ValueError(f"codes and scales must be uint8 [{rows}, >= {64 * steps}] and [{rows}, >= {4 * steps}] with unit "
+                         f"inner stride on one device, got {c.dtype} {tuple(c.shape)} on {c.device} and {s.dtype} "
+                         f"{tuple(s.shape)} on {s.device}")
 
 
 def mxfp4_quantize(x: torch.Tensor) -> MXFP4Tensor:
@@ -79,11 +79,12 @@ def mxfp4_quantize(x: torch.Tensor) -> MXFP4Tensor:
     dt = _dtype(x, "x")
     x2, rows, n, ldx = _rows(x, "x")
     steps = (n + 127) // 128
-    q = MXFP4Tensor(torch.empty((rows, 64 * steps), dtype=torch.uint8, device=x.device),
-                    torch.empty((rows, 4 * steps), dtype=torch.uint8, device=x.device), tuple(x.shape))
+    codes = torch.empty((rows, 64 * steps), dtype=torch.uint8, device=x.device)
+    scales = torch.empty((rows, 4 * steps), dtype=torch.uint8, device=x.device)
+    t = LrqMxfp4(codes.data_ptr(), 64 * steps, scales.data_ptr(), 4 * steps, rows, n)
     with _on(x.device):
-        call("lrq_mxfp4_quantize", _p(x2), ldx, dt, ctypes.byref(q.descriptor()), _stream(x.device))
-    return q
+        call("lrq_mxfp4_quantize", _p(x2), ldx, dt, ctypes.byref(t), _stream(x.device))
+    return MXFP4Tensor(codes, scales, tuple(x.shape))
 
 
 def mxfp4_dequantize(q: MXFP4Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:

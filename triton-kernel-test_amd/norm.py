@@ -58,7 +58,7 @@ def _rows(x: torch.Tensor, name: str) -> tuple[torch.Tensor, int, int, int]:
 
 
 def _like(t: Optional[torch.Tensor], x: torch.Tensor, name: str) -> Optional[torch.Tensor]:
-    if t is not None and (t.shape != x.shape or t.dtype != x.dtype or t.device != x.device):
+    if t is not None and (t.shape != x.shape or t.dtype is not x.dtype or t.device != x.device):
         raise ValueError(f"{name} must be {x.dtype} {tuple(x.shape)} on {x.device}, got {t.dtype} {tuple(t.shape)} "
                          f"on {t.device}")
     return t
@@ -69,22 +69,27 @@ def _new(x: torch.Tensor) -> torch.Tensor:
     return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
 
 
-def _weights(weight, bias, x: torch.Tensor):
-    n = x.shape[-1]
+def _weights(weight, bias, n: int, device: torch.device):
+    """(weight, bias, their dtype) ready for the kernels."""
     for t, name in ((weight, "weight"), (bias, "bias")):
-        if t is not None and (tuple(t.shape) != (n,) or t.device != x.device):
-            raise ValueError(f"{name} must be [{n}] on {x.device}, got {tuple(t.shape)} on {t.device}")
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise ValueError("weight and bias must have one dtype")
-    some = weight if weight is not None else bias
-    dt = _lib.LRQ_F32 if some is None else _dtype(some, "weight")
-    return (None if weight is None else weight.contiguous(), None if bias is None else bias.contiguous(), dt)
+        if t is not None and (t.dim() != 1 or t.shape[0] != n or t.device != device):
+            raise ValueError(f"{name} must be [{n}] on {device}, got {tuple(t.shape)} on {t.device}")
+    if weight is None:
+        if bias is None:
+            return None, None, _lib.LRQ_F32
+        return None, bias.contiguous(), _dtype(bias, "bias")
+    if bias is not None:
+        if bias.dtype is not weight.dtype:
+            raise ValueError("weight and bias must have one dtype")
+        bias = bias.contiguous()
+    return weight.contiguous(), bias, _dtype(weight, "weight")
 
 
 def _statistics(mean: torch.Tensor, rstd: torch.Tensor, x: torch.Tensor):
+    lead, device = x.shape[:-1], x.device
     for t, name in ((mean, "mean"), (rstd, "rstd")):
-        if t.dtype != torch.float32 or t.shape != x.shape[:-1] or t.device != x.device:
-            raise ValueError(f"{name} must be fp32 {tuple(x.shape[:-1])} on {x.device}")
+        if t.dtype is not torch.float32 or t.shape != lead or t.device != device:
+            raise ValueError(f"{name} must be fp32 {tuple(lead)} on {device}")
     return mean.contiguous(), rstd.contiguous()
 
 
@@ -123,7 +128,7 @@ def layer_norm_forward(x: torch.Tensor, weight: Optional[torch.Tensor] = None, b
     _require_device(x, weight, bias)
     dt = _dtype(x, "x")
     x2, rows, n, ldx = _rows(x, "x")
-    w, b, wdt = _weights(weight, bias, x)
+    w, b, wdt = _weights(weight, bias, n, x.device)
     y = _new(x)
     mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
     rstd = torch.empty_like(mean)
@@ -137,9 +142,9 @@ def _backward(drop, dy, dh, h, weight, mean, rstd, weight_grad: bool, fused: boo
     dt = _dtype(h, "x")
     _like(dy, h, "dy")
     _like(dh, h, "dh")
-    w, _, wdt = _weights(weight, None, h)
     mean, rstd = _statistics(mean, rstd, h)
     dy2, rows, n, lddy = _rows(dy, "dy")
+    w, _, wdt = _weights(weight, None, n, h.device)
     h2, _, _, ldh = _rows(h, "x")
     dh2, lddh = (None, 0) if dh is None else _rows(dh, "dh")[::3]
     dx = _new(h) if want_dx else None
@@ -195,7 +200,7 @@ def dropout_add_layer_norm_forward(x: torch.Tensor, residual: Optional[torch.Ten
     _like(residual, x, "residual")
     x2, rows, n, ldx = _rows(x, "x")
     r2, ldr = (None, 0) if residual is None else _rows(residual, "residual")[::3]
-    w, b, wdt = _weights(weight, bias, x)
+    w, b, wdt = _weights(weight, bias, n, x.device)
     drop, _state = _drop(p, seed, x.device)
     y = _new(x)
     h = _new(x)
