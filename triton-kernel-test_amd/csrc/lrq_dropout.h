@@ -56,6 +56,8 @@ __device__ __forceinline__ uint32_t xor3(uint32_t a, uint32_t b, uint32_t c) {
 
 __device__ __forceinline__ u32x4 philox(uint64_t q, const DropKey& key) {
   uint32_t c0 = (uint32_t)q, c1 = (uint32_t)(q >> 32), c2 = key.c2, c3 = key.c3, k0 = key.k0, k1 = key.k1;
+  // opaque, or the rounds' twenty keys are kept in scalar registers over the caller's loop and crowd out its own values
+  asm volatile("" : "+s"(k0), "+s"(k1));
 #pragma unroll
   for (int r = 0; r < 10; ++r) {
     const uint64_t p0 = (uint64_t)c0 * 0xD2511F53u, p1 = (uint64_t)c2 * 0xCD9E8D57u;

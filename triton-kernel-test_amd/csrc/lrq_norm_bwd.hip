@@ -35,7 +35,8 @@ __device__ __forceinline__ void norm_outputs(const NormBwd& a, const DropKey& ke
 template <int DT, int LANES, int C, bool FUSED>
 __global__ __launch_bounds__(C == 4 ? 512 : 1024) void k_norm_bwd(NormBwd a) {
   constexpr int ES = Elem<DT>::kBytes, L = LANES == 16 ? 16 : 64;
-  constexpr bool kPrefetch = C == 1;  // (more leave no registers for a second row)
+  // (four chunks a thread, or fp32 rows and the generator, leave no registers for a second row or for what is kept)
+  constexpr bool kPrefetch = C == 1 && !(FUSED && DT == kF32), kKeep = kPrefetch;
   __shared__ float red[2][16][2];
   extern __shared__ float sums[];  // [groups][threads of a row * 8 C], with weight gradients only
   const int tpr = LANES ? LANES : 64 * a.waves, kCols = tpr * 8 * C;
@@ -102,7 +103,7 @@ __global__ __launch_bounds__(C == 4 ? 512 : 1024) void k_norm_bwd(NormBwd a) {
     if constexpr (kPrefetch) next = load(row + step);
     else cur = load(row);
     float s1 = 0.f, s2 = 0.f;
-    float ge[C == 1 ? 8 : 1], ze[C == 1 ? 8 : 1];  // dy w and z, kept for the output where registers allow
+    float ge[kKeep ? 8 : 1], ze[kKeep ? 8 : 1];  // dy w and z, kept for the output where registers allow
 #pragma unroll
     for (int j = 0; j < C; ++j) {
       float g[8], z[8];
@@ -117,7 +118,7 @@ __global__ __launch_bounds__(C == 4 ? 512 : 1024) void k_norm_bwd(NormBwd a) {
         gb[j][e] += g[e];
         s1 += gg;
         s2 = __builtin_fmaf(gg, zz, s2);
-        if constexpr (C == 1) ge[e] = gg, ze[e] = zz;
+        if constexpr (kKeep) ge[e] = gg, ze[e] = zz;
       }
       if constexpr (C > 1) __builtin_amdgcn_sched_barrier(0);
     }
@@ -139,7 +140,7 @@ __global__ __launch_bounds__(C == 4 ? 512 : 1024) void k_norm_bwd(NormBwd a) {
 #pragma unroll
       for (int j = 0; j < C; ++j) {
         float g[8], z[8];
-        if constexpr (C == 1) {
+        if constexpr (kKeep) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) g[e] = ge[e], z[e] = ze[e];
         } else {
