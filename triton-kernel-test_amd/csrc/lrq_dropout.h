@@ -71,14 +71,16 @@ __device__ __forceinline__ u32x4 philox(uint64_t q, const DropKey& key) {
   return u32x4{c0, c1, c2, c3};
 }
 
-// f[e] = kept ? f[e] * scale : 0 for the chunk q (a dropped NaN or infinity gives 0).
-__device__ __forceinline__ void drop_chunk(const Drop& d, const DropKey& key, uint64_t q, float* f) {
-  const u32x4 w = philox(q, key);
+// f[e] = kept ? f[e] * scale : 0 for a chunk with the block w (a dropped NaN or infinity gives 0).
+__device__ __forceinline__ void drop_words(const Drop& d, const u32x4& w, float* f) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const uint32_t u = (e & 1) ? w[e / 2] >> 16 : w[e / 2] & 0xffffu;
     f[e] = u < d.keep ? f[e] * d.scale : 0.f;
   }
+}
+__device__ __forceinline__ void drop_chunk(const Drop& d, const DropKey& key, uint64_t q, float* f) {
+  drop_words(d, philox(q, key), f);
 }
 
 }  // namespace lrq

@@ -9,10 +9,10 @@ __device__ __forceinline__ Chunk<DT> ld_dh(const NormBwd& a, int64_t row, int c,
   return ld_chunk<DT>(a.dh + row * a.lddh * Elem<DT>::kBytes + 8u * Elem<DT>::kBytes * (uint32_t)c, a.dh != nullptr ? k : 0);
 }
 
-// dresidual and dx of one chunk from the norm's input gradient dn and dh.
+// dresidual and dx of one chunk from the norm's input gradient dn, dh and the chunk's random numbers.
 template <int DT, bool FUSED>
-__device__ __forceinline__ void norm_outputs(const NormBwd& a, const DropKey& key, int64_t row, int c, int nc, int k,
-                                             float* d, const Chunk<DT>& dh) {
+__device__ __forceinline__ void norm_outputs(const NormBwd& a, int64_t row, int c, int k, float* d, const Chunk<DT>& dh,
+                                             const u32x4& words) {
   constexpr int ES = Elem<DT>::kBytes;
   if (k <= 0) return;
   if constexpr (FUSED) {
@@ -23,7 +23,7 @@ __device__ __forceinline__ void norm_outputs(const NormBwd& a, const DropKey& ke
       for (int e = 0; e < 8; ++e) d[e] = q[e] + d[e];
     }
     if (a.dres != nullptr) st_chunk<DT>(a.dres + row * a.lddr * ES + 8u * ES * (uint32_t)c, narrow<DT>(d), k);
-    if (a.drop.keep < 65536u) drop_chunk(a.drop, key, (uint64_t)row * nc + c, d);
+    if (a.drop.keep < 65536u) drop_words(a.drop, words, d);
   }
   if (!FUSED || a.dx != nullptr) st_chunk<DT>(a.dx + row * a.lddx * ES + 8u * ES * (uint32_t)c, narrow<DT>(d), k);
 }
@@ -102,6 +102,10 @@ __global__ __launch_bounds__(C == 4 ? 512 : 1024) void k_norm_bwd(NormBwd a) {
     Row next;
     if constexpr (kPrefetch) next = load(row + step);
     else cur = load(row);
+    u32x4 words{};  // drawn now, under the loads, with one chunk a thread
+    if constexpr (FUSED && C == 1) {
+      if (a.drop.keep < 65536u) words = philox((uint64_t)row * nc + t, key);
+    }
     float s1 = 0.f, s2 = 0.f;
     float ge[kKeep ? 8 : 1], ze[kKeep ? 8 : 1];  // dy w and z, kept for the output where registers allow
 #pragma unroll
@@ -159,7 +163,10 @@ __global__ __launch_bounds__(C == 4 ? 512 : 1024) void k_norm_bwd(NormBwd a) {
         // asked for here: asked for ahead of the sums it holds up the rows in flight ([16384, 4096]: 127 against 143 us)
         Chunk<DT> dh;
         if constexpr (FUSED) dh = ld_dh<DT>(a, row, t + j * tpr, valid[j]);
-        norm_outputs<DT, FUSED>(a, key, row, t + j * tpr, nc, valid[j], g, dh);
+        if constexpr (FUSED && C > 1) {
+          if (a.drop.keep < 65536u) words = philox((uint64_t)row * nc + t + j * tpr, key);
+        }
+        norm_outputs<DT, FUSED>(a, row, t + j * tpr, valid[j], g, dh, words);
         if constexpr (C > 1) __builtin_amdgcn_sched_barrier(0);  // one chunk's temporaries at a time
       }
     }
@@ -225,8 +232,12 @@ __global__ __launch_bounds__(1024) void k_norm_bwd_wide(NormBwd a) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) g[e] = rstd * (g[e] - s1 - z[e] * s2);
       Chunk<DT> dh;
-      if constexpr (FUSED) dh = ld_dh<DT>(a, row, c, k);
-      norm_outputs<DT, FUSED>(a, key, row, c, nc, k, g, dh);
+      u32x4 words{};
+      if constexpr (FUSED) {
+        dh = ld_dh<DT>(a, row, c, k);
+        if (a.drop.keep < 65536u) words = philox((uint64_t)row * nc + c, key);
+      }
+      norm_outputs<DT, FUSED>(a, row, c, k, g, dh, words);
     }
   }
 }
