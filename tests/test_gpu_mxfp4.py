@@ -119,6 +119,113 @@ def test_gemm(pkg, dev, m, n, k):
         R.assert_within(pkg.mxfp4_gemm(a, w, dt), ref, bound, f"{dt}")
 
 
+def _grid(shape, dev, seed, values=(0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)):
+    g = torch.Generator(device=dev).manual_seed(seed)
+    v = torch.tensor(values, device=dev)[torch.randint(len(values), shape, generator=g, device=dev)]
+    return v * (2 * torch.randint(2, shape, generator=g, device=dev) - 1).to(v.dtype)
+
+
+# (m, n, k, which product, whether the contraction is split over workgroups): each height of each kernel, both ways
+PLANS = [(100, 200, 72, "linear", False), (40, 100, 1200, "linear", True), (4100, 260, 72, "linear", False),
+         (2050, 100, 3300, "linear", True), (600, 6500, 72, "linear", False), (4100, 100, 13000, "linear", True),
+         (3, 40, 9000, "linear", False), (9, 8300, 300, "linear", False), (4, 8200, 1000, "linear", False),
+         (16, 300, 5000, "linear", False), (40, 100, 72, "back", False), (40, 1300, 72, "back", True),
+         (4100, 100, 300, "back", False), (2050, 4100, 72, "back", True), (2050, 100, 2000, "back", False),
+         (4100, 4100, 72, "back", True), (40, 100, 72, "gemm", False), (40, 100, 2000, "gemm", True),
+         (600, 6500, 72, "gemm", False), (4100, 100, 9000, "gemm", True), (2050, 4100, 72, "gemm", False),
+         (2048, 4096, 49152, "gemm", True)]
+
+
+@pytest.mark.parametrize("m,n,k,which,split", PLANS)
+def test_every_plan_is_exact_on_small_numbers(pkg, dev, m, n, k, which, split):
+    """Multiples of 1/2 (1/4 for two MXFP4 operands) whose sums stay below 2^22: fp32 holds every partial sum exactly in
+    any order, so the outputs are those of 64 bits, rounded once in bf16; a block left out or taken twice shows."""
+    import ctypes
+    L = importlib.import_module("triton-kernel-test_amd._lib")
+    print(f"[mx] plan {which} {m} {n} {k}", flush=True)
+    w = _grid((n, k), dev, 1)
+    wq = pkg.mxfp4_quantize(w)
+    assert torch.equal(pkg.mxfp4_dequantize(wq, torch.float32), w)
+    if which == "gemm":
+        x = _grid((m, k), dev, 2)
+        xq = pkg.mxfp4_quantize(x)
+        ref = x.double() @ w.double().T
+        run = lambda dt: pkg.mxfp4_gemm(xq, wq, dt)
+        ws = L.call_raw("lrq_mxfp4_gemm_workspace", ctypes.byref(xq.descriptor()), ctypes.byref(wq.descriptor()))
+    else:
+        x = _grid((m, k if which == "linear" else n), dev, 2, (0.0, 1.0, 2.0))
+        ref = x.double() @ (w.double().T if which == "linear" else w.double())
+        xb = x.to(torch.bfloat16)
+        run = lambda dt: (pkg.mxfp4_linear if which == "linear" else pkg.mxfp4_linear_backward)(xb, wq, dt)
+        ws = L.call_raw("lrq_mxfp4_linear_workspace", m, ctypes.byref(wq.descriptor()), int(which == "back"))
+    assert (ws > 0) == split
+    assert float(ref.abs().max()) < 2 ** 22
+    assert torch.equal(run(torch.float32).double(), ref)
+    assert torch.equal(run(torch.bfloat16), ref.to(torch.float32).to(torch.bfloat16))
+
+
+def test_products_over_the_range_of_scales(pkg, dev):
+    """Every scale from 2^-127 (elements below the smallest normal number) to 2^125, picked out by one-hot operands."""
+    n, k = 64, 256
+    codes = torch.randint(0, 256, (n, 128), generator=_gen(5), dtype=torch.uint8)
+    scales = (torch.arange(n * 8) % 253).to(torch.uint8).reshape(n, 8)
+    w = pkg.MXFP4Tensor(codes.to(dev), scales.to(dev), (n, k))
+    w64 = R.mx_values(R.mx_nibbles(codes), scales.long(), k)
+    eye, eye_n = (torch.eye(i, dtype=torch.bfloat16, device=dev) for i in (k, n))
+    assert torch.equal(pkg.mxfp4_dequantize(w, torch.float32).cpu().double(), w64)
+    assert torch.equal(pkg.mxfp4_linear(eye, w, torch.float32).cpu().double(), w64.T)
+    assert torch.equal(pkg.mxfp4_linear(eye[:9], w, torch.float32).cpu().double(), w64.T[:9])
+    assert torch.equal(pkg.mxfp4_linear_backward(eye_n, w, torch.float32).cpu().double(), w64)
+    assert torch.equal(pkg.mxfp4_gemm(pkg.mxfp4_quantize(eye), w, torch.float32).cpu().double(), w64.T)
+
+
+def test_past_32_bits(pkg, dev):
+    """An activation of more than 2^32 bytes: its last rows, quantised and multiplied, are those of the rows alone."""
+    rows, k, n = 524300, 4104, 40
+    x = torch.zeros(rows, k, dtype=torch.bfloat16, device=dev)
+    tail = _grid((3, k), dev, 3).to(torch.bfloat16)
+    x[-3:] = tail
+    q, qt = pkg.mxfp4_quantize(x), pkg.mxfp4_quantize(tail)
+    assert torch.equal(q.codes[-3:], qt.codes) and torch.equal(q.scales[-3:], qt.scales)
+    assert torch.equal(pkg.mxfp4_dequantize(q)[-3:], tail)
+    w = _grid((n, k), dev, 4)
+    wq = pkg.mxfp4_quantize(w)
+    ref = tail.double() @ w.double().T  # exact in fp32, as above
+    for y in (pkg.mxfp4_linear(x, wq, torch.float32), pkg.mxfp4_gemm(q, wq, torch.float32)):
+        assert torch.equal(y[-3:].double(), ref) and not y[:-3].any()
+    # and as the output of the gradient
+    dy = torch.zeros(rows, n, dtype=torch.bfloat16, device=dev)
+    dy[-3:] = tail[:, :n]
+    dx = pkg.mxfp4_linear_backward(dy, wq)
+    assert torch.equal(dx[-3:].float(), (tail[:, :n].double() @ w.double()).float().to(torch.bfloat16).float())
+    assert not dx[:-3].any()
+    del x, q, dx
+
+
+def test_two_graphs_with_split_products(pkg, dev):
+    """Two captured graphs and eager calls, each with workspaces of its own, replayed in turn."""
+    x, w, _ = _operands(pkg, dev, 40, 100, 2048, 11)
+    x2 = x.flip(0).contiguous()
+    a, a2 = pkg.mxfp4_quantize(x), pkg.mxfp4_quantize(x2)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for xx, aa in ((x, a), (x2, a2)):
+        g = torch.cuda.CUDAGraph()
+        print("[mx] capture", flush=True)
+        with torch.cuda.graph(g):
+            outs.append((pkg.mxfp4_linear(xx, w), pkg.mxfp4_gemm(aa, w)))
+        graphs.append(g)
+    want = [(pkg.mxfp4_linear(xx, w), pkg.mxfp4_gemm(aa, w)) for xx, aa in ((x, a), (x2, a2))]
+    for _ in range(3):
+        for g in graphs:
+            g.replay()
+        again = pkg.mxfp4_linear(x, w)
+        torch.cuda.synchronize()
+        assert torch.equal(again, want[0][0])
+        for out, exp in zip(outs, want):
+            assert torch.equal(out[0], exp[0]) and torch.equal(out[1], exp[1])
+
+
 def test_products_map_every_element(pkg, dev):
     """One-hot operands pick single elements of the weight: any swap of rows, columns, nibbles or scales shows."""
     n, k = 150, 300
