@@ -171,9 +171,9 @@ __global__ __launch_bounds__(512) void k_mx_gemm(GemmArgs p) {
   const auto read_scales = [&](int step, int phase, int ring) {
     const char* sc = sm + kRing + ring * G::kScales + 4 * min(step - scale_base(step - phase, steps), 3);
 #pragma unroll
-    for (int i = 0; i < MT; ++i) na[i] = ld4(sc + 16 * (ra + 32 * i)) >> (8 * h);
+    for (int i = 0; i < MT; ++i) na[i] = ld4(sc + 16 * (ra + 32 * i));
 #pragma unroll
-    for (int t = 0; t < 2; ++t) nb[t] = ld4(sc + 1024 * MT + 16 * (rb + 32 * t)) >> (8 * h);
+    for (int t = 0; t < 2; ++t) nb[t] = ld4(sc + 1024 * MT + 16 * (rb + 32 * t));
   };
   // the scales' loads are ahead of the codes of the step before theirs
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(kLoads * 2));
@@ -183,25 +183,29 @@ __global__ __launch_bounds__(512) void k_mx_gemm(GemmArgs p) {
   int buf = 0, ring = 0;
   for (int step = at.first; step < at.last; ++step) {
     const int phase = (step - at.first) & 3, ahead = min(step + kDeep - 1, at.last - 1), to = (buf + kDeep - 1) & (kDeep - 1);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) sa[i] = na[i] >> (8 * h);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) sb[t] = nb[t] >> (8 * h);
+    __builtin_amdgcn_sched_barrier(0);  // (the wait for these is not to cover the reads that follow)
     read(1, buf);
-#pragma unroll
-    for (int i = 0; i < MT; ++i) sa[i] = na[i];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) sb[t] = nb[t];
-    __builtin_amdgcn_sched_barrier(0);
     if (phase == 0 && steps >= 4) issue_scales(step + 4, ring ^ 1);
+    __builtin_amdgcn_sched_barrier(0);
+    // No branch from here to the end of the step, and the order is held: the compiler would sink the instructions into
+    // the block behind it and issue the loads at once.
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
 #pragma unroll
       for (int t = 0; t < 2; ++t) acc[i][t] = mfma_mx<0>(va[0][i], vb[0][t], acc[i][t], sa[i], sb[t]);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int k = i * kLoads / MT; k < (i + 1) * kLoads / MT; ++k) issue_codes(ahead, to, k);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    // the next step's loads, not those of the two steps after it (nor the scales among them)
-    if (phase < 2 && steps >= 4) __builtin_amdgcn_s_waitcnt(vmcnt_imm(kLoads * (kDeep - 2) + 1));
-    else __builtin_amdgcn_s_waitcnt(vmcnt_imm(kLoads * (kDeep - 2)));
+    // the next step's loads, not those of the two steps after it (the scales are ahead of the last of these)
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(kLoads * (kDeep - 2)));
     lds_meet();  // every wave's are in, and every wave has read all of this step's buffer
-    if (phase == 3) ring ^= 1;
+    ring ^= (phase + 1) >> 2;
     buf = (buf + 1) & (kDeep - 1);
     read(0, buf);
     read_scales(step + 1, (phase + 1) & 3, ring);
