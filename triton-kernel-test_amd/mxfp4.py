@@ -79,8 +79,8 @@ def mxfp4_quantize(x: torch.Tensor) -> MXFP4Tensor:
     dt = _dtype(x, "x")
     x2, rows, n, ldx = _rows(x, "x")
     steps = (n + 127) // 128
-    codes = torch.empty((rows, 64 * steps), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((rows, 4 * steps), dtype=torch.uint8, device=x.device)
+    codes = x.new_empty((rows, 64 * steps), dtype=torch.uint8)
+    scales = x.new_empty((rows, 4 * steps), dtype=torch.uint8)
     t = LrqMxfp4(codes.data_ptr(), 64 * steps, scales.data_ptr(), 4 * steps, rows, n)
     with _on(x.device):
         call("lrq_mxfp4_quantize", _p(x2), ldx, dt, ctypes.byref(t), _stream(x.device))
@@ -90,7 +90,7 @@ def mxfp4_quantize(x: torch.Tensor) -> MXFP4Tensor:
 def mxfp4_dequantize(q: MXFP4Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values of q (exact in bf16 and fp32)."""
     t = q.descriptor()
-    out = torch.empty(q.shape, dtype=dtype, device=q.device)
+    out = q.codes.new_empty(q.shape, dtype=dtype)
     with _on(q.device):
         call("lrq_mxfp4_dequantize", ctypes.byref(t), _p(out), q.cols, _dtype(out, "the output"), _stream(q.device))
     return out
@@ -117,19 +117,19 @@ def mxfp4_gemm(a: MXFP4Tensor, b: MXFP4Tensor, out_dtype: torch.dtype = torch.bf
     ta = a.descriptor()
     if a.cols != b.cols:
         raise ValueError(f"operands have {a.cols} and {b.cols} columns")
-    out = torch.empty(tuple(a.shape[:-1]) + (b.rows,), dtype=out_dtype, device=a.device)
-    ws, ws_bytes = _workspace(a.device, "lrq_mxfp4_gemm_workspace", ctypes.byref(ta), ctypes.byref(tb))
+    out = a.codes.new_empty(tuple(a.shape[:-1]) + (b.rows,), dtype=out_dtype)
+    ws, ws_bytes = _workspace(out, "lrq_mxfp4_gemm_workspace", ctypes.byref(ta), ctypes.byref(tb))
     with _on(a.device):
         call("lrq_mxfp4_gemm", ctypes.byref(ta), ctypes.byref(tb), _p(out), b.rows, f32, _p(ws), ws_bytes,
              _stream(a.device))
     return out
 
 
-def _workspace(device, query: str, *args):
+def _workspace(like: torch.Tensor, query: str, *args):
     n = call_raw(query, *args)
     if n < 0:
         check(n, query)
-    return (torch.empty(n // 4, dtype=torch.float32, device=device) if n else None), n
+    return (like.new_empty(n // 4, dtype=torch.float32) if n else None), n
 
 
 def _operand(x: torch.Tensor, cols: int, name: str):
@@ -153,10 +153,10 @@ def _product(name: str, x: torch.Tensor, w: MXFP4Tensor, out_dtype, transposed: 
     t = _matrix(w, x.device)
     depth, cols = (w.rows, w.cols) if transposed else (w.cols, w.rows)
     x2, rows, ld = _operand(x, depth, "dy" if transposed else "x")
-    out = torch.empty(tuple(x.shape[:-1]) + (cols,), dtype=out_dtype, device=x.device)
+    out = x.new_empty(x.shape[:-1] + (cols,), dtype=out_dtype)
     if depth == 0:
         return out.zero_()
-    ws, ws_bytes = _workspace(x.device, "lrq_mxfp4_linear_workspace", rows, ctypes.byref(t), transposed)
+    ws, ws_bytes = _workspace(out, "lrq_mxfp4_linear_workspace", rows, ctypes.byref(t), transposed)
     with _on(x.device):
         call(name, _p(x2), ld, rows, ctypes.byref(t), _p(out), cols, f32, _p(ws), ws_bytes, _stream(x.device))
     return out

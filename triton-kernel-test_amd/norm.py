@@ -40,7 +40,7 @@ def _dtype(t: torch.Tensor, name: str) -> int:
 
 
 # Small batches are bound by the host (a call of a few rows: 10 us for 3 us of kernel), so the usual case, contiguous
-# operands, takes as few torch calls as it can: no views, empty_like for the outputs.
+# operands, takes as few torch calls as it can: no views, empty_like and new_empty for the outputs (half of empty's time).
 def _rows(x: torch.Tensor, name: str) -> tuple[torch.Tensor, int, int, int]:
     """x as rows: (a tensor to take the pointer of, rows, row width, row stride); rows do not overlap (an expanded
     gradient is copied)."""
@@ -66,7 +66,7 @@ def _like(t: Optional[torch.Tensor], x: torch.Tensor, name: str) -> Optional[tor
 
 def _new(x: torch.Tensor) -> torch.Tensor:
     """A contiguous tensor of x's shape and type."""
-    return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    return torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
 
 
 def _weights(weight, bias, n: int, device: torch.device):
@@ -130,7 +130,7 @@ def layer_norm_forward(x: torch.Tensor, weight: Optional[torch.Tensor] = None, b
     x2, rows, n, ldx = _rows(x, "x")
     w, b, wdt = _weights(weight, bias, n, x.device)
     y = _new(x)
-    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
     rstd = torch.empty_like(mean)
     with _on(x.device):
         call("lrq_layer_norm_fwd", None, _p(x2), ldx, None, 0, dt, _p(w), _p(b), wdt, rows, n, eps, None, 0, _p(y), n,
@@ -155,8 +155,8 @@ def _backward(drop, dy, dh, h, weight, mean, rstd, weight_grad: bool, fused: boo
         ws_bytes = _lib.call_raw("lrq_layer_norm_bwd_workspace", rows, n)
         if ws_bytes < 0:
             _lib.check(ws_bytes, "lrq_layer_norm_bwd_workspace")
-        ws = torch.empty(max(ws_bytes // 4, 1), dtype=torch.float32, device=h.device)
-        dw = torch.empty(n, dtype=torch.float32, device=h.device) if w is None else torch.empty_like(w)
+        ws = h.new_empty(max(ws_bytes // 4, 1), dtype=torch.float32)
+        dw = h.new_empty(n, dtype=torch.float32) if w is None else torch.empty_like(w)
         db = torch.empty_like(dw)
     with _on(h.device):
         call("lrq_layer_norm_bwd", drop, _p(dy2), lddy, _p(dh2), lddh, _p(h2), ldh, dt, _p(w), wdt, _p(mean), _p(rstd),
@@ -204,7 +204,7 @@ def dropout_add_layer_norm_forward(x: torch.Tensor, residual: Optional[torch.Ten
     drop, _state = _drop(p, seed, x.device)
     y = _new(x)
     h = _new(x)
-    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
     rstd = torch.empty_like(mean)
     with _on(x.device):
         call("lrq_layer_norm_fwd", ctypes.byref(drop), _p(x2), ldx, _p(r2), ldr, dt, _p(w), _p(b), wdt, rows, n, eps, _p(h),
