@@ -151,22 +151,25 @@ __global__ __launch_bounds__(512) void k_mx_gemm(GemmArgs p) {
 
   if (steps >= 4) issue_scales(at.first, 0);
   else short_scales(ps, steps, ls + 16 * lane);
+  const auto issue_step = [&](int step, int buf, int k) { issue_codes(min(step, at.last - 1), buf, k); };
+  constexpr int kEarly = kLoads / 2;  // loads of a step that are issued in the half step before the others
 #pragma unroll
-  for (int d = 0; d < kDeep - 1; ++d)
+  for (int d = 0; d < kDeep; ++d)
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) issue_codes(min(at.first + d, at.last - 1), d, i);
-  // The operands of instruction column q of a step, read from LDS while the column before runs: that of a step's
-  // first column is the last of the step before, so the step's loads are waited for, and the workgroup meets, in the
-  // middle of the step before.
+    for (int i = 0; i < (d < kDeep - 1 ? kLoads : kEarly); ++i) issue_step(at.first + d, d, i);
+  // The operands of instruction column q of a step are read from LDS while the column before runs: those of a step's
+  // first column during the last of the step before, so the step's loads are waited for, and the workgroup meets, in the
+  // middle of the step before.  Reads and loads go out one at a time between the instructions: a wave that issues them
+  // together stands in their queue with the matrix unit idle.
   const int ra = 32 * MT * wm + c, rb = 64 * wn + c, slot = c >> 2 & 3;
+  constexpr int kMfma = 2 * MT, kPieces = MT + 2, kPer = (kPieces + kMfma - 1) / kMfma;
   u32x4 va[2][MT], vb[2][2];
   uint32_t sa[MT], sb[2], na[MT], nb[2];
-  const auto read = [&](int q, int buf) {
+  const auto read = [&](int q, int buf, int j) {
     const char* st = sm + buf * kStage;
-#pragma unroll
-    for (int t = 0; t < 2; ++t) vb[q][t] = ld16(st + kA + 64 * (rb + 32 * t) + 16 * ((2 * q + h) ^ slot));
-#pragma unroll
-    for (int i = 0; i < MT; ++i) va[q][i] = ld16(st + 64 * (ra + 32 * i) + 16 * ((2 * q + h) ^ slot));
+    const int o = 16 * ((2 * q + h) ^ slot);
+    if (j < 2) vb[q][j < 2 ? j : 0] = ld16(st + kA + 64 * (rb + 32 * j) + o);
+    else va[q][j - 2] = ld16(st + 64 * (ra + 32 * (j - 2)) + o);
   };
   const auto read_scales = [&](int step, int phase, int ring) {
     const char* sc = sm + kRing + ring * G::kScales + 4 * min(step - scale_base(step - phase, steps), 3);
@@ -175,46 +178,44 @@ __global__ __launch_bounds__(512) void k_mx_gemm(GemmArgs p) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) nb[t] = ld4(sc + 1024 * MT + 16 * (rb + 32 * t));
   };
-  // the scales' loads are ahead of the codes of the step before theirs
-  __builtin_amdgcn_s_waitcnt(vmcnt_imm(kLoads * 2));
+  // Instruction m of a column, then its share of the next column's reads (the first ones' share) and of the loads (the
+  // last ones').  The order is held, and there is no branch in a step: the compiler would sink the instructions into
+  // the block behind it and issue everything else first.
+#define LRQ_COLUMN(Q, SEL, BUF, STEP, TO, FIRST, COUNT)                                                       \
+  _Pragma("unroll") for (int m = 0; m < kMfma; ++m) {                                                         \
+    acc[m / 2][m % 2] = mfma_mx<SEL>(va[Q][m / 2], vb[Q][m % 2], acc[m / 2][m % 2], sa[m / 2], sb[m % 2]);    \
+    __builtin_amdgcn_sched_barrier(0);                                                                        \
+    if (Q == 1 && m == 0) read_scales(step + 1, (phase + 1) & 3, ring);                                       \
+    _Pragma("unroll") for (int j = m * kPer; j < (m + 1) * kPer; ++j) if (j < kPieces) read(1 - Q, BUF, j);   \
+    if (m >= kMfma - (COUNT)) issue_step(STEP, TO, (FIRST) + m - (kMfma - (COUNT)));                          \
+    __builtin_amdgcn_sched_barrier(0);                                                                        \
+  }
+  // the scales' loads are ahead of the codes
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(kLoads * 2 + kEarly));
   lds_meet();
-  read(0, 0);
+#pragma unroll
+  for (int j = 0; j < kPieces; ++j) read(0, 0, j);
   read_scales(at.first, 0, 0);
   int buf = 0, ring = 0;
   for (int step = at.first; step < at.last; ++step) {
-    const int phase = (step - at.first) & 3, ahead = min(step + kDeep - 1, at.last - 1), to = (buf + kDeep - 1) & (kDeep - 1);
+    const int phase = (step - at.first) & 3;
+    if (phase == 0 && steps >= 4) issue_scales(step + 4, ring ^ 1);
 #pragma unroll
     for (int i = 0; i < MT; ++i) sa[i] = na[i] >> (8 * h);
 #pragma unroll
     for (int t = 0; t < 2; ++t) sb[t] = nb[t] >> (8 * h);
-    __builtin_amdgcn_sched_barrier(0);  // (the wait for these is not to cover the reads that follow)
-    read(1, buf);
-    if (phase == 0 && steps >= 4) issue_scales(step + 4, ring ^ 1);
     __builtin_amdgcn_sched_barrier(0);
-    // No branch from here to the end of the step, and the order is held: the compiler would sink the instructions into
-    // the block behind it and issue the loads at once.
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t) acc[i][t] = mfma_mx<0>(va[0][i], vb[0][t], acc[i][t], sa[i], sb[t]);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int k = i * kLoads / MT; k < (i + 1) * kLoads / MT; ++k) issue_codes(ahead, to, k);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    // the next step's loads, not those of the two steps after it (the scales are ahead of the last of these)
+    LRQ_COLUMN(0, 0, buf, step + kDeep - 1, (buf + kDeep - 1) & (kDeep - 1), kEarly, kLoads - kEarly)
+    // the next step's loads, not those of the two steps after it (the scales are done three steps on, in time)
     __builtin_amdgcn_s_waitcnt(vmcnt_imm(kLoads * (kDeep - 2)));
     lds_meet();  // every wave's are in, and every wave has read all of this step's buffer
     ring ^= (phase + 1) >> 2;
+    const int free = buf;
     buf = (buf + 1) & (kDeep - 1);
-    read(0, buf);
-    read_scales(step + 1, (phase + 1) & 3, ring);
     __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int t = 0; t < 2; ++t) acc[i][t] = mfma_mx<2>(va[1][i], vb[1][t], acc[i][t], sa[i], sb[t]);
+    LRQ_COLUMN(1, 2, buf, step + kDeep, free, 0, kEarly)
   }
+#undef LRQ_COLUMN
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // the last loads write LDS: let them end before the workgroup does
   char* out = (char*)p.out + (p.splits > 1 ? (int64_t)at.z * p.a.rows * p.ldo * 4 : 0);
   const int64_t n = at.n0 + 64 * wn + 2 * c;
