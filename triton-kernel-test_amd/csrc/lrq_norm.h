@@ -16,8 +16,8 @@
 namespace lrq {
 
 // Rows of up to 16 chunks take 16 threads, up to 64 chunks a wave, wider ones as many whole waves as they need (LANES 0,
-// waves at run time): 5120 columns are five waves of two chunks a thread with nothing idle.  A workgroup's row groups
-// walk rows g, g + G, ... (G = groups in the grid).
+// waves at run time): 5120 columns are five waves of two chunks a thread (forward) or ten of one (backward), with nothing
+// idle.  A workgroup's row groups walk rows g, g + G, ... (G = groups in the grid).
 struct RowShape {
   int lanes;   // 16, 64, or 0: several waves
   int chunks;  // a thread
