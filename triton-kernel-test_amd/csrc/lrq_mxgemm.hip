@@ -40,6 +40,8 @@ __device__ __forceinline__ void ld_to_lds(const void* g, char* lds) {
 }
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef u32x4 u32x4_dword __attribute__((aligned(4)));
+__device__ __forceinline__ u32x4 ld16_any(const uint8_t* p) { return *reinterpret_cast<const u32x4_dword*>(p); }
 
 __device__ __forceinline__ f32x16 mfma_32x32x16(u32x4 a, u32x4 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -265,7 +267,16 @@ __global__ __launch_bounds__(64 * WAVES) void k_mx_token(const uint16_t* x, int6
     for (int u = 0; u < D; ++u) {
       const int s = min(s0 + u, last - 1);
       c[u] = ld16_stream(codes + 64 * (int64_t)s);
-      sc[u] = ld4(scales + 4 * (int64_t)s);
+    }
+    if (s0 + D <= w.steps) {  // 16 bytes of scales a load, four steps
+#pragma unroll
+      for (int u = 0; u < D; u += 4) {
+        const u32x4 v = ld16_any(scales + 4 * (int64_t)(s0 + u));
+        sc[u] = v[0], sc[u + 1] = v[1], sc[u + 2] = v[2], sc[u + 3] = v[3];
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < D; ++u) sc[u] = ld4(scales + 4 * (int64_t)min(s0 + u, last - 1));
     }
     __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
     asm volatile("" ::: "memory");
