@@ -240,7 +240,9 @@ __global__ __launch_bounds__(512) void k_mx_gemm(GemmArgs p) {
 // of them for each of the step's four matrix instructions, and X is read in the same order.  Everything a wave needs
 // for its next D steps is in flight at once: X's columns go to the wave's own part of LDS (16-byte piece i of row r in
 // slot i ^ r, so that the 16 rows' reads fall in different banks), the codes and scales to registers.  The time is the
-// codes' arrival after a fixed 5 us: one row by [14336, 4096] 11 us for 31 MB, by [4096, 4096] 5 us for 9 MB.
+// codes' arrival after a fixed 4 us: one row by [14336, 4096] 8.4 us for 31 MB (9.8 from HBM), by [4096, 4096] 4.6 us for
+// 9 MB; 16 rows 13.0 and 5.4 us, where every workgroup reads all of X through L2.  A dword of scales a step in place of 16
+// bytes for four took 10.8 us.
 template <int ROWS, int WAVES, bool F32>
 __global__ __launch_bounds__(64 * WAVES) void k_mx_token(const uint16_t* x, int64_t ldx, int rows, Mx w, void* out,
                                                          int64_t ldo) {
@@ -724,7 +726,8 @@ static int mx_linear(const void* x, int64_t ldx, int64_t rows, const lrq_mxfp4* 
                       : launch((k_mx_token<r(), waves(), false>), grid, dim3(64 * waves()), 0, s, px, ldx, (int)rows, w, out, ldo);
     };
     // four waves a workgroup (8 steps each of 4096 columns: one round of loads); eight where workgroups are few and the
-    // runs long, 11.6 against 12.4 us on 4096 rows of 14336 columns (but 6.6 against 5.2 us on 4096 of 4096)
+    // runs long, 11.3 against 13.3 us on 4096 rows of 14336 columns (but 6.3 against 5.2 us on 4096 of 4096); with 16
+    // rows, whose runs are of four steps, there always
 #define LRQ_GO(R, W) return go(integral_constant<int, R>{}, integral_constant<int, W>{})
     if (rows <= 4) {
       if (grid.x >= 512 || w.steps <= 64) LRQ_GO(4, 4);
