@@ -117,7 +117,7 @@ def mxfp4_gemm(a: MXFP4Tensor, b: MXFP4Tensor, out_dtype: torch.dtype = torch.bf
     ta = a.descriptor()
     if a.cols != b.cols:
         raise ValueError(f"operands have {a.cols} and {b.cols} columns")
-    out = a.codes.new_empty(tuple(a.shape[:-1]) + (b.rows,), dtype=out_dtype)
+    out = a.codes.new_empty((ta.rows, tb.rows) if len(a.shape) == 2 else tuple(a.shape[:-1]) + (tb.rows,), dtype=out_dtype)
     ws, ws_bytes = _workspace(out, "lrq_mxfp4_gemm_workspace", ctypes.byref(ta), ctypes.byref(tb))
     with _on(a.device):
         call("lrq_mxfp4_gemm", ctypes.byref(ta), ctypes.byref(tb), _p(out), b.rows, f32, _p(ws), ws_bytes,
@@ -153,7 +153,7 @@ def _product(name: str, x: torch.Tensor, w: MXFP4Tensor, out_dtype, transposed: 
     t = _matrix(w, x.device)
     depth, cols = (w.rows, w.cols) if transposed else (w.cols, w.rows)
     x2, rows, ld = _operand(x, depth, "dy" if transposed else "x")
-    out = x.new_empty(x.shape[:-1] + (cols,), dtype=out_dtype)
+    out = x.new_empty((x.shape[0], cols) if x.dim() == 2 else x.shape[:-1] + (cols,), dtype=out_dtype)
     if depth == 0:
         return out.zero_()
     ws, ws_bytes = _workspace(out, "lrq_mxfp4_linear_workspace", rows, ctypes.byref(t), transposed)

@@ -130,7 +130,7 @@ def layer_norm_forward(x: torch.Tensor, weight: Optional[torch.Tensor] = None, b
     x2, rows, n, ldx = _rows(x, "x")
     w, b, wdt = _weights(weight, bias, n, x.device)
     y = _new(x)
-    mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    mean = x.new_empty((rows,) if x.dim() == 2 else x.shape[:-1], dtype=torch.float32)
     rstd = torch.empty_like(mean)
     with _on(x.device):
         call("lrq_layer_norm_fwd", None, _p(x2), ldx, None, 0, dt, _p(w), _p(b), wdt, rows, n, eps, None, 0, _p(y), n,
@@ -204,7 +204,7 @@ def dropout_add_layer_norm_forward(x: torch.Tensor, residual: Optional[torch.Ten
     drop, _state = _drop(p, seed, x.device)
     y = _new(x)
     h = _new(x)
-    mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    mean = x.new_empty((rows,) if x.dim() == 2 else x.shape[:-1], dtype=torch.float32)
     rstd = torch.empty_like(mean)
     with _on(x.device):
         call("lrq_layer_norm_fwd", ctypes.byref(drop), _p(x2), ldx, _p(r2), ldr, dt, _p(w), _p(b), wdt, rows, n, eps, _p(h),
