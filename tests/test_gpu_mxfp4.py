@@ -320,6 +320,35 @@ def test_deterministic_and_captured(pkg, dev):
         assert torch.equal(a, b)
 
 
+def test_one_dimensional_rows_and_two_streams(pkg, dev):
+    x, w, _ = _operands(pkg, dev, 40, 300, 2048, 15)
+    assert torch.equal(pkg.mxfp4_linear(x[5], w), pkg.mxfp4_linear(x[5:6], w)[0])
+    q1, q2 = pkg.mxfp4_quantize(x[5]), pkg.mxfp4_quantize(x[5:6])
+    assert q1.shape == (2048,) and torch.equal(q1.codes, q2.codes)
+    assert torch.equal(pkg.mxfp4_dequantize(q1), pkg.mxfp4_dequantize(q2)[0])
+    assert torch.equal(pkg.mxfp4_gemm(q1, w), pkg.mxfp4_gemm(q2, w)[0])
+    dy = torch.randn(40, 300, generator=_gen(16)).to(torch.bfloat16).to(dev)
+    assert torch.equal(pkg.mxfp4_linear_backward(dy[5], w), pkg.mxfp4_linear_backward(dy[5:6], w)[0])
+    xs = [x, x.flip(0).contiguous()]
+    qs = [pkg.mxfp4_quantize(t) for t in xs]
+
+    def step(i):
+        return pkg.mxfp4_linear(xs[i], w), pkg.mxfp4_gemm(qs[i], w), pkg.mxfp4_linear_backward(dy, w)
+
+    want = [step(0), step(1)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(4):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(step(i))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for g in got[i]:
+            for a, e in zip(g, want[i]):
+                assert torch.equal(a, e)
+
+
 def test_autograd_linear(pkg, dev):
     AG = importlib.import_module("triton-kernel-test_amd.autograd")
     x, w, w64 = _operands(pkg, dev, 12, 96, 256, 12)

@@ -471,3 +471,86 @@ def test_captured_graphs_draw_new_masks(pkg, dev):
     for i in range(len(seen)):
         for j in range(i):
             assert not torch.equal(seen[i], seen[j])
+
+
+def test_fused_norm_without_weights_and_one_dimensional(pkg, dev):
+    """The fused pass normalises h as the plain one does, whatever weights there are; one-dimensional operands."""
+    x, res = _x((21, 700), torch.bfloat16, dev, 161), _x((21, 700), torch.bfloat16, dev, 162)
+    dy = _x((21, 700), torch.bfloat16, dev, 163, 0.0)
+    for wdt in (torch.bfloat16, torch.float16):
+        w, b = _w(700, wdt, dev, 164)
+        for ww, bb in ((None, None), (w, None), (None, b), (w, b)):
+            y, h, mean, rstd = pkg.dropout_add_layer_norm_forward(x, res, ww, bb, 0.3, 5)
+            yp, mp, rp = pkg.layer_norm_forward(h, ww, bb)
+            assert torch.equal(_bits(y), _bits(yp)) and torch.equal(mean, mp) and torch.equal(rstd, rp)
+            got = pkg.dropout_add_layer_norm_backward(dy, None, h, ww, mean, rstd, 0.3, 5)
+            want = pkg.layer_norm_backward(dy, h, ww, mean, rstd)
+            for g, e in zip(got[1:], want):
+                assert torch.equal(g, e)
+    y1, m1, r1 = pkg.layer_norm_forward(x[3], None, None)
+    y2, m2, r2 = pkg.layer_norm_forward(x[3:4], None, None)
+    assert m1.shape == () and torch.equal(y1, y2[0]) and torch.equal(m1, m2[0])
+    dx, dw, db = pkg.layer_norm_backward(dy[3], x[3], None, m1, r1)
+    assert torch.equal(dx, pkg.layer_norm_backward(dy[3:4], x[3:4], None, m2, r2)[0][0]) and dw.shape == (700,)
+    assert torch.equal(pkg.dropout(x[3], 0.3, 9), pkg.dropout(x[3:4], 0.3, 9)[0])
+    assert pkg.dropout(x[3, 3], 1.0, 9).shape == () and not pkg.dropout(x[3, 3], 1.0, 9).any()
+
+
+def test_two_streams_at_once(pkg, dev):
+    x = [_x((3000, 1024), torch.bfloat16, dev, 171 + i) for i in range(2)]
+    w, b = _w(1024, torch.bfloat16, dev, 173)
+
+    def step(i):
+        y, h, mean, rstd = pkg.dropout_add_layer_norm_forward(x[i], x[1 - i], w, b, 0.1, (6, i))
+        return (y, *pkg.dropout_add_layer_norm_backward(x[i], h, h, w, mean, rstd, 0.1, (6, i)))
+
+    want = [step(0), step(1)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(4):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(step(i))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for g in got[i]:
+            for a, e in zip(g, want[i]):
+                assert torch.equal(a, e)
+
+
+def test_captured_training_step(pkg, dev):
+    """Forward and backward of the block captured whole: every replay equals the eager step at the seed tensor's value."""
+    AG = importlib.import_module("triton-kernel-test_amd.autograd")
+    x, res = (_x((70, 256), torch.bfloat16, dev, 181 + i).requires_grad_() for i in range(2))
+    w, b = (t.requires_grad_() for t in _w(256, torch.bfloat16, dev, 183))
+    q = pkg.mxfp4_quantize(_x((128, 256), torch.bfloat16, dev, 184))
+    dy, dh = _x((70, 128), torch.bfloat16, dev, 185, 0.0), _x((70, 256), torch.bfloat16, dev, 186, 0.0)
+    state = torch.tensor([3, 0], dtype=torch.int64, device=dev)
+    leaves = (x, res, w, b)
+
+    def step():
+        y, h = AG.dropout_add_layer_norm(x, res, w, b, 0.2, (state, 1))
+        return torch.autograd.grad([AG.mxfp4_linear(y, q), h], leaves, [dy, dh])
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    print("[norm] capture", flush=True)
+    with torch.cuda.graph(graph):
+        outs = step()
+    for i in range(3):
+        state[1] = i
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [o.clone() for o in outs]
+        y, h, mean, rstd = pkg.dropout_add_layer_norm_forward(x.detach(), res.detach(), w.detach(), b.detach(), 0.2,
+                                                              (state, 1))
+        g = pkg.mxfp4_linear_backward(dy, q)
+        want = pkg.dropout_add_layer_norm_backward(g, dh, h, w.detach(), mean, rstd, 0.2, (state, 1))
+        for a, e in zip(got, want):
+            assert torch.equal(a, e), i
