@@ -333,9 +333,10 @@ struct TileArgs {
 //   TRANS true: the lane's two columns are one code byte of each W row.  The transposing LDS read gives it that byte
 //   of 8 rows at once; each is widened with its own row's scale and the halves of two rows are paired by v_perm_b32.
 //
-// 512 rows by [14336, 4096]: 54 us, and 56 us and a join of 8 us for the gradient (1.1 and 1.0 PFLOP/s; 42 us each at the
-// 1.44 PFLOP/s of a large bf16 product on random data, which power limits); 4096 rows: 412 and 410 us (1.17).  224 of 256
-// CUs have a tile of 512 rows.  Reading the operands of the next instruction a step ahead in registers took the same time.
+// 512 rows by [14336, 4096]: 54 to 56 us, and 56 us and a join of 8 us for the gradient (1.1 and 1.0 PFLOP/s; 42 us each at
+// the 1.44 PFLOP/s of a large bf16 product on random data, which power limits: on zeros a step takes 1.27 us, on random
+// data 1.4 to 1.7, its instructions alone 0.96 at 2.1 GHz); 4096 rows: 412 to 422 us (1.15).  224 of 256 CUs have a tile of
+// 512 rows.
 template <bool TRANS, int MT>
 struct TileLds {
   static constexpr int kA = 32 * MT * 256, kB = 16384, kS = TRANS ? 3072 : 0, kStage = kA + kB + kS, kDeep = 3;
@@ -355,12 +356,12 @@ __global__ __launch_bounds__(512) void k_mx_tile(TileArgs a) {
 
   // x: instruction i of wave w fills rows 4 (MT w + i) .. + 3 of the tile; chunk q of row r sits in slot q ^ (r % 16)
   const char* px[MT];
-  int qx[MT];
+  int full[MT];  // this lane's chunk is one of x's in steps below it
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
-    const int r = 4 * (MT * wave + i) + (lane >> 4);
-    qx[i] = (lane & 15) ^ (r & 15);
-    px[i] = (const char*)(a.x + min(m0 + r, a.rows - 1) * a.ldx + 8 * qx[i]);
+    const int r = 4 * (MT * wave + i) + (lane >> 4), q = (lane & 15) ^ (r & 15);
+    full[i] = (a.chunks - q + 15) >> 4;
+    px[i] = (const char*)(a.x + min(m0 + r, a.rows - 1) * a.ldx + 8 * q);
   }
   // codes: TRANS false: 256 rows of 64 bytes, 16-byte piece q of row r in slot q ^ (r / 4 % 4), LDS row 64 wn + 32 t + c
   // holding W row 64 wn + 2 c + t; TRANS true: 128 rows of 128 bytes, piece q of row r in slot q ^ (r / 2 % 4).  Both
@@ -377,35 +378,27 @@ __global__ __launch_bounds__(512) void k_mx_tile(TileArgs a) {
       pb[i] = a.w.codes + w_row(r) * a.w.ldc + 16 * ((lane & 3) ^ (r >> 2 & 3));
     } else {
       rb[i] = 8 * in + (lane >> 3);
-      pb[i] = a.w.codes + rb[i] * a.w.ldc + min(n0 / 2 + 16 * ((lane & 7) ^ (rb[i] >> 1 & 3)), 64 * (int64_t)a.w.steps - 16);
+      pb[i] = a.w.codes + min(n0 / 2 + 16 * ((lane & 7) ^ (rb[i] >> 1 & 3)), 64 * (int64_t)a.w.steps - 16);
     }
   }
   const int rs = TRANS ? (threadIdx.x & 255) >> 1 : 64 * (wave & 3) + lane;
   if constexpr (!TRANS) ps = a.w.scales + w_row(rs) * a.w.lds;
-  else ps = a.w.scales + rs * a.w.lds + min(n0 / 32 + 4 * (lane & 1), 4 * (int64_t)a.w.steps - 4);
+  else ps = a.w.scales + min(n0 / 32 + 4 * (lane & 1), 4 * (int64_t)a.w.steps - 4);
 
-  // part i < 4 of a step's loads
+  // part i < 4 of a step's loads (no branch: see the loop)
   const auto issue = [&](int step, int buf, int i) {
     char* st = sm + buf * kStage;
     if (i < MT) {
       const int k = i < MT ? i : 0;
-      const char* g = px[k] + 256 * (int64_t)step;
-      if (16 * step + 16 > a.chunks && 16 * step + qx[k] >= a.chunks) g = (const char*)&kZeroChunk;
+      const char* g = step < full[k] ? px[k] + 256 * (int64_t)step : (const char*)&kZeroChunk;
       ld_to_lds<16>(g, st + 1024 * (MT * wave + i));
     }
     if constexpr (!TRANS) {
       if (i < 2) ld_to_lds<16>(pb[i & 1] + 64 * (int64_t)step, st + kA + 1024 * (2 * wave + i));
-    } else {
-      const int64_t r0 = 128 * (int64_t)step, most = a.w.rows - 1 - r0;  // rows past W's last: that one (their x is zero)
-      const bool whole = most >= 127;
-      if (i < 2) {
-        const int64_t r = whole ? r0 : r0 + min((int64_t)rb[i & 1], most) - rb[i & 1];
-        ld_to_lds<16>(pb[i & 1] + r * a.w.ldc, st + kA + 1024 * (2 * wave + i));
-      }
-      if (i == 2 && wave < 4) {
-        const int64_t r = whole ? r0 : r0 + min((int64_t)rs, most) - rs;
-        ld_to_lds<4>(ps + r * a.w.lds, st + kA + kB + 256 * wave);
-      }
+    } else {  // rows past W's last: that one (their x is zero)
+      const uint32_t r0 = 128 * (uint32_t)step, most = (uint32_t)a.w.rows - 1;
+      if (i < 2) ld_to_lds<16>(pb[i & 1] + (int64_t)min(r0 + rb[i & 1], most) * a.w.ldc, st + kA + 1024 * (2 * wave + i));
+      if (i == 2 && wave < 4) ld_to_lds<4>(ps + (int64_t)min(r0 + rs, most) * a.w.lds, st + kA + kB + 256 * wave);
     }
   };
   // TRANS false: W's scales, four steps at a time (waves 4 .. 7 load the same again)
@@ -429,38 +422,44 @@ __global__ __launch_bounds__(512) void k_mx_tile(TileArgs a) {
   for (int d = 0; d < 2; ++d)
 #pragma unroll
     for (int i = 0; i < 4; ++i) issue(min(first + d, last - 1), d, i);
-  int buf = 0, ring = 0;
-  for (int step = first; step < last; ++step) {
-    // this step's loads, and its scales' (issued ahead of the codes of the step before), not those of the step after
-    const int phase = (step - first) & 3;
+  issue(min(first + 2, last - 1), 2, 0);
+
+  // TRANS: a step's scales arrive as [row][8]; the four of the thread that loaded them go to [block][row] as bf16, so
+  // that half of them are a conversion's scale operand as read.
+  const auto turn_scales = [&](int buf) {
     if constexpr (TRANS) {
-      if (wave < 4) __builtin_amdgcn_s_waitcnt(vmcnt_imm(MT + 3));
-      else __builtin_amdgcn_s_waitcnt(vmcnt_imm(MT + 2));
-    } else {
-      __builtin_amdgcn_s_waitcnt(vmcnt_imm(MT + 2));
-    }
-    char* st = sm + buf * kStage;
-    if constexpr (TRANS) {
-      // the scales arrive as [row][8]; this thread's four go to [block][row] as bf16, so that half of them are a
-      // conversion's scale operand as read
       if (wave < 4) {
-        const uint32_t s4 = ld4(st + kA + kB + 4 * threadIdx.x);
-        uint16_t* to = (uint16_t*)(st + kA + kB + 1024) + 512 * (lane & 1) + rs;
+        char* st = sm + buf * kStage + kA + kB;
+        const uint32_t s4 = ld4(st + 4 * threadIdx.x);
+        uint16_t* to = (uint16_t*)(st + 1024) + 512 * (lane & 1) + rs;
 #pragma unroll
         for (int k = 0; k < 4; ++k) to[128 * k] = (uint16_t)((s4 >> (8 * k) & 255u) << 7);
       }
     }
-    lds_meet();  // every wave's loads are in, and the buffer of the step before is free
-    const int ahead = min(step + 2, last - 1), to = buf == 0 ? 2 : buf - 1;
+  };
+  u32x4 xr[2][MT], b[2][2];
+  u32x4 code[2];           // TRANS false: this lane's codes of its two columns, and their scales
+  float scale[2];
+  u32x2 cols[4];           // TRANS: its code byte of 8 rows, for each instruction, and the rows' scales
+  u32x4 rows8[4];
+  const auto read_x = [&](int buf, int s, int i) {
+    const int r = 32 * i + c;
+    xr[s & 1][i] = ld16(sm + buf * kStage + 256 * r + 16 * ((8 * gq + 4 * h + s) ^ (r & 15)));
+  };
+  const auto read_w = [&](int buf, int step, int phase, int ring) {
+    char* st = sm + buf * kStage;
     if constexpr (!TRANS) {
-      if (phase == 2 && a.steps >= 4) issue_scales(step + 2, ring ^ 1);
-    }
-    u32x4 code[2];
-    float scale[2];
-    u32x2 cols[4];            // TRANS: this lane's code byte of 8 rows, for each instruction
-    u32x4 rows8[4];           // and the rows' scales
-    if constexpr (TRANS) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int r = 64 * wn + 32 * t + c;
+        code[t] = ld16(st + kA + 64 * r + 16 * ((2 * gq + h) ^ (r >> 2 & 3)));
+        scale[t] = e8m0_operand((uint8_t)sm[kRing + ring * T::kScales + 16 * r +
+                                            4 * min(step - scale_base(step - phase, a.steps), 3) + 2 * gq + h]);
+      }
+    } else {
       const int r0 = 64 * gq + 32 * h, blk = 2 * wn + (lane >> 4 & 1), r = r0 + (lane >> 1 & 7);
+#pragma unroll
+      for (int s = 0; s < 4; ++s) rows8[s] = ld16(st + kA + kB + 1024 + 2 * (128 * blk + r0 + 8 * s));
       // by hand, with its wait: for the builtin the compiler first drains the loads to LDS just issued
       const uint32_t p = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)(
           st + kA + 128 * r + 16 * (blk ^ (r >> 1 & 3)) + 8 * (lane & 1));
@@ -470,51 +469,80 @@ __global__ __launch_bounds__(512) void k_mx_tile(TileArgs a) {
                    : "=&v"(cols[0]), "=&v"(cols[1]), "=&v"(cols[2]), "=&v"(cols[3])
                    : "v"(p)
                    : "memory");
-#pragma unroll
-      for (int s = 0; s < 4; ++s) rows8[s] = ld16(st + kA + kB + 1024 + 2 * (128 * blk + r0 + 8 * s));
     }
+  };
+  // W's operand of instruction s
+  const auto widen_w = [&](int s) {
     if constexpr (!TRANS) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int r = 64 * wn + 32 * t + c;
-        code[t] = ld16(st + kA + 64 * r + 16 * ((2 * gq + h) ^ (r >> 2 & 3)));
-        scale[t] = e8m0_operand((uint8_t)sm[kRing + ring * T::kScales + 16 * r + 4 * (step - scale_base(step - phase, a.steps)) +
-                                            2 * gq + h]);
+      for (int t = 0; t < 2; ++t) b[s & 1][t] = fp4x8_to_bf16(code[t][s], scale[t]);
+    } else {
+      uint32_t e[8];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {  // the conversion reads the exponent field alone
+        const uint32_t cw = cols[s][i], s01 = rows8[s][2 * i], s23 = rows8[s][2 * i + 1];
+        e[4 * i + 0] = fp4_to_bf16x2<0>(cw, __uint_as_float(s01 << 16));
+        e[4 * i + 1] = fp4_to_bf16x2<1>(cw, __uint_as_float(s01));
+        e[4 * i + 2] = fp4_to_bf16x2<2>(cw, __uint_as_float(s23 << 16));
+        e[4 * i + 3] = fp4_to_bf16x2<3>(cw, __uint_as_float(s23));
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        b[s & 1][0][i] = __builtin_amdgcn_perm(e[2 * i + 1], e[2 * i], 0x05040100u);
+        b[s & 1][1][i] = __builtin_amdgcn_perm(e[2 * i + 1], e[2 * i], 0x07060302u);
       }
     }
+  };
+
+  // the first step's loads (and the scales ahead of them), not those of the next nor the part after it
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(MT + 4));
+  turn_scales(0);
+  lds_meet();
+  int buf = 0, ring = 0;
+  read_w(0, first, 0, 0);
+#pragma unroll
+  for (int i = 0; i < MT; ++i) read_x(0, 0, i);
+  widen_w(0);
+  // Everything of instruction s + 1 is read and widened while instruction s runs, that of a step's first during the last of
+  // the step before, ahead of which the step's loads are waited for and the workgroup meets.  From then on the old step's
+  // buffer is free: the loads of three steps on go there, a part with each instruction (at once they would queue up
+  // before the first of them).  The order is held, and there is no branch in a step: the compiler would sink the
+  // instructions into the block behind it.
+  for (int step = first; step < last; ++step) {
+    const int phase = (step - first) & 3, ahead = min(step + 2, last - 1), to = buf == 0 ? 2 : buf - 1;
+    if constexpr (!TRANS) {
+      if (phase == 0 && a.steps >= 4) issue_scales(step + 4, ring ^ 1);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    int now = buf;
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-      u32x4 b[2];
-      if constexpr (!TRANS) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t) b[t] = fp4x8_to_bf16(code[t][s], scale[t]);
-      } else {
-        uint32_t e[8];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {  // the conversion reads the exponent field alone
-          const uint32_t cw = cols[s][i], s01 = rows8[s][2 * i], s23 = rows8[s][2 * i + 1];
-          e[4 * i + 0] = fp4_to_bf16x2<0>(cw, __uint_as_float(s01 << 16));
-          e[4 * i + 1] = fp4_to_bf16x2<1>(cw, __uint_as_float(s01));
-          e[4 * i + 2] = fp4_to_bf16x2<2>(cw, __uint_as_float(s23 << 16));
-          e[4 * i + 3] = fp4_to_bf16x2<3>(cw, __uint_as_float(s23));
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          b[0][i] = __builtin_amdgcn_perm(e[2 * i + 1], e[2 * i], 0x05040100u);
-          b[1][i] = __builtin_amdgcn_perm(e[2 * i + 1], e[2 * i], 0x07060302u);
-        }
+      if (s == 3) {
+        // the next step's loads (four steps' scales are in by the time they are read)
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm(MT + 2));
+        now = buf == 2 ? 0 : buf + 1;
+        ring ^= (phase + 1) >> 2;
+        turn_scales(now);
+        lds_meet();
       }
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
-        const int r = 32 * i + c;
-        const u32x4 x = ld16(st + 256 * r + 16 * ((8 * gq + 4 * h + s) ^ (r & 15)));
 #pragma unroll
-        for (int t = 0; t < 2; ++t) acc[i][t] = mfma_32x32x16(x, b[t], acc[i][t]);
+        for (int t = 0; t < 2; ++t) acc[i][t] = mfma_32x32x16(xr[s & 1][i], b[s & 1][t], acc[i][t]);
+        __builtin_amdgcn_sched_barrier(0);
+        if (s == 3 && i == MT / 4) read_w(now, step + 1, (phase + 1) & 3, ring);
+        // (two at a time: the wait for them is not to meet the last one just issued)
+        if (2 * i < MT) read_x(now, (s + 1) & 3, 2 * i);
+        if (2 * i + 1 < MT) read_x(now, (s + 1) & 3, 2 * i + 1);
+        if (i == MT - 1) {
+          if (s < 3) issue(ahead, to, s + 1);
+          else issue(min(step + 3, last - 1), buf, 0);
+          widen_w((s + 1) & 3);
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
-      issue(ahead, to, s);  // spread over the step: issued at once the loads queue up before its first instruction
     }
-    if (phase == 3) ring ^= 1;
-    buf = buf == 2 ? 0 : buf + 1;
+    buf = now;
   }
 
   // The two halves' sums meet through LDS: half gq finishes half of the rows (MT 1: half 0 all of them).
