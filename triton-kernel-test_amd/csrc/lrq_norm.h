@@ -66,6 +66,7 @@ struct NormFwd {
   int n;
   int waves, groups;  // of a row, of a workgroup
   float eps;
+  bool past_l2;  // outputs stored past L2
   Drop drop;
 };
 
@@ -88,6 +89,7 @@ struct NormBwd {
   int64_t rows;
   int n;
   int waves, groups;  // of a row, of a workgroup
+  bool past_l2;       // outputs stored past L2
   Drop drop;
 };
 
