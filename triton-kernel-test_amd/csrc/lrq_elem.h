@@ -98,6 +98,14 @@ __device__ __forceinline__ void widen(const Chunk<DT>& c, float* f) {
   }
 }
 
+// Element e of those at p.
+template <int DT>
+__device__ __forceinline__ float ld_elem(const char* p, int e) {
+  if constexpr (DT == kF32) return reinterpret_cast<const float*>(p)[e];
+  const uint32_t v = reinterpret_cast<const uint16_t*>(p)[e];
+  return DT == kBf16 ? __uint_as_float(v << 16) : f16_val(v);
+}
+
 // Rounds to the element type, nearest even.
 template <int DT>
 __device__ __forceinline__ Chunk<DT> narrow(const float* f) {

@@ -9,10 +9,11 @@ __device__ __forceinline__ Chunk<DT> ld_dh(const NormBwd& a, int64_t row, int c,
   return ld_chunk<DT>(a.dh + row * a.lddh * Elem<DT>::kBytes + 8u * Elem<DT>::kBytes * (uint32_t)c, a.dh != nullptr ? k : 0);
 }
 
-// dresidual and dx of one chunk from the norm's input gradient dn, dh and the chunk's random numbers.
+// dresidual and dx of one chunk from the norm's input gradient dn, dh (a partial chunk that was not loaded whole: element
+// by element here) and the chunk's random numbers.
 template <int DT, bool FUSED, bool PAST>
 __device__ __forceinline__ void norm_outputs(const NormBwd& a, int64_t row, int c, int k, float* d, const Chunk<DT>& dh,
-                                             const u32x4& words) {
+                                             bool whole, const u32x4& words) {
   constexpr int ES = Elem<DT>::kBytes;
   if (k <= 0) return;
   if constexpr (FUSED) {
@@ -21,6 +22,12 @@ __device__ __forceinline__ void norm_outputs(const NormBwd& a, int64_t row, int 
       widen<DT>(dh, q);
 #pragma unroll
       for (int e = 0; e < 8; ++e) d[e] = q[e] + d[e];
+      if (!whole) {
+        const char* p = a.dh + row * a.lddh * ES + 8u * ES * (uint32_t)c;
+#pragma unroll
+        for (int e = 0; e < 7; ++e)
+          if (e < k) d[e] = ld_elem<DT>(p, e) + d[e];
+      }
     }
     if (a.dres != nullptr) st_chunk_past<DT>(PAST && a.past_l2, a.dres + row * a.lddr * ES + 8u * ES * (uint32_t)c, narrow<DT>(d), k);
     if (a.drop.keep < 65536u) drop_words(a.drop, words, d);
@@ -38,8 +45,14 @@ __device__ __forceinline__ void norm_outputs(const NormBwd& a, int64_t row, int 
 // (those two were 85 and 131 us; fp32 [8192, 4096] took 97 in place of 81 us so, and four chunks a thread 84 in place of 81).  One chunk a thread: two would hold twice the weights and sums, past
 // the registers.  Rows above 8192 columns take four and keep nothing ahead, [4096, 14336] 81 and 185 us.  No variant may use
 // scratch.
-template <int DT, int LANES, int C, bool FUSED>
+//
+// ODD: rows of one chunk a thread, eight elements at least, that end inside a chunk.  Apart from the others, which then have
+// whole chunks only (with 128 columns or fewer, or four chunks a thread, partial ones as well): tests of the width at run
+// time cost these 2 to 4 %.  [8192, 5003] 59 and 117 us, against 103 and 180 with partial chunks loaded by elements.
+template <int DT, int LANES, int C, bool FUSED, bool ODD>
 __global__ __launch_bounds__(C == 4 ? 512 : 1024) void k_norm_bwd(NormBwd a) {
+  static_assert(C == 1 || !ODD);
+  constexpr bool kPart = ODD || C > 1 || LANES == 16;
   constexpr int ES = Elem<DT>::kBytes, L = LANES == 16 ? 16 : 64;
   // (four chunks a thread, or fp32 rows and the generator, leave no registers for a second row or for what is kept)
   constexpr bool kPrefetch = C == 1 && !(FUSED && DT == kF32), kKeep = kPrefetch;
@@ -55,7 +68,7 @@ __global__ __launch_bounds__(C == 4 ? 512 : 1024) void k_norm_bwd(NormBwd a) {
 #pragma unroll
   for (int j = 0; j < C; ++j) {
     const int c = t + j * tpr;
-    valid[j] = c < nc ? min(8, n - 8 * c) : 0;
+    valid[j] = c < nc ? (kPart ? min(8, n - 8 * c) : 8) : 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) gw[j][e] = 0.f, gb[j][e] = 0.f;
   }
@@ -87,15 +100,15 @@ __global__ __launch_bounds__(C == 4 ? 512 : 1024) void k_norm_bwd(NormBwd a) {
   const int64_t idy = step * a.lddy * ES, ih = step * a.ldh * ES;
   const auto load = [&](int64_t row) {
     Row r;
-    const bool on = row < a.rows;
+    const bool on = row < a.rows, more = ODD && row + 1 < a.rows;
     r.mean = on ? a.mean[row] : 0.f;
     r.rstd = on ? a.rstd[row] : 0.f;
     if constexpr (C > 1) pdy = a.dy + row * a.lddy * ES, ph = a.h + row * a.ldh * ES;
 #pragma unroll
     for (int j = 0; j < C; ++j) {
       const uint32_t at = 8u * ES * (uint32_t)(t + j * tpr);
-      r.dy[j] = ld_chunk<DT>(pdy + at, on ? valid[j] : 0);
-      r.h[j] = ld_chunk<DT>(ph + at, on ? valid[j] : 0);
+      r.dy[j] = ld_chunk<DT>(pdy + at, on ? load_size(valid[j], more) : 0);
+      r.h[j] = ld_chunk<DT>(ph + at, on ? load_size(valid[j], more) : 0);
     }
     if constexpr (C == 1) pdy += idy, ph += ih;
     return r;
@@ -119,6 +132,7 @@ __global__ __launch_bounds__(C == 4 ? 512 : 1024) void k_norm_bwd(NormBwd a) {
       float g[8], z[8];
       const int jw = kHold ? j : 0;
       if constexpr (!kHold) weights(j, wt[0]);
+      if constexpr (ODD) mask_chunk<DT>(cur.dy[j], valid[j]), mask_chunk<DT>(cur.h[j], valid[j]);
       widen<DT>(cur.dy[j], g);
       widen<DT>(cur.h[j], z);
 #pragma unroll
@@ -168,11 +182,12 @@ __global__ __launch_bounds__(C == 4 ? 512 : 1024) void k_norm_bwd(NormBwd a) {
         for (int e = 0; e < 8; ++e) g[e] = __builtin_fmaf(z[e], c2, __builtin_fmaf(g[e], cur.rstd, -c1));
         // asked for here: asked for ahead of the sums it holds up the rows in flight ([16384, 4096]: 127 against 143 us)
         Chunk<DT> dh;
-        if constexpr (FUSED) dh = ld_dh<DT>(a, row, t + j * tpr, valid[j]);
+        const bool whole = !ODD || load_size(valid[j], row + 1 < a.rows) >= 8;
+        if constexpr (FUSED) dh = ld_dh<DT>(a, row, t + j * tpr, !ODD ? valid[j] : whole ? 8 : 0);
         if constexpr (FUSED && C > 1) {
           if (a.drop.keep < 65536u) words = philox((uint64_t)row * nc + t + j * tpr, key);
         }
-        norm_outputs<DT, FUSED, DT != kF32 && C == 1>(a, row, t + j * tpr, valid[j], g, dh, words);
+        norm_outputs<DT, FUSED, DT != kF32 && C == 1>(a, row, t + j * tpr, valid[j], g, dh, whole, words);
         if constexpr (C > 1) __builtin_amdgcn_sched_barrier(0);  // one chunk's temporaries at a time
       }
     }
@@ -243,7 +258,7 @@ __global__ __launch_bounds__(1024) void k_norm_bwd_wide(NormBwd a) {
         dh = ld_dh<DT>(a, row, c, k);
         if (a.drop.keep < 65536u) words = philox((uint64_t)row * nc + c, key);
       }
-      norm_outputs<DT, FUSED, false>(a, row, c, k, g, dh, words);
+      norm_outputs<DT, FUSED, false>(a, row, c, k, g, dh, true, words);
     }
   }
 }
@@ -346,10 +361,11 @@ static int norm_bwd(NormBwd a, hipStream_t s) {
     }
     return launch(kern, dim3((unsigned)p.grid), dim3(threads), lds, s, a);
   };
-  if (p.shape.lanes == 16) return go(k_norm_bwd<DT, 16, 1, FUSED>);
-  if (p.shape.lanes == 64) return go(k_norm_bwd<DT, 64, 1, FUSED>);
-  if (p.shape.chunks == 1) return go(k_norm_bwd<DT, 0, 1, FUSED>);
-  if constexpr (DT != kF32) return go(k_norm_bwd<DT, 0, 4, FUSED>);
+  const bool odd = a.n >= 8 && a.n % 8 != 0;
+  if (p.shape.lanes == 16) return odd ? go(k_norm_bwd<DT, 16, 1, FUSED, true>) : go(k_norm_bwd<DT, 16, 1, FUSED, false>);
+  if (p.shape.lanes == 64) return odd ? go(k_norm_bwd<DT, 64, 1, FUSED, true>) : go(k_norm_bwd<DT, 64, 1, FUSED, false>);
+  if (p.shape.chunks == 1) return odd ? go(k_norm_bwd<DT, 0, 1, FUSED, true>) : go(k_norm_bwd<DT, 0, 1, FUSED, false>);
+  if constexpr (DT != kF32) return go(k_norm_bwd<DT, 0, 4, FUSED, false>);
   return LRQ_ERR_UNSUPPORTED;  // (not reached: wide)
 }
 

@@ -60,6 +60,7 @@ __global__ __launch_bounds__(1024) void k_norm_fwd(NormFwd a) {
   const int grp = wave_row<LANES>(threadIdx.x / tpr), t = threadIdx.x - grp * tpr;
   const int wv = threadIdx.x >> 6, w0 = LANES ? 0 : grp * a.waves;  // this wave, its row's first
   const int n = a.n, nc = (n + 7) / 8;
+  const bool odd = n >= 8 && n % 8 != 0;  // rows end inside a chunk, and are as long as one
   int valid[C];
   float cnt = 0.f;
 #pragma unroll
@@ -101,7 +102,8 @@ __global__ __launch_bounds__(1024) void k_norm_fwd(NormFwd a) {
   const auto load = [&](int64_t row) {
     Row r;
 #pragma unroll
-    for (int j = 0; j < C; ++j) r.in[j] = ld_input<DT, FUSED>(a, row, t + j * tpr, row < a.rows ? valid[j] : 0);
+    for (int j = 0; j < C; ++j)  // (the sums leave out what is past the row)
+      r.in[j] = ld_input<DT, FUSED>(a, row, t + j * tpr, row < a.rows ? load_size(valid[j], odd && row + 1 < a.rows) : 0);
     return r;
   };
   const int64_t step = (int64_t)gridDim.x * a.groups;
