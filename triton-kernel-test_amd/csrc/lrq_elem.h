@@ -70,18 +70,6 @@ __device__ __forceinline__ void st_chunk(char* p, const Chunk<DT>& c, int valid)
   }
 }
 
-// Outputs larger than the L2s together (8 of 4 MB) are stored past them, which leaves them to what is read again; smaller
-// ones stay there for their reader.
-static constexpr int64_t kL2Bytes = 32 << 20;
-template <int DT>
-__device__ __forceinline__ void st_chunk_past(bool past_l2, char* p, const Chunk<DT>& c, int valid) {
-  if (past_l2) {
-    st_chunk<DT, true>(p, c, valid);
-  } else {
-    st_chunk<DT>(p, c, valid);
-  }
-}
-
 template <int DT>
 __device__ __forceinline__ void widen(const Chunk<DT>& c, float* f) {
   if constexpr (DT == kF32) {

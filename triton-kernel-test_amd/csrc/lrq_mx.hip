@@ -17,8 +17,7 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t v) {
 }
 
 // Four lanes a block, 8 columns each: 16-byte loads of consecutive lanes, one dword of codes a lane.  HBM-bound: bf16
-// [16384, 4096] 35 us (4.9 TB/s), and 26.5 us (6.4 TB/s) back, past L2 where the output is larger (27.7 us otherwise;
-// fp32 [8192, 4096] 52 in place of 26 us so).
+// [16384, 4096] 35 us (4.9 TB/s), and 28 us (6.1 TB/s) back.
 template <int DT>
 __global__ __launch_bounds__(256) void k_mx_quantize(const char* x, int64_t ldx, Mx q) {
   constexpr int ES = Elem<DT>::kBytes;
@@ -45,7 +44,7 @@ __global__ __launch_bounds__(256) void k_mx_quantize(const char* x, int64_t ldx,
 }
 
 template <int DT>
-__global__ __launch_bounds__(256) void k_mx_dequantize(Mx q, char* out, int64_t ldo, bool past_l2) {
+__global__ __launch_bounds__(256) void k_mx_dequantize(Mx q, char* out, int64_t ldo) {
   constexpr int ES = Elem<DT>::kBytes;
   const int chunks = (q.cols + 7) / 8;
   const int64_t total = q.rows * chunks;
@@ -58,7 +57,7 @@ __global__ __launch_bounds__(256) void k_mx_dequantize(Mx q, char* out, int64_t 
     const f32x2_t a = fp4_to_f32x2<0>(w, sf), b = fp4_to_f32x2<1>(w, sf), d = fp4_to_f32x2<2>(w, sf),
                   e = fp4_to_f32x2<3>(w, sf);
     v[0] = a[0], v[1] = a[1], v[2] = b[0], v[3] = b[1], v[4] = d[0], v[5] = d[1], v[6] = e[0], v[7] = e[1];
-    st_chunk_past<DT>(DT != kF32 && past_l2, out + (row * ldo + 8 * (int64_t)c) * ES, narrow<DT>(v), min(8, q.cols - 8 * c));
+    st_chunk<DT>(out + (row * ldo + 8 * (int64_t)c) * ES, narrow<DT>(v), min(8, q.cols - 8 * c));
   }
 }
 
@@ -96,11 +95,10 @@ extern "C" int lrq_mxfp4_dequantize(const lrq_mxfp4* t, void* out, int64_t ldo, 
   if (!aligned(out, dtype == LRQ_F32 ? 4 : 2)) return LRQ_ERR_ALIGN;
   const Mx q = make_mx(t);
   const dim3 grid = mx_grid(q.rows * ((q.cols + 7) / 8));
-  const bool past = q.rows * q.cols * 2 > kL2Bytes;
   hipStream_t s = (hipStream_t)stream;
   switch (dtype) {
-    case LRQ_BF16: return launch(k_mx_dequantize<kBf16>, grid, dim3(256), 0, s, q, (char*)out, ldo, past);
-    case LRQ_F16: return launch(k_mx_dequantize<kF16>, grid, dim3(256), 0, s, q, (char*)out, ldo, past);
-    default: return launch(k_mx_dequantize<kF32>, grid, dim3(256), 0, s, q, (char*)out, ldo, past);
+    case LRQ_BF16: return launch(k_mx_dequantize<kBf16>, grid, dim3(256), 0, s, q, (char*)out, ldo);
+    case LRQ_F16: return launch(k_mx_dequantize<kF16>, grid, dim3(256), 0, s, q, (char*)out, ldo);
+    default: return launch(k_mx_dequantize<kF32>, grid, dim3(256), 0, s, q, (char*)out, ldo);
   }
 }

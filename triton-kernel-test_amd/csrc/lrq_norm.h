@@ -81,7 +81,6 @@ struct NormFwd {
   int n;
   int waves, groups;  // of a row, of a workgroup
   float eps;
-  bool past_l2;  // outputs stored past L2
   Drop drop;
 };
 
@@ -104,7 +103,6 @@ struct NormBwd {
   int64_t rows;
   int n;
   int waves, groups;  // of a row, of a workgroup
-  bool past_l2;       // outputs stored past L2
   Drop drop;
 };
 

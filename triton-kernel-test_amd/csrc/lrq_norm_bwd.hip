@@ -11,7 +11,7 @@ __device__ __forceinline__ Chunk<DT> ld_dh(const NormBwd& a, int64_t row, int c,
 
 // dresidual and dx of one chunk from the norm's input gradient dn, dh (a partial chunk that was not loaded whole: element
 // by element here) and the chunk's random numbers.
-template <int DT, bool FUSED, bool PAST>
+template <int DT, bool FUSED>
 __device__ __forceinline__ void norm_outputs(const NormBwd& a, int64_t row, int c, int k, float* d, const Chunk<DT>& dh,
                                              bool whole, const u32x4& words) {
   constexpr int ES = Elem<DT>::kBytes;
@@ -29,10 +29,10 @@ __device__ __forceinline__ void norm_outputs(const NormBwd& a, int64_t row, int 
           if (e < k) d[e] = ld_elem<DT>(p, e) + d[e];
       }
     }
-    if (a.dres != nullptr) st_chunk_past<DT>(PAST && a.past_l2, a.dres + row * a.lddr * ES + 8u * ES * (uint32_t)c, narrow<DT>(d), k);
+    if (a.dres != nullptr) st_chunk<DT>(a.dres + row * a.lddr * ES + 8u * ES * (uint32_t)c, narrow<DT>(d), k);
     if (a.drop.keep < 65536u) drop_words(a.drop, words, d);
   }
-  if (!FUSED || a.dx != nullptr) st_chunk_past<DT>(PAST && a.past_l2, a.dx + row * a.lddx * ES + 8u * ES * (uint32_t)c, narrow<DT>(d), k);
+  if (!FUSED || a.dx != nullptr) st_chunk<DT>(a.dx + row * a.lddx * ES + 8u * ES * (uint32_t)c, narrow<DT>(d), k);
 }
 
 // One pass over dy and h.  A thread owns the same columns in every row of its group, so dy z and dy of the
@@ -40,11 +40,10 @@ __device__ __forceinline__ void norm_outputs(const NormBwd& a, int64_t row, int 
 // k_norm_wgrad adds the workgroups' sums in a fixed order.  The next row is already on the way while one is reduced and
 // written: up to sixteen waves a CU in 128 registers, and few workgroups, whose sums are few.
 //
-// HBM-bound: bf16 [16384, 4096] 69 us (5.8 TB/s), with dh, dropout and both outputs 125 us (5.4 TB/s); [8192, 5120] 50
-// and 96 us (ten waves, so one row at a time a CU: 4.4 TB/s).  16-bit outputs larger than the L2s are stored past them
-// (those two were 85 and 131 us; fp32 [8192, 4096] took 97 in place of 81 us so, and four chunks a thread 84 in place of 81).  One chunk a thread: two would hold twice the weights and sums, past
-// the registers.  Rows above 8192 columns take four and keep nothing ahead, [4096, 14336] 81 and 185 us.  No variant may use
-// scratch.
+// HBM-bound: bf16 [16384, 4096] 80 to 87 us (4.8 TB/s), with dh, dropout and both outputs 126 us (5.3 TB/s); [8192, 5120]
+// 49 and 94 us (ten waves, so one row at a time a CU: 4.5 TB/s).  One chunk a thread: two would hold twice the weights and
+// sums, past the registers.  Rows above 8192 columns take four and keep nothing ahead, [4096, 14336] 79 and 176 us.  No
+// variant may use scratch.
 //
 // ODD: rows of one chunk a thread, eight elements at least, that end inside a chunk.  Apart from the others, which then have
 // whole chunks only (with 128 columns or fewer, or four chunks a thread, partial ones as well): tests of the width at run
@@ -187,7 +186,7 @@ __global__ __launch_bounds__(C == 4 ? 512 : 1024) void k_norm_bwd(NormBwd a) {
         if constexpr (FUSED && C > 1) {
           if (a.drop.keep < 65536u) words = philox((uint64_t)row * nc + t + j * tpr, key);
         }
-        norm_outputs<DT, FUSED, DT != kF32 && C == 1>(a, row, t + j * tpr, valid[j], g, dh, whole, words);
+        norm_outputs<DT, FUSED>(a, row, t + j * tpr, valid[j], g, dh, whole, words);
         if constexpr (C > 1) __builtin_amdgcn_sched_barrier(0);  // one chunk's temporaries at a time
       }
     }
@@ -258,7 +257,7 @@ __global__ __launch_bounds__(1024) void k_norm_bwd_wide(NormBwd a) {
         dh = ld_dh<DT>(a, row, c, k);
         if (a.drop.keep < 65536u) words = philox((uint64_t)row * nc + c, key);
       }
-      norm_outputs<DT, FUSED, false>(a, row, c, k, g, dh, true, words);
+      norm_outputs<DT, FUSED>(a, row, c, k, g, dh, true, words);
     }
   }
 }
@@ -410,7 +409,7 @@ extern "C" int lrq_layer_norm_bwd(const lrq_dropout* drop, const void* dy, int64
     const bool fused = drop != nullptr || dh != nullptr || dresidual != nullptr;
     const NormBwd a{(const char*)dy, lddy, (const char*)dh, lddh, (const char*)h, ldh, mean, rstd, w, w_dtype, (char*)dx,
                     lddx, (char*)dresidual, ld_dresidual, wgrad ? (float*)workspace : nullptr, rows, (int)n,
-                    0, 0, rows * n * es > kL2Bytes, make_drop(drop)};
+                    0, 0, make_drop(drop)};
     const auto go = [&] {
       switch (dtype) {
         case LRQ_BF16: return fused ? norm_bwd<kBf16, true>(a, s) : norm_bwd<kBf16, false>(a, s);

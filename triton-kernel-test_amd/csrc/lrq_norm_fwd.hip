@@ -37,7 +37,7 @@ __device__ __forceinline__ void norm_input(const NormFwd& a, const DropKey& key,
       }
       // the statistics are those of h as stored
       const Chunk<DT> hc = narrow<DT>(v);
-      st_chunk_past<DT>(DT != kF32 && a.past_l2, a.h + row * a.ldh * Elem<DT>::kBytes + 8u * Elem<DT>::kBytes * (uint32_t)c, hc, k);
+      st_chunk<DT>(a.h + row * a.ldh * Elem<DT>::kBytes + 8u * Elem<DT>::kBytes * (uint32_t)c, hc, k);
       widen<DT>(hc, v);
     }
   }
@@ -47,11 +47,12 @@ __device__ __forceinline__ void norm_input(const NormFwd& a, const DropKey& key,
 // squared deviations from it) and the waves' parts are merged (Chan, Golub and LeVeque's update), so a
 // row costs one barrier and the variance never comes from a difference of large sums.
 //
-// HBM-bound: bf16 [16384, 4096] 46 us (5.8 TB/s; a copy reaches 5.2), with dropout and the residual 86 us (6.2 TB/s), whose
-// generator runs under the next row's loads.  16-bit outputs larger than the L2s are stored past them (49 and 94 us
-// otherwise; fp32 [8192, 4096] 54 in place of 49 us so).  Two chunks a thread (one above 512 columns costs a second row's worth of
-// waves and barriers); [8192, 5120] 33 and 62 us.  fp32 rows that start off alignment, [1003, 5003]: 14 us, two rounds of
-// rows for a load's latency each.
+// HBM-bound: bf16 [16384, 4096] 47 us (5.7 TB/s; a copy reaches 5.2), with dropout and the residual 93 us (5.8 TB/s), whose
+// generator runs under the next row's loads.  (Stored past the caches the outputs take 3 and 8 us less, and their reader
+// more than that longer: 78 against 75 us with a quantisation of y behind it.)  Two chunks a thread (one above 512 columns
+// costs a second row's worth of waves and barriers); [8192, 5120] 32 and 64 us, [8192, 5003] 34 and 69 us (rows that end
+// inside a chunk are read whole; 40 and 86 by elements).  fp32 [1003, 5003]: 13 us, two rounds of rows for a load's latency
+// each.
 template <int DT, int LANES, int C, bool FUSED, bool SAME>
 __global__ __launch_bounds__(1024) void k_norm_fwd(NormFwd a) {
   constexpr int ES = Elem<DT>::kBytes, L = LANES == 16 ? 16 : 64;
@@ -179,7 +180,7 @@ __global__ __launch_bounds__(1024) void k_norm_fwd(NormFwd a) {
       float o[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) o[e] = __builtin_fmaf((v[j][e] - mean) * rstd, wt[k][e], bs[k][e]);
-      st_chunk_past<DT>(DT != kF32 && a.past_l2, a.y + row * a.ldy * ES + 8u * ES * (uint32_t)(t + j * tpr), narrow<DT>(o), valid[j]);
+      st_chunk<DT>(a.y + row * a.ldy * ES + 8u * ES * (uint32_t)(t + j * tpr), narrow<DT>(o), valid[j]);
     }
   }
 }
@@ -283,7 +284,7 @@ extern "C" int lrq_layer_norm_fwd(const lrq_dropout* drop, const void* x, int64_
       !aligned(b, ws) || !aligned(mean, 4) || !aligned(rstd, 4))
     return LRQ_ERR_ALIGN;
   const NormFwd a{(const char*)x, ldx, (const char*)residual, ld_residual, (char*)h, ldh, (char*)y, ldy, mean, rstd, w, b,
-                  w_dtype, rows, (int)n, 0, 0, eps, n <= kNormMaxWidth && rows * n * es > kL2Bytes, make_drop(drop)};
+                  w_dtype, rows, (int)n, 0, 0, eps, make_drop(drop)};
   hipStream_t s = (hipStream_t)stream;
   switch (dtype) {
     case LRQ_BF16: return fused ? norm_fwd<kBf16, true>(a, s) : norm_fwd<kBf16, false>(a, s);
