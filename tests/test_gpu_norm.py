@@ -148,6 +148,42 @@ def test_layer_norm_strides_and_empty(pkg, dev):
     assert y.shape == (0, 333) and dx.shape == (0, 333) and not dw.any() and not db.any()
 
 
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("n", [1, 5, 9, 77, 333, 1001, 5003, 9001])
+def test_rows_of_a_buffer_of_nans(pkg, dev, n, dtype):
+    """Rows that end inside a chunk, with NaN and infinity right behind them (and behind the last): nothing of it shows."""
+    dt = DT[dtype]
+    print(f"[norm] nans n={n} {dtype}", flush=True)
+
+    def view(seed, pad):
+        buf = torch.full((20, n + pad), float("nan"), dtype=dt, device=dev)
+        buf[:, n:] = torch.tensor([float("inf"), float("nan"), float("-inf")] * 5, dtype=dt, device=dev)[:pad]
+        buf[1:18, :n] = _x((17, n), dt, dev, seed)
+        return buf, buf[1:18, :n]
+
+    (bx, x), (br, res), (by, dy), (bh, dh) = (view(200 + i, p) for i, p in enumerate((1, 3, 7, 13)))
+    kept = [t.clone() for t in (bx, br, by, bh)]
+    w, b = _w(n, dt, dev, 205)
+    c = [t.contiguous() for t in (x, res, dy, dh)]
+
+    def run(x, res, dy, dh):
+        y, mean, rstd = pkg.layer_norm_forward(x, w, b)
+        y2, h, m2, r2 = pkg.dropout_add_layer_norm_forward(x, res, w, b, 0.2, (SEED, 1))
+        return (y, mean, rstd, *pkg.layer_norm_backward(dy, x, w, mean, rstd), y2, h, m2, r2,
+                *pkg.dropout_add_layer_norm_backward(dy, dh, h, w, m2, r2, 0.2, (SEED, 1)),
+                pkg.dropout(x, 0.2, 3), pkg.dropout(x, 0.2, 3, residual=res), pkg.mxfp4_quantize(x).codes)
+
+    for got, want in zip(run(x, res, dy, dh), run(*c)):
+        assert torch.isfinite(got.float()).all() and torch.equal(got, want)
+    # the same where h, whose rows the backward pass reads, is such a view
+    _, mean, rstd = pkg.layer_norm_forward(x, w, b)
+    for got, want in zip(pkg.dropout_add_layer_norm_backward(dy, dh, x, w, mean, rstd, 0.2, 9),
+                         pkg.dropout_add_layer_norm_backward(c[2], c[3], c[0], w, mean, rstd, 0.2, 9)):
+        assert torch.equal(got, want)
+    for t, k in zip((bx, br, by, bh), kept):
+        assert torch.equal(_bits(t), _bits(k))
+
+
 # ---------------------------------------------------------------- dropout
 @pytest.mark.parametrize("dtype", list(DT))
 @pytest.mark.parametrize("shape", [(1, 1), (1, 7), (5, 8), (3, 9), (33, 1001), (2, 3, 77), (7, 4096), (2, 20000)])

@@ -34,13 +34,15 @@ __global__ __launch_bounds__(256) void k_dropout(DropArgs a) {
     const char* x = a.x + row * a.ldx * ES;
     const char* res = a.res + row * a.ldr * ES;
     char* out = a.out + row * a.ldo * ES;
+    const bool more = a.n >= 8 && row + 1 < a.rows;
     for (int c0 = blockIdx.y * a.tpr * kAhead + t; c0 < nc; c0 += a.tpr * kAhead * gridDim.y) {
       Chunk<DT> xc[kAhead], rc[kAhead];
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {
         const int64_t c = c0 + k * a.tpr;
-        xc[k] = ld_chunk<DT, true>(x + 8 * c * ES, (int)(a.n - 8 * c));
-        if constexpr (RES) rc[k] = ld_chunk<DT, true>(res + 8 * c * ES, (int)(a.n - 8 * c));
+        const int size = load_size((int)(a.n - 8 * c), more);
+        xc[k] = ld_chunk<DT, true>(x + 8 * c * ES, size);
+        if constexpr (RES) rc[k] = ld_chunk<DT, true>(res + 8 * c * ES, size);
       }
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {

@@ -45,21 +45,6 @@ __device__ __forceinline__ int wave_row(int grp) {
   return LANES == 16 ? grp : (int)__builtin_amdgcn_readfirstlane(grp);
 }
 
-// How many elements of a chunk to load: a row's partial chunk is read whole, up to 7 elements into what follows the row,
-// where a further row keeps that inside the tensor (element loads are joined as they arrive, so a thread that waits for
-// them holds up the rows in flight: bf16 [8192, 5003] backward 103 us).  What lies past the row is masked.
-__device__ __forceinline__ int load_size(int valid, bool more_rows) { return more_rows && valid > 0 ? 8 : valid; }
-
-template <int DT>
-__device__ __forceinline__ void mask_chunk(Chunk<DT>& c, int valid) {
-  if (valid >= 8) return;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    if constexpr (DT == kF32) c.v[e / 4][e % 4] = e < valid ? c.v[e / 4][e % 4] : 0u;
-    else c.v[0][e / 2] &= e < valid ? ~0u : (e & 1) ? 0xffffu : 0xffff0000u;
-  }
-}
-
 // The widest row of the register-resident kernels; wider rows sweep the row again.
 static constexpr int64_t kNormMaxWidth = 16384;
 
