@@ -106,7 +106,7 @@ def test_tile(m, n, k, trans):
     steps, wsteps = -(-depth // 128), -(-k // 128)
     ldc, lds, chunks = 64 * wsteps, 4 * wsteps, -(-depth // 8)
     ldx = 8 * chunks
-    ka, stage = 32 * mt * 256, 32 * mt * 256 + 16384 + (3072 if trans else 0)
+    ka, stage = 32 * mt * 256, 32 * mt * 256 + 16384 + (3 * 1024 if trans else 0)
     loop = 3 * stage + (0 if trans else 8192)
     assert max(loop, (4 * mt if mt >= 2 else 4) * 8192) <= 160 * 1024
     for m0, n0 in _tiles(m, 32 * mt, cols):

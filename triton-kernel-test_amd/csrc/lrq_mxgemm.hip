@@ -341,7 +341,7 @@ struct TileArgs {
 // 512 rows.
 template <bool TRANS, int MT>
 struct TileLds {
-  static constexpr int kA = 32 * MT * 256, kB = 16384, kS = TRANS ? 3072 : 0, kStage = kA + kB + kS, kDeep = 3;
+  static constexpr int kA = 32 * MT * 256, kB = 16384, kS = TRANS ? 3 * 1024 : 0, kStage = kA + kB + kS, kDeep = 3;
   static constexpr int kScales = TRANS ? 0 : 4096, kLoop = kDeep * kStage + 2 * kScales;
   static constexpr int kJoin = (MT >= 2 ? 8 * MT / 2 : 4) * 8192, kBytes = kLoop > kJoin ? kLoop : kJoin;
 };
@@ -466,10 +466,10 @@ __global__ __launch_bounds__(512) void k_mx_tile(TileArgs a) {
       const uint32_t p = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)(
           st + kA + 128 * r + 16 * (blk ^ (r >> 1 & 3)) + 8 * (lane & 1));
       asm volatile("ds_read_b64_tr_b8 %0, %4\n\tds_read_b64_tr_b8 %1, %4 offset:1024\n\t"
-                   "ds_read_b64_tr_b8 %2, %4 offset:2048\n\tds_read_b64_tr_b8 %3, %4 offset:3072\n\t"
+                   "ds_read_b64_tr_b8 %2, %4 offset:2048\n\tds_read_b64_tr_b8 %3, %4 offset:%5\n\t"
                    "s_waitcnt lgkmcnt(0)"
                    : "=&v"(cols[0]), "=&v"(cols[1]), "=&v"(cols[2]), "=&v"(cols[3])
-                   : "v"(p)
+                   : "v"(p), "n"(3 * 1024)
                    : "memory");
     }
   };
