@@ -159,14 +159,16 @@ def test_tile(m, n, k, trans):
 
 
 @pytest.mark.parametrize("rows,n,k", [(1, 1, 1), (1, 16, 32), (2, 17, 33), (4, 300, 4096), (5, 129, 1000), (16, 256, 128),
-                                      (3, 40, 9000), (9, 8300, 300), (16, 300, 5000), (1, 14336, 4096)])
+                                      (3, 40, 9000), (9, 8300, 300), (16, 300, 5000), (1, 14336, 4096), (7, 14336, 4096)])
 def test_token(rows, n, k):
     steps, cap = -(-k // 128), 4 if rows <= 4 else 16
-    wgs = -(-n // 16)
-    waves = (4 if wgs >= 512 or steps <= 64 else 8) if rows <= 4 else (4 if wgs >= 512 else 8)
+    tiles = -(-n // 16)
+    waves = (4 if tiles >= 512 or steps <= 64 else 8) if rows <= 4 else (4 if tiles >= 512 else 8)
+    cols = 2 if rows > 4 and tiles >= 512 else 1
+    wgs = -(-tiles // cols)
     depth = 8 if cap == 4 else 4
     krow, ldc, lds, ldx = 256 * depth, 64 * steps, 4 * steps, -(-k // 8) * 8
-    assert waves * cap * krow + waves * 1024 <= 160 * 1024
+    assert waves * cap * krow + waves * cols * 1024 <= 160 * 1024
     per = -(-steps // waves)
     j, g = LANE & 15, LANE >> 4
     for wave in range(waves):
@@ -179,7 +181,7 @@ def test_token(rows, n, k):
                     if at.size:
                         _inside(2 * (r * ldx + at), 16, 2 * rows * ldx, "x")
                     assert ((wave * cap + r) * krow + 1024 * i) + 1024 <= waves * cap * krow
-            for n0 in {0, 16 * (wgs - 1)}:
+            for n0 in {16 * cols * wg + 16 * t for wg in (0, wgs - 1) for t in range(cols)}:
                 w = np.minimum(n0 + j, n - 1)
                 for u in range(depth):
                     _inside(w * ldc + 16 * g + 64 * min(s0 + u, last - 1), 16, n * ldc, "codes")

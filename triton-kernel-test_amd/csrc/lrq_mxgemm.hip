@@ -237,30 +237,38 @@ __global__ __launch_bounds__(512) void k_mx_gemm(GemmArgs p) {
 }
 
 // ---------------------------------------------------------------- bf16 rows, few of them
-// Up to ROWS rows of X (a decoding step) by 16 rows of W a workgroup; each of its WAVES waves takes a run of the K steps
-// of 128 and they join in LDS.  Lane (j, g) reads the 16 code bytes of block g of W row j: its k are 32g .. 32g + 31, 8
+// Up to ROWS rows of X (a decoding step) by 16 COLS rows of W a workgroup; each of its WAVES waves takes a run of the K
+// steps of 128 and they join in LDS.  Lane (j, g) reads the 16 code bytes of block g of W row j: its k are 32g .. 32g + 31, 8
 // of them for each of the step's four matrix instructions, and X is read in the same order.  Everything a wave needs
 // for its next D steps is in flight at once: X's columns go to the wave's own part of LDS (16-byte piece i of row r in
 // slot i ^ r, so that the 16 rows' reads fall in different banks), the codes and scales to registers.  The time is the
 // codes' arrival after a fixed 4 us: one row by [14336, 4096] 8.4 us for 31 MB (9.8 from HBM), by [4096, 4096] 4.6 us for
-// 9 MB; 16 rows 13.0 and 5.4 us, where every workgroup reads all of X through L2.  A dword of scales a step in place of 16
-// bytes for four took 10.8 us.
-template <int ROWS, int WAVES, bool F32>
+// 9 MB.  Every workgroup reads all of X through L2, so with more than four rows it takes two tiles of W where that leaves
+// 256 workgroups: 16 rows by [14336, 4096] 12.1 us (one tile: 14.8), 5 rows 9.5 (10.4).  A dword of scales a step in place
+// of 16 bytes for four took 10.8 us.
+template <int ROWS, int WAVES, int COLS, bool F32>
 __global__ __launch_bounds__(64 * WAVES) void k_mx_token(const uint16_t* x, int64_t ldx, int rows, Mx w, void* out,
                                                          int64_t ldo) {
   constexpr int D = ROWS > 4 ? 4 : 8, kRow = 256 * D;
   __shared__ __attribute__((aligned(16))) char xs[WAVES][ROWS][kRow];
-  __shared__ f32x4 red[WAVES][64];
+  __shared__ f32x4 red[WAVES][COLS][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 15, g = lane >> 4;
-  const int64_t n0 = (int64_t)blockIdx.x * 16, rw = min(n0 + j, w.rows - 1);
+  const int64_t n0 = (int64_t)blockIdx.x * 16 * COLS;
   const int per = (w.steps + WAVES - 1) / WAVES, first = min(wave * per, w.steps), last = min(first + per, w.steps);
-  const uint8_t* codes = w.codes + rw * w.ldc + 16 * g;
-  const uint8_t* scales = w.scales + rw * w.lds;
+  const uint8_t *codes[COLS], *scales[COLS];
+#pragma unroll
+  for (int t = 0; t < COLS; ++t) {
+    const int64_t rw = min(n0 + 16 * t + j, w.rows - 1);
+    codes[t] = w.codes + rw * w.ldc + 16 * g;
+    scales[t] = w.scales + rw * w.lds;
+  }
   const int row = min(j, rows - 1);  // (lanes past X's rows repeat its last: their rows of the product are not stored)
-  f32x4 acc = zero4();
+  f32x4 acc[COLS];
+#pragma unroll
+  for (int t = 0; t < COLS; ++t) acc[t] = zero4();
   for (int s0 = first; s0 < last; s0 += D) {
-    u32x4 c[D];
-    uint32_t sc[D];
+    u32x4 c[COLS][D];
+    uint32_t sc[COLS][D];
     for (int r = 0; r < rows; ++r)
 #pragma unroll
       for (int i = 0; i < kRow / 1024; ++i) {
@@ -268,43 +276,53 @@ __global__ __launch_bounds__(64 * WAVES) void k_mx_token(const uint16_t* x, int6
         ld_to_lds<16>(k < w.cols ? (const void*)(x + r * ldx + k) : &kZeroChunk, &xs[wave][r][1024 * i]);
       }
 #pragma unroll
-    for (int u = 0; u < D; ++u) {
-      const int s = min(s0 + u, last - 1);
-      c[u] = ld16_stream(codes + 64 * (int64_t)s);
-    }
+    for (int t = 0; t < COLS; ++t)
+#pragma unroll
+      for (int u = 0; u < D; ++u) c[t][u] = ld16_stream(codes[t] + 64 * (int64_t)min(s0 + u, last - 1));
     if (s0 + D <= w.steps) {  // 16 bytes of scales a load, four steps
 #pragma unroll
-      for (int u = 0; u < D; u += 4) {
-        const u32x4 v = ld16_any(scales + 4 * (int64_t)(s0 + u));
-        sc[u] = v[0], sc[u + 1] = v[1], sc[u + 2] = v[2], sc[u + 3] = v[3];
-      }
+      for (int t = 0; t < COLS; ++t)
+#pragma unroll
+        for (int u = 0; u < D; u += 4) {
+          const u32x4 v = ld16_any(scales[t] + 4 * (int64_t)(s0 + u));
+          sc[t][u] = v[0], sc[t][u + 1] = v[1], sc[t][u + 2] = v[2], sc[t][u + 3] = v[3];
+        }
     } else {
 #pragma unroll
-      for (int u = 0; u < D; ++u) sc[u] = ld4(scales + 4 * (int64_t)min(s0 + u, last - 1));
+      for (int t = 0; t < COLS; ++t)
+#pragma unroll
+        for (int u = 0; u < D; ++u) sc[t][u] = ld4(scales[t] + 4 * (int64_t)min(s0 + u, last - 1));
     }
     __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
     asm volatile("" ::: "memory");
 #pragma unroll
     for (int u = 0; u < D; ++u) {
       if (s0 + u >= last) break;
-      const float sf = e8m0_operand(sc[u] >> (8 * g));
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        acc = mfma_16x16x32(ld16(&xs[wave][row][16 * ((16 * u + 4 * g + q) ^ row)]), fp4x8_to_bf16(c[u][q], sf), acc);
+      for (int q = 0; q < 4; ++q) {
+        const u32x4 x8 = ld16(&xs[wave][row][16 * ((16 * u + 4 * g + q) ^ row)]);
+#pragma unroll
+        for (int t = 0; t < COLS; ++t)
+          acc[t] = mfma_16x16x32(x8, fp4x8_to_bf16(c[t][u][q], e8m0_operand(sc[t][u] >> (8 * g))), acc[t]);
+      }
     }
     __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the reads are done before the next steps' X lands
   }
-  red[wave][lane] = acc;
+#pragma unroll
+  for (int t = 0; t < COLS; ++t) red[wave][t][lane] = acc[t];
   __syncthreads();
   if (threadIdx.x >= 256) return;
   // 16 columns of an output row to 16 threads
   const int l = (threadIdx.x & 15) + (threadIdx.x >> 2 & 48), v = threadIdx.x >> 4 & 3;
-  float sum = 0.f;
-#pragma unroll
-  for (int k = 0; k < WAVES; ++k) sum += red[k][l][v];
   const int m = 4 * (l >> 4) + v;
-  const int64_t n = n0 + (l & 15);
-  if (m < rows && n < w.rows) st_out<F32>(out, m * ldo + n, sum);
+#pragma unroll
+  for (int t = 0; t < COLS; ++t) {
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < WAVES; ++k) sum += red[k][t][l][v];
+    const int64_t n = n0 + 16 * t + (l & 15);
+    if (m < rows && n < w.rows) st_out<F32>(out, m * ldo + n, sum);
+  }
 }
 
 // ---------------------------------------------------------------- bf16 rows, many of them
@@ -750,21 +768,22 @@ static int mx_linear(const void* x, int64_t ldx, int64_t rows, const lrq_mxfp4* 
   const uint16_t* px = (const uint16_t*)x;
   if (!trans && rows <= 16) {
     using std::integral_constant;
-    const dim3 grid((unsigned)((w.rows + 15) / 16));
-    const auto go = [&](auto r, auto waves) {
-      return out_fp32 ? launch((k_mx_token<r(), waves(), true>), grid, dim3(64 * waves()), 0, s, px, ldx, (int)rows, w, out, ldo)
-                      : launch((k_mx_token<r(), waves(), false>), grid, dim3(64 * waves()), 0, s, px, ldx, (int)rows, w, out, ldo);
+    const int64_t tiles = (w.rows + 15) / 16;
+    const auto go = [&](auto r, auto waves, auto cols) {
+      const dim3 grid((unsigned)((tiles + cols() - 1) / cols()));
+      return out_fp32 ? launch((k_mx_token<r(), waves(), cols(), true>), grid, dim3(64 * waves()), 0, s, px, ldx, (int)rows, w, out, ldo)
+                      : launch((k_mx_token<r(), waves(), cols(), false>), grid, dim3(64 * waves()), 0, s, px, ldx, (int)rows, w, out, ldo);
     };
     // four waves a workgroup (8 steps each of 4096 columns: one round of loads); eight where workgroups are few and the
     // runs long, 11.3 against 13.3 us on 4096 rows of 14336 columns (but 6.3 against 5.2 us on 4096 of 4096); with 16
     // rows, whose runs are of four steps, there always
-#define LRQ_GO(R, W) return go(integral_constant<int, R>{}, integral_constant<int, W>{})
+#define LRQ_GO(R, W, C) return go(integral_constant<int, R>{}, integral_constant<int, W>{}, integral_constant<int, C>{})
     if (rows <= 4) {
-      if (grid.x >= 512 || w.steps <= 64) LRQ_GO(4, 4);
-      LRQ_GO(4, 8);
+      if (tiles >= 512 || w.steps <= 64) LRQ_GO(4, 4, 1);
+      LRQ_GO(4, 8, 1);
     }
-    if (grid.x >= 512) LRQ_GO(16, 4);
-    LRQ_GO(16, 8);
+    if (tiles >= 512) LRQ_GO(16, 4, 2);
+    LRQ_GO(16, 8, 1);
 #undef LRQ_GO
   }
   const SplitPlan p = split_plan(rows, t, trans);

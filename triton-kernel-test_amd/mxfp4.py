@@ -1,7 +1,7 @@
 """Microscaled 4-bit floating point (OCP MXFP4): quantisation, and products with operands held in it.
 
 A weight in MXFP4 takes 17/32 of a byte an element.  ``mxfp4_linear`` multiplies bf16 activations by it
-(a frozen base weight: the reference's profiles keep theirs in another 4-bit format through a closed
+(a frozen base weight: the reference's profiles keep theirs in another 4-bit format through another
 library) and ``mxfp4_linear_backward`` is the gradient for the activations; ``mxfp4_gemm`` multiplies two
 MXFP4 operands on the scaled matrix instructions.  ``autograd.mxfp4_linear`` and
 ``autograd.lora_linear_compressed`` (an ``MXFP4Tensor`` as its base weight) call them.
