@@ -41,16 +41,21 @@ __device__ __forceinline__ void norm_outputs(const NormBwd& a, int64_t row, int 
 // written: up to sixteen waves a CU in 128 registers, and few workgroups, whose sums are few.
 //
 // HBM-bound: bf16 [16384, 4096] 80 to 87 us (4.8 TB/s), with dh, dropout and both outputs 126 us (5.3 TB/s); [8192, 5120]
-// 49 and 94 us (ten waves, so one row at a time a CU: 4.5 TB/s).  One chunk a thread: two would hold twice the weights and
+// 49 and 86 us (ten waves, so one row at a time a CU: 4.9 TB/s).  One chunk a thread: two would hold twice the weights and
 // sums, past the registers.  Rows above 8192 columns take four and keep nothing ahead, [4096, 14336] 79 and 176 us.  No
 // variant may use scratch.
 //
 // ODD: rows of one chunk a thread, eight elements at least, that end inside a chunk.  Apart from the others, which then have
 // whole chunks only (with 128 columns or fewer, or four chunks a thread, partial ones as well): tests of the width at run
 // time cost these 2 to 4 %.  [8192, 5003] 59 and 117 us, against 103 and 180 with partial chunks loaded by elements.
-template <int DT, int LANES, int C, bool FUSED, bool ODD>
+//
+// EARLY: dh comes with its row, where the workgroup has one row at a time ([8192, 5120] 102 -> 86 us; behind the next row's
+// loads it waits for them).  With more rows in flight it comes when it is used ([16384, 4096] 130 against 135 us).
+enum { kNormPlain = 0, kNormOdd = 1, kNormEarly = 2 };
+template <int DT, int LANES, int C, bool FUSED, int MODE>
 __global__ __launch_bounds__(C == 4 ? 512 : 1024) void k_norm_bwd(NormBwd a) {
-  static_assert(C == 1 || !ODD);
+  constexpr bool ODD = MODE == kNormOdd, kDh = MODE == kNormEarly;
+  static_assert(C == 1 || MODE == kNormPlain);
   constexpr bool kPart = ODD || C > 1 || LANES == 16;
   constexpr int ES = Elem<DT>::kBytes, L = LANES == 16 ? 16 : 64;
   // (four chunks a thread, or fp32 rows and the generator, leave no registers for a second row or for what is kept)
@@ -87,7 +92,7 @@ __global__ __launch_bounds__(C == 4 ? 512 : 1024) void k_norm_bwd(NormBwd a) {
   DropKey key{};
   if constexpr (FUSED) key = drop_key(a.drop);
   struct Row {
-    Chunk<DT> dy[C], h[C];
+    Chunk<DT> dy[C], h[C], dh;  // (dh: kDh)
     float mean, rstd;
   };
   // a group past the last row works on zeros; elements past the row are zero in dy, so they add nothing to any sum (z is
@@ -109,6 +114,7 @@ __global__ __launch_bounds__(C == 4 ? 512 : 1024) void k_norm_bwd(NormBwd a) {
       r.dy[j] = ld_chunk<DT>(pdy + at, on ? load_size(valid[j], more) : 0);
       r.h[j] = ld_chunk<DT>(ph + at, on ? load_size(valid[j], more) : 0);
     }
+    if constexpr (kDh) r.dh = ld_dh<DT>(a, row, t, on ? valid[0] : 0);
     if constexpr (C == 1) pdy += idy, ph += ih;
     return r;
   };
@@ -179,10 +185,10 @@ __global__ __launch_bounds__(C == 4 ? 512 : 1024) void k_norm_bwd(NormBwd a) {
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) g[e] = __builtin_fmaf(z[e], c2, __builtin_fmaf(g[e], cur.rstd, -c1));
-        // asked for here: asked for ahead of the sums it holds up the rows in flight ([16384, 4096]: 127 against 143 us)
         Chunk<DT> dh;
         const bool whole = !ODD || load_size(valid[j], row + 1 < a.rows) >= 8;
-        if constexpr (FUSED) dh = ld_dh<DT>(a, row, t + j * tpr, !ODD ? valid[j] : whole ? 8 : 0);
+        if constexpr (kDh) dh = cur.dh;
+        else if constexpr (FUSED) dh = ld_dh<DT>(a, row, t + j * tpr, !ODD ? valid[j] : whole ? 8 : 0);
         if constexpr (FUSED && C > 1) {
           if (a.drop.keep < 65536u) words = philox((uint64_t)row * nc + t + j * tpr, key);
         }
@@ -361,10 +367,16 @@ static int norm_bwd(NormBwd a, hipStream_t s) {
     return launch(kern, dim3((unsigned)p.grid), dim3(threads), lds, s, a);
   };
   const bool odd = a.n >= 8 && a.n % 8 != 0;
-  if (p.shape.lanes == 16) return odd ? go(k_norm_bwd<DT, 16, 1, FUSED, true>) : go(k_norm_bwd<DT, 16, 1, FUSED, false>);
-  if (p.shape.lanes == 64) return odd ? go(k_norm_bwd<DT, 64, 1, FUSED, true>) : go(k_norm_bwd<DT, 64, 1, FUSED, false>);
-  if (p.shape.chunks == 1) return odd ? go(k_norm_bwd<DT, 0, 1, FUSED, true>) : go(k_norm_bwd<DT, 0, 1, FUSED, false>);
-  if constexpr (DT != kF32) return go(k_norm_bwd<DT, 0, 4, FUSED, false>);
+  if (p.shape.lanes == 16) return odd ? go(k_norm_bwd<DT, 16, 1, FUSED, kNormOdd>) : go(k_norm_bwd<DT, 16, 1, FUSED, kNormPlain>);
+  if (p.shape.lanes == 64) return odd ? go(k_norm_bwd<DT, 64, 1, FUSED, kNormOdd>) : go(k_norm_bwd<DT, 64, 1, FUSED, kNormPlain>);
+  if (p.shape.chunks == 1) {
+    if (odd) return go(k_norm_bwd<DT, 0, 1, FUSED, kNormOdd>);
+    if constexpr (FUSED && DT != kF32) {
+      if (p.groups == 1) return go(k_norm_bwd<DT, 0, 1, FUSED, kNormEarly>);
+    }
+    return go(k_norm_bwd<DT, 0, 1, FUSED, kNormPlain>);
+  }
+  if constexpr (DT != kF32) return go(k_norm_bwd<DT, 0, 4, FUSED, kNormPlain>);
   return LRQ_ERR_UNSUPPORTED;  // (not reached: wide)
 }
 
