@@ -42,7 +42,7 @@ __device__ __forceinline__ void norm_outputs(const NormBwd& a, int64_t row, int 
 //
 // HBM-bound: bf16 [16384, 4096] 80 to 87 us (4.8 TB/s), with dh, dropout and both outputs 126 us (5.3 TB/s); [8192, 5120]
 // 49 and 86 us (ten waves, so one row at a time a CU: 4.9 TB/s).  One chunk a thread: two would hold twice the weights and
-// sums, past the registers.  Rows above 8192 columns take four and keep nothing ahead, [4096, 14336] 79 and 176 us.  No
+// sums, past the registers.  Rows above 8192 columns take four and keep nothing ahead, [4096, 14336] 80 and 176 to 190 us.  No
 // variant may use scratch.
 //
 // ODD: rows of one chunk a thread, eight elements at least, that end inside a chunk.  Apart from the others, which then have
