@@ -31,6 +31,10 @@ HIPFLAGS = [
     "-ffp-contract=off",
     # MFMA results straight into VGPRs (no v_accvgpr_read round trips in the epilogues)
     "-mllvm", "-amdgpu-mfma-vgpr-form",
+    # every masked region restores its own mask.  Where two regions end together the compiler would leave out the inner
+    # restore, and spilled registers reloaded between the two ends then miss the lanes that skipped the inner region: a row
+    # loop whose step was reloaded so never ended.  Costs a scalar instruction a region: times are the same within noise.
+    "-mllvm", "-amdgpu-remove-redundant-endcf=0",
     # IEEE mode off: v_min/v_max of MFMA results need no canonicalising moves.  The kernels
     # assume finite inputs (NaN / Inf activations give unspecified codes, never a fault).
     "-fno-honor-nans", "-mno-amdgpu-ieee",
