@@ -35,10 +35,19 @@ HIPFLAGS = [
     # restore, and spilled registers reloaded between the two ends then miss the lanes that skipped the inner region: a row
     # loop whose step was reloaded so never ended.  Costs a scalar instruction a region: times are the same within noise.
     "-mllvm", "-amdgpu-remove-redundant-endcf=0",
-    # IEEE mode off: v_min/v_max of MFMA results need no canonicalising moves.  The kernels
-    # assume finite inputs (NaN / Inf activations give unspecified codes, never a fault).
-    "-fno-honor-nans", "-mno-amdgpu-ieee",
 ]
+
+# The compressed format assumes finite inputs (NaN / Inf activations give unspecified codes, never a fault).  IEEE mode
+# off: v_min/v_max of MFMA results need no canonicalising moves.
+FINITE_FLAGS = ["-fno-honor-nans", "-mno-amdgpu-ieee"]
+
+# The layer norm, dropout and MXFP4 kernels carry NaN and infinity through their row or block.  Without NaNs honoured
+# every operation on one would be undefined to the compiler, so these are built with the language's own arithmetic.
+CARRY_NAN = {"lrq_dropout", "lrq_mx", "lrq_mxgemm", "lrq_norm_bwd", "lrq_norm_fwd"}
+
+
+def flags(src: Path) -> list[str]:
+    return HIPFLAGS if src.stem in CARRY_NAN else HIPFLAGS + FINITE_FLAGS
 
 
 def hipcc() -> str:
@@ -50,7 +59,7 @@ def hipcc() -> str:
 
 def _compile(src: Path) -> Path:
     obj = BUILD / (src.stem + ".o")
-    cmd = [hipcc(), *HIPFLAGS, "-c", str(src), "-o", str(obj)]
+    cmd = [hipcc(), *flags(src), "-c", str(src), "-o", str(obj)]
     res = subprocess.run(cmd, capture_output=True, text=True)
     noise = "is not a recognized feature for this target"
     err = "\n".join(l for l in (res.stderr or "").splitlines() if noise not in l)

@@ -26,6 +26,12 @@ struct Chunk {
 
 typedef u32x4 u32x4_any __attribute__((aligned(2)));
 
+template <int DT>
+__device__ __forceinline__ void pin(Chunk<DT>& c) {
+#pragma unroll
+  for (int k = 0; k < Elem<DT>::kVecs; ++k) pin(c.v[k]);
+}
+
 // `valid` elements of the chunk at p (8 or more: the whole chunk; 0 or less: none); the others are 0.
 template <int DT, bool STREAM = false>
 __device__ __forceinline__ Chunk<DT> ld_chunk(const char* p, int valid) {

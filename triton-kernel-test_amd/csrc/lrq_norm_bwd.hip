@@ -119,7 +119,14 @@ __global__ __launch_bounds__(C == 4 ? 512 : 1024) void k_norm_bwd(NormBwd a) {
     return r;
   };
   Row cur;
-  if constexpr (kPrefetch) cur = load(row0);
+  if constexpr (kPrefetch) {
+    cur = load(row0);
+    // here ahead of the loop, or the wait for it is in the loop, where it meets the next row's loads as well
+    asm volatile("" : "+v"(cur.mean), "+v"(cur.rstd));
+    pin(cur.dy[0]);
+    pin(cur.h[0]);
+    if constexpr (kDh) pin(cur.dh);
+  }
   for (int64_t r0 = (int64_t)blockIdx.x * a.groups; r0 < a.rows; r0 += step) {
     const int64_t row = r0 + grp;
     const bool on = row < a.rows;

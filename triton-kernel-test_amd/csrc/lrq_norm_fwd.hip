@@ -110,7 +110,15 @@ __global__ __launch_bounds__(1024) void k_norm_fwd(NormFwd a) {
   const int64_t step = (int64_t)gridDim.x * a.groups;
   constexpr bool kPrefetch = C == 1 || !FUSED || DT != kF32;  // (two fp32 rows of two inputs: too many registers)
   Row cur;
-  if constexpr (kPrefetch) cur = load((int64_t)blockIdx.x * a.groups + grp);
+  if constexpr (kPrefetch) {
+    cur = load((int64_t)blockIdx.x * a.groups + grp);
+    // here ahead of the loop, or the wait for it is in the loop, where it meets the next row's loads as well
+#pragma unroll
+    for (int j = 0; j < C; ++j) {
+      pin(cur.in[j].x);
+      if constexpr (FUSED) pin(cur.in[j].res);
+    }
+  }
   // Every thread takes every step (barriers): a group past the last row works on zeros.  The next row is on its way
   // while this one is reduced and written.
   for (int64_t r0 = (int64_t)blockIdx.x * a.groups; r0 < a.rows; r0 += step) {
