@@ -49,3 +49,25 @@ def test_no_kernel_spills(tmp_path):
         assert sum(stem in n for n in mine) >= least, stem
     bad = {n: v for n, v in mine.items() if v != (0, 0)}
     assert not bad, bad
+
+
+def test_no_kernel_spills_scalars(tmp_path):
+    """Nor do they spill scalar registers (to lanes of a vector register, which a kernel short of those then lacks)."""
+    L = importlib.import_module("triton-kernel-test_amd._lib")
+    readelf = Path("/opt/rocm/llvm/bin/llvm-readelf")
+    readelf = str(readelf) if readelf.exists() else shutil.which("llvm-readelf")
+    if not L.LIB_PATH.exists() or readelf is None:
+        pytest.skip("needs the built library and llvm-readelf")
+    bad, count = {}, 0
+    for i, obj in enumerate(_code_objects(L.LIB_PATH.read_bytes())):
+        f = tmp_path / f"{i}.elf"
+        f.write_bytes(obj)
+        notes = subprocess.run([readelf, "--notes", str(f)], capture_output=True, text=True, check=True).stdout
+        for kernel in notes.split("\n  - .agpr_count:")[1:]:
+            name = re.search(r"\.symbol:\s+'?(\S+?)\.kd", kernel).group(1)
+            if re.search(r"k_(norm|dropout|mx)_?", name):
+                count += 1
+                spilled = int(re.search(r"\.sgpr_spill_count:\s+(\d+)", kernel).group(1))
+                if spilled:
+                    bad[name] = spilled
+    assert count >= 100 and not bad, (count, bad)

@@ -32,6 +32,10 @@ __device__ __forceinline__ void pin(Chunk<DT>& c) {
   for (int k = 0; k < Elem<DT>::kVecs; ++k) pin(c.v[k]);
 }
 
+// What is compared with v is compared afresh behind this: a partial chunk's seven comparisons and the tests of a whole one,
+// kept over a loop, take a pair of scalar registers each, for every chunk of a thread.
+__device__ __forceinline__ void opaque(int& v) { asm volatile("" : "+v"(v)); }
+
 // `valid` elements of the chunk at p (8 or more: the whole chunk; 0 or less: none); the others are 0.
 template <int DT, bool STREAM = false>
 __device__ __forceinline__ Chunk<DT> ld_chunk(const char* p, int valid) {

@@ -124,6 +124,10 @@ __global__ __launch_bounds__(1024) void k_norm_fwd(NormFwd a) {
   for (int64_t r0 = (int64_t)blockIdx.x * a.groups; r0 < a.rows; r0 += step) {
     const int64_t row = r0 + grp;
     const bool on = row < a.rows;
+    if constexpr (FUSED && C > 1) {  // (its scalar registers do not hold them all)
+#pragma unroll
+      for (int j = 0; j < C; ++j) opaque(valid[j]);
+    }
     Row next;
     if constexpr (kPrefetch) next = load(row + step);
     else cur = load(row);
