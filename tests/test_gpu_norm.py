@@ -184,6 +184,32 @@ def test_rows_of_a_buffer_of_nans(pkg, dev, n, dtype):
         assert torch.equal(_bits(t), _bits(k))
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("n", [4, 12, 256, 300, 1000, 1003, 5003, 9001, 16387])
+def test_layer_norm_backward_of_large_means(pkg, dev, n, dtype):
+    """Rows of 2^96 with a mean of that and a reciprocal deviation of 2^33: every z is 0, while (0 - mean) rstd of a place
+    past the row's end overflows.  dx = rstd (g - mean(g)), dw = 0."""
+    dt = DT[dtype]
+    print(f"[norm] large means n={n} {dtype}", flush=True)
+    rows = 5
+    x = torch.full((rows, n), 2.0 ** 96, dtype=dt, device=dev)
+    dy = _x((rows, n), dt, dev, 300 + n, 0.1)
+    mean, rstd = torch.full((rows,), 2.0 ** 96, device=dev), torch.full((rows,), 2.0 ** 33, device=dev)
+    g = dy.double().cpu()
+    ref = 2.0 ** 33 * (g - g.mean(-1, keepdim=True))
+    # the sum's roundings and the division's, the two terms' difference; the factor is a power of two
+    adds = R.Norm64(x[:1], None, None, EPS).adds
+    e = 2.0 ** 33 * R.U * ((adds + 4) * g.abs().mean(-1, keepdim=True) + 4 * g.abs())
+    bound = R.half_step(dt) * (ref.abs() + e) + e
+    dx, dw, db = pkg.layer_norm_backward(dy, x, None, mean, rstd)
+    R.assert_within(dx, ref, bound, "dx")
+    assert not dw.any()
+    R.assert_within(db, g.sum(0), (rows + 8) * R.U * g.abs().sum(0), "db")
+    dx2, dres, dw, _ = pkg.dropout_add_layer_norm_backward(dy, None, x, None, mean, rstd, 0.0, 0)
+    R.assert_within(dres, ref, bound, "dresidual")
+    assert not dw.any()
+
+
 # ---------------------------------------------------------------- dropout
 @pytest.mark.parametrize("dtype", list(DT))
 @pytest.mark.parametrize("shape", [(1, 1), (1, 7), (5, 8), (3, 9), (33, 1001), (2, 3, 77), (7, 4096), (2, 20000)])

@@ -9,6 +9,14 @@ __device__ __forceinline__ Chunk<DT> ld_dh(const NormBwd& a, int64_t row, int c,
   return ld_chunk<DT>(a.dh + row * a.lddh * Elem<DT>::kBytes + 8u * Elem<DT>::kBytes * (uint32_t)c, a.dh != nullptr ? k : 0);
 }
 
+// Elements past the row (a chunk holds `valid`) take the row's mean in place of h, so that their z is 0: (0 - mean) rstd may
+// overflow where no element of the row does, and their dy of 0 times that is NaN.
+__device__ __forceinline__ void fill_mean(float* h, int valid, float mean) {
+  if (valid >= 8) return;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) h[e] = e < valid ? h[e] : mean;
+}
+
 // dresidual and dx of one chunk from the norm's input gradient dn, dh (a partial chunk that was not loaded whole: element
 // by element here) and the chunk's random numbers.
 template <int DT, bool FUSED>
@@ -95,8 +103,8 @@ __global__ __launch_bounds__(C == 4 ? 512 : 1024) void k_norm_bwd(NormBwd a) {
     Chunk<DT> dy[C], h[C], dh;  // (dh: kDh)
     float mean, rstd;
   };
-  // a group past the last row works on zeros; elements past the row are zero in dy, so they add nothing to any sum (z is
-  // finite there for finite statistics; a row whose statistics are not finite is lost anyway)
+  // a group past the last row works on zeros; elements past the row have a dy and a z of zero and add nothing to any sum (a
+  // row whose statistics are not finite is lost anyway)
   int slot = 0;
   const int64_t step = (int64_t)gridDim.x * a.groups, row0 = (int64_t)blockIdx.x * a.groups + grp;
   // the row to load, stepped along (with four chunks a thread computed instead: no registers to spare)
@@ -148,9 +156,10 @@ __global__ __launch_bounds__(C == 4 ? 512 : 1024) void k_norm_bwd(NormBwd a) {
       float g[8], z[8];
       const int jw = kHold ? j : 0;
       if constexpr (!kHold) weights(j, wt[0]);
-      if constexpr (ODD) mask_chunk<DT>(cur.dy[j], valid[j]), mask_chunk<DT>(cur.h[j], valid[j]);
+      if constexpr (ODD) mask_chunk<DT>(cur.dy[j], valid[j]);
       widen<DT>(cur.dy[j], g);
       widen<DT>(cur.h[j], z);
+      fill_mean(z, valid[j], cur.mean);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float zz = (z[e] - cur.mean) * cur.rstd, gg = g[e] * wt[jw][e];
@@ -179,6 +188,7 @@ __global__ __launch_bounds__(C == 4 ? 512 : 1024) void k_norm_bwd(NormBwd a) {
       const float c1 = cur.rstd * (s1 * rn), c2 = -cur.rstd * (s2 * rn);
 #pragma unroll
       for (int j = 0; j < C; ++j) {
+        if constexpr (C > 1) opaque(valid[j]);
         float g[8], z[8];
         if constexpr (kKeep) {
 #pragma unroll
@@ -246,6 +256,7 @@ __global__ __launch_bounds__(1024) void k_norm_bwd_wide(NormBwd a) {
       if (a.w != nullptr) ld_weight(a.w, a.wdt, 8 * (int64_t)c, k, w);
       widen<DT>(ld_chunk<DT>(a.dy + (row * a.lddy + 8 * (int64_t)c) * ES, k), g);
       widen<DT>(ld_chunk<DT>(a.h + (row * a.ldh + 8 * (int64_t)c) * ES, k), z);
+      fill_mean(z, k, mean);
 #pragma unroll
       for (int e = 0; e < 8; ++e) z[e] = (z[e] - mean) * rstd, g[e] *= w[e];
     };
