@@ -184,6 +184,34 @@ def test_dropout_probability_and_seed(pkg):
             N._drop(0.25, bad, dev)
 
 
+def test_no_dropout_needs_no_seed(pkg):
+    N, dev = pkg.norm, torch.device("cpu")
+    d, s = N._drop(0.0, None, dev)
+    assert d.keep == 65536 and d.state is None and s is None
+    for p in (1e-9, 0.5, 1.0):
+        with pytest.raises(ValueError):
+            N._drop(p, None, dev)
+
+
+@pytest.mark.gpu
+def test_no_dropout_needs_no_seed_on_the_device(pkg, dev):
+    """p = 0 without a seed: dropout is the identity (plus the residual), its gradient too, in every form."""
+    AG = pkg.autograd
+    x, r = (torch.randn(5, 40, device=dev).requires_grad_() for _ in range(2))
+    assert torch.equal(pkg.dropout(x.detach(), 0.0, None), x)
+    dy = torch.randn(5, 40, device=dev)
+    y = AG.dropout(x, 0.0, None, residual=r)
+    y.backward(dy)
+    assert torch.equal(y, r + x) and torch.equal(x.grad, dy) and torch.equal(r.grad, dy)
+    want = AG.dropout_add_layer_norm(x, r, None, None, 0.0, 7)
+    for got, e in zip(AG.dropout_add_layer_norm(x, r, None, None, 0.0, None), want):
+        assert torch.equal(got, e)
+    y, h, mean, rstd = pkg.dropout_add_layer_norm_forward(x.detach(), r.detach(), None, None, 0.0, None)
+    assert torch.equal(y, want[0]) and torch.equal(h, want[1])
+    got = pkg.dropout_add_layer_norm_backward(dy, None, h, None, mean, rstd, 0.0, None)
+    assert torch.equal(got[0], pkg.dropout_add_layer_norm_backward(dy, None, h, None, mean, rstd, 0.0, 7)[0])
+
+
 @pytest.mark.gpu
 def test_python_refusals(pkg, dev):
     x = torch.zeros(4, 8, dtype=torch.bfloat16, device=dev)

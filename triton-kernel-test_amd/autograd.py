@@ -207,8 +207,7 @@ class _DropoutAddLayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, weight, bias, p, seed, eps):
         ctx.p, ctx.seed, state = _seeded(p, seed)
-        y, h, mean, rstd = _norm.dropout_add_layer_norm_forward(x, residual, weight, bias, p, 0 if seed is None else seed,
-                                                                eps)
+        y, h, mean, rstd = _norm.dropout_add_layer_norm_forward(x, residual, weight, bias, p, seed, eps)
         ctx.save_for_backward(h, weight, mean, rstd, state)
         ctx.bias_dtype = None if bias is None else bias.dtype
         ctx.set_materialize_grads(False)
@@ -221,7 +220,7 @@ class _DropoutAddLayerNorm(torch.autograd.Function):
         if dy is None and dh is None:
             return (None,) * 7
         dy = torch.zeros_like(h) if dy is None else dy
-        seed = 0 if ctx.p == 0.0 else _with_state(ctx.seed, state)
+        seed = _with_state(ctx.seed, state)
         _, need_r, need_w, need_b = ctx.needs_input_grad[:4]
         dx, dres, dw, db = _norm.dropout_add_layer_norm_backward(dy, dh, h, weight, mean, rstd, ctx.p, seed,
                                                                  weight_grad=need_w or need_b)

@@ -11,8 +11,8 @@ Dropout's mask is a function of (seed, offset, row, column) and is never stored:
 gradient with the same seed is the backward pass.  ``seed`` is an int, a pair (seed, offset), or an int64
 device tensor of those two words, alone or with a further offset as (tensor, offset): such a tensor
 is read when the kernel runs, so a captured graph draws a new mask in each replay if its second word is
-advanced in between (give each dropout of the graph an offset of its own).  An element takes 16 random bits:
-p is rounded to a multiple of 1 / 65536 (at least one for p > 0, at most 65535 for p < 1).
+advanced in between (give each dropout of the graph an offset of its own).  With p = 0 it may be None.  An element
+takes 16 random bits: p is rounded to a multiple of 1 / 65536 (at least one for p > 0, at most 65535 for p < 1).
 """
 
 from __future__ import annotations
@@ -115,6 +115,8 @@ def _drop(p: float, seed, device: torch.device) -> tuple[LrqDropout, Optional[to
         state, seed = seed, 0
         if state.dtype != torch.int64 or state.numel() != 2 or state.device != device or not state.is_contiguous():
             raise ValueError(f"a seed tensor must be two contiguous int64 words on {device}")
+    if seed is None and keep == 65536:  # nothing is drawn
+        seed = 0
     if isinstance(seed, bool) or not isinstance(seed, int) or isinstance(offset, bool) or not isinstance(offset, int):
         raise ValueError("seed and offset must be ints")
     m = (1 << 64) - 1
