@@ -76,22 +76,24 @@ class LoRALinearCompressed(torch.autograd.Function):
     def forward(ctx, x, w, a, b, basis: Optional[LowRankBasis], bits: int, group: int, fused: bool = True,
                 dropout_p: float = 0.0, seed=None):
         ctx.p, ctx.seed, state = _seeded(dropout_p, seed)
-        ctx.mx = w if isinstance(w, _mx.MXFP4Tensor) else None
-        if ctx.p == 0.0 and ctx.mx is None:
+        mx = isinstance(w, _mx.MXFP4Tensor)
+        if ctx.p == 0.0 and not mx:
             y = compute_lora(x, w, a, b)
         else:
             x2 = _flat(x)
             xd = _norm.dropout(x2, ctx.p, seed) if ctx.p > 0.0 else x2
-            base = _mx.mxfp4_linear(x2, w) if ctx.mx is not None else x2 @ w.mT
+            base = _mx.mxfp4_linear(x2, w) if mx else x2 @ w.mT
             y = torch.addmm(base, xd @ a, b).reshape(x.shape[:-1] + (w.shape[0],))
         ctx.c = encode(x.detach(), basis, bits=bits, group_size=group)
         ctx.fused = fused
-        ctx.save_for_backward(None if ctx.mx is not None else w, a, b, state)
+        ctx.mx, weight = _weight(w) if mx else (None, (w,))
+        ctx.save_for_backward(a, b, state, *weight)
         return y
 
     @staticmethod
     def backward(ctx, dy):
-        w, a, b, state = ctx.saved_tensors
+        a, b, state, *weight = ctx.saved_tensors
+        w = weight[0] if ctx.mx is None else _saved_weight(ctx.mx, *weight)
         c, ctx.c = ctx.c, None
         dy2 = _flat(dy)
         codes = ctx.fused and ctx.p == 0.0 and _codes_gemm_ok(c, a, dy2)
@@ -103,7 +105,7 @@ class LoRALinearCompressed(torch.autograd.Function):
                 dx, da, db = compute_lora_gradient(dy2, _flat(decode(c)), w, a, b)
         else:
             g = dy2 @ b.mT
-            dx = _mx.mxfp4_linear_backward(dy2, ctx.mx) if ctx.mx is not None else dy2 @ w
+            dx = _mx.mxfp4_linear_backward(dy2, w) if ctx.mx is not None else dy2 @ w
             if ctx.p > 0.0:
                 dx = _norm.dropout(g @ a.mT, ctx.p, _with_state(ctx.seed, state), residual=dx)
             else:
@@ -235,16 +237,29 @@ def dropout_add_layer_norm(x: torch.Tensor, residual: Optional[torch.Tensor], we
     return _DropoutAddLayerNorm.apply(x, residual, weight, bias, p, seed, eps)
 
 
+def _weight(w: "_mx.MXFP4Tensor"):
+    """(what the context keeps of w, the tensors to save): the backward pass refuses a weight changed in between.  Tensors
+    made in inference mode carry no version and cannot be saved; such a weight is kept as it is."""
+    if w.codes.is_inference() or w.scales.is_inference():
+        return w, (None, None)
+    return w.shape, (w.codes, w.scales)
+
+
+def _saved_weight(kept, codes, scales):
+    return kept if codes is None else _mx.MXFP4Tensor(codes, scales, kept)
+
+
 class _MXFP4Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, out_dtype):
-        ctx.w = w
+        ctx.w, weight = _weight(w)
+        ctx.save_for_backward(*weight)
         return _mx.mxfp4_linear(x, w, out_dtype)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        return _mx.mxfp4_linear_backward(dy.to(torch.bfloat16), ctx.w), None, None
+        return _mx.mxfp4_linear_backward(dy.to(torch.bfloat16), _saved_weight(ctx.w, *ctx.saved_tensors)), None, None
 
 
 def mxfp4_linear(x: torch.Tensor, w: "_mx.MXFP4Tensor", out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
