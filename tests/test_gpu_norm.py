@@ -34,8 +34,8 @@ def _bits(t):
     return t.view(torch.int16 if t.element_size() == 2 else torch.int32)
 
 
-# row widths: one element, inside a chunk, one chunk, the limits of each register geometry (16, 64, 256 and 1024
-# threads, one to three chunks each) and past the last one; odd widths start rows off every alignment
+# row widths: one element, inside a chunk, one chunk, the limits of each register geometry (16 lanes, a wave or several whole
+# waves a row, of one, two or four chunks a thread) and past the last one; odd widths start rows off every alignment
 WIDTHS = [1, 3, 8, 77, 128, 129, 512, 1000, 1024, 1025, 2048, 2050, 4096, 4099, 5120, 6144, 6145, 8192, 8200, 16384,
           16385, 20011]
 
@@ -81,6 +81,63 @@ def test_layer_norm_many_rows(pkg, dev, rows, n):
     for got, g2, r, bound, name in zip(first, again, refs, bounds, ("dx", "dw", "db")):
         R.assert_within(got, r, bound, name)
         assert torch.equal(_bits(got), _bits(g2)), name
+
+
+# (rows, columns) whose row groups walk several rows each: 16 lanes, a wave and several waves a row, rows of whole chunks and
+# rows that end inside one, wave counts that do and do not divide a workgroup's sixteen, one group a workgroup and several
+GEOMETRIES = [(17000, 96), (17000, 100), (17000, 5), (5000, 512), (5000, 333), (3000, 1000), (3000, 1003), (2700, 1300),
+              (2700, 1304), (1500, 2000), (1500, 2003), (1700, 2500), (1700, 2504), (1100, 2900), (1100, 2904), (1100, 3500),
+              (1100, 3504), (1030, 4096), (530, 4500), (530, 4504), (1003, 5003), (600, 5120), (530, 8000), (530, 8190),
+              (520, 9001), (520, 9008), (530, 16390)]
+
+
+def _backward_plan(rows, n, fp32):
+    """The backward pass's launch (csrc/lrq_norm_bwd.hip, csrc/lrq_norm.h): kind of rows, lanes and chunks a thread, groups of
+    a workgroup, workgroups, parts of the weight gradients."""
+    nc = -(-n // 8)
+    if n > (8192 if fp32 else 16384):
+        return "wide", 0, 0, 1, min(rows, 512), min(-(-rows // 4), 64)
+    chunks = 1 if nc <= 1024 else 4
+    lanes = 16 if nc <= 16 else 64 if nc <= 64 * chunks else 0
+    waves = -(-nc // (64 * chunks))
+    most = 64 * (8 if chunks == 4 else 16) // lanes if lanes else max(1, (8 if chunks == 4 else 16) // waves)
+    groups = min(most, max(1, 4 * -(-rows // 1024) if lanes == 16 else -(-rows // 256)))
+    grid = min(-(-rows // groups), 256)
+    kind = "plain" if chunks > 1 or n < 8 or n % 8 == 0 else "odd"
+    return kind, lanes, chunks, groups, grid, grid
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("rows,n", GEOMETRIES)
+def test_layer_norm_of_every_geometry(pkg, dev, rows, n, dtype):
+    """Plain and fused, both ways, with dh and the weights' gradients, against 64 bits."""
+    dt, p, seed = DT[dtype], 0.2, (SEED, 9)
+    print(f"[norm] geometry rows={rows} n={n} {dtype}", flush=True)
+    x, res, dy, dh = (_x((rows, n), dt, dev, 400 + i, 0.1) for i in range(4))
+    w, b = _w(n, dt, dev, 404)
+    y, mean, rstd = pkg.layer_norm_forward(x, w, b, EPS)
+    plain = pkg.layer_norm_backward(dy, x, w, mean, rstd)
+    y2, h, mean2, rstd2 = pkg.dropout_add_layer_norm_forward(x, res, w, b, p, seed, EPS)
+    fused = pkg.dropout_add_layer_norm_backward(dy, dh, h, w, mean2, rstd2, p, seed)
+    torch.cuda.synchronize()
+    ref = R.Norm64(x, w, b, EPS)
+    R.assert_within(y, ref.y, ref.bound_y(dt), "y")
+    refs, bounds, _ = ref.grads(dy, dt, dt)
+    for got, r, bound, name in zip(plain, refs, bounds, ("dx", "dw", "db")):
+        R.assert_within(got, r, bound, name)
+    d64, mask = R.drop64(x, p, *seed)
+    h64 = res.double().cpu() + d64
+    e = 3 * R.U * (d64.abs() + res.double().cpu().abs())
+    R.assert_within(h, h64, R.half_step(dt) * (h64.abs() + e) + e + R.smallest(dt), "h")
+    ref = R.Norm64(h, w, b, EPS)
+    R.assert_within(y2, ref.y, ref.bound_y(dt), "fused y")
+    (rd, rdw, rdb), (bd, bw, bb), e_d = ref.grads(dy, dt, dt, dh=dh)
+    R.assert_within(fused[1], rd, bd, "dresidual")
+    rdx = rd * mask
+    e = e_d * mask + 2 * R.U * rdx.abs()
+    R.assert_within(fused[0], rdx, R.half_step(dt) * (rdx.abs() + e) + e + R.smallest(dt), "fused dx")
+    R.assert_within(fused[2], rdw, bw, "fused dw")
+    R.assert_within(fused[3], rdb, bb, "fused db")
 
 
 def test_layer_norm_without_weights_and_mixed_types(pkg, dev):
