@@ -191,3 +191,45 @@ def test_token(rows, n, k):
                 else:
                     for u in range(depth):
                         _inside(w * lds + 4 * min(s0 + u, last - 1), 4, n * lds, "scales")
+
+
+def _matrix(pkg, rows, cols):
+    steps = -(-cols // 128)
+    return pkg._lib.LrqMxfp4(0x10000, 64 * steps, 0x20000, 4 * steps, rows, cols)
+
+
+@pytest.mark.parametrize("m,n,k", SIZES)
+def test_the_plans_are_the_librarys(pkg, m, n, k):
+    """The splits that the replays above take are those whose parts the library asks a workspace for."""
+    import ctypes
+
+    def want(splits, rows, cols):
+        return splits * rows * (-(-cols // 4) * 4) * 4 if splits > 1 else 0
+
+    a, w = ctypes.byref(_matrix(pkg, m, k)), ctypes.byref(_matrix(pkg, n, k))
+    _, splits = _plan(m, n, k, 64, (0.35, 0.4, 0.6), lambda s, t: (s + 3) * t, 4)
+    assert pkg._lib.call_raw("lrq_mxfp4_gemm_workspace", a, w) == want(splits, m, n)
+    for trans in (0, 1):
+        cols, depth = (k, n) if trans else (n, k)
+        _, splits = _plan(m, cols, depth, 32, (0.6, 1.0, 1.6) if trans else (0.53, 0.72, 1.4), lambda s, t: s * t + 9, 2)
+        if not trans and m <= 16:
+            splits = 1  # the few-row kernel
+        assert pkg._lib.call_raw("lrq_mxfp4_linear_workspace", m, w, trans) == want(splits, m, cols)
+
+
+def _distinct(inst, count, what):
+    """Every (wave, load) pair's kilobyte, all pairs counted: each of `count` once."""
+    flat = np.concatenate([np.broadcast_to(i, (8, 1)).ravel() for i in inst])
+    assert flat.size == count and sorted(flat.tolist()) == list(range(count)), what
+
+
+@pytest.mark.parametrize("mt", [1, 2, 4])
+def test_no_two_waves_load_to_the_same_place(mt):
+    if mt >= 2:
+        _distinct([mt // 2 * WAVE + i for i in range(mt // 2)], 4 * mt, "both operands: A")
+    else:  # the upper four waves load the same again: from the same rows to the same place
+        inst = (WAVE & 3).ravel()
+        assert inst[:4].tolist() == inst[4:].tolist() == [0, 1, 2, 3]
+    _distinct([2 * WAVE + i for i in range(2)], 16, "both operands: B")
+    _distinct([mt * WAVE + i for i in range(mt)], 8 * mt, "x")
+    _distinct([2 * WAVE + i for i in range(2)], 16, "codes")
