@@ -82,6 +82,8 @@ class LoRALinearCompressed(torch.autograd.Function):
         else:
             x2 = _flat(x)
             xd = _norm.dropout(x2, ctx.p, seed) if ctx.p > 0.0 else x2
+            # the base product in x's type before the branch is added, as compute_lora has it: in fp32 it would be
+            # written and read again at twice the bytes
             base = _mx.mxfp4_linear(x2, w) if mx else x2 @ w.mT
             y = torch.addmm(base, xd @ a, b).reshape(x.shape[:-1] + (w.shape[0],))
         ctx.c = encode(x.detach(), basis, bits=bits, group_size=group)
@@ -107,6 +109,7 @@ class LoRALinearCompressed(torch.autograd.Function):
             g = dy2 @ b.mT
             dx = _mx.mxfp4_linear_backward(dy2, w) if ctx.mx is not None else dy2 @ w
             if ctx.p > 0.0:
+                # (dy W and g A^T rounded to dy's type ahead of their sum, which takes them from memory)
                 dx = _norm.dropout(g @ a.mT, ctx.p, _with_state(ctx.seed, state), residual=dx)
             else:
                 dx = torch.addmm(dx, g, a.mT)
@@ -259,6 +262,7 @@ class _MXFP4Linear(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
+        # the product's rows are bf16, a matrix instruction's operand beside the widened weight; dx, of x's type, is bf16 too
         return _mx.mxfp4_linear_backward(dy.to(torch.bfloat16), _saved_weight(ctx.w, *ctx.saved_tensors)), None, None
 
 

@@ -1,7 +1,7 @@
 // Dropout and dropout + residual add: out = residual + (kept ? x * 65536 / keep : 0); the numbers are
 // those of lrq_dropout.h.  The same call on the output's gradient is dropout's backward pass.
-// HBM-bound by its traffic (x, the residual, out); the generator's ten rounds run under it: bf16 [16384, 4096] 45.5 us
-// (5.9 TB/s), with a residual 63 us (6.4 TB/s); a copy reaches 5.2.
+// HBM-bound by its traffic (x, the residual, out); the generator's ten rounds run under it: bf16 [16384, 4096] 45 us
+// (6.0 TB/s), with a residual 61 to 64 us (6.3 to 6.6 TB/s); a copy reaches 5.2.
 #include "lrq_dropout.h"
 
 #include <algorithm>

@@ -101,7 +101,7 @@ __device__ __forceinline__ void short_scales(const uint8_t* row, int steps, char
 // [4096, 4096] x [14336, 4096]: 146 to 157 us on different cards, 3.1 to 3.3 PFLOP/s.  A step's instructions alone take
 // 0.48 us of the matrix unit at 2.1 GHz; a step takes 0.78 us on zeros and 0.9 to 1.1 us on random data, where the card
 // lowers its clock for power; 15 us are the output's 117 MB, which no other workgroup's work covers (144 KB of LDS: one
-// workgroup a CU).
+// workgroup a CU).  The last of four rounds of tiles is half empty.
 template <int MT>
 struct GemmLds {
   static constexpr int kA = 64 * MT * 64, kB = 16384, kStage = kA + kB, kDeep = 4;
@@ -242,10 +242,11 @@ __global__ __launch_bounds__(512) void k_mx_gemm(GemmArgs p) {
 // of them for each of the step's four matrix instructions, and X is read in the same order.  Everything a wave needs
 // for its next D steps is in flight at once: X's columns go to the wave's own part of LDS (16-byte piece i of row r in
 // slot i ^ r, so that the 16 rows' reads fall in different banks), the codes and scales to registers.  The time is the
-// codes' arrival after a fixed 4 us: one row by [14336, 4096] 8.4 us for 31 MB (9.8 from HBM), by [4096, 4096] 4.6 us for
-// 9 MB.  Every workgroup reads all of X through L2, so with more than four rows it takes two tiles of W where that leaves
-// 256 workgroups: 16 rows by [14336, 4096] 12.1 us (one tile: 14.8), 5 rows 9.5 (10.4).  A dword of scales a step in place
-// of 16 bytes for four took 10.8 us.
+// codes' arrival after a fixed 4 us: one row by [14336, 4096] 8.4 to 9.8 us for 31 MB where they lie in the last-level
+// cache and 10.8 to 11.8 from HBM, by [4096, 4096] 4.6 us for 9 MB.  Every workgroup reads all of X through L2, so with
+// more than four rows it takes two tiles of W where that leaves 256 workgroups: 16 rows by [14336, 4096] 12.1 us, 12.8 to
+// 13.0 from HBM (one tile: 14.8), 5 rows 9.5 (10.4).  A dword of scales a step in place of 16 bytes for four took 10.8 us
+// for one row, against 8.4.
 template <int ROWS, int WAVES, int COLS, bool F32>
 __global__ __launch_bounds__(64 * WAVES) void k_mx_token(const uint16_t* x, int64_t ldx, int rows, Mx w, void* out,
                                                          int64_t ldo) {
@@ -353,10 +354,10 @@ struct TileArgs {
 //   TRANS true: the lane's two columns are one code byte of each W row.  The transposing LDS read gives it that byte
 //   of 8 rows at once; each is widened with its own row's scale and the halves of two rows are paired by v_perm_b32.
 //
-// 512 rows by [14336, 4096]: 54 to 56 us, and 56 us and a join of 8 us for the gradient (1.1 and 1.0 PFLOP/s; 42 us each at
-// the 1.44 PFLOP/s of a large bf16 product on random data, which power limits: on zeros a step takes 1.27 us, on random
-// data 1.4 to 1.7, its instructions alone 0.96 at 2.1 GHz); 4096 rows: 412 to 422 us (1.15).  224 of 256 CUs have a tile of
-// 512 rows.
+// 512 rows by [14336, 4096]: 54 to 62 us, and 56 to 63 us and a join of 8 us for the gradient (1.0 to 1.1 PFLOP/s; 42 us
+// each at the 1.44 PFLOP/s of a large bf16 product on random data, which power limits: on zeros a step takes 1.27 us, on
+// random data 1.4 to 1.7, its instructions alone 0.96 at 2.1 GHz); 4096 rows: 412 to 443 us (1.1 to 1.2).  224 of 256 CUs
+// have a tile of 512 rows.
 template <bool TRANS, int MT>
 struct TileLds {
   static constexpr int kA = 32 * MT * 256, kB = 16384, kS = TRANS ? 3 * 1024 : 0, kStage = kA + kB + kS, kDeep = 3;

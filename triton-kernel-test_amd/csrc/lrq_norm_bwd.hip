@@ -48,14 +48,15 @@ __device__ __forceinline__ void norm_outputs(const NormBwd& a, int64_t row, int 
 // k_norm_wgrad adds the workgroups' sums in a fixed order.  The next row is already on the way while one is reduced and
 // written: up to sixteen waves a CU in 128 registers, and few workgroups, whose sums are few.
 //
-// HBM-bound: bf16 [16384, 4096] 80 to 87 us (4.8 TB/s), with dh, dropout and both outputs 126 us (5.3 TB/s); [8192, 5120]
-// 49 and 86 us (ten waves, so one row at a time a CU: 4.9 TB/s).  One chunk a thread: two would hold twice the weights and
-// sums, past the registers.  Rows above 8192 columns take four and keep nothing ahead, [4096, 14336] 80 and 176 to 190 us.  No
-// variant may use scratch.
+// HBM-bound: bf16 [16384, 4096] 77 to 86 us (4.7 to 5.2 TB/s), with dh, dropout and both outputs 124 to 134 us (5.0 to 5.4
+// TB/s); [8192, 5120] 45 and 84 us (ten waves, so one row at a time a CU: 5.0 TB/s).  One chunk a thread: two hold twice the
+// weights and sums, 119 registers of 128 at least and spills besides.  Rows above 8192 columns take four and keep nothing
+// ahead, [4096, 14336] 84 and 190 us.  No variant may use scratch or spill.
 //
 // ODD: rows of one chunk a thread, eight elements at least, that end inside a chunk.  Apart from the others, which then have
 // whole chunks only (with 128 columns or fewer, or four chunks a thread, partial ones as well): tests of the width at run
-// time cost these 2 to 4 %.  [8192, 5003] 59 and 117 us, against 103 and 180 with partial chunks loaded by elements.
+// time cost these 2 to 4 %.  [8192, 5003] 55 to 65 and 114 to 118 us, against 103 and 180 with partial chunks loaded by
+// elements; fused, dh comes behind the next row's loads.
 //
 // EARLY: dh comes with its row, where the workgroup has one row at a time ([8192, 5120] 102 -> 86 us; behind the next row's
 // loads it waits for them).  With more rows in flight it comes when it is used ([16384, 4096] 130 against 135 us).
@@ -238,7 +239,9 @@ __global__ __launch_bounds__(C == 4 ? 512 : 1024) void k_norm_bwd(NormBwd a) {
 }
 
 // Rows wider than the registers hold: one workgroup a row, swept twice; its weight gradients come from
-// k_norm_cols.
+// k_norm_cols, so dy and h are read three times.  With k_norm_cols (30 us) bf16 [2048, 20000] 90 us, with dh, dropout and both
+// outputs 131; fp32 [4096, 14336] 272 (112 of them k_norm_cols) and 365, [2048, 32768] 312 (114) and 413: 2.6 to 2.7 and 3.1 to
+// 3.3 TB/s of what has to move once.
 template <int DT, bool FUSED>
 __global__ __launch_bounds__(1024) void k_norm_bwd_wide(NormBwd a) {
   constexpr int ES = Elem<DT>::kBytes;

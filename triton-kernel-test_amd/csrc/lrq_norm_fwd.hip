@@ -47,12 +47,12 @@ __device__ __forceinline__ void norm_input(const NormFwd& a, const DropKey& key,
 // squared deviations from it) and the waves' parts are merged (Chan, Golub and LeVeque's update), so a
 // row costs one barrier and the variance never comes from a difference of large sums.
 //
-// HBM-bound: bf16 [16384, 4096] 47 us (5.7 TB/s; a copy reaches 5.2), with dropout and the residual 93 us (5.8 TB/s), whose
-// generator runs under the next row's loads.  (Stored past the caches the outputs take 3 and 8 us less, and their reader
-// more than that longer: 78 against 75 us with a quantisation of y behind it.)  Two chunks a thread (one above 512 columns
-// costs a second row's worth of waves and barriers); [8192, 5120] 32 and 64 us, [8192, 5003] 34 and 69 us (rows that end
-// inside a chunk are read whole; 40 and 86 by elements).  fp32 [1003, 5003]: 13 us, two rounds of rows for a load's latency
-// each.
+// HBM-bound: bf16 [16384, 4096] 46 to 53 us (5.0 to 5.8 TB/s; a copy reaches 5.2), with dropout and the residual 97 to 100 us
+// (5.4 TB/s), whose generator runs under the next row's loads.  (Stored past the caches the outputs take 3 and 8 us less,
+// and their reader more than that longer: 78 against 75 us with a quantisation of y behind it.)  Two chunks a thread (one
+// above 512 columns costs a second row's worth of waves and barriers); [8192, 5120] 29 and 56 to 65 us, [8192, 5003] 33 and 69
+// to 73 us (rows that end inside a chunk are read whole; 40 and 86 by elements).  fp32 [1003, 5003]: 13 to 16 us, two rounds of
+// rows for a load's latency each.
 template <int DT, int LANES, int C, bool FUSED, bool SAME>
 __global__ __launch_bounds__(1024) void k_norm_fwd(NormFwd a) {
   constexpr int ES = Elem<DT>::kBytes, L = LANES == 16 ? 16 : 64;
@@ -210,7 +210,9 @@ __device__ __forceinline__ float block_sum1024(float v, float* red) {
 }
 
 // Rows wider than the registers hold: one workgroup a row, which is swept three times (the mean, the
-// deviations, the output); after the first the row comes from L2.
+// deviations, the output); after the first the row comes from L2.  bf16 [2048, 20000] 43 us (3.8 TB/s of what it has to
+// move), with dropout and the residual 96 (3.4); fp32 [2048, 32768] 167 (3.2) and 265 us (4.1).  Bound by its own waits: a
+// sweep's loads have nothing of another row in flight beside them but the CU's second workgroup's.
 template <int DT, bool FUSED>
 __global__ __launch_bounds__(1024) void k_norm_fwd_wide(NormFwd a) {
   constexpr int ES = Elem<DT>::kBytes;
