@@ -442,6 +442,67 @@ int lrq_mxfp4_linear_t(const void* y, int64_t ldy, int64_t rows, const lrq_mxfp4
  * LRQ_ERR_*.  Host only. */
 int64_t lrq_mxfp4_linear_workspace(int64_t rows, const lrq_mxfp4* w, int32_t transposed);
 
+/* ------------------------------------------------------------------ root-mean-square norm, 8-bit floating point
+ * A matrix [rows, cols] in e4m3 (OCP 8-bit floating point, largest 448): codes, ld_codes bytes a row (16-byte aligned rows,
+ * ld_codes >= 128 * ceil(cols / 128)), padding columns code 0; scales, ld_scales bytes a row (4-byte aligned rows, ld_scales
+ * >= ceil(cols / 128) rounded up to 4), hold one E8M0 exponent for 128 columns of a row (block 1) or of 128 rows (block 128:
+ * ceil(rows / 128) rows of scales). */
+typedef struct lrq_fp8 {
+  void* codes;
+  int64_t ld_codes;
+  void* scales;
+  int64_t ld_scales;
+  int64_t rows, cols;
+  int32_t block;
+} lrq_fp8;
+
+/* Quantise x[rows, cols], or with transpose x[cols, rows] (block 1 only): t = x^T.  A block's scale is the smallest power of
+ * two, 2^-127 at least, that its largest magnitude exceeds at most 448 times; elements round to the nearest code, ties
+ * to the even one.  A block with an infinity or a NaN becomes NaN (scale 255, codes 0). */
+int lrq_fp8_quantize(const void* x, int64_t ldx, int32_t dtype, const lrq_fp8* t, int32_t transpose, void* stream);
+
+/* out[rows, cols] = the values of t, rounded to dtype (exact in bf16 and fp32 down to their smallest normal numbers). */
+int lrq_fp8_dequantize(const lrq_fp8* t, void* out, int64_t ldo, int32_t dtype, void* stream);
+
+/* out[a.rows, b.rows] = a b^T, both e4m3 with the same cols (any blocks); fp32 accumulation, out of out_dtype.  The
+ * contraction may be split over workgroups: `workspace` (16-byte aligned, lrq_fp8_gemm_workspace(a, b, 0) bytes) takes
+ * their fp32 sums, which are added in a fixed order. */
+int lrq_fp8_gemm(const lrq_fp8* a, const lrq_fp8* b, void* out, int64_t ldo, int32_t out_dtype, void* workspace,
+                 int64_t workspace_bytes, void* stream);
+
+/* out[a.rows, b.cols] = a b with a.cols == b.rows and b of block 128: the gradient of a linear layer's input.  `workspace`:
+ * lrq_fp8_gemm_workspace(a, b, 1) bytes. */
+int lrq_fp8_gemm_nn(const lrq_fp8* a, const lrq_fp8* b, void* out, int64_t ldo, int32_t out_dtype, void* workspace,
+                    int64_t workspace_bytes, void* stream);
+
+/* Workspace bytes (>= 0) of lrq_fp8_gemm (nn == 0) or lrq_fp8_gemm_nn, or a negative LRQ_ERR_*.  Host only. */
+int64_t lrq_fp8_gemm_workspace(const lrq_fp8* a, const lrq_fp8* b, int32_t nn);
+
+/* lrq_fp8_gemm with a = x[rows, w.cols] of bf16 or fp16 quantised on the way (blocks of 1 x 128), for at most
+ * LRQ_FP8_LINEAR_ROWS rows; w.cols a multiple of 8. */
+#define LRQ_FP8_LINEAR_ROWS 16
+int lrq_fp8_linear(const void* x, int64_t ldx, int32_t dtype, int64_t rows, const lrq_fp8* w, void* out, int64_t ldo,
+                   int32_t out_dtype, void* stream);
+
+/* y = h * rstd * w per row of n columns, rstd = 1 / sqrt(mean(h^2) + eps) (fp32 [rows], kept for the backward pass).
+ * h == NULL: the rows are x's (residual NULL).  Otherwise h = residual + x (residual may be NULL), rounded to dtype, is
+ * written and normalised as stored.  w (of w_dtype) may be NULL: 1.  Exactly one of y (of dtype) and q is given: q, of block 1
+ * and [rows, n], takes y quantised as by lrq_fp8_quantize, from its fp32 values. */
+int lrq_rms_norm_fwd(const void* x, int64_t ldx, const void* residual, int64_t ld_residual, int32_t dtype, const void* w,
+                     int32_t w_dtype, int64_t rows, int64_t n, float eps, void* h, int64_t ldh, void* y, int64_t ldy,
+                     const lrq_fp8* q, float* rstd, void* stream);
+
+/* Gradients of lrq_rms_norm_fwd from dy and, if not NULL, dh (the gradient of h from its other uses): dx = dh + (gradient
+ * through the norm), for x and the residual alike.  h: the rows that were normalised.  dw (w_dtype) may be NULL; otherwise
+ * it is summed over the rows in a fixed order through `workspace` (4-byte aligned, lrq_rms_norm_bwd_workspace(rows, n)
+ * bytes); rows == 0 writes zeros to it. */
+int lrq_rms_norm_bwd(const void* dy, int64_t lddy, const void* dh, int64_t lddh, const void* h, int64_t ldh, int32_t dtype,
+                     const void* w, int32_t w_dtype, const float* rstd, int64_t rows, int64_t n, void* dx, int64_t lddx,
+                     void* dw, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Workspace bytes of lrq_rms_norm_bwd with a weight gradient (>= 0), or a negative LRQ_ERR_*.  Host only. */
+int64_t lrq_rms_norm_bwd_workspace(int64_t rows, int64_t n);
+
 /* ------------------------------------------------------------------ misc */
 const char* lrq_status_string(int status);
 int32_t lrq_abi_version(void);

@@ -25,6 +25,7 @@ LRQ_GEMM_T_SCRATCH_BYTES = 16 * 1024 * 1024  # include/lrq.h
 LRQ_BF16 = 0
 LRQ_F16 = 1
 LRQ_F32 = 2
+LRQ_FP8_LINEAR_ROWS = 16
 
 
 class LrqTensors(ctypes.Structure):
@@ -55,9 +56,17 @@ class LrqMxfp4(ctypes.Structure):
                 ("rows", c_int64), ("cols", c_int64)]
 
 
+class LrqFp8(ctypes.Structure):
+    """Mirror of ``lrq_fp8`` in include/lrq.h."""
+
+    _fields_ = [("codes", c_void_p), ("ld_codes", c_int64), ("scales", c_void_p), ("ld_scales", c_int64),
+                ("rows", c_int64), ("cols", c_int64), ("block", c_int32)]
+
+
 _T = POINTER(LrqTensors)
 _D = POINTER(LrqDropout)
 _M = POINTER(LrqMxfp4)
+_E = POINTER(LrqFp8)
 
 # name -> (restype, argtypes); must cover every function declared in include/*.h (the drop-in
 # ABI in lrq.h and the test hooks in lrq_test_hooks.h)
@@ -134,6 +143,17 @@ SIGNATURES = {
     "lrq_mxfp4_linear_t": (c_int32, [c_void_p, c_int64, c_int64, _M, c_void_p, c_int64, c_int32, c_void_p, c_int64,
                                      c_void_p]),
     "lrq_mxfp4_linear_workspace": (c_int64, [c_int64, _M, c_int32]),
+    "lrq_fp8_quantize": (c_int32, [c_void_p, c_int64, c_int32, _E, c_int32, c_void_p]),
+    "lrq_fp8_dequantize": (c_int32, [_E, c_void_p, c_int64, c_int32, c_void_p]),
+    "lrq_fp8_gemm": (c_int32, [_E, _E, c_void_p, c_int64, c_int32, c_void_p, c_int64, c_void_p]),
+    "lrq_fp8_gemm_nn": (c_int32, [_E, _E, c_void_p, c_int64, c_int32, c_void_p, c_int64, c_void_p]),
+    "lrq_fp8_gemm_workspace": (c_int64, [_E, _E, c_int32]),
+    "lrq_fp8_linear": (c_int32, [c_void_p, c_int64, c_int32, c_int64, _E, c_void_p, c_int64, c_int32, c_void_p]),
+    "lrq_rms_norm_fwd": (c_int32, [c_void_p, c_int64, c_void_p, c_int64, c_int32, c_void_p, c_int32, c_int64, c_int64,
+                                   c_float, c_void_p, c_int64, c_void_p, c_int64, _E, c_void_p, c_void_p]),
+    "lrq_rms_norm_bwd": (c_int32, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int32, c_void_p, c_int32,
+                                   c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p]),
+    "lrq_rms_norm_bwd_workspace": (c_int64, [c_int64, c_int64]),
     "lrq_status_string": (ctypes.c_char_p, [c_int32]),
     "lrq_abi_version": (c_int32, []),
 }
@@ -205,5 +225,5 @@ def call(name: str, *args) -> None:
         check(st, name)
 
 
-__all__ = ["LrqTensors", "LrqDropout", "LrqMxfp4", "load", "call", "call_raw", "check", "status_string", "missing_symbols", "SIGNATURES",
+__all__ = ["LrqTensors", "LrqDropout", "LrqMxfp4", "LrqFp8", "load", "call", "call_raw", "check", "status_string", "missing_symbols", "SIGNATURES",
            "LIB_PATH", "LRQ_FLAG_HADAMARD", "c_size_t"]

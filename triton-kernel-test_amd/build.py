@@ -29,25 +29,28 @@ HIPFLAGS = [
     f"--offload-arch={ARCH}", "-O3", "-fPIC", "-std=c++17", "-Wall", "-Wno-unused-function",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     "-ffp-contract=off",
-    # MFMA results straight into VGPRs (no v_accvgpr_read round trips in the epilogues)
-    "-mllvm", "-amdgpu-mfma-vgpr-form",
     # every masked region restores its own mask.  Where two regions end together the compiler would leave out the inner
     # restore, and spilled registers reloaded between the two ends then miss the lanes that skipped the inner region: a row
     # loop whose step was reloaded so never ended.  Costs a scalar instruction a region: times are the same within noise.
     "-mllvm", "-amdgpu-remove-redundant-endcf=0",
 ]
 
+# MFMA results straight into VGPRs (no v_accvgpr_read round trips in the epilogues).  Not for the 8-bit products, whose sums
+# are all the accumulation registers of a wave: in VGPR form they would be copied there and back in each step.
+VGPR_FORM = ["-mllvm", "-amdgpu-mfma-vgpr-form"]
+ACC_FORM = {"lrq_fp8gemm"}
+
 # The compressed format assumes finite inputs (NaN / Inf activations give unspecified codes, never a fault).  IEEE mode
 # off: v_min/v_max of MFMA results need no canonicalising moves.
 FINITE_FLAGS = ["-fno-honor-nans", "-mno-amdgpu-ieee"]
 
-# The layer norm, dropout and MXFP4 kernels carry NaN and infinity through their row or block.  Without NaNs honoured
+# The norm, dropout, MXFP4 and 8-bit kernels carry NaN and infinity through their row or block.  Without NaNs honoured
 # every operation on one would be undefined to the compiler, so these are built with the language's own arithmetic.
-CARRY_NAN = {"lrq_dropout", "lrq_mx", "lrq_mxgemm", "lrq_norm_bwd", "lrq_norm_fwd"}
+CARRY_NAN = {"lrq_dropout", "lrq_fp8", "lrq_fp8gemm", "lrq_mx", "lrq_mxgemm", "lrq_norm_bwd", "lrq_norm_fwd", "lrq_rms"}
 
 
 def flags(src: Path) -> list[str]:
-    return HIPFLAGS if src.stem in CARRY_NAN else HIPFLAGS + FINITE_FLAGS
+    return HIPFLAGS + ([] if src.stem in ACC_FORM else VGPR_FORM) + ([] if src.stem in CARRY_NAN else FINITE_FLAGS)
 
 
 def hipcc() -> str:
