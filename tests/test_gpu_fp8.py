@@ -1,0 +1,371 @@
+"""e4m3 with a power-of-two scale for 128: quantisation to the bit, products and gradients against 64-bit forms."""
+
+import importlib
+
+import pytest
+import torch
+
+import opref8 as R
+from opref import assert_within
+
+pytestmark = pytest.mark.gpu
+BF, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def _x(rows, n, dtype, seed=0, scale=1.0):
+    g = torch.Generator().manual_seed(1000 * rows + n + seed)
+    x = torch.randn(rows, n, generator=g)
+    x[:, ::37] *= 20.0
+    return (scale * x).to(dtype).cuda()
+
+
+def _same(q, x, tall, what=""):
+    codes, scales = R.quantize(x, tall)
+    steps = -(-x.shape[1] // 128)
+    assert torch.equal(q.codes.view(torch.uint8).cpu().long(), codes), f"{what}: codes"
+    assert torch.equal(q.scales.cpu().long()[:, :steps], scales), f"{what}: scales"
+
+
+SIZES = [(1, 1), (1, 128), (3, 129), (128, 128), (129, 64), (130, 300), (257, 1000), (16, 4096)]
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32], ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("rows,n", SIZES)
+def test_quantize(pkg, rows, n, dtype):
+    x = _x(rows, n, dtype)
+    _same(pkg.fp8_quantize(x), x, 1, "rows")
+    _same(pkg.fp8_quantize(x, 128), x, 128, "square")
+    q = pkg.fp8_quantize(x, transpose=True)
+    assert q.shape == (n, rows) and q.block == 1
+    _same(q, x.T, 1, "transpose")
+
+
+def test_quantize_strided(pkg):
+    """Rows apart, odd starts, columns of a wider matrix, three dimensions, an expanded row."""
+    base = _x(70, 700, BF)
+    for x in (base[::2, 3:400], base[:, 5:], base.T, base[1:2].expand(9, 700)):
+        _same(pkg.fp8_quantize(x), x, 1)
+        _same(pkg.fp8_quantize(x, 128), x, 128)
+        _same(pkg.fp8_quantize(x, transpose=True), x.T, 1)
+    x = base.reshape(7, 10, 700)
+    q = pkg.fp8_quantize(x)
+    assert q.shape == x.shape
+    _same(q, base, 1)
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32], ids=["bf16", "fp16", "fp32"])
+def test_quantize_edges(pkg, dtype):
+    """Zeros of both signs, the smallest and largest numbers, powers of two around 448, ties, and blocks lost to NaN."""
+    inf, nan = float("inf"), float("nan")
+    t = torch.finfo(dtype)
+    rows = [[0.0], [-0.0, 0.0], [t.smallest_normal], [t.smallest_normal * t.eps], [t.max], [-t.max, t.smallest_normal],
+            [448.0, 1.0], [449.0 if dtype != BF else 450.0, 1.0], [447.0 if dtype != BF else 446.0, 1.0], [1.75], [1.7578125],
+            [17.0, 19.0, 21.0, 448.0], [2.0 ** -10, 3 * 2.0 ** -10, 5 * 2.0 ** -10, 448.0], [2.0 ** -11, -2.0 ** -10, 400.0],
+            [inf, 1.0], [1.0, nan], [-inf], [1.0, 2.0]]
+    x = torch.zeros(len(rows), 300, dtype=F32)
+    for i, r in enumerate(rows):
+        x[i, 60:60 + len(r)] = torch.tensor(r)
+        x[i, 140:140 + len(r)] = torch.tensor(r[::-1])
+    x[:, 299] = 3.0
+    x = x.to(dtype).cuda()
+    _same(pkg.fp8_quantize(x), x, 1, "rows")
+    _same(pkg.fp8_quantize(x.T.contiguous(), transpose=True), x, 1, "transpose")
+    for i in range(len(rows)):
+        _same(pkg.fp8_quantize(x[i:i + 1], 128), x[i:i + 1], 128, f"square {rows[i]}")
+    d = pkg.fp8_dequantize(pkg.fp8_quantize(x), F32)
+    lost = ~torch.isfinite(x).cpu()
+    assert torch.equal(torch.isnan(d).cpu()[:, :128].any(1), lost[:, :128].any(1)) and not torch.isnan(d[:, 256:]).any()
+
+
+def test_dequantize_every_code(pkg):
+    """All 256 codes under small, middle and large scales, NaN scales among them, in blocks of both kinds."""
+    codes = torch.arange(256, dtype=torch.uint8).repeat(6, 1).cuda()
+    scales = torch.tensor([0, 1, 119, 127, 246, 255], dtype=torch.uint8).reshape(6, 1).repeat(1, 4).cuda()
+    q = pkg.FP8Tensor(codes, scales, (6, 256), 1)
+    ref = R.tensor_values(q)
+    got = pkg.fp8_dequantize(q, F32).cpu().double()
+    assert torch.equal(torch.nan_to_num(got), torch.nan_to_num(ref)) and torch.equal(torch.isnan(got), torch.isnan(ref))
+    for s in (100, 127, 140):
+        q = pkg.FP8Tensor(codes, torch.full((1, 4), s, dtype=torch.uint8).cuda(), (6, 256), 128)
+        got = pkg.fp8_dequantize(q, BF).cpu().double()
+        assert torch.equal(torch.nan_to_num(got), torch.nan_to_num(R.tensor_values(q)))
+
+
+def test_from_parts(pkg):
+    w = _x(300, 400, F32, scale=0.02)
+    q = pkg.fp8_quantize(w, 128)
+    ref = R.tensor_values(q)
+    c, s = q.codes[:, :400], q.scales[:, :4]
+    f32 = torch.exp2(s.float() - 127)
+    for scales in (s, f32, f32.cpu().to(torch.float8_e8m0fnu).cuda()):
+        p = pkg.fp8_from_parts(c.contiguous(), scales, 128)
+        assert torch.equal(R.tensor_values(p), ref)
+        p.descriptor()
+    with pytest.raises(ValueError, match="powers of two"):
+        pkg.fp8_from_parts(c, f32 * 1.5)
+    with pytest.raises(ValueError, match="scales must be"):
+        pkg.fp8_from_parts(c, f32[:1])
+    whole = pkg.fp8_quantize(_x(256, 512, F32), 128)
+    p = pkg.fp8_from_parts(whole.codes, whole.scales, 128)
+    assert p.codes.data_ptr() == whole.codes.data_ptr()  # nothing to lay out
+
+
+# M x K x N: the few-row kernel's and the tiles' edges, one step and many, ragged sizes, contractions that are split
+SHAPES = [(1, 1, 1), (1, 128, 16), (3, 300, 33), (16, 1000, 100), (17, 256, 40), (33, 129, 20), (64, 640, 80), (65, 128, 256),
+          (70, 513, 300), (130, 384, 257), (257, 1030, 130), (300, 2048, 520), (100, 9000, 64), (520, 200, 700)]
+
+
+@pytest.mark.parametrize("m,k,n", SHAPES)
+@pytest.mark.parametrize("ba,bb", [(1, 128), (1, 1), (128, 128), (128, 1)])
+def test_gemm(pkg, m, k, n, ba, bb):
+    a, b = pkg.fp8_quantize(_x(m, k, BF), ba), pkg.fp8_quantize(_x(n, k, F32, 1, 0.02), bb)
+    va, vb = R.tensor_values(a), R.tensor_values(b)
+    for dtype in (F32, BF, F16):
+        ref, bound = R.product(va, vb.T, dtype)
+        assert_within(pkg.fp8_gemm(a, b, dtype), ref, bound, f"{m}x{k}x{n} {dtype}")
+
+
+@pytest.mark.parametrize("m,k,n", SHAPES)
+@pytest.mark.parametrize("ba", [1, 128])
+def test_gemm_nn(pkg, m, k, n, ba):
+    """dy w: the contraction runs over w's rows."""
+    a, b = pkg.fp8_quantize(_x(m, n, BF), ba), pkg.fp8_quantize(_x(n, k, F32, 1, 0.02), 128)
+    va, vb = R.tensor_values(a), R.tensor_values(b)
+    for dtype in (F32, BF, F16):
+        ref, bound = R.product(va, vb, dtype)
+        assert_within(pkg.fp8_linear_backward(a, b, dtype), ref, bound, f"{m}x{n}x{k} {dtype}")
+
+
+@pytest.mark.parametrize("m,k,n", [(5, 128, 16), (40, 1000, 300), (300, 700, 520)])
+def test_small_integers_are_exact(pkg, m, k, n):
+    """Codes of small integers, scales of different powers of two: every sum is exact, so every code and scale has met its
+    own partner."""
+    g = torch.Generator().manual_seed(m)
+    steps = -(-k // 128)
+    c = torch.zeros(m, 128 * steps)
+    c[:, :k] = torch.randint(-3, 4, (m, k), generator=g).float()
+    w = torch.zeros(n, 128 * steps)
+    w[:, :k] = torch.randint(-3, 4, (n, k), generator=g).float()
+    f8 = torch.float8_e4m3fn
+    wide = -(-steps // 4) * 4
+    sa = torch.randint(125, 130, (m, wide), generator=g).to(torch.uint8)
+    sb = torch.randint(125, 130, (-(-n // 128), wide), generator=g).to(torch.uint8)
+    a = pkg.FP8Tensor(c.to(f8).cuda(), sa.cuda(), (m, k), 1)
+    b = pkg.FP8Tensor(w.to(f8).cuda(), sb.cuda(), (n, k), 128)
+    ref = R.tensor_values(a) @ R.tensor_values(b).T
+    assert torch.equal(pkg.fp8_gemm(a, b, F32).cpu().double(), ref)
+    wide = -(-(-(-n // 128)) // 4) * 4
+    d = torch.zeros(m, -(-n // 128) * 128)
+    d[:, :n] = torch.randint(-3, 4, (m, n), generator=g).float()
+    dy = pkg.FP8Tensor(d.to(f8).cuda(), torch.randint(125, 130, (m, wide), generator=g).to(torch.uint8).cuda(), (m, n), 1)
+    ref = R.tensor_values(dy) @ R.tensor_values(b)
+    assert torch.equal(pkg.fp8_linear_backward(dy, b, F32).cpu().double(), ref)
+
+
+def test_operands_apart(pkg):
+    """Rows of codes and scales apart, an operand that starts inside another, float8 scales, three dimensions, no rows."""
+    a, b = pkg.fp8_quantize(_x(90, 500, BF)), pkg.fp8_quantize(_x(200, 500, BF, 1), 128)
+    want = pkg.fp8_gemm(a, b)
+
+    def apart(q):
+        c = torch.full((q.codes.shape[0], 800), 0x7F, dtype=torch.uint8).cuda()
+        s = torch.full((q.scales.shape[0], 12), 255, dtype=torch.uint8).cuda()
+        c[:, 16:16 + 512] = q.codes.view(torch.uint8)
+        s[:, 4:8] = q.scales
+        return pkg.FP8Tensor(c[:, 16:528], s[:, 4:8].view(torch.float8_e8m0fnu), q.shape, q.block)
+    assert torch.equal(pkg.fp8_gemm(apart(a), apart(b)), want)
+    dy = pkg.fp8_quantize(_x(90, 200, BF, 2))
+    assert torch.equal(pkg.fp8_linear_backward(dy, apart(b)), pkg.fp8_linear_backward(dy, b))
+    few = pkg.FP8Tensor(a.codes[:7], a.scales[:7], (7, 500), 1)
+    assert torch.equal(pkg.fp8_gemm(apart(few), apart(b)), pkg.fp8_gemm(few, b))
+    three = pkg.FP8Tensor(a.codes, a.scales, (9, 10, 500), 1)
+    assert torch.equal(pkg.fp8_gemm(three, b), want.reshape(9, 10, 200))
+    none = pkg.fp8_quantize(_x(90, 500, BF)[:0])
+    assert pkg.fp8_gemm(none, b).shape == (0, 200)
+    assert pkg.fp8_linear(_x(90, 500, BF)[:0], b).shape == (0, 200)
+
+
+@pytest.mark.parametrize("dtype", [BF, F16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("m", [1, 2, 7, 16])
+def test_linear_quantises_as_the_quantiser(pkg, m, dtype):
+    """Few 16-bit rows are quantised inside the product: the same bits as in two calls, special values among them."""
+    w = pkg.fp8_quantize(_x(300, 1000, F32, 1, 0.02), 128)
+    x = _x(m, 1000, dtype)
+    x[0, :128] = 0.0
+    x[m - 1, 400] = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    assert torch.equal(pkg.fp8_linear(x, w, F32), pkg.fp8_gemm(pkg.fp8_quantize(x), w, F32))
+    wide = torch.zeros(m, 1203, dtype=dtype, device="cuda")
+    wide[:, 3:1003] = x
+    assert torch.equal(pkg.fp8_linear(wide[:, 3:1003], w, F32), pkg.fp8_linear(x, w, F32))
+    x[m - 1, 999] = float("nan")
+    y = pkg.fp8_linear(x, w)
+    assert torch.isnan(y[m - 1]).all() and torch.isfinite(y[:m - 1]).all()
+
+
+@pytest.mark.parametrize("m", [5, 40, 200])
+def test_nan_stays_in_its_row(pkg, m):
+    x = _x(m, 300, BF)
+    x[m - 1, 7] = float("inf")
+    x[0, 299] = float("nan")
+    w = pkg.fp8_quantize(_x(260, 300, F32, 1), 128)
+    y = pkg.fp8_linear(x, w)
+    assert torch.isnan(y[0]).all() and torch.isnan(y[m - 1]).all() and torch.isfinite(y[1:m - 1]).all()
+    bad = _x(260, 300, F32, 1)
+    bad[130, 5] = float("nan")  # rows 128 .. 255 share the block
+    y = pkg.fp8_linear(_x(m, 300, BF), pkg.fp8_quantize(bad, 128))
+    assert torch.isnan(y[:, 128:256]).all() and torch.isfinite(y[:, :128]).all() and torch.isfinite(y[:, 256:]).all()
+    dx = pkg.fp8_linear_backward(_x(m, 260, BF), pkg.fp8_quantize(bad, 128))
+    assert torch.isnan(dx[:, :128]).all() and torch.isfinite(dx[:, 128:]).all()
+
+
+def test_rows_behind_the_output_are_left(pkg):
+    """The C entry writes [rows, cols] of a wider, longer output and nothing else."""
+    L = pkg._lib
+    import ctypes
+    for m, k, n in ((5, 256, 50), (40, 256, 50), (100, 256, 300)):
+        a, b = pkg.fp8_quantize(_x(m, k, BF)), pkg.fp8_quantize(_x(n, k, BF, 1), 128)
+        out = torch.full((m + 3, n + 5), 7.0, dtype=BF, device="cuda")
+        ta, tb = a.descriptor(), b.descriptor()
+        nb = L.call_raw("lrq_fp8_gemm_workspace", ctypes.byref(ta), ctypes.byref(tb), 0)
+        ws = torch.empty(max(nb // 4, 4), device="cuda")
+        L.call("lrq_fp8_gemm", ctypes.byref(ta), ctypes.byref(tb), ctypes.c_void_p(out.data_ptr()), n + 5, L.LRQ_BF16,
+               ctypes.c_void_p(ws.data_ptr()), nb, ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+        assert torch.equal(out[:m, :n], pkg.fp8_gemm(a, b))
+        assert (out[m:] == 7).all() and (out[:, n:] == 7).all()
+
+
+@pytest.mark.parametrize("rows,k,n", [(1, 128, 128), (100, 300, 200), (257, 513, 130), (1000, 256, 384)])
+def test_weight_gradient(pkg, rows, k, n):
+    dy, x = _x(rows, n, BF, 3, 0.02), _x(rows, k, BF)
+    va = R.values(*R.quantize(dy.T, 1), rows, 1)
+    vb = R.values(*R.quantize(x.T, 1), rows, 1)
+    ref, bound = R.product(va, vb.T, F32)
+    assert_within(pkg.fp8_weight_gradient(dy, x, F32), ref, bound, "dw")
+    assert pkg.fp8_weight_gradient(dy[:0], x[:0]).eq(0).all()
+
+
+def test_same_result_every_time(pkg):
+    x = _x(100, 9000, BF)
+    w = pkg.fp8_quantize(_x(64, 9000, BF, 1), 128)
+    y = pkg.fp8_linear(x, w, F32)
+    for _ in range(3):
+        assert torch.equal(pkg.fp8_linear(x, w, F32), y)
+
+
+def test_streams_and_graphs(pkg):
+    """Two streams at once, and a captured step replayed on new inputs between eager calls."""
+    w = pkg.fp8_quantize(_x(520, 1100, F32, 1), 128)
+    xs = [_x(m, 1100, BF, m) for m in (1, 12, 50, 300)]
+    want = [(pkg.fp8_linear(x, w), pkg.fp8_linear_backward(_x(x.shape[0], 520, BF), w)) for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in xs]
+    got = []
+    for x, s in zip(xs, streams):
+        with torch.cuda.stream(s):
+            got.append((pkg.fp8_linear(x, w), pkg.fp8_linear_backward(_x(x.shape[0], 520, BF), w)))
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    static = torch.empty(300, 1100, dtype=BF, device="cuda")
+
+    def step():
+        y = pkg.fp8_linear(static, w)
+        return y, pkg.fp8_linear_backward(y, w), pkg.fp8_weight_gradient(y, static)
+    static.copy_(xs[3])
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i in range(3):
+        static.copy_(_x(300, 1100, BF, 50 + i))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, step()):
+            assert torch.equal(a, b)
+
+
+def test_offsets_past_32_bits(pkg):
+    """Operands of more than 4 GiB: the last rows come out right (not to the bit as alone, where the contraction is split)."""
+    k, n, rows = 4096, 512, (1 << 20) + 300
+    w = pkg.fp8_quantize(_x(n, k, BF, 1), 128)
+    tail = _x(300, k, BF)
+    codes = torch.zeros(rows, k, dtype=torch.uint8, device="cuda")
+    scales = torch.full((rows, 32), 127, dtype=torch.uint8, device="cuda")
+    q = pkg.fp8_quantize(tail)
+    codes[-300:], scales[-300:] = q.codes.view(torch.uint8), q.scales
+    y = pkg.fp8_gemm(pkg.FP8Tensor(codes, scales, (rows, k), 1), w, F32)
+    ref, bound = R.product(R.tensor_values(q), R.tensor_values(w).T, F32)
+    assert_within(y[-300:], ref, bound, "the last rows")
+    assert y[:1000].eq(0).all()
+    del y, codes
+    x = torch.zeros(rows, k, dtype=BF, device="cuda")
+    x[-300:] = tail
+    big = pkg.fp8_quantize(x)
+    assert torch.equal(big.codes[-300:].view(torch.uint8), q.codes.view(torch.uint8))
+
+
+# ---------------------------------------------------------------- autograd
+@pytest.fixture(scope="module")
+def AG(pkg):
+    return importlib.import_module("triton-kernel-test_amd.autograd")
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32], ids=["bf16", "fp16", "fp32"])
+def test_linear_gradients(pkg, AG, dtype):
+    x, w = _x(150, 300, dtype).requires_grad_(), _x(200, 300, dtype, 1, 0.02).requires_grad_()
+    dy = _x(150, 200, dtype, 2)
+    y = AG.fp8_linear(x, w)
+    y.backward(dy)
+    q = pkg.fp8_quantize(w.detach(), 128)
+    assert y.dtype == dtype and torch.equal(y, pkg.fp8_linear(x.detach(), q, dtype))
+    assert torch.equal(x.grad, pkg.fp8_linear_backward(dy, q, dtype)) and x.grad.dtype == dtype
+    assert torch.equal(w.grad, pkg.fp8_weight_gradient(dy, x.detach(), dtype)) and w.grad.dtype == dtype
+    x2 = x.detach().reshape(10, 15, 300).requires_grad_()
+    y2 = AG.fp8_linear(x2, q)
+    y2.backward(dy.reshape(10, 15, 200))
+    assert torch.equal(y2.reshape(150, 200), y) and torch.equal(x2.grad.reshape(150, 300), x.grad)
+    with torch.inference_mode():
+        assert torch.equal(AG.fp8_linear(x, q), y)
+
+
+def test_linear_is_its_formula(pkg, AG):
+    """The gradients of quantised products against those of the products themselves: two operands' roundings, at most
+    half a step of 2^-4 each where nothing underflows."""
+    x, w, dy = _x(256, 384, F32), _x(128, 384, F32, 1), _x(256, 128, F32, 2)
+    xg, wg = x.clone().requires_grad_(), w.clone().requires_grad_()
+    AG.fp8_linear(xg, wg).backward(dy)
+    for got, ref, mag in ((xg.grad, dy.double() @ w.double(), dy.abs().double() @ w.abs().double()),
+                          (wg.grad, dy.T.double() @ x.double(), dy.T.abs().double() @ x.abs().double())):
+        # elements under 2^-6 of the scaled range lose up to 2^-10 of it, 2^-19 of the block's largest: within 0.01 of
+        # these sums, whose terms are of one order
+        e = (2 * 2.0 ** -4 + 2.0 ** -8 + 0.01) * mag
+        assert ((got.double() - ref).abs() <= e).all()
+
+
+def test_changed_weight_is_refused(pkg, AG):
+    q = pkg.fp8_quantize(_x(200, 300, BF, 1), 128)
+    x = _x(20, 300, BF).requires_grad_()
+    y = AG.fp8_linear(x, q)
+    q.scales.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+def test_lora_on_an_8_bit_base(pkg, AG):
+    x = _x(128, 512, BF).requires_grad_()
+    q = pkg.fp8_quantize(_x(256, 512, BF, 1, 0.02), 128)
+    a = (_x(512, 16, BF, 2, 0.02)).requires_grad_()
+    b = (_x(16, 256, BF, 3, 0.02)).requires_grad_()
+    dy = _x(128, 256, BF, 4)
+    y = AG.lora_linear_compressed(x, q, a, b, bits=4, group=64)
+    y.backward(dy)
+    xd = x.detach()
+    want = torch.addmm(pkg.fp8_linear(xd, q), xd @ a.detach(), b.detach())
+    assert torch.equal(y, want)
+    g = dy @ b.detach().mT
+    assert torch.equal(x.grad, torch.addmm(pkg.fp8_linear_backward(dy, q), g, a.detach().mT))
+    assert a.grad.shape == a.shape and torch.isfinite(a.grad).all() and b.grad.shape == b.shape

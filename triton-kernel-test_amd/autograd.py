@@ -19,8 +19,9 @@ round trip part of autograd:
   stores every saved bf16 activation with a suitable last dimension in the compressed format
   and decodes it when backward asks for it, for any model.
 * ``layer_norm``, ``dropout``, ``dropout_add_layer_norm`` and ``mxfp4_linear`` are the operators of
-  ``norm.py`` and ``mxfp4.py`` with their gradients; ``lora_linear_compressed`` takes an MXFP4 base
-  weight and LoRA dropout.
+  ``norm.py`` and ``mxfp4.py`` with their gradients, ``rms_norm``, ``add_rms_norm``, ``fp8_linear`` and
+  ``rms_norm_linear`` those of ``rms.py`` and ``fp8.py``; ``lora_linear_compressed`` takes an MXFP4 or
+  8-bit base weight and LoRA dropout.
 * ``fit_basis`` builds the rank-r basis V from a sample of activation rows (top right singular
   vectors), the counterpart of the reference's low-rank factors of x.
 
@@ -34,12 +35,15 @@ from typing import Callable, Optional
 import torch
 from torch.autograd.function import once_differentiable
 
+from . import fp8 as _f8
 from . import mxfp4 as _mx
 from . import norm as _norm
+from . import rms as _rms
 from .api import CompressedActivation, LowRankBasis, decode, encode, lora_grads
 
 __all__ = ["compute_lora", "compute_lora_gradient", "LoRALinearCompressed", "lora_linear_compressed",
-           "compressed_saved_tensors", "fit_basis", "layer_norm", "dropout", "dropout_add_layer_norm", "mxfp4_linear"]
+           "compressed_saved_tensors", "fit_basis", "layer_norm", "dropout", "dropout_add_layer_norm", "mxfp4_linear",
+           "rms_norm", "add_rms_norm", "fp8_linear", "rms_norm_linear"]
 
 
 def compute_lora(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
@@ -69,14 +73,14 @@ class LoRALinearCompressed(torch.autograd.Function):
 
     Gradients: dx, dA, dB of compute_lora_gradient on the decoded x; W gets none.  ``fused``
     reads the codes directly for dA and x A (no decoded x), see the module docstring.  W may be an
-    ``MXFP4Tensor`` [out, in].  With ``dropout_p`` the LoRA branch reads dropout(x): y = x W^T + (dropout(x) A) B, its
+    ``MXFP4Tensor`` or ``FP8Tensor`` [out, in].  With ``dropout_p`` the LoRA branch reads dropout(x): y = x W^T + (dropout(x) A) B, its
     mask drawn again from ``seed`` in the backward pass, where x is decoded for it."""
 
     @staticmethod
     def forward(ctx, x, w, a, b, basis: Optional[LowRankBasis], bits: int, group: int, fused: bool = True,
                 dropout_p: float = 0.0, seed=None):
         ctx.p, ctx.seed, state = _seeded(dropout_p, seed)
-        mx = isinstance(w, _mx.MXFP4Tensor)
+        mx = isinstance(w, (_mx.MXFP4Tensor, _f8.FP8Tensor))
         if ctx.p == 0.0 and not mx:
             y = compute_lora(x, w, a, b)
         else:
@@ -84,7 +88,7 @@ class LoRALinearCompressed(torch.autograd.Function):
             xd = _norm.dropout(x2, ctx.p, seed) if ctx.p > 0.0 else x2
             # the base product in x's type before the branch is added, as compute_lora has it: in fp32 it would be
             # written and read again at twice the bytes
-            base = _mx.mxfp4_linear(x2, w) if mx else x2 @ w.mT
+            base = _product(x2, w) if mx else x2 @ w.mT
             y = torch.addmm(base, xd @ a, b).reshape(x.shape[:-1] + (w.shape[0],))
         ctx.c = encode(x.detach(), basis, bits=bits, group_size=group)
         ctx.fused = fused
@@ -107,7 +111,7 @@ class LoRALinearCompressed(torch.autograd.Function):
                 dx, da, db = compute_lora_gradient(dy2, _flat(decode(c)), w, a, b)
         else:
             g = dy2 @ b.mT
-            dx = _mx.mxfp4_linear_backward(dy2, w) if ctx.mx is not None else dy2 @ w
+            dx = _product_backward(dy2, w) if ctx.mx is not None else dy2 @ w
             if ctx.p > 0.0:
                 # (dy W and g A^T rounded to dy's type ahead of their sum, which takes them from memory)
                 dx = _norm.dropout(g @ a.mT, ctx.p, _with_state(ctx.seed, state), residual=dx)
@@ -136,8 +140,8 @@ def _codes_gemm_ok(c: CompressedActivation, a: torch.Tensor, dy2: torch.Tensor) 
 
 def lora_linear_compressed(x, w, a, b, basis: Optional[LowRankBasis] = None, bits: int = 4, group: int = 64,
                            fused: bool = True, dropout_p: float = 0.0, seed=None):
-    """The LoRA layer that saves x compressed (``LoRALinearCompressed``).  w: dense [out, in] or an
-    ``MXFP4Tensor``; ``dropout_p`` > 0 needs a ``seed`` (``norm.dropout``'s), a new one for every step and layer."""
+    """The LoRA layer that saves x compressed (``LoRALinearCompressed``).  w: dense [out, in], an
+    ``MXFP4Tensor`` or an ``FP8Tensor``; ``dropout_p`` > 0 needs a ``seed`` (``norm.dropout``'s), a new one for every step and layer."""
     return LoRALinearCompressed.apply(x, w, a, b, basis, bits, group, fused, dropout_p, seed)
 
 
@@ -240,16 +244,28 @@ def dropout_add_layer_norm(x: torch.Tensor, residual: Optional[torch.Tensor], we
     return _DropoutAddLayerNorm.apply(x, residual, weight, bias, p, seed, eps)
 
 
-def _weight(w: "_mx.MXFP4Tensor"):
-    """(what the context keeps of w, the tensors to save): the backward pass refuses a weight changed in between.  Tensors
-    made in inference mode carry no version and cannot be saved; such a weight is kept as it is."""
+def _weight(w):
+    """(what the context keeps of an MXFP4 or 8-bit w, the tensors to save): the backward pass refuses a weight changed in
+    between.  Tensors made in inference mode carry no version and cannot be saved; such a weight is kept as it is."""
     if w.codes.is_inference() or w.scales.is_inference():
         return w, (None, None)
-    return w.shape, (w.codes, w.scales)
+    return (w.shape, getattr(w, "block", None)), (w.codes, w.scales)
 
 
 def _saved_weight(kept, codes, scales):
-    return kept if codes is None else _mx.MXFP4Tensor(codes, scales, kept)
+    if codes is None:
+        return kept
+    shape, block = kept
+    return _mx.MXFP4Tensor(codes, scales, shape) if block is None else _f8.FP8Tensor(codes, scales, shape, block)
+
+
+def _product(x, w):
+    return _mx.mxfp4_linear(x, w) if isinstance(w, _mx.MXFP4Tensor) else _f8.fp8_linear(x, w, x.dtype)
+
+
+def _product_backward(dy, w):
+    return (_mx.mxfp4_linear_backward(dy, w) if isinstance(w, _mx.MXFP4Tensor)
+            else _f8.fp8_linear_backward(dy, w, dy.dtype))
 
 
 class _MXFP4Linear(torch.autograd.Function):
@@ -269,6 +285,155 @@ class _MXFP4Linear(torch.autograd.Function):
 def mxfp4_linear(x: torch.Tensor, w: "_mx.MXFP4Tensor", out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """x w^T for a frozen MXFP4 weight (``mxfp4.mxfp4_linear``), with the gradient for x (taken from dy in bf16)."""
     return _MXFP4Linear.apply(x, w, out_dtype)
+
+
+class _RmsNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, eps):
+        y, rstd = _rms.rms_norm_forward(x, weight, eps)
+        ctx.save_for_backward(x, weight, rstd)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, rstd = ctx.saved_tensors
+        dx, dw = _rms.rms_norm_backward(dy, x, weight, rstd, weight_grad=ctx.needs_input_grad[1])
+        return dx, dw, None
+
+
+def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float = 1e-6) -> torch.Tensor:
+    """Root-mean-square norm over the last axis (``rms.rms_norm_forward``) with gradients for x and weight; the sum of
+    the weight's gradient is skipped where it needs none."""
+    return _RmsNorm.apply(x, weight, eps)
+
+
+class _AddRmsNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, weight, eps):
+        y, h, rstd = _rms.add_rms_norm_forward(x, residual, weight, eps)
+        ctx.save_for_backward(h, weight, rstd)
+        ctx.set_materialize_grads(False)
+        return y, h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dh):
+        h, weight, rstd = ctx.saved_tensors
+        if dy is None:  # the norm's output went unused
+            return dh, dh, None, None
+        dx, dw = _rms.rms_norm_backward(dy, h, weight, rstd, dh, weight_grad=ctx.needs_input_grad[2])
+        return dx, dx if ctx.needs_input_grad[1] else None, dw, None
+
+
+def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float = 1e-6):
+    """(y, h) of h = residual + x, y = rms_norm(h), in one kernel each way; h is the residual stream that the next block
+    adds to."""
+    return _AddRmsNorm.apply(x, residual, weight, eps)
+
+
+class _FP8Linear(torch.autograd.Function):
+    """A frozen 8-bit weight."""
+
+    @staticmethod
+    def forward(ctx, x, w, out_dtype):
+        ctx.w, weight = _weight(w)
+        ctx.save_for_backward(*weight)
+        ctx.dtype = x.dtype
+        return _f8.fp8_linear(x, w, out_dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        return _f8.fp8_linear_backward(dy, _saved_weight(ctx.w, *ctx.saved_tensors), ctx.dtype), None, None
+
+
+class _FP8LinearTrained(torch.autograd.Function):
+    """A dense weight, quantised here; x is kept for the weight's gradient in 8 bits, as that product reads it."""
+
+    @staticmethod
+    def forward(ctx, x, w, out_dtype):
+        q = _f8.fp8_quantize(w, 128)
+        ctx.shape, ctx.dtype, ctx.w_dtype = q.shape, x.dtype, w.dtype
+        ctx.tokens = x.numel() // x.shape[-1] if x.shape[-1] else 0
+        xt = _f8.fp8_quantize(x, transpose=True) if ctx.needs_input_grad[1] and ctx.tokens else None
+        ctx.save_for_backward(*((q.codes, q.scales) if ctx.needs_input_grad[0] else (None, None)),
+                              *((xt.codes, xt.scales) if xt is not None else (None, None)))
+        return _f8.fp8_linear(x, q, out_dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        codes, scales, xc, xs = ctx.saved_tensors
+        dx = dw = None
+        if ctx.needs_input_grad[0]:
+            dx = _f8.fp8_linear_backward(dy, _f8.FP8Tensor(codes, scales, ctx.shape, 128), ctx.dtype)
+        if ctx.needs_input_grad[1]:
+            if ctx.tokens:
+                dw = _f8.fp8_gemm(_f8.fp8_quantize(dy, transpose=True),
+                                  _f8.FP8Tensor(xc, xs, (ctx.shape[1], ctx.tokens), 1), ctx.w_dtype)
+            else:
+                dw = torch.zeros(ctx.shape, dtype=ctx.w_dtype, device=dy.device)
+        return dx, dw, None
+
+
+def fp8_linear(x: torch.Tensor, w, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """x w^T in 8 bits (``fp8.fp8_linear``), of x's type unless ``out_dtype`` says otherwise.  w: an ``FP8Tensor`` of block
+    128 (frozen: a gradient for x alone) or a dense [out, in] weight, which is quantised in each call and gets its
+    gradient; all products of the backward pass are in 8 bits too."""
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    if isinstance(w, _f8.FP8Tensor):
+        return _FP8Linear.apply(x, w, out_dtype)
+    if not isinstance(w, torch.Tensor) or w.dim() != 2:
+        raise ValueError("the weight must be an FP8Tensor or a dense matrix")
+    return _FP8LinearTrained.apply(x, w, out_dtype)
+
+
+class _RmsNormLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, norm_weight, eps, weights):
+        if residual is None:
+            q, rstd = _rms.rms_norm_forward(x, norm_weight, eps, fp8=True)
+            h = x
+        else:
+            q, h, rstd = _rms.add_rms_norm_forward(x, residual, norm_weight, eps, fp8=True)
+        kept = [_weight(w) for w in weights]
+        ctx.w = [k for k, _ in kept]
+        ctx.save_for_backward(h, norm_weight, rstd, *(t for _, ts in kept for t in ts))
+        ctx.add = residual is not None
+        ctx.set_materialize_grads(False)
+        y = tuple(_f8.fp8_linear(q, w, x.dtype) for w in weights)
+        return y + (h,) if ctx.add else y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, *grads):
+        h, norm_weight, rstd, *saved = ctx.saved_tensors
+        dh = grads[len(ctx.w)] if ctx.add else None
+        some = [(g, _saved_weight(k, *saved[2 * i:2 * i + 2])) for i, (g, k) in enumerate(zip(grads, ctx.w)) if g is not None]
+        if not some:
+            return dh, dh if ctx.add else None, None, None, None
+        # several products' gradients are added in fp32 and rounded once, as a single one is
+        parts = [_f8.fp8_linear_backward(g, w, h.dtype if len(some) == 1 else torch.float32) for g, w in some]
+        dn = parts[0]
+        for p in parts[1:]:
+            dn = dn.add_(p)
+        dx, dw = _rms.rms_norm_backward(dn.to(h.dtype), h, norm_weight, rstd, dh, weight_grad=ctx.needs_input_grad[2])
+        return dx, dx if ctx.add and ctx.needs_input_grad[1] else None, dw, None, None
+
+
+def rms_norm_linear(x: torch.Tensor, norm_weight: Optional[torch.Tensor], weights, residual: Optional[torch.Tensor] = None,
+                    eps: float = 1e-6):
+    """The pre-norm of a layer and the products behind it: n = rms_norm(residual + x), quantised as it leaves the norm,
+    times the frozen 8-bit weight(s).  ``weights``: an ``FP8Tensor`` of block 128, or several that share n (query, key and
+    value).  Returns a y for each weight (one y for a single FP8Tensor), and with a residual also h = residual + x, last.
+    Gradients go to x, the residual and the norm's weight; n itself is not kept."""
+    single = isinstance(weights, _f8.FP8Tensor)
+    ws = (weights,) if single else tuple(weights)
+    if not ws or not all(isinstance(w, _f8.FP8Tensor) for w in ws):
+        raise ValueError("weights must be FP8Tensors")
+    out = _RmsNormLinear.apply(x, residual, norm_weight, eps, ws)
+    return out[0] if single and residual is None else out
 
 
 class compressed_saved_tensors(torch.autograd.graph.saved_tensors_hooks):
