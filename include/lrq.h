@@ -480,7 +480,7 @@ int64_t lrq_fp8_gemm_workspace(const lrq_fp8* a, const lrq_fp8* b, int32_t nn);
 
 /* lrq_fp8_gemm with a = x[rows, w.cols] of bf16 or fp16 quantised on the way (blocks of 1 x 128), for at most
  * LRQ_FP8_LINEAR_ROWS rows; w.cols a multiple of 8. */
-#define LRQ_FP8_LINEAR_ROWS 16
+#define LRQ_FP8_LINEAR_ROWS 4
 int lrq_fp8_linear(const void* x, int64_t ldx, int32_t dtype, int64_t rows, const lrq_fp8* w, void* out, int64_t ldo,
                    int32_t out_dtype, void* stream);
 

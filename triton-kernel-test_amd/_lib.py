@@ -25,7 +25,7 @@ LRQ_GEMM_T_SCRATCH_BYTES = 16 * 1024 * 1024  # include/lrq.h
 LRQ_BF16 = 0
 LRQ_F16 = 1
 LRQ_F32 = 2
-LRQ_FP8_LINEAR_ROWS = 16
+LRQ_FP8_LINEAR_ROWS = 4
 
 
 class LrqTensors(ctypes.Structure):

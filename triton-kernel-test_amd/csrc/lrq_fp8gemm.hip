@@ -69,6 +69,7 @@ struct TokenArgs {
   const uint8_t* xs;
   int64_t ldxs;
   int xshift, rows;
+  int own;        // rows of W a workgroup
   Fp8 w;
   void* out;
   int64_t ldo;
@@ -77,122 +78,98 @@ struct TokenArgs {
 
 typedef uint32_t u32_byte __attribute__((aligned(1)));
 
-// Up to 16 TM rows of X by 16 TN rows of W a workgroup; its waves take runs of the K steps and join in LDS.  W is the
-// instruction's first operand, so that a lane ends with four neighbouring outputs of one row of X.  XT kX8: X in e4m3; kBf16, kF16: 16-bit
-// rows (TM 1), quantised by every workgroup for itself.
+// Up to 16 rows of X by `own` rows of W (16 TN at most) a workgroup; its waves take runs of the K steps, D of them with all loads in flight at
+// once, and join in LDS.  W is the instruction's first operand, so that a lane ends with four neighbouring outputs of one
+// row of X.  Lane (j, g) holds pieces g and g + 4 of row j's 128 bytes (any order of K serves that both operands share): each
+// load of W takes 64 neighbouring bytes of 16 rows.
+//
+// XT kX8: X in e4m3, read as the operand.  kBf16, kF16: four 16-bit rows at most, quantised by every wave for its own steps:
+// 16 lanes a row, 8 elements each, then through LDS to the operand's lanes.
 enum { kX8 = 3 };
-template <int XT, int TM, int TN, int WAVES, int D>
+template <int XT, int TN, int WAVES, int D>
 __global__ __launch_bounds__(64 * WAVES) void k_fp8_token(TokenArgs a) {
-  static_assert(XT == kX8 || TM == 1);
-  __shared__ f32x4 red[WAVES][TM * TN][64];
+  static_assert(D <= 8);  // two dwords of scales
+  constexpr bool k8 = XT == kX8;
+  __shared__ f32x4 red[WAVES][TN][64];
+  __shared__ __attribute__((aligned(16))) char xq[k8 ? 1 : WAVES][4][128];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 15, g = lane >> 4;
-  const int64_t n0 = (int64_t)blockIdx.x * 16 * TN;
+  const int64_t n0 = (int64_t)blockIdx.x * a.own, n1 = min(n0 + a.own, a.w.rows);
   const int steps = a.w.steps, first = steps * wave / WAVES, last = steps * (wave + 1) / WAVES;
   const int sw4 = (steps + 3) / 4 * 4;
-  const uint8_t *wp[TN], *wsc[TN], *xsc[TM];
-  const char* xp[TM];
+  const uint8_t *wp[TN], *wsc[TN];
 #pragma unroll
   for (int t = 0; t < TN; ++t) {
-    const int64_t r = min(n0 + 16 * t + j, a.w.rows - 1);
-    wp[t] = a.w.codes + r * a.w.ldc + 32 * g;
+    const int64_t r = min(n0 + 16 * t + j, n1 - 1);
+    wp[t] = a.w.codes + r * a.w.ldc + 16 * g;
     wsc[t] = a.w.scales + (r >> a.w.shift) * a.w.lds;
   }
+  const int xr = min(j, a.rows - 1);  // (lanes past X's rows repeat its last: what they add is not stored)
+  const char* xp = a.x + xr * a.ldx + 16 * g;
+  const uint8_t* xsc = a.xs + (xr >> a.xshift) * a.ldxs;
+  f32x4 acc[TN];
 #pragma unroll
-  for (int t = 0; t < TM; ++t) {  // (lanes past X's rows repeat its last: what they add is not stored)
-    const int64_t r = min(16 * t + j, a.rows - 1);
-    xp[t] = a.x + r * a.ldx + (XT == kX8 ? 32 : 64) * g;
-    if constexpr (XT == kX8) xsc[t] = a.xs + (r >> a.xshift) * a.ldxs;
-  }
-  f32x4 acc[TM][TN];
-#pragma unroll
-  for (int i = 0; i < TM; ++i)
-#pragma unroll
-    for (int t = 0; t < TN; ++t) acc[i][t] = zero4();
-  constexpr int kXv = XT == kX8 ? 2 : 4;
-  struct Group {
-    Frag w[TN][D];
-    u32x4 x[TM][D][kXv];
-    uint32_t sw[TN], sx[TM];
-  };
-  const auto load = [&](int s0) {
-    Group r;
-    const int base = min(s0, sw4 - 4);
+  for (int t = 0; t < TN; ++t) acc[t] = zero4();
+  for (int s0 = first; s0 < last; s0 += D) {
+    Frag w[TN][D], x8[k8 ? D : 1];
+    Chunk<k8 ? kBf16 : XT> x16[k8 ? 1 : D];
+    constexpr int kDw = (D + 3) / 4;
+    uint32_t sw[TN][kDw], sx[kDw];
+    const int n = min(D, last - s0);
 #pragma unroll
     for (int u = 0; u < D; ++u) {
-      const int s = min(s0 + u, last - 1);
+      if (u < n) {
 #pragma unroll
-      for (int t = 0; t < TN; ++t) {
-        r.w[t][u].v[0] = ld16_stream(wp[t] + 128 * (int64_t)s);
-        r.w[t][u].v[1] = ld16_stream(wp[t] + 128 * (int64_t)s + 16);
-      }
-#pragma unroll
-      for (int t = 0; t < TM; ++t)
-#pragma unroll
-        for (int q = 0; q < kXv; ++q) {
-          if constexpr (XT == kX8) {
-            r.x[t][u][q] = ld16(xp[t] + 128 * (int64_t)s + 16 * q);
-          } else {
-            const int k = 128 * s + 32 * g + 8 * q;
-            r.x[t][u][q] = u32x4{0u, 0u, 0u, 0u};
-            if (k < a.w.cols) r.x[t][u][q] = *reinterpret_cast<const u32x4_any*>(xp[t] + 256 * (int64_t)s + 16 * q);
-          }
+        for (int t = 0; t < TN; ++t) {
+          w[t][u].v[0] = ld16_stream(wp[t] + 128 * (int64_t)(s0 + u));
+          w[t][u].v[1] = ld16_stream(wp[t] + 128 * (int64_t)(s0 + u) + 64);
         }
+        if constexpr (k8) {
+          x8[u].v[0] = ld16(xp + 128 * (int64_t)(s0 + u));
+          x8[u].v[1] = ld16(xp + 128 * (int64_t)(s0 + u) + 64);
+        } else {
+          const int k = 128 * (s0 + u) + 8 * j;
+          x16[u] = ld_chunk<XT>(a.x + min(g, a.rows - 1) * a.ldx + 2 * (int64_t)k, k < a.w.cols ? 8 : 0);
+        }
+      }
+    }
+    // scales of steps s0 + 4 d .. + 3, as far as the row goes
+    int base[kDw];
+#pragma unroll
+    for (int d = 0; d < kDw; ++d) {
+      base[d] = min(s0 + 4 * d, sw4 - 4);
+#pragma unroll
+      for (int t = 0; t < TN; ++t) sw[t][d] = *reinterpret_cast<const u32_byte*>(wsc[t] + base[d]);
+      if constexpr (k8) sx[d] = *reinterpret_cast<const u32_byte*>(xsc + base[d]);
     }
 #pragma unroll
-    for (int t = 0; t < TN; ++t) r.sw[t] = *reinterpret_cast<const u32_byte*>(wsc[t] + base);
-#pragma unroll
-    for (int t = 0; t < TM; ++t) r.sx[t] = XT == kX8 ? *reinterpret_cast<const u32_byte*>(xsc[t] + base) : 0u;
-    return r;
-  };
-  if (first < last) {
-    Group cur = load(first);
-    for (int s0 = first; s0 < last; s0 += D) {
-      const Group next = load(min(s0 + D, last - 1));
-      const int base = min(s0, sw4 - 4);
-#pragma unroll
-      for (int u = 0; u < D; ++u) {
-        if (s0 + u < last) {
-          const int sh = 8 * (s0 + u - base);
-          Frag x[TM];
-          uint32_t sx[TM];
-#pragma unroll
-          for (int i = 0; i < TM; ++i) {
-            if constexpr (XT == kX8) {
-              x[i].v[0] = cur.x[i][u][0], x[i].v[1] = cur.x[i][u][1];
-              sx[i] = cur.sx[i] >> sh;
-            } else {
-              float v[4][8];
-              uint32_t top = 0;
-#pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                Chunk<XT> c;
-                c.v[0] = cur.x[i][u][q];
-                widen<XT>(c, v[q]);
-                top = max(top, top8(v[q]));
-              }
-              sx[i] = fp8_scale(row_top(top));
-#pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                const u32x2 c = fp8_codes8(v[q], sx[i]);
-                x[i].v[q / 2][2 * (q & 1)] = c[0], x[i].v[q / 2][2 * (q & 1) + 1] = c[1];
-              }
-            }
-          }
-#pragma unroll
-          for (int t = 0; t < TN; ++t)
-#pragma unroll
-            for (int i = 0; i < TM; ++i) acc[i][t] = mfma8_16(cur.w[t][u], x[i], acc[i][t], cur.sw[t] >> sh, sx[i]);
-        }
+    for (int u = 0; u < D; ++u) {
+      if (u >= n) break;
+      const int sh = 8 * (s0 + u - base[u / 4]);
+      Frag x;
+      uint32_t s;
+      if constexpr (k8) {
+        x = x8[u];
+        s = sx[u / 4] >> sh;
+      } else {
+        float v[8];
+        widen<XT>(x16[u], v);
+        const uint32_t mine = fp8_scale(lanes16_max(top8(v)));
+        st8(&xq[wave][g][16 * (j / 2 ^ g) + 8 * (j & 1)], fp8_codes8(v, mine));
+        const int r = j & 3;  // (rows past four: their products are not stored)
+        s = (uint32_t)__shfl((int)mine, 16 * r);
+        asm volatile("" ::: "memory");
+        x.v[0] = ld16(&xq[wave][r][16 * (g ^ r)]);
+        x.v[1] = ld16(&xq[wave][r][16 * ((g + 4) ^ r)]);
+        asm volatile("" ::: "memory");
       }
-      cur = next;
+#pragma unroll
+      for (int t = 0; t < TN; ++t) acc[t] = mfma8_16(w[t][u], x, acc[t], sw[t][u / 4] >> sh, s);
     }
   }
 #pragma unroll
-  for (int i = 0; i < TM; ++i)
-#pragma unroll
-    for (int t = 0; t < TN; ++t) red[wave][i * TN + t][lane] = acc[i][t];
+  for (int t = 0; t < TN; ++t) red[wave][t][lane] = acc[t];
   __syncthreads();
-  for (int p = wave; p < TM * TN; p += WAVES) {
+  for (int p = wave; p < TN; p += WAVES) {
     f32x4 s = red[0][p][lane];
 #pragma unroll
     for (int k = 1; k < WAVES; ++k) {
@@ -200,14 +177,13 @@ __global__ __launch_bounds__(64 * WAVES) void k_fp8_token(TokenArgs a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[e] += v[e];
     }
-    const int m = 16 * (p / TN) + j;
-    const int64_t n = n0 + 16 * (p % TN) + 4 * g;
-    if (m >= a.rows) continue;
+    const int64_t n = n0 + 16 * p + 4 * g;
+    if (j >= a.rows) continue;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      if (n + e >= a.w.rows) break;
-      if (a.odt == kF32) reinterpret_cast<float*>(a.out)[m * a.ldo + n + e] = s[e];
-      else reinterpret_cast<uint16_t*>(a.out)[m * a.ldo + n + e] = bits16(s[e], a.odt);
+      if (n + e >= n1) break;
+      if (a.odt == kF32) reinterpret_cast<float*>(a.out)[j * a.ldo + n + e] = s[e];
+      else reinterpret_cast<uint16_t*>(a.out)[j * a.ldo + n + e] = bits16(s[e], a.odt);
     }
   }
 }
@@ -239,56 +215,62 @@ struct Tile8Args {
   int64_t ldo;
   int64_t cols;   // of the output
   int odt;
-  int tiles_m, tiles_n, splits;
+  int tiles_m, tiles_m2, tiles_n, splits, big;
   int steps;      // contraction steps of 128
 };
 
 // Workgroup: 64 MT rows of X by 256 output columns, four waves in two rows of two, each 32 MT x 128 of it in 32x32x64
-// instructions: one wave a SIMD, whose sums take half of its registers.  K goes through LDS in half steps of 64 bytes a
-// row, four deep, straight from memory, one barrier each.
+// instructions: one wave a SIMD, whose sums take half of its registers.  K goes through LDS in steps of 128 bytes a row,
+// straight from memory, whole cache lines at a time (with 64 bytes a row the L2s were asked twice as often, 66 % of their
+// cycles, and 8192^3 took 480 us).
 //
-// LDS: X and (NN false) W have rows of 64 bytes, row r's 16-byte piece q in slot q ^ (r / 4 % 4): 16 lanes of a read cover
-// all banks.  NN: 64 rows of W of 256 bytes, piece q of row r in slot q ^ (r % 8); the transposing read gives a lane its
+// LDS: X and (NN false) W have rows of 128 bytes, row r's 16-byte piece p in slot p ^ (r / 2 % 8): 16 lanes of a read cover
+// all banks.  NN: 128 rows of W of 256 bytes, piece p of row r in slot p ^ (r % 8); the transposing read gives a lane its
 // column of 8 rows.
 template <bool NN, int MT>
 struct Tile8Lds {
-  static constexpr int kX = 64 * MT * 64, kW = 16384, kStage = kX + kW, kDeep = 4, kRing = kDeep * kStage;
+  static constexpr int kX = 64 * MT * 128, kW = 32768, kStage = kX + kW, kDeep = MT >= 3 ? 2 : 3, kRing = kDeep * kStage;
   static constexpr int kScales = 2048, kLoop = kRing + 2 * kScales;
-  static constexpr int kPitch = 128 * 4 + 16, kOut = 4 * 32 * kPitch, kBytes = kLoop > kOut ? kLoop : kOut;
+  static constexpr int kOut = 4 * 32 * (128 * 4 + 16), kBytes = kLoop > kOut ? kLoop : kOut;
+  static_assert(kBytes <= 160 * 1024);
 };
+// Workgroup `id` of `tiles_m` by tiles_n tiles for each split, from row m1 on.
 template <bool NN, int MT, int OT>
-__global__ __launch_bounds__(256, 1) void k_fp8_tile(Tile8Args a) {
+__device__ __forceinline__ void fp8_tile(const Tile8Args& a, char* sm, uint32_t id, uint32_t tiles_m, int64_t m1) {
   using T = Tile8Lds<NN, MT>;
-  constexpr int kX = T::kX, kStage = T::kStage, kLoads = MT + 4;
-  extern __shared__ __attribute__((aligned(16))) char sm[];
+  constexpr int kX = T::kX, kStage = T::kStage, kDeep = T::kDeep, kLx = 2 * MT, kLoads = kLx + 8;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave >> 1, wn = wave & 1, c = lane & 31, h = lane >> 5;
-  const uint32_t tiles = a.tiles_m * a.tiles_n, id = xcd_tile(blockIdx.x, gridDim.x);
+  const uint32_t tiles = tiles_m * a.tiles_n;
   const uint32_t z = __builtin_amdgcn_readfirstlane(id / tiles), tile = id - z * tiles;
-  const uint32_t tn = __builtin_amdgcn_readfirstlane(tile / a.tiles_m), tm = tile - tn * a.tiles_m;
-  const int64_t m0 = (int64_t)tm * 64 * MT, n0 = (int64_t)tn * 256;
+  // runs of kBand tiles down, then across: the 32 tiles that an XCD's CUs work on share 8 rows and 4 columns of tiles
+  constexpr uint32_t kBand = 8;
+  const uint32_t band = __builtin_amdgcn_readfirstlane(tile / (kBand * a.tiles_n)), in = tile - band * kBand * a.tiles_n;
+  const uint32_t tall = min(kBand, tiles_m - band * kBand);
+  const uint32_t tn = __builtin_amdgcn_readfirstlane(in / tall), tm = band * kBand + in - tn * tall;
+  const int64_t m0 = m1 + (int64_t)tm * 64 * MT, n0 = (int64_t)tn * 256;
   const int first = __builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)a.steps * z / (uint32_t)a.splits));
   const int last = __builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)a.steps * (z + 1) / (uint32_t)a.splits));
 
-  // loads of 1 KB: 16 rows of 64 bytes (NN W: 4 rows of 256), at 32-bit offsets from the tile's first row
+  // loads of 1 KB: 8 rows of 128 bytes (NN W: 4 rows of 256), at 32-bit offsets from the tile's first row
   const uint32_t sm0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)sm;
   const uint8_t* bx = a.x.codes + m0 * a.x.ldc;
   const uint8_t* bw = NN ? a.w.codes + n0 : a.w.codes + n0 * a.w.ldc;
-  uint32_t ox[MT], ow[4];
-  int rw[4];
+  uint32_t ox[kLx], ow[8];
 #pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    const int r = 16 * (MT * wave + i) + (lane >> 2);
-    ox[i] = (uint32_t)min((int64_t)r, a.x.rows - 1 - m0) * (uint32_t)a.x.ldc + 16 * ((lane & 3) ^ (r >> 2 & 3));
+  for (int i = 0; i < kLx; ++i) {
+    const int r = 8 * (kLx * wave + i) + (lane >> 3);
+    ox[i] = (uint32_t)min((int64_t)r, a.x.rows - 1 - m0) * (uint32_t)a.x.ldc + 16 * ((lane & 7) ^ (r >> 1 & 7));
   }
+  // NN: row 32 wave + 4 i + lane / 16 of a step, whose piece does not depend on i / 2
+  const int rw = 32 * wave + (lane >> 4);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < (NN ? 2 : 8); ++i) {
     if constexpr (!NN) {
-      const int r = 16 * (4 * wave + i) + (lane >> 2);
-      ow[i] = (uint32_t)min((int64_t)r, a.w.rows - 1 - n0) * (uint32_t)a.w.ldc + 16 * ((lane & 3) ^ (r >> 2 & 3));
+      const int r = 8 * (8 * wave + i) + (lane >> 3);
+      ow[i] = (uint32_t)min((int64_t)r, a.w.rows - 1 - n0) * (uint32_t)a.w.ldc + 16 * ((lane & 7) ^ (r >> 1 & 7));
     } else {
-      rw[i] = 4 * (4 * wave + i) + (lane >> 4);
-      ow[i] = (uint32_t)min((int64_t)16 * ((lane & 15) ^ (rw[i] & 7)), 128 * (int64_t)a.w.steps - 16 - n0);
+      ow[i] = (uint32_t)min((int64_t)16 * ((lane & 15) ^ ((rw + 4 * i) & 7)), 128 * (int64_t)a.w.steps - 16 - n0);
     }
   }
   // four steps' scales of 64 rows a load; NN: of this wave's 128 columns, four steps are four rows of scales
@@ -298,19 +280,19 @@ __global__ __launch_bounds__(256, 1) void k_fp8_tile(Tile8Args a) {
   const uint32_t osw = NN ? (uint32_t)(kb & ~3) : (uint32_t)(min(n0 + 64 * wave + lane, a.w.rows - 1) >> a.w.shift) * (uint32_t)a.w.lds;
   const int blocks = (int)((a.w.rows + 127) >> 7);
 
-  // load i of half step u (u counts from the contraction's start)
-  const auto issue = [&](int u, int buf, int i) {
+  // load i of a step
+  const auto issue = [&](int step, int buf, int i) {
     const uint32_t st = sm0 + buf * kStage;
-    if (i < MT) {
-      ld_to_lds8<16, NN>(bx + 64 * (int64_t)u, ox[i < MT ? i : 0], st + 1024 * (MT * wave + i));
+    if (i < kLx) {
+      ld_to_lds8<16, NN>(bx + 128 * (int64_t)step, ox[i < kLx ? i : 0], st + 1024 * (kLx * wave + i));
     } else {
-      const int k = (i - MT) & 3;
-      const uint32_t to = st + kX + 1024 * (4 * wave + k);
+      const int k = (i - kLx) & 7;
+      const uint32_t to = st + kX + 1024 * (8 * wave + k);
       if constexpr (!NN) {
-        ld_to_lds8<16, NN>(bw + 64 * (int64_t)u, ow[k], to);
+        ld_to_lds8<16, NN>(bw + 128 * (int64_t)step, ow[k], to);
       } else {  // rows past W's last: that one (their x is zero)
-        const uint32_t end = (uint32_t)a.w.rows - 1, r0 = min(64u * (uint32_t)u, end);
-        ld_to_lds8<16, NN>(bw + (int64_t)r0 * a.w.ldc, min((uint32_t)rw[k], end - r0) * (uint32_t)a.w.ldc + ow[k], to);
+        const uint32_t end = (uint32_t)a.w.rows - 1 - 128u * (uint32_t)step;
+        ld_to_lds8<16, NN>(bw + 128 * (int64_t)step * a.w.ldc, min((uint32_t)(rw + 4 * k), end) * (uint32_t)a.w.ldc + ow[k & 1], to);
       }
     }
   };
@@ -322,24 +304,29 @@ __global__ __launch_bounds__(256, 1) void k_fp8_tile(Tile8Args a) {
     else ld_to_lds8<4, NN>(a.w.scales, (uint32_t)min(4 * gr + (lane & 3), blocks - 1) * (uint32_t)a.w.lds + osw, sc + 1024 + 256 * wave);
   };
 
+  // operands of half Q of a step (64 of K): piece 4 Q + 2 h + q of a row
   Frag fx[2][MT], fw[2][4];
   uint32_t sx[MT], sw[4];
-  const auto read_x = [&](int set, int buf, int i, int q) {
+  const auto read_x = [&](int half, int buf, int i, int q) {
     const int r = 32 * MT * wm + 32 * i + c;
-    fx[set][i].v[q] = ld16(sm + buf * kStage + 64 * r + 16 * ((2 * h + q) ^ (r >> 2 & 3)));
+    fx[half][i].v[q] = ld16(sm + buf * kStage + 128 * r + 16 * ((4 * half + 2 * h + q) ^ (r >> 1 & 7)));
   };
-  const auto read_w = [&](int set, int buf, int t, int q) {
+  const auto read_w = [&](int half, int buf, int t, int q) {
     const char* st = sm + buf * kStage + kX;
     if constexpr (!NN) {
       const int r = 128 * wn + 32 * t + c;
-      fw[set][t].v[q] = ld16(st + 64 * r + 16 * ((2 * h + q) ^ (r >> 2 & 3)));
+      fw[half][t].v[q] = ld16(st + 128 * r + 16 * ((4 * half + 2 * h + q) ^ (r >> 1 & 7)));
     } else {
-      const int r = 32 * h + 16 * q + (lane >> 1 & 7), piece = 8 * wn + 2 * t + (lane >> 4 & 1);
+      const int r = 64 * half + 32 * h + 16 * q + (lane >> 1 & 7), piece = 8 * wn + 2 * t + (lane >> 4 & 1);
       typedef int i32x2 __attribute__((ext_vector_type(2)));
       const auto p = (__attribute__((address_space(3))) i32x2*)(st + 256 * r + 16 * (piece ^ (r & 7)) + 8 * (lane & 1));
       const i32x2 lo = __builtin_amdgcn_ds_read_tr8_b64_v2i32(p), hi = __builtin_amdgcn_ds_read_tr8_b64_v2i32(p + 8 * 32);
-      fw[set][t].v[q] = u32x4{(uint32_t)lo[0], (uint32_t)lo[1], (uint32_t)hi[0], (uint32_t)hi[1]};
+      fw[half][t].v[q] = u32x4{(uint32_t)lo[0], (uint32_t)lo[1], (uint32_t)hi[0], (uint32_t)hi[1]};
     }
+  };
+  const auto read_piece = [&](int half, int buf, int p) {
+    if (p < 8) read_w(half, buf, p >> 1, p & 1);
+    else read_x(half, buf, (p - 8) >> 1, p & 1);
   };
   const auto read_scales = [&](int step) {
     const char* sc = sm + T::kRing + (step >> 2 & 1) * T::kScales;
@@ -362,55 +349,61 @@ __global__ __launch_bounds__(256, 1) void k_fp8_tile(Tile8Args a) {
 #pragma unroll
       for (int v = 0; v < 16; ++v) acc[i][t][v] = 0.f;
 
+  // Half 1 of a step is read from LDS behind the first instructions of half 0, half 0 of the next step behind those of half 1.
+  // The workgroup meets twice in a step: once all of it has been read, whose place the loads of kDeep steps on then take,
+  // and before half 1, when the next step's loads are in.  The loads go out evenly over the rest of the step: they are
+  // 16 TB/s of the L2s' at full speed, and 1.5 to 2 at a time 8192^3 took 440 us, at 1 behind each instruction of half 1 404,
+  // so 395.  The order is held: the compiler would issue all loads first.
+  constexpr int kMfma = 4 * MT, kPieces = 2 * (MT + 4), kReads = (kPieces + kMfma / 2 - 1) / (kMfma / 2);
+  constexpr int kFirst = 3 * kLoads / 8;  // of a step's loads: behind the second half of half 0's instructions
   issue_scales(first >> 2);
   issue_scales((first >> 2) + 1);
-  const int end = 2 * last - 1;
 #pragma unroll
-  for (int d = 0; d < 4; ++d)
+  for (int d = 0; d < kDeep; ++d)
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) issue(min(2 * first + d, end), d, i);
-  __builtin_amdgcn_s_waitcnt(vmcnt_imm(3 * kLoads));
+    for (int i = 0; i < kLoads; ++i) issue(min(first + d, last - 1), d, i);
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm((kDeep - 1) * kLoads));
   lds_meet();
 #pragma unroll
-  for (int q = 0; q < 2; ++q) {
-#pragma unroll
-    for (int i = 0; i < MT; ++i) read_x(0, 0, i, q);
-#pragma unroll
-    for (int t = 0; t < 4; ++t) read_w(0, 0, t, q);
-  }
+  for (int p = 0; p < kPieces; ++p) read_piece(0, 0, p);
   read_scales(first);
   int buf = 0;
   for (int step = first; step < last; ++step) {
+    const int next = buf + 1 == kDeep ? 0 : buf + 1;
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      // the next half step's loads are in, not those of the two after it, and every wave has read all of this one's buffer
-      __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * kLoads));
-      lds_meet();
-      const int u = 2 * step + q, next = (buf + 1) & 3;
-      if (q == 0 && (step & 3) == 0 && step > first) issue_scales((step >> 2) + 1);
+    for (int m = 0; m < kMfma; ++m) {
+      const int i = m >> 2, t = m & 3, late = m - kMfma / 2;
+      acc[i][t] = mfma8_32(fw[0][t], fx[0][i], acc[i][t], sw[NN ? 0 : t], sx[i]);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int m = 0; m < 4 * MT; ++m) {
-        const int i = m >> 2, t = m & 3;
-        acc[i][t] = mfma8_32(fw[q][t], fx[q][i], acc[i][t], sw[NN ? 0 : t], sx[i]);
-        __builtin_amdgcn_sched_barrier(0);
-        constexpr int kPieces = 2 * (MT + 4), kPer = (kPieces + 4 * MT - 1) / (4 * MT);
+      for (int p = kReads * m; p < kReads * (m + 1); ++p)
+        if (p < kPieces) read_piece(1, buf, p);
+      if (late == 0) lds_meet();
 #pragma unroll
-        for (int p = kPer * m; p < kPer * (m + 1); ++p) {
-          if (p < 8) read_w(1 - q, next, p >> 1, p & 1);
-          else if (p < kPieces) read_x(1 - q, next, (p - 8) >> 1, p & 1);
-        }
-        constexpr int kGap = 4 * MT / kLoads > 0 ? 4 * MT / kLoads : 1, kEach = (kLoads + 4 * MT - 1) / (4 * MT);
-        if (m % kGap == kGap - 1) {
-#pragma unroll
-          for (int i2 = kEach * (m / kGap); i2 < kEach * (m / kGap + 1); ++i2)
-            if (i2 < kLoads) issue(min(u + 4, end), buf, i2);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      if (q == 1) read_scales(min(step + 1, last - 1));
-      buf = next;
+      for (int l = 0; l < kFirst; ++l)
+        if (l * (kMfma / 2) / kFirst == late) issue(min(step + kDeep, last - 1), buf, l);
+      __builtin_amdgcn_sched_barrier(0);
     }
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm((kDeep - 2) * kLoads + kFirst));
+    lds_meet();
+    if ((step & 3) == 0 && step > first) issue_scales((step >> 2) + 1);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int m = 0; m < kMfma; ++m) {
+      const int i = m >> 2, t = m & 3;
+      acc[i][t] = mfma8_32(fw[1][t], fx[1][i], acc[i][t], sw[NN ? 0 : t], sx[i]);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int l = 0; l < kLoads - kFirst; ++l)
+        if (l * kMfma / (kLoads - kFirst) == m) issue(min(step + kDeep, last - 1), buf, kFirst + l);
+#pragma unroll
+      for (int p = kReads * m; p < kReads * (m + 1); ++p)
+        if (p < kPieces) read_piece(0, next, p);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    read_scales(min(step + 1, last - 1));
+    buf = next;
   }
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // the last loads write LDS
   lds_meet();
@@ -448,6 +441,18 @@ __global__ __launch_bounds__(256, 1) void k_fp8_tile(Tile8Args a) {
   }
 }
 
+// The first `big` workgroups' tiles have 64 MT rows, the others' 64 MT2 of the rows behind them: where tiles of one height
+// leave the last round of workgroups half empty, lower ones fill it.
+template <bool NN, int MT, int MT2, int OT>
+__global__ __launch_bounds__(256, 1) void k_fp8_tile(Tile8Args a) {
+  extern __shared__ __attribute__((aligned(16))) char sm[];
+  if (MT == MT2 || blockIdx.x < (uint32_t)a.big) {
+    fp8_tile<NN, MT, OT>(a, sm, xcd_tile(blockIdx.x, a.big), a.tiles_m, 0);
+  } else if constexpr (MT != MT2) {
+    fp8_tile<NN, MT2, OT>(a, sm, xcd_tile(blockIdx.x - a.big, gridDim.x - a.big), a.tiles_m2, (int64_t)a.tiles_m * 64 * MT);
+  }
+}
+
 // out[rows, cols] = the splits' sums, in their order; 4 columns a thread.
 __global__ __launch_bounds__(256) void k_fp8_join(const float* part, int splits, int64_t rows, int64_t cols, int64_t ldp,
                                                   void* out, int64_t ldo, int odt) {
@@ -471,30 +476,47 @@ __global__ __launch_bounds__(256) void k_fp8_join(const float* part, int splits,
 }
 
 struct Plan8 {
-  int mt;  // 64 mt rows a workgroup; 0: the few-row kernel
-  int64_t tiles_m, tiles_n;
+  int mt, mt2;               // 64 mt rows a workgroup, mt2 behind them; 0: the few-row kernel
+  int64_t tiles_m, tiles_m2, tiles_n;
   int splits, steps;
 };
 
-static constexpr int kTokenRows = 64;
+static constexpr int kTokenRows = 16;
 
-// The tile's height and how often the contraction is split over workgroups, by the rounds of workgroups that the grid takes.
+// The tiles' heights and how often the contraction is split over workgroups, by the rounds of workgroups that the grid takes
+// (one runs on a CU at a time).
 static Plan8 plan8(const lrq_fp8* a, const lrq_fp8* b, bool nn) {
-  constexpr double kStep[3] = {0.45, 0.6, 1.0}, kFixed = 6.0, kJoin = 4.0, kPerByte = 2.0 / 4.0e6;
-  const int64_t rows = a->rows, cols = nn ? b->cols : b->rows;
+  constexpr double kStep[4] = {0.62, 0.86, 1.19, 1.44}, kFixed[4] = {1.5, 5.5, 5.0, 6.0}, kJoin = 4.0, kPerByte = 2.0 / 4.0e6;
+  constexpr int kCus = 256;  // a fixed count, so that the workspace and the order of the sums depend on the shape alone
+  const int64_t rows = a->rows, cols = nn ? b->cols : b->rows, tiles_n = (cols + 255) / 256;
   const int steps = (int)((a->cols + 127) / 128);
-  if (!nn && rows <= kTokenRows) return Plan8{0, 0, 0, 1, steps};
+  if (!nn && rows <= kTokenRows) return Plan8{0, 0, 0, 0, 0, 1, steps};
   Plan8 best{};
   double least = 0.;
-  for (int i = 0; i < 3; ++i) {
-    Plan8 p{1 << i, 0, (cols + 255) / 256, 1, steps};
-    p.tiles_m = (rows + 64 * p.mt - 1) / (64 * p.mt);
+  const auto take = [&](const Plan8& p, double cost) {
+    if (best.mt == 0 || cost < least) best = p, least = cost;
+  };
+  for (int mt = 1; mt <= 4; ++mt) {
+    Plan8 p{mt, mt, (rows + 64 * mt - 1) / (64 * mt), 0, tiles_n, 1, steps};
     for (; p.splits <= 16 && p.splits <= std::max(1, steps / 4); ++p.splits) {
-      const double rounds = (double)((p.tiles_m * p.tiles_n * p.splits + 255) / 256);
-      const double cost = rounds * ((steps + p.splits - 1) / p.splits * kStep[i] + kFixed) +
-                          (p.splits > 1 ? kJoin + kPerByte * 4. * p.splits * rows * cols : 0.);
-      if (best.mt == 0 || cost < least) best = p, least = cost;
+      const double rounds = (double)((p.tiles_m * tiles_n * p.splits + kCus - 1) / kCus);
+      take(p, rounds * ((steps + p.splits - 1) / p.splits * kStep[mt - 1] + kFixed[mt - 1]) +
+                  (p.splits > 1 ? kJoin + kPerByte * 4. * p.splits * rows * cols : 0.));
     }
+  }
+  // high tiles first and low ones behind them, each to the CU that is free first
+  const double high = steps * kStep[3] + kFixed[3], low = steps * kStep[1] + kFixed[1];
+  for (int64_t m = rows / 256, end = std::max<int64_t>(0, m - 8); m > end && m * tiles_n >= kCus; --m) {
+    const Plan8 p{4, 2, m, (rows - 256 * m + 127) / 128, tiles_n, 1, steps};
+    const int64_t full = m * tiles_n / kCus, over = m * tiles_n % kCus;
+    if (p.tiles_m2 == 0) continue;
+    double now = full * high, behind = now + high, ends = over > 0 ? behind : now;  // of the CUs without, with one more high tile
+    for (int64_t left = p.tiles_m2 * tiles_n; left > 0;) {
+      const bool ahead = over == 0 || now <= behind;
+      left -= ahead ? kCus - over : over;
+      ends = std::max(ends, (ahead ? now : behind) += low);
+    }
+    take(p, ends);
   }
   return best;
 }
@@ -521,13 +543,22 @@ static int validate_pair(const lrq_fp8* a, const lrq_fp8* b, bool nn) {
   return nn && b->block != 128 ? LRQ_ERR_UNSUPPORTED : LRQ_OK;
 }
 
-template <int XT, int TM>
-static int token(const TokenArgs& a, hipStream_t s) {
-  const int64_t tiles = (a.w.rows + 15) / 16;
-  constexpr int D = XT == kX8 ? (TM == 4 ? 1 : 2) : 2;
-  // one tile of W a workgroup where that fills the CUs no more than twice
-  if (tiles > 1024) return launch((k_fp8_token<XT, TM, 2, 4, D>), dim3((unsigned)((tiles + 1) / 2)), dim3(256), 0, s, a);
-  return launch((k_fp8_token<XT, TM, 1, 8, D>), dim3((unsigned)tiles), dim3(512), 0, s, a);
+template <int XT>
+static int token(TokenArgs a, hipStream_t s) {
+  using std::integral_constant;
+  const int64_t n = a.w.rows;
+  const auto go = [&](auto tn, auto waves, auto d, int64_t wgs) {
+    a.own = (int)std::min<int64_t>(16 * tn(), ((n + wgs - 1) / wgs + 3) / 4 * 4);
+    return launch((k_fp8_token<XT, tn(), waves(), d()>), dim3((unsigned)((n + a.own - 1) / a.own)), dim3(64 * waves()), 0, s, a);
+  };
+#define LRQ_GO(TN, WAVES, WGS) return go(integral_constant<int, TN>{}, integral_constant<int, WAVES>{}, integral_constant<int, 4>{}, WGS)
+  // Every CU the same bytes of W, which come to it at about 18 GB/s whatever the others do: a workgroup a CU, of
+  // as many rows as that makes ([5120, 5120] by one row 8.9 us; whole tiles of 16 rows, 320 of them: 11.5).  More than 32
+  // rows a CU: two workgroups, whose starts and ends overlap ([14336, 4096] 13.7 us against 15.5 with one of 56 rows).
+  if (n <= 4096) LRQ_GO(1, 16, 256);
+  if (n <= 8192) LRQ_GO(2, 16, 256);
+  LRQ_GO(2, 8, 512 * ((n + 16383) / 16384));
+#undef LRQ_GO
 }
 
 static int fp8_product(const lrq_fp8* ta, const lrq_fp8* tb, bool nn, void* out, int64_t ldo, int32_t odt, void* workspace,
@@ -539,8 +570,8 @@ static int fp8_product(const lrq_fp8* ta, const lrq_fp8* tb, bool nn, void* out,
   const Plan8 p = plan8(ta, tb, nn);
   const Fp8 x = make_fp8(ta), w = make_fp8(tb);
   if (p.mt == 0) {
-    const TokenArgs a{(const char*)x.codes, x.ldc, x.scales, x.lds, x.shift, (int)rows, w, out, ldo, odt};
-    return rows <= 16 ? token<kX8, 1>(a, s) : rows <= 32 ? token<kX8, 2>(a, s) : token<kX8, 4>(a, s);
+    const TokenArgs a{(const char*)x.codes, x.ldc, x.scales, x.lds, x.shift, (int)rows, 0, w, out, ldo, odt};
+    return token<kX8>(a, s);
   }
   const int64_t need = parts_bytes(p.splits, rows, cols), ldp = (cols + 3) / 4 * 4;
   if (need > 0) {
@@ -548,26 +579,28 @@ static int fp8_product(const lrq_fp8* ta, const lrq_fp8* tb, bool nn, void* out,
     if (!aligned(workspace, 16)) return LRQ_ERR_ALIGN;
     if (workspace_bytes < need) return LRQ_ERR_WORKSPACE;
   }
-  const int64_t wgs = p.tiles_m * p.tiles_n * p.splits;
+  const int64_t big = p.tiles_m * p.tiles_n * p.splits, wgs = big + p.tiles_m2 * p.tiles_n;
   if (wgs > INT32_MAX) return LRQ_ERR_SHAPE;
-  const Tile8Args a{x, w, need ? workspace : out, need ? ldp : ldo, cols, need ? (int)kF32 : odt, (int)p.tiles_m, (int)p.tiles_n,
-                    p.splits, p.steps};
+  const Tile8Args a{x, w, need ? workspace : out, need ? ldp : ldo, cols, need ? (int)kF32 : odt, (int)p.tiles_m,
+                    (int)p.tiles_m2, (int)p.tiles_n, p.splits, (int)big, p.steps};
   const auto go = [&](auto kern, int lds) {
     const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (e != hipSuccess) return (int)e;
     return launch(kern, dim3((unsigned)wgs), dim3(256), (size_t)lds, s, a);
   };
-  const auto with = [&](auto mt) {
+  const auto with = [&](auto mt, auto mt2) {
+    constexpr int kLds = std::max(Tile8Lds<true, mt()>::kBytes, Tile8Lds<true, mt2()>::kBytes);
     const auto typed = [&](auto ot) {
-      return nn ? go(k_fp8_tile<true, mt(), ot()>, Tile8Lds<true, mt()>::kBytes)
-                : go(k_fp8_tile<false, mt(), ot()>, Tile8Lds<false, mt()>::kBytes);
+      return nn ? go(k_fp8_tile<true, mt(), mt2(), ot()>, kLds) : go(k_fp8_tile<false, mt(), mt2(), ot()>, kLds);
     };
     if (a.odt == kBf16) return typed(std::integral_constant<int, kBf16>{});
     return a.odt == kF16 ? typed(std::integral_constant<int, kF16>{}) : typed(std::integral_constant<int, kF32>{});
   };
-  if (p.mt == 4) LRQ_TRY(with(std::integral_constant<int, 4>{}));
-  else if (p.mt == 2) LRQ_TRY(with(std::integral_constant<int, 2>{}));
-  else LRQ_TRY(with(std::integral_constant<int, 1>{}));
+  using std::integral_constant;
+  if (p.mt == 4) LRQ_TRY(with(integral_constant<int, 4>{}, integral_constant<int, 2>{}));
+  else if (p.mt == 3) LRQ_TRY(with(integral_constant<int, 3>{}, integral_constant<int, 3>{}));
+  else if (p.mt == 2) LRQ_TRY(with(integral_constant<int, 2>{}, integral_constant<int, 2>{}));
+  else LRQ_TRY(with(integral_constant<int, 1>{}, integral_constant<int, 1>{}));
   if (need == 0) return LRQ_OK;
   const dim3 grid((unsigned)std::min<int64_t>((rows * (ldp / 4) + 255) / 256, (int64_t)cu_count() * 32));
   return launch(k_fp8_join, grid, dim3(256), 0, s, (const float*)workspace, p.splits, rows, cols, ldp, out, ldo, odt);
@@ -603,7 +636,7 @@ extern "C" int lrq_fp8_linear(const void* x, int64_t ldx, int32_t dtype, int64_t
   if (ldx < t->cols) return LRQ_ERR_SHAPE;
   if (!aligned(x, 2)) return LRQ_ERR_ALIGN;
   LRQ_TRY(validate_out8(out, ldo, t->rows, out_dtype));
-  const TokenArgs a{(const char*)x, 2 * ldx, nullptr, 0, 0, (int)rows, make_fp8(t), out, ldo, out_dtype};
+  const TokenArgs a{(const char*)x, 2 * ldx, nullptr, 0, 0, (int)rows, 0, make_fp8(t), out, ldo, out_dtype};
   hipStream_t s = (hipStream_t)stream;
-  return dtype == LRQ_BF16 ? token<kBf16, 1>(a, s) : token<kF16, 1>(a, s);
+  return dtype == LRQ_BF16 ? token<kBf16>(a, s) : token<kF16>(a, s);
 }
