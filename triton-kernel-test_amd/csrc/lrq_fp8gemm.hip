@@ -215,7 +215,7 @@ struct Tile8Args {
   int64_t ldo;
   int64_t cols;   // of the output
   int odt;
-  int tiles_m, tiles_m2, tiles_n, splits, big;
+  int tiles_m, tiles_n, splits;
   int steps;      // contraction steps of 128
 };
 
@@ -234,21 +234,21 @@ struct Tile8Lds {
   static constexpr int kOut = 4 * 32 * (128 * 4 + 16), kBytes = kLoop > kOut ? kLoop : kOut;
   static_assert(kBytes <= 160 * 1024);
 };
-// Workgroup `id` of `tiles_m` by tiles_n tiles for each split, from row m1 on.
 template <bool NN, int MT, int OT>
-__device__ __forceinline__ void fp8_tile(const Tile8Args& a, char* sm, uint32_t id, uint32_t tiles_m, int64_t m1) {
+__global__ __launch_bounds__(256, 1) void k_fp8_tile(Tile8Args a) {
   using T = Tile8Lds<NN, MT>;
   constexpr int kX = T::kX, kStage = T::kStage, kDeep = T::kDeep, kLx = 2 * MT, kLoads = kLx + 8;
+  extern __shared__ __attribute__((aligned(16))) char sm[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave >> 1, wn = wave & 1, c = lane & 31, h = lane >> 5;
-  const uint32_t tiles = tiles_m * a.tiles_n;
+  const uint32_t tiles = a.tiles_m * a.tiles_n, id = xcd_tile(blockIdx.x, gridDim.x);
   const uint32_t z = __builtin_amdgcn_readfirstlane(id / tiles), tile = id - z * tiles;
   // runs of kBand tiles down, then across: the 32 tiles that an XCD's CUs work on share 8 rows and 4 columns of tiles
   constexpr uint32_t kBand = 8;
   const uint32_t band = __builtin_amdgcn_readfirstlane(tile / (kBand * a.tiles_n)), in = tile - band * kBand * a.tiles_n;
-  const uint32_t tall = min(kBand, tiles_m - band * kBand);
+  const uint32_t tall = min(kBand, a.tiles_m - band * kBand);
   const uint32_t tn = __builtin_amdgcn_readfirstlane(in / tall), tm = band * kBand + in - tn * tall;
-  const int64_t m0 = m1 + (int64_t)tm * 64 * MT, n0 = (int64_t)tn * 256;
+  const int64_t m0 = (int64_t)tm * 64 * MT, n0 = (int64_t)tn * 256;
   const int first = __builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)a.steps * z / (uint32_t)a.splits));
   const int last = __builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)a.steps * (z + 1) / (uint32_t)a.splits));
 
@@ -441,18 +441,6 @@ __device__ __forceinline__ void fp8_tile(const Tile8Args& a, char* sm, uint32_t 
   }
 }
 
-// The first `big` workgroups' tiles have 64 MT rows, the others' 64 MT2 of the rows behind them: where tiles of one height
-// leave the last round of workgroups half empty, lower ones fill it.
-template <bool NN, int MT, int MT2, int OT>
-__global__ __launch_bounds__(256, 1) void k_fp8_tile(Tile8Args a) {
-  extern __shared__ __attribute__((aligned(16))) char sm[];
-  if (MT == MT2 || blockIdx.x < (uint32_t)a.big) {
-    fp8_tile<NN, MT, OT>(a, sm, xcd_tile(blockIdx.x, a.big), a.tiles_m, 0);
-  } else if constexpr (MT != MT2) {
-    fp8_tile<NN, MT2, OT>(a, sm, xcd_tile(blockIdx.x - a.big, gridDim.x - a.big), a.tiles_m2, (int64_t)a.tiles_m * 64 * MT);
-  }
-}
-
 // out[rows, cols] = the splits' sums, in their order; 4 columns a thread.
 __global__ __launch_bounds__(256) void k_fp8_join(const float* part, int splits, int64_t rows, int64_t cols, int64_t ldp,
                                                   void* out, int64_t ldo, int odt) {
@@ -476,47 +464,34 @@ __global__ __launch_bounds__(256) void k_fp8_join(const float* part, int splits,
 }
 
 struct Plan8 {
-  int mt, mt2;               // 64 mt rows a workgroup, mt2 behind them; 0: the few-row kernel
-  int64_t tiles_m, tiles_m2, tiles_n;
+  int mt;  // 64 mt rows a workgroup; 0: the few-row kernel
+  int64_t tiles_m, tiles_n;
   int splits, steps;
 };
 
 static constexpr int kTokenRows = 16;
 
-// The tiles' heights and how often the contraction is split over workgroups, by the rounds of workgroups that the grid takes
-// (one runs on a CU at a time).
+// The tile's height and how often the contraction is split over workgroups: one workgroup runs on a CU at a time, so a
+// grid takes rounds of its steps; every split writes and re-reads fp32 parts.  Times in us, as measured (a step of
+// each height; a workgroup's start and end; the join's launch; its bytes at 4 TB/s).  A last round that does not
+// fill the card runs at higher clocks: half full it takes 0.8 of a full one.
 static Plan8 plan8(const lrq_fp8* a, const lrq_fp8* b, bool nn) {
   constexpr double kStep[4] = {0.62, 0.86, 1.19, 1.44}, kFixed[4] = {1.5, 5.5, 5.0, 6.0}, kJoin = 4.0, kPerByte = 2.0 / 4.0e6;
   constexpr int kCus = 256;  // a fixed count, so that the workspace and the order of the sums depend on the shape alone
   const int64_t rows = a->rows, cols = nn ? b->cols : b->rows, tiles_n = (cols + 255) / 256;
   const int steps = (int)((a->cols + 127) / 128);
-  if (!nn && rows <= kTokenRows) return Plan8{0, 0, 0, 0, 0, 1, steps};
+  if (!nn && rows <= kTokenRows) return Plan8{0, 0, 0, 1, steps};
   Plan8 best{};
   double least = 0.;
-  const auto take = [&](const Plan8& p, double cost) {
-    if (best.mt == 0 || cost < least) best = p, least = cost;
-  };
   for (int mt = 1; mt <= 4; ++mt) {
-    Plan8 p{mt, mt, (rows + 64 * mt - 1) / (64 * mt), 0, tiles_n, 1, steps};
+    Plan8 p{mt, (rows + 64 * mt - 1) / (64 * mt), tiles_n, 1, steps};
     for (; p.splits <= 16 && p.splits <= std::max(1, steps / 4); ++p.splits) {
-      const double rounds = (double)((p.tiles_m * tiles_n * p.splits + kCus - 1) / kCus);
-      take(p, rounds * ((steps + p.splits - 1) / p.splits * kStep[mt - 1] + kFixed[mt - 1]) +
-                  (p.splits > 1 ? kJoin + kPerByte * 4. * p.splits * rows * cols : 0.));
+      const int64_t wgs = p.tiles_m * tiles_n * p.splits, over = wgs % kCus;
+      const double rounds = (double)(wgs / kCus) + (over ? 0.6 + 0.4 * (double)over / kCus : 0.);
+      const double cost = rounds * ((steps + p.splits - 1) / p.splits * kStep[mt - 1] + kFixed[mt - 1]) +
+                          (p.splits > 1 ? kJoin + kPerByte * 4. * p.splits * rows * cols : 0.);
+      if (best.mt == 0 || cost < least) best = p, least = cost;
     }
-  }
-  // high tiles first and low ones behind them, each to the CU that is free first
-  const double high = steps * kStep[3] + kFixed[3], low = steps * kStep[1] + kFixed[1];
-  for (int64_t m = rows / 256, end = std::max<int64_t>(0, m - 8); m > end && m * tiles_n >= kCus; --m) {
-    const Plan8 p{4, 2, m, (rows - 256 * m + 127) / 128, tiles_n, 1, steps};
-    const int64_t full = m * tiles_n / kCus, over = m * tiles_n % kCus;
-    if (p.tiles_m2 == 0) continue;
-    double now = full * high, behind = now + high, ends = over > 0 ? behind : now;  // of the CUs without, with one more high tile
-    for (int64_t left = p.tiles_m2 * tiles_n; left > 0;) {
-      const bool ahead = over == 0 || now <= behind;
-      left -= ahead ? kCus - over : over;
-      ends = std::max(ends, (ahead ? now : behind) += low);
-    }
-    take(p, ends);
   }
   return best;
 }
@@ -579,28 +554,28 @@ static int fp8_product(const lrq_fp8* ta, const lrq_fp8* tb, bool nn, void* out,
     if (!aligned(workspace, 16)) return LRQ_ERR_ALIGN;
     if (workspace_bytes < need) return LRQ_ERR_WORKSPACE;
   }
-  const int64_t big = p.tiles_m * p.tiles_n * p.splits, wgs = big + p.tiles_m2 * p.tiles_n;
+  const int64_t wgs = p.tiles_m * p.tiles_n * p.splits;
   if (wgs > INT32_MAX) return LRQ_ERR_SHAPE;
   const Tile8Args a{x, w, need ? workspace : out, need ? ldp : ldo, cols, need ? (int)kF32 : odt, (int)p.tiles_m,
-                    (int)p.tiles_m2, (int)p.tiles_n, p.splits, (int)big, p.steps};
+                    (int)p.tiles_n, p.splits, p.steps};
   const auto go = [&](auto kern, int lds) {
     const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (e != hipSuccess) return (int)e;
     return launch(kern, dim3((unsigned)wgs), dim3(256), (size_t)lds, s, a);
   };
-  const auto with = [&](auto mt, auto mt2) {
-    constexpr int kLds = std::max(Tile8Lds<true, mt()>::kBytes, Tile8Lds<true, mt2()>::kBytes);
-    const auto typed = [&](auto ot) {
-      return nn ? go(k_fp8_tile<true, mt(), mt2(), ot()>, kLds) : go(k_fp8_tile<false, mt(), mt2(), ot()>, kLds);
-    };
-    if (a.odt == kBf16) return typed(std::integral_constant<int, kBf16>{});
-    return a.odt == kF16 ? typed(std::integral_constant<int, kF16>{}) : typed(std::integral_constant<int, kF32>{});
-  };
   using std::integral_constant;
-  if (p.mt == 4) LRQ_TRY(with(integral_constant<int, 4>{}, integral_constant<int, 2>{}));
-  else if (p.mt == 3) LRQ_TRY(with(integral_constant<int, 3>{}, integral_constant<int, 3>{}));
-  else if (p.mt == 2) LRQ_TRY(with(integral_constant<int, 2>{}, integral_constant<int, 2>{}));
-  else LRQ_TRY(with(integral_constant<int, 1>{}, integral_constant<int, 1>{}));
+  const auto with = [&](auto mt) {
+    const auto typed = [&](auto ot) {
+      return nn ? go(k_fp8_tile<true, mt(), ot()>, Tile8Lds<true, mt()>::kBytes)
+                : go(k_fp8_tile<false, mt(), ot()>, Tile8Lds<false, mt()>::kBytes);
+    };
+    if (a.odt == kBf16) return typed(integral_constant<int, kBf16>{});
+    return a.odt == kF16 ? typed(integral_constant<int, kF16>{}) : typed(integral_constant<int, kF32>{});
+  };
+  if (p.mt == 4) LRQ_TRY(with(integral_constant<int, 4>{}));
+  else if (p.mt == 3) LRQ_TRY(with(integral_constant<int, 3>{}));
+  else if (p.mt == 2) LRQ_TRY(with(integral_constant<int, 2>{}));
+  else LRQ_TRY(with(integral_constant<int, 1>{}));
   if (need == 0) return LRQ_OK;
   const dim3 grid((unsigned)std::min<int64_t>((rows * (ldp / 4) + 255) / 256, (int64_t)cu_count() * 32));
   return launch(k_fp8_join, grid, dim3(256), 0, s, (const float*)workspace, p.splits, rows, cols, ldp, out, ldo, odt);
