@@ -78,7 +78,7 @@ struct TokenArgs {
 
 typedef uint32_t u32_byte __attribute__((aligned(1)));
 
-// Up to 16 rows of X by `own` rows of W (16 TN at most) a workgroup; its waves take runs of the K steps, D of them with all loads in flight at
+// Up to 16 TM rows of X by `own` rows of W (16 TN at most) a workgroup; its waves take runs of the K steps, D of them with all loads in flight at
 // once, and join in LDS.  W is the instruction's first operand, so that a lane ends with four neighbouring outputs of one
 // row of X.  Lane (j, g) holds pieces g and g + 4 of row j's 128 bytes (any order of K serves that both operands share): each
 // load of W takes 64 neighbouring bytes of 16 rows.
@@ -86,11 +86,11 @@ typedef uint32_t u32_byte __attribute__((aligned(1)));
 // XT kX8: X in e4m3, read as the operand.  kBf16, kF16: four 16-bit rows at most, quantised by every wave for its own steps:
 // 16 lanes a row, 8 elements each, then through LDS to the operand's lanes.
 enum { kX8 = 3 };
-template <int XT, int TN, int WAVES, int D>
+template <int XT, int TM, int TN, int WAVES, int D>
 __global__ __launch_bounds__(64 * WAVES) void k_fp8_token(TokenArgs a) {
-  static_assert(D <= 8);  // two dwords of scales
   constexpr bool k8 = XT == kX8;
-  __shared__ f32x4 red[WAVES][TN][64];
+  static_assert(D <= 4 && (k8 || TM == 1));  // (a dword holds four steps' scales)
+  __shared__ f32x4 red[WAVES][TM * TN][64];
   __shared__ __attribute__((aligned(16))) char xq[k8 ? 1 : WAVES][4][128];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 15, g = lane >> 4;
   const int64_t n0 = (int64_t)blockIdx.x * a.own, n1 = min(n0 + a.own, a.w.rows);
@@ -103,18 +103,24 @@ __global__ __launch_bounds__(64 * WAVES) void k_fp8_token(TokenArgs a) {
     wp[t] = a.w.codes + r * a.w.ldc + 16 * g;
     wsc[t] = a.w.scales + (r >> a.w.shift) * a.w.lds;
   }
-  const int xr = min(j, a.rows - 1);  // (lanes past X's rows repeat its last: what they add is not stored)
-  const char* xp = a.x + xr * a.ldx + 16 * g;
-  const uint8_t* xsc = a.xs + (xr >> a.xshift) * a.ldxs;
-  f32x4 acc[TN];
+  const char* xp[TM];
+  const uint8_t* xsc[TM];
 #pragma unroll
-  for (int t = 0; t < TN; ++t) acc[t] = zero4();
+  for (int i = 0; i < TM; ++i) {  // (lanes past X's rows repeat its last: what they add is not stored)
+    const int64_t r = min(16 * i + j, a.rows - 1);
+    xp[i] = a.x + r * a.ldx + 16 * g;
+    xsc[i] = a.xs + (r >> a.xshift) * a.ldxs;
+  }
+  f32x4 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int t = 0; t < TN; ++t) acc[i][t] = zero4();
   for (int s0 = first; s0 < last; s0 += D) {
-    Frag w[TN][D], x8[k8 ? D : 1];
+    Frag w[TN][D], x8[k8 ? TM : 1][k8 ? D : 1];
     Chunk<k8 ? kBf16 : XT> x16[k8 ? 1 : D];
-    constexpr int kDw = (D + 3) / 4;
-    uint32_t sw[TN][kDw], sx[kDw];
-    const int n = min(D, last - s0);
+    uint32_t sw[TN], sx[TM];
+    const int n = min(D, last - s0), base = min(s0, sw4 - 4);
 #pragma unroll
     for (int u = 0; u < D; ++u) {
       if (u < n) {
@@ -124,52 +130,55 @@ __global__ __launch_bounds__(64 * WAVES) void k_fp8_token(TokenArgs a) {
           w[t][u].v[1] = ld16_stream(wp[t] + 128 * (int64_t)(s0 + u) + 64);
         }
         if constexpr (k8) {
-          x8[u].v[0] = ld16(xp + 128 * (int64_t)(s0 + u));
-          x8[u].v[1] = ld16(xp + 128 * (int64_t)(s0 + u) + 64);
+#pragma unroll
+          for (int i = 0; i < TM; ++i) {
+            x8[i][u].v[0] = ld16(xp[i] + 128 * (int64_t)(s0 + u));
+            x8[i][u].v[1] = ld16(xp[i] + 128 * (int64_t)(s0 + u) + 64);
+          }
         } else {
           const int k = 128 * (s0 + u) + 8 * j;
           x16[u] = ld_chunk<XT>(a.x + min(g, a.rows - 1) * a.ldx + 2 * (int64_t)k, k < a.w.cols ? 8 : 0);
         }
       }
     }
-    // scales of steps s0 + 4 d .. + 3, as far as the row goes
-    int base[kDw];
 #pragma unroll
-    for (int d = 0; d < kDw; ++d) {
-      base[d] = min(s0 + 4 * d, sw4 - 4);
+    for (int t = 0; t < TN; ++t) sw[t] = *reinterpret_cast<const u32_byte*>(wsc[t] + base);
+    if constexpr (k8) {
 #pragma unroll
-      for (int t = 0; t < TN; ++t) sw[t][d] = *reinterpret_cast<const u32_byte*>(wsc[t] + base[d]);
-      if constexpr (k8) sx[d] = *reinterpret_cast<const u32_byte*>(xsc + base[d]);
+      for (int i = 0; i < TM; ++i) sx[i] = *reinterpret_cast<const u32_byte*>(xsc[i] + base);
     }
 #pragma unroll
     for (int u = 0; u < D; ++u) {
       if (u >= n) break;
-      const int sh = 8 * (s0 + u - base[u / 4]);
-      Frag x;
-      uint32_t s;
+      const int sh = 8 * (s0 + u - base);
       if constexpr (k8) {
-        x = x8[u];
-        s = sx[u / 4] >> sh;
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+          for (int t = 0; t < TN; ++t) acc[i][t] = mfma8_16(w[t][u], x8[i][u], acc[i][t], sw[t] >> sh, sx[i] >> sh);
       } else {
         float v[8];
         widen<XT>(x16[u], v);
         const uint32_t mine = fp8_scale(lanes16_max(top8(v)));
         st8(&xq[wave][g][16 * (j / 2 ^ g) + 8 * (j & 1)], fp8_codes8(v, mine));
         const int r = j & 3;  // (rows past four: their products are not stored)
-        s = (uint32_t)__shfl((int)mine, 16 * r);
+        const uint32_t s = (uint32_t)__shfl((int)mine, 16 * r);
+        Frag x;
         asm volatile("" ::: "memory");
         x.v[0] = ld16(&xq[wave][r][16 * (g ^ r)]);
         x.v[1] = ld16(&xq[wave][r][16 * ((g + 4) ^ r)]);
         asm volatile("" ::: "memory");
-      }
 #pragma unroll
-      for (int t = 0; t < TN; ++t) acc[t] = mfma8_16(w[t][u], x, acc[t], sw[t][u / 4] >> sh, s);
+        for (int t = 0; t < TN; ++t) acc[0][t] = mfma8_16(w[t][u], x, acc[0][t], sw[t] >> sh, s);
+      }
     }
   }
 #pragma unroll
-  for (int t = 0; t < TN; ++t) red[wave][t][lane] = acc[t];
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int t = 0; t < TN; ++t) red[wave][i * TN + t][lane] = acc[i][t];
   __syncthreads();
-  for (int p = wave; p < TN; p += WAVES) {
+  for (int p = wave; p < TM * TN; p += WAVES) {
     f32x4 s = red[0][p][lane];
 #pragma unroll
     for (int k = 1; k < WAVES; ++k) {
@@ -177,13 +186,13 @@ __global__ __launch_bounds__(64 * WAVES) void k_fp8_token(TokenArgs a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[e] += v[e];
     }
-    const int64_t n = n0 + 16 * p + 4 * g;
-    if (j >= a.rows) continue;
+    const int64_t n = n0 + 16 * (p % TN) + 4 * g, m = 16 * (p / TN) + j;
+    if (m >= a.rows) continue;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       if (n + e >= n1) break;
-      if (a.odt == kF32) reinterpret_cast<float*>(a.out)[j * a.ldo + n + e] = s[e];
-      else reinterpret_cast<uint16_t*>(a.out)[j * a.ldo + n + e] = bits16(s[e], a.odt);
+      if (a.odt == kF32) reinterpret_cast<float*>(a.out)[m * a.ldo + n + e] = s[e];
+      else reinterpret_cast<uint16_t*>(a.out)[m * a.ldo + n + e] = bits16(s[e], a.odt);
     }
   }
 }
@@ -432,7 +441,7 @@ __global__ __launch_bounds__(256, 1) void k_fp8_tile(Tile8Args a) {
       }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
-#pragma unroll 1
+#pragma unroll 4
     for (int r = 0; r < 32; r += 64 / kPer) {
       Out16<OT> o{ld16(mine + (r + lane / kPer) * kPitch + 16 * (lane % kPer))};
       if (m + r < a.x.rows) o.store(out + ((m + r) * a.ldo + n) * ES, valid);
@@ -469,26 +478,30 @@ struct Plan8 {
   int splits, steps;
 };
 
-static constexpr int kTokenRows = 16;
+// Rows that the few-row kernel takes: 16, and up to 32 except by few long rows of W (32 rows by [4096, 4096] 9.7 us and by
+// [14336, 4096] 19.3 against 13.9 and 20.0 in tiles, but by [4096, 14336] 26.7 against 20.5).
+static bool few_rows(int64_t rows, int64_t cols, int steps) { return rows <= 16 || (rows <= 32 && (steps <= 64 || cols > 8192)); }
 
 // The tile's height and how often the contraction is split over workgroups: one workgroup runs on a CU at a time, so a
 // grid takes rounds of its steps; every split writes and re-reads fp32 parts.  Times in us, as measured (a step of
-// each height; a workgroup's start and end; the join's launch; its bytes at 4 TB/s).  A last round that does not
-// fill the card runs at higher clocks: half full it takes 0.8 of a full one.
+// each height; a workgroup's start and end; the join's launch; its bytes at 4 TB/s).  A round that does not fill
+// the card runs at higher clocks: half full, one of high tiles takes 0.8 of a full one; low ones wait for memory.
 static Plan8 plan8(const lrq_fp8* a, const lrq_fp8* b, bool nn) {
-  constexpr double kStep[4] = {0.62, 0.86, 1.19, 1.44}, kFixed[4] = {1.5, 5.5, 5.0, 6.0}, kJoin = 4.0, kPerByte = 2.0 / 4.0e6;
+  constexpr double kStep[4] = {0.72, 0.86, 1.19, 1.44}, kEmpty[4] = {1., 0.9, 0.6, 0.6}, kFixed[4] = {1.5, 5.5, 5.0, 6.0}, kJoin = 4.0, kPerByte = 2.0 / 4.0e6;
+  constexpr double kOnce = 0.86;  // of the lowest, where one row of tiles reads all of W from memory
   constexpr int kCus = 256;  // a fixed count, so that the workspace and the order of the sums depend on the shape alone
   const int64_t rows = a->rows, cols = nn ? b->cols : b->rows, tiles_n = (cols + 255) / 256;
   const int steps = (int)((a->cols + 127) / 128);
-  if (!nn && rows <= kTokenRows) return Plan8{0, 0, 0, 1, steps};
+  if (!nn && few_rows(rows, cols, steps)) return Plan8{0, 0, 0, 1, steps};
   Plan8 best{};
   double least = 0.;
   for (int mt = 1; mt <= 4; ++mt) {
     Plan8 p{mt, (rows + 64 * mt - 1) / (64 * mt), tiles_n, 1, steps};
     for (; p.splits <= 16 && p.splits <= std::max(1, steps / 4); ++p.splits) {
       const int64_t wgs = p.tiles_m * tiles_n * p.splits, over = wgs % kCus;
-      const double rounds = (double)(wgs / kCus) + (over ? 0.6 + 0.4 * (double)over / kCus : 0.);
-      const double cost = rounds * ((steps + p.splits - 1) / p.splits * kStep[mt - 1] + kFixed[mt - 1]) +
+      const double rounds = (double)(wgs / kCus) + (over == 0 ? 0. : kEmpty[mt - 1] + (1. - kEmpty[mt - 1]) * (double)over / kCus);
+      const double step = p.tiles_m == 1 && mt == 1 ? kOnce : kStep[mt - 1];
+      const double cost = rounds * ((steps + p.splits - 1) / p.splits * step + kFixed[mt - 1]) +
                           (p.splits > 1 ? kJoin + kPerByte * 4. * p.splits * rows * cols : 0.);
       if (best.mt == 0 || cost < least) best = p, least = cost;
     }
@@ -518,21 +531,27 @@ static int validate_pair(const lrq_fp8* a, const lrq_fp8* b, bool nn) {
   return nn && b->block != 128 ? LRQ_ERR_UNSUPPORTED : LRQ_OK;
 }
 
-template <int XT>
+template <int XT, int TM>
 static int token(TokenArgs a, hipStream_t s) {
   using std::integral_constant;
   const int64_t n = a.w.rows;
   const auto go = [&](auto tn, auto waves, auto d, int64_t wgs) {
     a.own = (int)std::min<int64_t>(16 * tn(), ((n + wgs - 1) / wgs + 3) / 4 * 4);
-    return launch((k_fp8_token<XT, tn(), waves(), d()>), dim3((unsigned)((n + a.own - 1) / a.own)), dim3(64 * waves()), 0, s, a);
+    return launch((k_fp8_token<XT, TM, tn(), waves(), d()>), dim3((unsigned)((n + a.own - 1) / a.own)), dim3(64 * waves()), 0, s, a);
   };
-#define LRQ_GO(TN, WAVES, WGS) return go(integral_constant<int, TN>{}, integral_constant<int, WAVES>{}, integral_constant<int, 4>{}, WGS)
+#define LRQ_GO(TN, WAVES, D, WGS) return go(integral_constant<int, TN>{}, integral_constant<int, WAVES>{}, integral_constant<int, D>{}, WGS)
   // Every CU the same bytes of W, which come to it at about 18 GB/s whatever the others do: a workgroup a CU, of
   // as many rows as that makes ([5120, 5120] by one row 8.9 us; whole tiles of 16 rows, 320 of them: 11.5).  More than 32
   // rows a CU: two workgroups, whose starts and ends overlap ([14336, 4096] 13.7 us against 15.5 with one of 56 rows).
-  if (n <= 4096) LRQ_GO(1, 16, 256);
-  if (n <= 8192) LRQ_GO(2, 16, 256);
-  LRQ_GO(2, 8, 512 * ((n + 16383) / 16384));
+  if constexpr (TM == 1) {
+    if (n <= 4096) LRQ_GO(1, 16, 4, 256);
+    if (n <= 8192) LRQ_GO(2, 16, 4, 256);
+    LRQ_GO(2, 8, 4, 512 * ((n + 16383) / 16384));
+  } else {  // X is read again by every workgroup, at twice the bytes: more rows of W to each
+    if (n <= 4096) LRQ_GO(1, 16, 2, 256);
+    if (n <= 8192) LRQ_GO(2, 16, 2, 256);
+    LRQ_GO(4, 8, 1, 256 * ((n + 16383) / 16384));
+  }
 #undef LRQ_GO
 }
 
@@ -546,7 +565,7 @@ static int fp8_product(const lrq_fp8* ta, const lrq_fp8* tb, bool nn, void* out,
   const Fp8 x = make_fp8(ta), w = make_fp8(tb);
   if (p.mt == 0) {
     const TokenArgs a{(const char*)x.codes, x.ldc, x.scales, x.lds, x.shift, (int)rows, 0, w, out, ldo, odt};
-    return token<kX8>(a, s);
+    return rows <= 16 ? token<kX8, 1>(a, s) : token<kX8, 2>(a, s);
   }
   const int64_t need = parts_bytes(p.splits, rows, cols), ldp = (cols + 3) / 4 * 4;
   if (need > 0) {
@@ -613,5 +632,5 @@ extern "C" int lrq_fp8_linear(const void* x, int64_t ldx, int32_t dtype, int64_t
   LRQ_TRY(validate_out8(out, ldo, t->rows, out_dtype));
   const TokenArgs a{(const char*)x, 2 * ldx, nullptr, 0, 0, (int)rows, 0, make_fp8(t), out, ldo, out_dtype};
   hipStream_t s = (hipStream_t)stream;
-  return dtype == LRQ_BF16 ? token<kBf16>(a, s) : token<kF16>(a, s);
+  return dtype == LRQ_BF16 ? token<kBf16, 1>(a, s) : token<kF16, 1>(a, s);
 }
