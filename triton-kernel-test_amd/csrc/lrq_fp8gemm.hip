@@ -457,7 +457,7 @@ __global__ __launch_bounds__(256) void k_fp8_join(const float* part, int splits,
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
     const int64_t m = i / quads, n = 4 * (i - m * quads);
     f32x4 s = *(const f32x4*)(part + m * ldp + n);
-#pragma unroll 4
+#pragma unroll 8
     for (int z = 1; z < splits; ++z) {
       const f32x4 v = *(const f32x4*)(part + ((int64_t)z * rows + m) * ldp + n);
 #pragma unroll
