@@ -218,8 +218,13 @@ struct Out16 {
   }
 };
 
+struct Operand8 {
+  const uint8_t *codes, *scales;
+  uint32_t ldc, lds, rows;
+  int steps, shift;
+};
 struct Tile8Args {
-  Fp8 x, w;
+  Operand8 x, w;
   void* out;      // [splits][x.rows][ldo] fp32 parts where splits > 1
   int64_t ldo;
   int64_t cols;   // of the output
@@ -236,16 +241,17 @@ struct Tile8Args {
 // LDS: X and (NN false) W have rows of 128 bytes, row r's 16-byte piece p in slot p ^ (r / 2 % 8): 16 lanes of a read cover
 // all banks.  NN: 128 rows of W of 256 bytes, piece p of row r in slot p ^ (r % 8); the transposing read gives a lane its
 // column of 8 rows.
-template <bool NN, int MT>
+template <int MT>
 struct Tile8Lds {
   static constexpr int kX = 64 * MT * 128, kW = 32768, kStage = kX + kW, kDeep = MT >= 3 ? 2 : 3, kRing = kDeep * kStage;
   static constexpr int kScales = 2048, kLoop = kRing + 2 * kScales;
-  static constexpr int kOut = 4 * 32 * (128 * 4 + 16), kBytes = kLoop > kOut ? kLoop : kOut;
-  static_assert(kBytes <= 160 * 1024);
+  static constexpr int kOut = 4 * 32 * (128 + 16);  // of the output, in the ring's place
+  static_assert(kLoop <= 160 * 1024 && kOut <= kLoop);
 };
+
 template <bool NN, int MT, int OT>
 __global__ __launch_bounds__(256, 1) void k_fp8_tile(Tile8Args a) {
-  using T = Tile8Lds<NN, MT>;
+  using T = Tile8Lds<MT>;
   constexpr int kX = T::kX, kStage = T::kStage, kDeep = T::kDeep, kLx = 2 * MT, kLoads = kLx + 8;
   extern __shared__ __attribute__((aligned(16))) char sm[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -257,63 +263,72 @@ __global__ __launch_bounds__(256, 1) void k_fp8_tile(Tile8Args a) {
   const uint32_t band = __builtin_amdgcn_readfirstlane(tile / (kBand * a.tiles_n)), in = tile - band * kBand * a.tiles_n;
   const uint32_t tall = min(kBand, a.tiles_m - band * kBand);
   const uint32_t tn = __builtin_amdgcn_readfirstlane(in / tall), tm = band * kBand + in - tn * tall;
-  const int64_t m0 = (int64_t)tm * 64 * MT, n0 = (int64_t)tn * 256;
-  const int first = __builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)a.steps * z / (uint32_t)a.splits));
-  const int last = __builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)a.steps * (z + 1) / (uint32_t)a.splits));
+  const uint32_t m0 = tm * 64 * MT, n0 = tn * 256;
+  // a split's steps: whole groups of four, whose scales come together
+  const uint32_t groups = (uint32_t)(a.steps + 3) >> 2;
+  const int first = 4 * __builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)groups * z / (uint32_t)a.splits));
+  const int last = min(4 * (int)__builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)groups * (z + 1) / (uint32_t)a.splits)), a.steps);
 
-  // loads of 1 KB: 8 rows of 128 bytes (NN W: 4 rows of 256), at 32-bit offsets from the tile's first row
+  // ---- loads of 1 KB: 8 rows of 128 bytes (NN W: 4 rows of 256), at 32-bit offsets from a tile's first row
   const uint32_t sm0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)sm;
-  const uint8_t* bx = a.x.codes + m0 * a.x.ldc;
-  const uint8_t* bw = NN ? a.w.codes + n0 : a.w.codes + n0 * a.w.ldc;
-  uint32_t ox[kLx], ow[8];
+  const int rw = 32 * wave + (lane >> 4);  // NN: row rw + 4 i of a step, whose piece does not depend on i / 2
+  struct {
+    const uint8_t *x, *w;
+    uint32_t row;
+  } to;  // the step that is loaded next (row: NN, of W)
+  const auto point = [&](int step) {
+    to.row = 128u * (uint32_t)step;
+    to.x = a.x.codes + (uint64_t)m0 * a.x.ldc + to.row;
+    to.w = NN ? a.w.codes + n0 + (uint64_t)to.row * a.w.ldc : a.w.codes + (uint64_t)n0 * a.w.ldc + to.row;
+  };
+  uint32_t ox[kLx], ow[NN ? 2 : 8];
+  const uint32_t mx = min(64u * MT, a.x.rows - m0) - 1;
 #pragma unroll
   for (int i = 0; i < kLx; ++i) {
     const int r = 8 * (kLx * wave + i) + (lane >> 3);
-    ox[i] = (uint32_t)min((int64_t)r, a.x.rows - 1 - m0) * (uint32_t)a.x.ldc + 16 * ((lane & 7) ^ (r >> 1 & 7));
+    ox[i] = min((uint32_t)r, mx) * a.x.ldc + 16 * ((lane & 7) ^ (r >> 1 & 7));
   }
-  // NN: row 32 wave + 4 i + lane / 16 of a step, whose piece does not depend on i / 2
-  const int rw = 32 * wave + (lane >> 4);
+  if constexpr (!NN) {
+    const uint32_t mw = min(256u, a.w.rows - n0) - 1;
 #pragma unroll
-  for (int i = 0; i < (NN ? 2 : 8); ++i) {
-    if constexpr (!NN) {
+    for (int i = 0; i < 8; ++i) {
       const int r = 8 * (8 * wave + i) + (lane >> 3);
-      ow[i] = (uint32_t)min((int64_t)r, a.w.rows - 1 - n0) * (uint32_t)a.w.ldc + 16 * ((lane & 7) ^ (r >> 1 & 7));
-    } else {
-      ow[i] = (uint32_t)min((int64_t)16 * ((lane & 15) ^ ((rw + 4 * i) & 7)), 128 * (int64_t)a.w.steps - 16 - n0);
+      ow[i] = min((uint32_t)r, mw) * a.w.ldc + 16 * ((lane & 7) ^ (r >> 1 & 7));
     }
+  } else {
+    const uint32_t mw = min(256u, 128u * (uint32_t)a.w.steps - n0) - 16;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) ow[i] = min((uint32_t)(16 * ((lane & 15) ^ ((rw + 4 * i) & 7))), mw);
   }
-  // four steps' scales of 64 rows a load; NN: of this wave's 128 columns, four steps are four rows of scales
-  const int is = min(wave, MT - 1);
-  const uint32_t osx = (uint32_t)(min(m0 + 64 * is + lane, a.x.rows - 1) >> a.x.shift) * (uint32_t)a.x.lds;
-  const int kb = (int)min((n0 + 128 * wn) >> 7, (int64_t)a.w.steps - 1);
-  const uint32_t osw = NN ? (uint32_t)(kb & ~3) : (uint32_t)(min(n0 + 64 * wave + lane, a.w.rows - 1) >> a.w.shift) * (uint32_t)a.w.lds;
-  const int blocks = (int)((a.w.rows + 127) >> 7);
-
-  // load i of a step
-  const auto issue = [&](int step, int buf, int i) {
+  // load i of the step
+  const auto issue = [&](int buf, int i) {
     const uint32_t st = sm0 + buf * kStage;
     if (i < kLx) {
-      ld_to_lds8<16, NN>(bx + 128 * (int64_t)step, ox[i < kLx ? i : 0], st + 1024 * (kLx * wave + i));
+      ld_to_lds8<16, NN>(to.x, ox[i < kLx ? i : 0], st + 1024 * (kLx * wave + i));
     } else {
       const int k = (i - kLx) & 7;
-      const uint32_t to = st + kX + 1024 * (8 * wave + k);
+      const uint32_t lds = st + kX + 1024 * (8 * wave + k);
       if constexpr (!NN) {
-        ld_to_lds8<16, NN>(bw + 128 * (int64_t)step, ow[k], to);
+        ld_to_lds8<16, NN>(to.w, ow[k], lds);
       } else {  // rows past W's last: that one (their x is zero)
-        const uint32_t end = (uint32_t)a.w.rows - 1 - 128u * (uint32_t)step;
-        ld_to_lds8<16, NN>(bw + 128 * (int64_t)step * a.w.ldc, min((uint32_t)(rw + 4 * k), end) * (uint32_t)a.w.ldc + ow[k & 1], to);
+        const uint32_t end = a.w.rows - 1 - to.row;
+        ld_to_lds8<16, NN>(to.w, min((uint32_t)(rw + 4 * k), end) * a.w.ldc + ow[k & 1], lds);
       }
     }
   };
-  const auto issue_scales = [&](int group) {
-    const uint32_t sc = sm0 + T::kRing + (group & 1) * T::kScales;
-    const int gr = min(group, (a.steps - 1) >> 2);
-    ld_to_lds8<4, NN>(a.x.scales + 4 * gr, osx, sc + 256 * is);
-    if constexpr (!NN) ld_to_lds8<4, NN>(a.w.scales + 4 * gr, osw, sc + 1024 + 256 * wave);
-    else ld_to_lds8<4, NN>(a.w.scales, (uint32_t)min(4 * gr + (lane & 3), blocks - 1) * (uint32_t)a.w.lds + osw, sc + 1024 + 256 * wave);
+  // four steps' scales of 64 rows a load; NN: of this wave's 128 columns, four steps are four rows of scales
+  const int is = min(wave, MT - 1);
+  const int block = min((int)(n0 >> 7) + wn, a.w.steps - 1);  // NN
+  const uint32_t osx = (min(m0 + 64 * is + lane, a.x.rows - 1) >> a.x.shift) * a.x.lds;
+  const uint32_t osw = NN ? (uint32_t)(block & ~3) : (min(n0 + 64 * wave + lane, a.w.rows - 1) >> a.w.shift) * a.w.lds;
+  const auto issue_scales = [&](int group, int slot) {
+    const uint32_t sc = sm0 + T::kRing + slot * T::kScales;
+    ld_to_lds8<4, NN>(a.x.scales + 4 * group, osx, sc + 256 * is);
+    if constexpr (!NN) ld_to_lds8<4, NN>(a.w.scales + 4 * group, osw, sc + 1024 + 256 * wave);
+    else ld_to_lds8<4, NN>(a.w.scales, (uint32_t)min(4 * group + (lane & 3), a.steps - 1) * a.w.lds + osw, sc + 1024 + 256 * wave);
   };
 
-  // operands of half Q of a step (64 of K): piece 4 Q + 2 h + q of a row
+  // ---- operands of half Q of a step (64 of K): piece 4 Q + 2 h + q of a row
   Frag fx[2][MT], fw[2][4];
   uint32_t sx[MT], sw[4];
   const auto read_x = [&](int half, int buf, int i, int q) {
@@ -337,8 +352,8 @@ __global__ __launch_bounds__(256, 1) void k_fp8_tile(Tile8Args a) {
     if (p < 8) read_w(half, buf, p >> 1, p & 1);
     else read_x(half, buf, (p - 8) >> 1, p & 1);
   };
-  const auto read_scales = [&](int step) {
-    const char* sc = sm + T::kRing + (step >> 2 & 1) * T::kScales;
+  const auto read_scales = [&](int step, int slot) {
+    const char* sc = sm + T::kRing + slot * T::kScales;
     const int sh = 8 * (step & 3);
 #pragma unroll
     for (int i = 0; i < MT; ++i) sx[i] = ld4(sc + 4 * (32 * MT * wm + 32 * i + c)) >> sh;
@@ -346,17 +361,9 @@ __global__ __launch_bounds__(256, 1) void k_fp8_tile(Tile8Args a) {
 #pragma unroll
       for (int t = 0; t < 4; ++t) sw[t] = ld4(sc + 1024 + 4 * (128 * wn + 32 * t + c)) >> sh;
     } else {
-      sw[0] = ld4(sc + 1024 + 256 * wave + 4 * (step & 3)) >> (8 * (kb & 3));
+      sw[0] = ld4(sc + 1024 + 256 * wave + 4 * (step & 3)) >> (8 * (block & 3));
     }
   };
-
-  f32x16 acc[MT][4];
-#pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-      for (int v = 0; v < 16; ++v) acc[i][t][v] = 0.f;
 
   // Half 1 of a step is read from LDS behind the first instructions of half 0, half 0 of the next step behind those of half 1.
   // The workgroup meets twice in a step: once all of it has been read, whose place the loads of kDeep steps on then take,
@@ -365,88 +372,107 @@ __global__ __launch_bounds__(256, 1) void k_fp8_tile(Tile8Args a) {
   // so 395.  The order is held: the compiler would issue all loads first.
   constexpr int kMfma = 4 * MT, kPieces = 2 * (MT + 4), kReads = (kPieces + kMfma / 2 - 1) / (kMfma / 2);
   constexpr int kFirst = 3 * kLoads / 8;  // of a step's loads: behind the second half of half 0's instructions
-  issue_scales(first >> 2);
-  issue_scales((first >> 2) + 1);
+  f32x16 acc[MT][4];
 #pragma unroll
-  for (int d = 0; d < kDeep; ++d)
+  for (int i = 0; i < MT; ++i)
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) issue(min(first + d, last - 1), d, i);
+    for (int t = 0; t < 4; ++t) acc[i][t] = f32x16{};
+  issue_scales(first >> 2, 0);
+#pragma unroll
+  for (int d = 0; d < kDeep; ++d) {
+    point(min(first + d, last - 1));
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) issue(d, i);
+  }
+  point(first + kDeep);
   __builtin_amdgcn_s_waitcnt(vmcnt_imm((kDeep - 1) * kLoads));
   lds_meet();
 #pragma unroll
   for (int p = 0; p < kPieces; ++p) read_piece(0, 0, p);
-  read_scales(first);
-  int buf = 0;
-  for (int step = first; step < last; ++step) {
-    const int next = buf + 1 == kDeep ? 0 : buf + 1;
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int m = 0; m < kMfma; ++m) {
-      const int i = m >> 2, t = m & 3, late = m - kMfma / 2;
-      acc[i][t] = mfma8_32(fw[0][t], fx[0][i], acc[i][t], sw[NN ? 0 : t], sx[i]);
+  read_scales(first, 0);
+  // The loads are kDeep steps ahead; the last steps repeat the last's.  A loop for each, so that a step has no branch but
+  // that of the scales: the compiler would move the instructions behind it.
+  int buf = 0, slot = 0;  // of the step, of its scales
+  for (int part = 0, step = first; part < 2; ++part) {
+    const int end = part ? last : max(first, last - kDeep);
+    const uint64_t ix = part ? 0 : 128, iw = part ? 0 : NN ? 128 * (uint64_t)a.w.ldc : 128;
+    if (part) point(last - 1);
+    for (; step < end; ++step) {
+      const int next = buf + 1 == kDeep ? 0 : buf + 1;
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int p = kReads * m; p < kReads * (m + 1); ++p)
-        if (p < kPieces) read_piece(1, buf, p);
-      if (late == 0) lds_meet();
+      for (int m = 0; m < kMfma; ++m) {
+        const int i = m >> 2, t = m & 3, late = m - kMfma / 2;
+        acc[i][t] = mfma8_32(fw[0][t], fx[0][i], acc[i][t], sw[NN ? 0 : t], sx[i]);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int l = 0; l < kFirst; ++l)
-        if (l * (kMfma / 2) / kFirst == late) issue(min(step + kDeep, last - 1), buf, l);
+        for (int p = kReads * m; p < kReads * (m + 1); ++p)
+          if (p < kPieces) read_piece(1, buf, p);
+        if (late == 0) lds_meet();
+#pragma unroll
+        for (int l = 0; l < kFirst; ++l)
+          if (l * (kMfma / 2) / kFirst == late) issue(buf, l);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      __builtin_amdgcn_s_waitcnt(vmcnt_imm((kDeep - 2) * kLoads + kFirst));
+      lds_meet();
+      if ((step & 3) == 0 && step + 4 < last) issue_scales((step >> 2) + 1, slot ^ 1);
       __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int m = 0; m < kMfma; ++m) {
+        const int i = m >> 2, t = m & 3;
+        acc[i][t] = mfma8_32(fw[1][t], fx[1][i], acc[i][t], sw[NN ? 0 : t], sx[i]);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int l = 0; l < kLoads - kFirst; ++l)
+          if (l * kMfma / (kLoads - kFirst) == m) issue(buf, kFirst + l);
+#pragma unroll
+        for (int p = kReads * m; p < kReads * (m + 1); ++p)
+          if (p < kPieces) read_piece(0, next, p);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      to.x += ix, to.w += iw, to.row += (uint32_t)ix;
+      slot ^= (step & 3) == 3 ? 1 : 0;
+      read_scales(step + 1, slot);  // (of no use behind the last step)
+      buf = next;
     }
-    __builtin_amdgcn_s_waitcnt(vmcnt_imm((kDeep - 2) * kLoads + kFirst));
-    lds_meet();
-    if ((step & 3) == 0 && step > first) issue_scales((step >> 2) + 1);
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int m = 0; m < kMfma; ++m) {
-      const int i = m >> 2, t = m & 3;
-      acc[i][t] = mfma8_32(fw[1][t], fx[1][i], acc[i][t], sw[NN ? 0 : t], sx[i]);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int l = 0; l < kLoads - kFirst; ++l)
-        if (l * kMfma / (kLoads - kFirst) == m) issue(min(step + kDeep, last - 1), buf, kFirst + l);
-#pragma unroll
-      for (int p = kReads * m; p < kReads * (m + 1); ++p)
-        if (p < kPieces) read_piece(0, next, p);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    read_scales(min(step + 1, last - 1));
-    buf = next;
   }
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // the last loads write LDS
   lds_meet();
 
-  // Out through LDS, 32 rows of the wave's 128 columns at a time: a lane has four neighbouring columns of one row, and leaves
-  // with 16 bytes beside its neighbours'.
-  constexpr int ES = Elem<OT>::kBytes, kPitch = 128 * ES + 16, kWide = 16 / ES, kPer = 128 / kWide;
+  // Out through LDS, 32 rows by 128 bytes of the wave's columns at a time: a lane has four neighbouring columns of one row,
+  // and leaves with 16 bytes beside its neighbours'.
+  constexpr int ES = Elem<OT>::kBytes, kPitch = 128 + 16, kWide = 16 / ES, kCols = 128 / ES, kTs = kCols / 32;
   char* mine = sm + wave * 32 * kPitch;
   char* out = (char*)a.out + (a.splits > 1 ? (int64_t)z * a.x.rows * a.ldo * 4 : 0);
-  const int64_t n = n0 + 128 * wn + kWide * (lane % kPer);
-  const int valid = (int)min((int64_t)kWide, a.cols - n);
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
-    const int64_t m = m0 + 32 * MT * wm + 32 * i + lane / kPer;
-    __builtin_amdgcn_sched_barrier(0);
+    const int64_t m = (int64_t)m0 + 32 * MT * wm + 32 * i + lane / 8;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) asm volatile("" : "+a"(acc[i][t]));  // not read before: no registers for all of them
+    for (int t0 = 0; t0 < 4; t0 += kTs) {
+      const int64_t n = (int64_t)n0 + 128 * wn + 32 * t0 + kWide * (lane % 8);
+      const int valid = (int)min((int64_t)kWide, a.cols - n);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+      for (int t = t0; t < t0 + kTs; ++t) {
+        asm volatile("" : "+a"(acc[i][t]));  // not read before: no registers for all of them
 #pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        const f32x4 s = {acc[i][t][4 * v], acc[i][t][4 * v + 1], acc[i][t][4 * v + 2], acc[i][t][4 * v + 3]};
-        char* to = mine + c * kPitch + ES * (32 * t + 8 * v + 4 * h);
-        if constexpr (OT == kF32) st16(to, __builtin_bit_cast(u32x4, s));
-        else st8(to, u32x2{pack16(s[0], s[1], OT), pack16(s[2], s[3], OT)});
+        for (int v = 0; v < 4; ++v) {
+          const f32x4 s = {acc[i][t][4 * v], acc[i][t][4 * v + 1], acc[i][t][4 * v + 2], acc[i][t][4 * v + 3]};
+          char* st = mine + c * kPitch + ES * (32 * (t - t0) + 8 * v + 4 * h);
+          if constexpr (OT == kF32) st16(st, __builtin_bit_cast(u32x4, s));
+          else st8(st, u32x2{pack16(s[0], s[1], OT), pack16(s[2], s[3], OT)});
+        }
       }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll 4
-    for (int r = 0; r < 32; r += 64 / kPer) {
-      Out16<OT> o{ld16(mine + (r + lane / kPer) * kPitch + 16 * (lane % kPer))};
-      if (m + r < a.x.rows) o.store(out + ((m + r) * a.ldo + n) * ES, valid);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      Out16<OT> o[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o[r].v = ld16(mine + (8 * r + lane / 8) * kPitch + 16 * (lane % 8));
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (m + 8 * r < a.x.rows) o[r].store(out + ((m + 8 * r) * a.ldo + n) * ES, valid);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }
 }
 
@@ -526,7 +552,7 @@ static int validate_pair(const lrq_fp8* a, const lrq_fp8* b, bool nn) {
   if (a->cols != (nn ? b->rows : b->cols)) return LRQ_ERR_SHAPE;
   for (const lrq_fp8* t : {a, b}) {  // 32-bit offsets within a tile's codes and from the first scale
     const int64_t tall = (t->rows + t->block - 1) / t->block;
-    if (t->ld_codes >= 1 << 24 || (tall > 0 && t->ld_scales > UINT32_MAX / tall)) return LRQ_ERR_SHAPE;
+    if (t->ld_codes >= 1 << 24 || t->ld_scales > INT32_MAX || (tall > 0 && t->ld_scales > UINT32_MAX / tall)) return LRQ_ERR_SHAPE;
   }
   return nn && b->block != 128 ? LRQ_ERR_UNSUPPORTED : LRQ_OK;
 }
@@ -575,19 +601,20 @@ static int fp8_product(const lrq_fp8* ta, const lrq_fp8* tb, bool nn, void* out,
   }
   const int64_t wgs = p.tiles_m * p.tiles_n * p.splits;
   if (wgs > INT32_MAX) return LRQ_ERR_SHAPE;
-  const Tile8Args a{x, w, need ? workspace : out, need ? ldp : ldo, cols, need ? (int)kF32 : odt, (int)p.tiles_m,
-                    (int)p.tiles_n, p.splits, p.steps};
-  const auto go = [&](auto kern, int lds) {
-    const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    if (e != hipSuccess) return (int)e;
-    return launch(kern, dim3((unsigned)wgs), dim3(256), (size_t)lds, s, a);
+  const auto operand = [](const Fp8& t) {
+    return Operand8{t.codes, t.scales, (uint32_t)t.ldc, (uint32_t)t.lds, (uint32_t)t.rows, t.steps, t.shift};
   };
+  const Tile8Args a{operand(x), operand(w), need ? workspace : out, need ? ldp : ldo, cols, need ? (int)kF32 : odt, (int)p.tiles_m,
+                    (int)p.tiles_n, p.splits, p.steps};
   using std::integral_constant;
   const auto with = [&](auto mt) {
-    const auto typed = [&](auto ot) {
-      return nn ? go(k_fp8_tile<true, mt(), ot()>, Tile8Lds<true, mt()>::kBytes)
-                : go(k_fp8_tile<false, mt(), ot()>, Tile8Lds<false, mt()>::kBytes);
+    const auto go = [&](auto kern) {
+      constexpr int kLds = Tile8Lds<mt()>::kLoop;
+      const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+      if (e != hipSuccess) return (int)e;
+      return launch(kern, dim3((unsigned)wgs), dim3(256), (size_t)kLds, s, a);
     };
+    const auto typed = [&](auto ot) { return nn ? go(k_fp8_tile<true, mt(), ot()>) : go(k_fp8_tile<false, mt(), ot()>); };
     if (a.odt == kBf16) return typed(integral_constant<int, kBf16>{});
     return a.odt == kF16 ? typed(integral_constant<int, kF16>{}) : typed(integral_constant<int, kF32>{});
   };
