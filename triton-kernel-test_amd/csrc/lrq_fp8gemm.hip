@@ -37,21 +37,17 @@ __device__ __forceinline__ uint32_t pack16(float a, float b, int dt) {
   return dt == kBf16 ? pack_bf16x2(a, b) : (uint32_t)f16_bits(a) | (uint32_t)f16_bits(b) << 16;
 }
 
-// 64 lanes' 16 (4) bytes at base + off to LDS, lane l's at lds + 16 l (4 l); base and lds are the wave's.  ASM: the compiler
-// does not see the load.  It has no output register; its end is counted by vmcnt as that of any other, and all waits for
-// it are written out.  (The transposing LDS reads have no other use: behind a load to LDS that the compiler knows of, it lets
-// each of them wait until every load is in.)
-template <int BYTES, bool ASM>
+// 64 lanes' 16 (4) bytes at base + off to LDS, lane l's at lds + 16 l (4 l); base and lds are the wave's.  In assembly: the
+// compiler does not see the load, which has no output register and whose end is counted by vmcnt as that of any other;
+// all waits for it are written out.  (Behind a load to LDS that the compiler knows of, it lets each transposing LDS read wait
+// until every load is in; and it takes a 64-bit addition for each address, 2 % of a product.)  m0 has no other use in the
+// kernels that call it.
+template <int BYTES>
 __device__ __forceinline__ void ld_to_lds8(const uint8_t* base, uint32_t off, uint32_t lds) {
-  if constexpr (!ASM) {
-    const auto l = (__attribute__((address_space(3))) void*)(uintptr_t)lds;
-    if constexpr (BYTES == 16) __builtin_amdgcn_global_load_lds(base + off, l, 16, 0, 0);
-    else __builtin_amdgcn_global_load_lds(base + off, l, 4, 0, 0);
-  } else if constexpr (BYTES == 16) {  // (m0 has no other use in these kernels)
+  if constexpr (BYTES == 16)
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory");
-  } else {
+  else
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory");
-  }
 }
 
 // The largest of v over the lanes j, j + 16, j + 32, j + 48, in all of them.
@@ -304,15 +300,15 @@ __global__ __launch_bounds__(256, 1) void k_fp8_tile(Tile8Args a) {
   const auto issue = [&](int buf, int i) {
     const uint32_t st = sm0 + buf * kStage;
     if (i < kLx) {
-      ld_to_lds8<16, NN>(to.x, ox[i < kLx ? i : 0], st + 1024 * (kLx * wave + i));
+      ld_to_lds8<16>(to.x, ox[i < kLx ? i : 0], st + 1024 * (kLx * wave + i));
     } else {
       const int k = (i - kLx) & 7;
       const uint32_t lds = st + kX + 1024 * (8 * wave + k);
       if constexpr (!NN) {
-        ld_to_lds8<16, NN>(to.w, ow[k], lds);
+        ld_to_lds8<16>(to.w, ow[k], lds);
       } else {  // rows past W's last: that one (their x is zero)
         const uint32_t end = a.w.rows - 1 - to.row;
-        ld_to_lds8<16, NN>(to.w, min((uint32_t)(rw + 4 * k), end) * a.w.ldc + ow[k & 1], lds);
+        ld_to_lds8<16>(to.w, min((uint32_t)(rw + 4 * k), end) * a.w.ldc + ow[k & 1], lds);
       }
     }
   };
@@ -323,9 +319,9 @@ __global__ __launch_bounds__(256, 1) void k_fp8_tile(Tile8Args a) {
   const uint32_t osw = NN ? (uint32_t)(block & ~3) : (min(n0 + 64 * wave + lane, a.w.rows - 1) >> a.w.shift) * a.w.lds;
   const auto issue_scales = [&](int group, int slot) {
     const uint32_t sc = sm0 + T::kRing + slot * T::kScales;
-    ld_to_lds8<4, NN>(a.x.scales + 4 * group, osx, sc + 256 * is);
-    if constexpr (!NN) ld_to_lds8<4, NN>(a.w.scales + 4 * group, osw, sc + 1024 + 256 * wave);
-    else ld_to_lds8<4, NN>(a.w.scales, (uint32_t)min(4 * group + (lane & 3), a.steps - 1) * a.w.lds + osw, sc + 1024 + 256 * wave);
+    ld_to_lds8<4>(a.x.scales + 4 * group, osx, sc + 256 * is);
+    if constexpr (!NN) ld_to_lds8<4>(a.w.scales + 4 * group, osw, sc + 1024 + 256 * wave);
+    else ld_to_lds8<4>(a.w.scales, (uint32_t)min(4 * group + (lane & 3), a.steps - 1) * a.w.lds + osw, sc + 1024 + 256 * wave);
   };
 
   // ---- operands of half Q of a step (64 of K): piece 4 Q + 2 h + q of a row
