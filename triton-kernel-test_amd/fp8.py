@@ -12,7 +12,6 @@ from __future__ import annotations
 
 import ctypes
 import math
-from dataclasses import dataclass
 from typing import Union
 
 import torch
@@ -28,7 +27,6 @@ __all__ = ["FP8Tensor", "fp8_from_parts", "fp8_quantize", "fp8_dequantize", "fp8
 _BYTES = (torch.uint8, torch.float8_e4m3fn, torch.float8_e8m0fnu)
 
 
-@dataclass(eq=False)
 class FP8Tensor:
     """A tensor [..., cols] in e4m3; rows are its leading dimensions flattened.
 
@@ -36,14 +34,46 @@ class FP8Tensor:
     one E8M0 exponent for 128 columns of ``block`` (1 or 128) rows, [ceil(rows / block), >= ceil(cols / 128) rounded up to
     4]."""
 
-    codes: torch.Tensor
-    scales: torch.Tensor
-    shape: tuple
-    block: int = 1
+    # What the library makes lies in one allocation, codes first, whose views are taken when they are asked for: a call on few
+    # rows is bound by the host, and an allocation and two views are 3 us of it.
+    __slots__ = ("_codes", "_scales", "shape", "block", "_buf")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape, block: int = 1):
+        self._codes, self._scales, self.shape, self.block, self._buf = codes, scales, tuple(shape), block, None
+
+    def _views(self):
+        c, steps, wide = self._buf, _steps(self.shape[-1]), _wide(self.shape[-1])
+        rows = math.prod(self.shape[:-1])
+        tall = (rows + self.block - 1) // self.block
+        self._codes = c.as_strided((rows, 128 * steps), (128 * steps, 1)).view(torch.float8_e4m3fn)
+        self._scales = c.as_strided((tall, wide), (wide, 1), c.storage_offset() + rows * 128 * steps)
+
+    @property
+    def codes(self) -> torch.Tensor:
+        if self._codes is None:
+            self._views()
+        return self._codes
+
+    @codes.setter
+    def codes(self, t: torch.Tensor):
+        self._scales, self._codes, self._buf = self.scales, t, None
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            self._views()
+        return self._scales
+
+    @scales.setter
+    def scales(self, t: torch.Tensor):
+        self._codes, self._scales, self._buf = self.codes, t, None
+
+    def __repr__(self) -> str:
+        return f"FP8Tensor(shape={self.shape}, block={self.block}, device={self.device})"
 
     @property
     def rows(self) -> int:
-        return self.codes.shape[0]
+        return math.prod(self.shape[:-1])
 
     @property
     def cols(self) -> int:
@@ -51,7 +81,7 @@ class FP8Tensor:
 
     @property
     def device(self) -> torch.device:
-        return self.codes.device
+        return (self._codes if self._buf is None else self._buf).device
 
     def nbytes(self) -> int:
         return self.codes.numel() + self.scales.numel()
@@ -60,8 +90,7 @@ class FP8Tensor:
         return FP8Tensor(self.codes.to(device), self.scales.to(device), self.shape, self.block)
 
     def descriptor(self) -> LrqFp8:
-        c, s, shape, block = self.codes, self.scales, self.shape, self.block
-        _require_device(c, s)
+        shape, block, buf = self.shape, self.block, self._buf
         cols = shape[-1] if len(shape) else 0
         if cols <= 0:
             raise ValueError("an FP8 tensor needs rows of at least one element")
@@ -69,7 +98,14 @@ class FP8Tensor:
             raise ValueError(f"a scale is for 1 or 128 rows, got {block}")
         rows = shape[0] if len(shape) == 2 else math.prod(shape[:-1])
         steps = (cols + 127) // 128
-        tall, wide = (rows + block - 1) // block, (steps + 3) // 4 * 4
+        wide = (steps + 3) // 4 * 4
+        if buf is not None:
+            p = buf.data_ptr()
+            return LrqFp8(p, 128 * steps, p + rows * 128 * steps, wide, rows, cols, block)
+        c, s = self._codes, self._scales
+        tall = (rows + block - 1) // block
+        if not (c.is_cuda and s.is_cuda):
+            _require_device(c, s)
         if c.dim() == 2 and s.dim() == 2 and c.dtype in _BYTES and s.dtype in _BYTES and c.device == s.device:
             (cr, cw), (sr, sw), (ldc, c1), (lds, s1) = c.shape, s.shape, c.stride(), s.stride()
             if cr == rows and sr == tall and cw >= 128 * steps and sw >= wide and c1 == 1 and s1 == 1:
@@ -83,14 +119,24 @@ class FP8Tensor:
                          f"{tuple(s.shape)} on {s.device}")
 
 
+def _steps(cols: int) -> int:
+    return (cols + 127) // 128
+
+
+def _wide(cols: int) -> int:
+    return (_steps(cols) + 3) // 4 * 4
+
+
 def _empty(like: torch.Tensor, rows: int, cols: int, shape, block: int) -> tuple[FP8Tensor, LrqFp8]:
     """An FP8 tensor to be written, and its descriptor."""
     steps = (cols + 127) // 128
-    wide = (steps + 3) // 4 * 4
-    codes = like.new_empty((rows, 128 * steps), dtype=torch.float8_e4m3fn)
-    scales = like.new_empty(((rows + block - 1) // block, wide), dtype=torch.uint8)
-    return (FP8Tensor(codes, scales, shape, block),
-            LrqFp8(codes.data_ptr(), 128 * steps, scales.data_ptr(), wide, rows, cols, block))
+    wide, codes = (steps + 3) // 4 * 4, rows * 128 * steps
+    q = FP8Tensor.__new__(FP8Tensor)
+    q._codes = q._scales = None
+    q.shape, q.block = tuple(shape), block
+    q._buf = buf = like.new_empty(codes + (rows if block == 1 else (rows + 127) // 128) * wide, dtype=torch.uint8)
+    p = buf.data_ptr()
+    return q, LrqFp8(p, 128 * steps, p + codes, wide, rows, cols, block)
 
 
 def fp8_from_parts(codes: torch.Tensor, scales: torch.Tensor, block: int = 128) -> FP8Tensor:
@@ -139,7 +185,7 @@ def fp8_quantize(x: torch.Tensor, block: int = 1, transpose: bool = False) -> FP
             raise ValueError("the transpose of no rows has rows of no elements")
         q, t = _empty(x, n, rows, (n, rows), 1)
     else:
-        q, t = _empty(x, rows, n, tuple(x.shape), block)
+        q, t = _empty(x, rows, n, x.shape, block)
     with _on(x.device):
         call("lrq_fp8_quantize", _p(x2), ldx, dt, ctypes.byref(t), int(transpose), _stream(x.device))
     return q
@@ -148,7 +194,7 @@ def fp8_quantize(x: torch.Tensor, block: int = 1, transpose: bool = False) -> FP
 def fp8_dequantize(q: FP8Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values of q (exact in bf16 and fp32)."""
     t = q.descriptor()
-    out = q.codes.new_empty(q.shape, dtype=dtype)
+    out = (q._codes if q._buf is None else q._buf).new_empty(q.shape, dtype=dtype)
     with _on(q.device):
         call("lrq_fp8_dequantize", ctypes.byref(t), _p(out), q.cols, _dtype(out, "the output"), _stream(q.device))
     return out
@@ -172,13 +218,16 @@ def _matrix(w: FP8Tensor, device: torch.device) -> LrqFp8:
 def _product(name: str, a: FP8Tensor, tb: LrqFp8, cols: int, out_dtype, nn: int) -> torch.Tensor:
     dt = _out_dtype(out_dtype)
     ta = a.descriptor()
-    out = a.codes.new_empty((ta.rows, cols) if len(a.shape) == 2 else tuple(a.shape[:-1]) + (cols,), dtype=out_dtype)
-    n = call_raw("lrq_fp8_gemm_workspace", ctypes.byref(ta), ctypes.byref(tb), nn)
-    if n < 0:
-        check(n, "lrq_fp8_gemm_workspace")
-    ws = out.new_empty(n // 4, dtype=torch.float32) if n else None
-    with _on(a.device):
-        call(name, ctypes.byref(ta), ctypes.byref(tb), _p(out), cols, dt, _p(ws), n, _stream(a.device))
+    rows, any_ = ta.rows, a._codes if a._buf is None else a._buf
+    out = any_.new_empty((rows, cols) if len(a.shape) == 2 else a.shape[:-1] + (cols,), dtype=out_dtype)
+    device, pa, pb, ws, n = out.device, ctypes.byref(ta), ctypes.byref(tb), None, 0
+    if nn or rows > 16:  # (fewer rows split nothing over workgroups)
+        n = call_raw("lrq_fp8_gemm_workspace", pa, pb, nn)
+        if n < 0:
+            check(n, "lrq_fp8_gemm_workspace")
+        ws = out.new_empty(n // 4, dtype=torch.float32) if n else None
+    with _on(device):
+        call(name, pa, pb, out.data_ptr(), cols, dt, _p(ws), n, _stream(device))
     return out
 
 

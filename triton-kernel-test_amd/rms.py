@@ -25,21 +25,24 @@ __all__ = ["rms_norm_forward", "add_rms_norm_forward", "rms_norm_backward"]
 def _forward(x, residual, weight, eps, fp8: bool, add: bool):
     _require_device(x, residual, weight)
     dt = _dtype(x, "x")
-    _like(residual, x, "residual")
     x2, rows, n, ldx = _rows(x, "x")
-    r2, ldr = (None, 0) if residual is None else _rows(residual, "residual")[::3]
-    w, _, wdt = _weights(weight, None, n, x.device)
+    device, r2, ldr, w, wdt = x.device, None, 0, None, _lib.LRQ_F32
+    if residual is not None:
+        _like(residual, x, "residual")
+        r2, ldr = _rows(residual, "residual")[::3]
+    if weight is not None:
+        w, _, wdt = _weights(weight, None, n, device)
     h = _new(x) if add else None
     if fp8:
-        y, t = _empty(x, rows, n, tuple(x.shape), 1)
+        y, t = _empty(x, rows, n, x.shape, 1)
         py, pq = None, ctypes.byref(t)
     else:
         y = _new(x)
-        py, pq = _p(y), None
+        py, pq = y.data_ptr(), None
     rstd = x.new_empty((rows,) if x.dim() == 2 else x.shape[:-1], dtype=torch.float32)
-    with _on(x.device):
-        call("lrq_rms_norm_fwd", _p(x2), ldx, _p(r2), ldr, dt, _p(w), wdt, rows, n, eps, _p(h), n, py, n, pq, _p(rstd),
-             _stream(x.device))
+    with _on(device):
+        call("lrq_rms_norm_fwd", x2.data_ptr(), ldx, _p(r2), ldr, dt, _p(w), wdt, rows, n, eps, _p(h), n, py, n, pq,
+             rstd.data_ptr(), _stream(device))
     return y, h, rstd
 
 
