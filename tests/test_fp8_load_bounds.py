@@ -1,4 +1,4 @@
-"""The loads of the 8-bit products, replayed in numpy from the launch arithmetic of csrc/lrq_fp8gemm.hip for every tile height
+"""The loads of the 8-bit products, replayed in numpy from the launch arithmetic of csrc/lrq_fp8gemm.hip for every tile
 and split the host may choose: every read lies in its operand, every LDS write in the part of the allocation it belongs to,
 no two loads of a step write the same bytes, and the transposing and plain LDS reads find the element they are meant to."""
 
@@ -19,8 +19,11 @@ def _lds(dests, low, high, what):
     assert all(a[1] <= b[0] for a, b in zip(spans, spans[1:])), f"{what}: two loads write the same bytes"
 
 
-def _deep(mt):
-    return 2 if mt >= 3 else 3
+TILES = [(1, 4), (2, 2), (2, 4), (3, 4), (4, 4)]  # 64 mt rows by 64 nb columns
+
+
+def _deep(mt, nb):
+    return (160 * 1024 - 4096) // (64 * (mt + nb) * 128)
 
 
 def _runs(steps, splits):
@@ -33,29 +36,32 @@ SIZES = [(1, 1, 1), (17, 100, 520), (65, 257, 136), (129, 260, 640), (300, 513, 
          (40, 1300, 2640), (300, 500, 6000), (2050, 4100, 72), (600, 1300, 13000), (512, 14336, 4096)]
 
 
-def _lds_sizes(mt):
-    kx, kw = 64 * mt * 128, 32768
+def _lds_sizes(mt, nb):
+    kx, kw = 64 * mt * 128, 64 * nb * 128
     stage = kx + kw
-    ring = _deep(mt) * stage
+    ring = _deep(mt, nb) * stage
+    assert _deep(mt, nb) >= 2
     loop = ring + 2 * 2048
     assert loop <= 160 * 1024 and 4 * 32 * 144 <= loop
     return kx, stage, ring
 
 
 @pytest.mark.parametrize("nn", [False, True])
-@pytest.mark.parametrize("mt", [1, 2, 3, 4])
+@pytest.mark.parametrize("mt,nb", TILES)
 @pytest.mark.parametrize("m,n,k", SIZES)
-def test_tile(m, n, k, mt, nn):
+def test_tile(m, n, k, mt, nb, nn):
     """x [m, depth], w [n, k]: depth = k, output columns n; NN: depth = n, output columns k."""
     depth, cols = (n, k) if nn else (k, n)
     steps, wsteps = -(-depth // 128), -(-k // 128)
     ldx, ldw, ldsx, ldsw = 128 * steps, 128 * wsteps, -(-steps // 4) * 4, -(-wsteps // 4) * 4
-    kx, stage, ring = _lds_sizes(mt)
-    klx = 2 * mt
+    kx, stage, ring = _lds_sizes(mt, nb)
+    klx, klw = 2 * mt, 2 * nb
+    lanes, even = 4 * nb, 1 if nb == 2 else 2
+    each = 64 // lanes
     wrows = -(-n // 128)
-    for splits in {1, 2, 3, 16} if steps >= 64 else {1, 2} if steps >= 8 else {1}:
+    for splits in {min(wanted, max(1, steps // 4)) for wanted in (1, 2, 3, 16)}:  # none without a step
         for m0 in {0, (m - 1) // (64 * mt) * 64 * mt}:
-            for n0 in {0, (cols - 1) // 256 * 256}:
+            for n0 in {0, (cols - 1) // (64 * nb) * 64 * nb}:
                 for first, last in _runs(steps, splits):
                     assert 0 <= first < last <= steps and first % 4 == 0
                     # X
@@ -71,24 +77,25 @@ def test_tile(m, n, k, mt, nn):
                     _lds(dest, 0, kx, "X")
                     # W
                     dest = []
-                    for i in range(8):
+                    for i in range(klw):
                         if not nn:
-                            r = 8 * (8 * WAVE + i) + (LANE >> 3)
-                            ow = np.minimum(r, min(256, n - n0) - 1) * ldw + 16 * ((LANE & 7) ^ (r >> 1 & 7))
+                            r = 8 * (klw * WAVE + i) + (LANE >> 3)
+                            ow = np.minimum(r, min(64 * nb, n - n0) - 1) * ldw + 16 * ((LANE & 7) ^ (r >> 1 & 7))
                             for step in (first, last - 1):
                                 _inside(n0 * ldw + 128 * step + ow, 16, n * ldw, "W codes")
                         else:
-                            r = 32 * WAVE + 4 * i + (LANE >> 4)
-                            ow = np.minimum(16 * ((LANE & 15) ^ (r & 7)), min(256, 128 * wsteps - n0) - 16)
-                            assert (((32 * WAVE + 4 * (i & 1) + (LANE >> 4)) & 7) == (r & 7)).all()  # offset i & 1 serves
+                            r = 32 * WAVE + each * i + LANE // lanes
+                            ow = np.minimum(16 * ((LANE % lanes) ^ (r & 7)), min(64 * nb, 128 * wsteps - n0) - 16)
+                            assert (((32 * WAVE + each * (i % even) + LANE // lanes) & 7) == (r & 7)).all()  # offset i % even serves
                             for step in (first, last - 1):
                                 row = np.minimum(r, n - 1 - 128 * step)
                                 _inside((128 * step + row) * ldw + n0 + ow, 16, n * ldw, "W codes")
-                        dest += [(kx + 1024 * v, 1024) for v in np.unique(8 * WAVE + i)]
+                        dest += [(kx + 1024 * v, 1024) for v in np.unique(klw * WAVE + i)]
                     _lds(dest, kx, stage, "W")
                     # scales: group g in slot (g - first / 4) % 2; every step's are loaded ahead of it
                     part = np.minimum(WAVE, mt - 1)
-                    dest = [(ring + 256 * v, 256) for v in np.unique(part)] + [(ring + 1024 + 256 * v, 256) for v in range(4)]
+                    wpart = WAVE if nn else np.minimum(WAVE, nb - 1)
+                    dest = [(ring + 256 * v, 256) for v in np.unique(part)] + [(ring + 1024 + 256 * v, 256) for v in np.unique(wpart)]
                     _lds(dest, ring, ring + 2048, "scales")
                     slot, held = 0, {0: first // 4}
                     for step in range(first, last):
@@ -105,10 +112,10 @@ def test_tile(m, n, k, mt, nn):
                         if not nn:
                             for shift in (0, 7):
                                 tall = -(-n // (1 << shift))
-                                row = np.minimum(n0 + 64 * WAVE + LANE, n - 1) >> shift
+                                row = np.minimum(n0 + 64 * wpart + LANE, n - 1) >> shift
                                 _inside(row * ldsw + 4 * g, 4, tall * ldsw, "W scales")
                         else:
-                            block = np.minimum(n0 // 128 + (WAVE & 1), wsteps - 1)
+                            block = np.minimum((n0 + 32 * nb * (WAVE & 1)) // 128, wsteps - 1)
                             row = np.minimum(4 * g + (LANE & 3), steps - 1)
                             _inside(row * ldsw + (block & ~3), 4, wrows * ldsw, "W scales")
 
@@ -143,32 +150,34 @@ def test_reads_of_rows(mt):
                 assert all(len(set(banks[16 * g:16 * g + 16])) == 16 for g in range(4))
 
 
-def test_reads_of_columns():
+@pytest.mark.parametrize("nb", [2, 4])
+def test_reads_of_columns(nb):
     """NN: the transposing read of lane (c, h), half Q, piece q, gives bytes of column 32 t + c in rows 64 Q + 32 h + 16 q ..
     + 15, in the order in which X's operand has them."""
-    image = np.full((128 * 256, 2), -1)  # (row of the step, column of the tile)
+    lanes = 4 * nb
+    image = np.full((128 * 64 * nb, 2), -1)  # (row of the step, column of the tile)
     for wave in range(4):
-        for i in range(8):
-            r = 32 * wave + 4 * i + (LANE >> 4)
+        for i in range(2 * nb):
+            r = 32 * wave + 64 // lanes * i + LANE // lanes
             for b in range(16):
-                image[1024 * (8 * wave + i) + 16 * LANE + b] = np.stack([r, 16 * ((LANE & 15) ^ (r & 7)) + b], 1)
+                image[1024 * (2 * nb * wave + i) + 16 * LANE + b] = np.stack([r, 16 * ((LANE % lanes) ^ (r & 7)) + b], 1)
     assert (image >= 0).all()
     for wn in range(2):
-        for t in range(4):
+        for t in range(nb):
             for half in range(2):
                 for q in range(2):
                     r = 64 * half + 32 * (LANE >> 5) + 16 * q + (LANE >> 1 & 7)
-                    piece = 8 * wn + 2 * t + (LANE >> 4 & 1)
-                    p = 256 * r + 16 * (piece ^ (r & 7)) + 8 * (LANE & 1)
+                    piece = 2 * nb * wn + 2 * t + (LANE >> 4 & 1)
+                    p = 64 * nb * r + 16 * (piece ^ (r & 7)) + 8 * (LANE & 1)
                     for second in range(2):
-                        at = p + 8 * 256 * second
+                        at = p + 8 * 64 * nb * second
                         for lane in range(64):
                             group, i = lane & ~15, lane & 15
                             # 16 lanes read 8 rows of 16 bytes, two lanes a row; lane i is given byte i of each
                             for e in range(8):
                                 src = at[group + 2 * e + i // 8] + i % 8
                                 row, col = image[src]
-                                assert col == 128 * wn + 32 * t + (lane & 31)
+                                assert col == 32 * nb * wn + 32 * t + (lane & 31)
                                 assert row == 64 * half + 32 * (lane >> 5) + 16 * q + 8 * second + e
 
 

@@ -136,6 +136,18 @@ def test_gemm_nn(pkg, m, k, n, ba):
         assert_within(pkg.fp8_linear_backward(a, b, dtype), ref, bound, f"{m}x{n}x{k} {dtype}")
 
 
+# depth by columns: what each tile is chosen for (64 x 256, 128 x 128 split and not, 128 x 256, 192 x 256, 256 x 256)
+@pytest.mark.parametrize("m,depth,cols", [(50, 256, 4100), (90, 4000, 256), (129, 1100, 2100), (700, 256, 6001), (1500, 300, 11000),
+                                          (1000, 300, 8200)])
+@pytest.mark.parametrize("nn", [False, True])
+def test_every_tile(pkg, m, depth, cols, nn):
+    a = pkg.fp8_quantize(_x(m, depth, BF))
+    b = pkg.fp8_quantize(_x(*((depth, cols) if nn else (cols, depth)), F32, 1, 0.02), 128)
+    va, vb = R.tensor_values(a), R.tensor_values(b)
+    ref, bound = R.product(va, vb if nn else vb.T, F32)
+    assert_within((pkg.fp8_linear_backward if nn else pkg.fp8_gemm)(a, b, F32), ref, bound, f"{m}x{depth}x{cols}")
+
+
 @pytest.mark.parametrize("m,k,n", [(5, 128, 16), (40, 1000, 300), (300, 700, 520)])
 def test_small_integers_are_exact(pkg, m, k, n):
     """Codes of small integers, scales of different powers of two: every sum is exact, so every code and scale has met its

@@ -229,26 +229,26 @@ struct Tile8Args {
   int steps;      // contraction steps of 128
 };
 
-// Workgroup: 64 MT rows of X by 256 output columns, four waves in two rows of two, each 32 MT x 128 of it in 32x32x64
+// Workgroup: 64 MT rows of X by 64 NB output columns, four waves in two rows of two, each 32 MT x 32 NB of it in 32x32x64
 // instructions: one wave a SIMD, whose sums take half of its registers.  K goes through LDS in steps of 128 bytes a row,
 // straight from memory, whole cache lines at a time (with 64 bytes a row the L2s were asked twice as often, 66 % of their
 // cycles, and 8192^3 took 480 us).
 //
 // LDS: X and (NN false) W have rows of 128 bytes, row r's 16-byte piece p in slot p ^ (r / 2 % 8): 16 lanes of a read cover
-// all banks.  NN: 128 rows of W of 256 bytes, piece p of row r in slot p ^ (r % 8); the transposing read gives a lane its
+// all banks.  NN: 128 rows of W of 64 NB bytes, piece p of row r in slot p ^ (r % 8); the transposing read gives a lane its
 // column of 8 rows.
-template <int MT>
+template <int MT, int NB>
 struct Tile8Lds {
-  static constexpr int kX = 64 * MT * 128, kW = 32768, kStage = kX + kW, kDeep = MT >= 3 ? 2 : 3, kRing = kDeep * kStage;
+  static constexpr int kX = 64 * MT * 128, kW = 64 * NB * 128, kStage = kX + kW, kDeep = (160 * 1024 - 4096) / kStage, kRing = kDeep * kStage;
   static constexpr int kScales = 2048, kLoop = kRing + 2 * kScales;
   static constexpr int kOut = 4 * 32 * (128 + 16);  // of the output, in the ring's place
   static_assert(kLoop <= 160 * 1024 && kOut <= kLoop);
 };
 
-template <bool NN, int MT, int OT>
+template <bool NN, int MT, int NB, int OT>
 __global__ __launch_bounds__(256, 1) void k_fp8_tile(Tile8Args a) {
-  using T = Tile8Lds<MT>;
-  constexpr int kX = T::kX, kStage = T::kStage, kDeep = T::kDeep, kLx = 2 * MT, kLoads = kLx + 8;
+  using T = Tile8Lds<MT, NB>;
+  constexpr int kX = T::kX, kStage = T::kStage, kDeep = T::kDeep, kLx = 2 * MT, kLw = 2 * NB, kLoads = kLx + kLw;
   extern __shared__ __attribute__((aligned(16))) char sm[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave >> 1, wn = wave & 1, c = lane & 31, h = lane >> 5;
@@ -259,15 +259,17 @@ __global__ __launch_bounds__(256, 1) void k_fp8_tile(Tile8Args a) {
   const uint32_t band = __builtin_amdgcn_readfirstlane(tile / (kBand * a.tiles_n)), in = tile - band * kBand * a.tiles_n;
   const uint32_t tall = min(kBand, a.tiles_m - band * kBand);
   const uint32_t tn = __builtin_amdgcn_readfirstlane(in / tall), tm = band * kBand + in - tn * tall;
-  const uint32_t m0 = tm * 64 * MT, n0 = tn * 256;
+  const uint32_t m0 = tm * 64 * MT, n0 = tn * 64 * NB;
   // a split's steps: whole groups of four, whose scales come together
   const uint32_t groups = (uint32_t)(a.steps + 3) >> 2;
   const int first = 4 * __builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)groups * z / (uint32_t)a.splits));
   const int last = min(4 * (int)__builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)groups * (z + 1) / (uint32_t)a.splits)), a.steps);
 
-  // ---- loads of 1 KB: 8 rows of 128 bytes (NN W: 4 rows of 256), at 32-bit offsets from a tile's first row
+  // ---- loads of 1 KB: 8 rows of 128 bytes (NN W: 16 / NB rows of 64 NB), at 32-bit offsets from a tile's first row
   const uint32_t sm0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)sm;
-  const int rw = 32 * wave + (lane >> 4);  // NN: row rw + 4 i of a step, whose piece does not depend on i / 2
+  // NN: row rw + kRows i of a step; its piece depends on the row's last three bits, so on i % 2 at most
+  constexpr int kLanes = 4 * NB, kRows = 64 / kLanes, kEven = kRows == 8 ? 1 : 2;
+  const int rw = 32 * wave + lane / kLanes;
   struct {
     const uint8_t *x, *w;
     uint32_t row;
@@ -277,7 +279,7 @@ __global__ __launch_bounds__(256, 1) void k_fp8_tile(Tile8Args a) {
     to.x = a.x.codes + (uint64_t)m0 * a.x.ldc + to.row;
     to.w = NN ? a.w.codes + n0 + (uint64_t)to.row * a.w.ldc : a.w.codes + (uint64_t)n0 * a.w.ldc + to.row;
   };
-  uint32_t ox[kLx], ow[NN ? 2 : 8];
+  uint32_t ox[kLx], ow[NN ? kEven : kLw];
   const uint32_t mx = min(64u * MT, a.x.rows - m0) - 1;
 #pragma unroll
   for (int i = 0; i < kLx; ++i) {
@@ -285,16 +287,16 @@ __global__ __launch_bounds__(256, 1) void k_fp8_tile(Tile8Args a) {
     ox[i] = min((uint32_t)r, mx) * a.x.ldc + 16 * ((lane & 7) ^ (r >> 1 & 7));
   }
   if constexpr (!NN) {
-    const uint32_t mw = min(256u, a.w.rows - n0) - 1;
+    const uint32_t mw = min(64u * NB, a.w.rows - n0) - 1;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = 8 * (8 * wave + i) + (lane >> 3);
+    for (int i = 0; i < kLw; ++i) {
+      const int r = 8 * (kLw * wave + i) + (lane >> 3);
       ow[i] = min((uint32_t)r, mw) * a.w.ldc + 16 * ((lane & 7) ^ (r >> 1 & 7));
     }
   } else {
-    const uint32_t mw = min(256u, 128u * (uint32_t)a.w.steps - n0) - 16;
+    const uint32_t mw = min(64u * NB, 128u * (uint32_t)a.w.steps - n0) - 16;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) ow[i] = min((uint32_t)(16 * ((lane & 15) ^ ((rw + 4 * i) & 7))), mw);
+    for (int i = 0; i < kEven; ++i) ow[i] = min((uint32_t)(16 * ((lane % kLanes) ^ ((rw + kRows * i) & 7))), mw);
   }
   // load i of the step
   const auto issue = [&](int buf, int i) {
@@ -302,31 +304,31 @@ __global__ __launch_bounds__(256, 1) void k_fp8_tile(Tile8Args a) {
     if (i < kLx) {
       ld_to_lds8<16>(to.x, ox[i < kLx ? i : 0], st + 1024 * (kLx * wave + i));
     } else {
-      const int k = (i - kLx) & 7;
-      const uint32_t lds = st + kX + 1024 * (8 * wave + k);
+      const int k = i >= kLx ? i - kLx : 0;
+      const uint32_t lds = st + kX + 1024 * (kLw * wave + k);
       if constexpr (!NN) {
         ld_to_lds8<16>(to.w, ow[k], lds);
       } else {  // rows past W's last: that one (their x is zero)
         const uint32_t end = a.w.rows - 1 - to.row;
-        ld_to_lds8<16>(to.w, min((uint32_t)(rw + 4 * k), end) * a.w.ldc + ow[k & 1], lds);
+        ld_to_lds8<16>(to.w, min((uint32_t)(rw + kRows * k), end) * a.w.ldc + ow[k % kEven], lds);
       }
     }
   };
-  // four steps' scales of 64 rows a load; NN: of this wave's 128 columns, four steps are four rows of scales
-  const int is = min(wave, MT - 1);
-  const int block = min((int)(n0 >> 7) + wn, a.w.steps - 1);  // NN
+  // four steps' scales of 64 rows a load; NN: of the block of 128 columns that this wave's are in, four steps are four rows
+  const int is = min(wave, MT - 1), iw = min(wave, NB - 1);
+  const int block = min((int)(n0 + 32 * NB * wn) >> 7, a.w.steps - 1);  // NN
   const uint32_t osx = (min(m0 + 64 * is + lane, a.x.rows - 1) >> a.x.shift) * a.x.lds;
-  const uint32_t osw = NN ? (uint32_t)(block & ~3) : (min(n0 + 64 * wave + lane, a.w.rows - 1) >> a.w.shift) * a.w.lds;
+  const uint32_t osw = NN ? (uint32_t)(block & ~3) : (min(n0 + 64 * iw + lane, a.w.rows - 1) >> a.w.shift) * a.w.lds;
   const auto issue_scales = [&](int group, int slot) {
     const uint32_t sc = sm0 + T::kRing + slot * T::kScales;
     ld_to_lds8<4>(a.x.scales + 4 * group, osx, sc + 256 * is);
-    if constexpr (!NN) ld_to_lds8<4>(a.w.scales + 4 * group, osw, sc + 1024 + 256 * wave);
+    if constexpr (!NN) ld_to_lds8<4>(a.w.scales + 4 * group, osw, sc + 1024 + 256 * iw);
     else ld_to_lds8<4>(a.w.scales, (uint32_t)min(4 * group + (lane & 3), a.steps - 1) * a.w.lds + osw, sc + 1024 + 256 * wave);
   };
 
   // ---- operands of half Q of a step (64 of K): piece 4 Q + 2 h + q of a row
-  Frag fx[2][MT], fw[2][4];
-  uint32_t sx[MT], sw[4];
+  Frag fx[2][MT], fw[2][NB];
+  uint32_t sx[MT], sw[NB];
   const auto read_x = [&](int half, int buf, int i, int q) {
     const int r = 32 * MT * wm + 32 * i + c;
     fx[half][i].v[q] = ld16(sm + buf * kStage + 128 * r + 16 * ((4 * half + 2 * h + q) ^ (r >> 1 & 7)));
@@ -334,19 +336,19 @@ __global__ __launch_bounds__(256, 1) void k_fp8_tile(Tile8Args a) {
   const auto read_w = [&](int half, int buf, int t, int q) {
     const char* st = sm + buf * kStage + kX;
     if constexpr (!NN) {
-      const int r = 128 * wn + 32 * t + c;
+      const int r = 32 * NB * wn + 32 * t + c;
       fw[half][t].v[q] = ld16(st + 128 * r + 16 * ((4 * half + 2 * h + q) ^ (r >> 1 & 7)));
     } else {
-      const int r = 64 * half + 32 * h + 16 * q + (lane >> 1 & 7), piece = 8 * wn + 2 * t + (lane >> 4 & 1);
+      const int r = 64 * half + 32 * h + 16 * q + (lane >> 1 & 7), piece = 2 * NB * wn + 2 * t + (lane >> 4 & 1);
       typedef int i32x2 __attribute__((ext_vector_type(2)));
-      const auto p = (__attribute__((address_space(3))) i32x2*)(st + 256 * r + 16 * (piece ^ (r & 7)) + 8 * (lane & 1));
-      const i32x2 lo = __builtin_amdgcn_ds_read_tr8_b64_v2i32(p), hi = __builtin_amdgcn_ds_read_tr8_b64_v2i32(p + 8 * 32);
+      const auto p = (__attribute__((address_space(3))) i32x2*)(st + 64 * NB * r + 16 * (piece ^ (r & 7)) + 8 * (lane & 1));
+      const i32x2 lo = __builtin_amdgcn_ds_read_tr8_b64_v2i32(p), hi = __builtin_amdgcn_ds_read_tr8_b64_v2i32(p + 64 * NB);
       fw[half][t].v[q] = u32x4{(uint32_t)lo[0], (uint32_t)lo[1], (uint32_t)hi[0], (uint32_t)hi[1]};
     }
   };
   const auto read_piece = [&](int half, int buf, int p) {
-    if (p < 8) read_w(half, buf, p >> 1, p & 1);
-    else read_x(half, buf, (p - 8) >> 1, p & 1);
+    if (p < 2 * NB) read_w(half, buf, p >> 1, p & 1);
+    else read_x(half, buf, (p - 2 * NB) >> 1, p & 1);
   };
   const auto read_scales = [&](int step, int slot) {
     const char* sc = sm + T::kRing + slot * T::kScales;
@@ -355,7 +357,7 @@ __global__ __launch_bounds__(256, 1) void k_fp8_tile(Tile8Args a) {
     for (int i = 0; i < MT; ++i) sx[i] = ld4(sc + 4 * (32 * MT * wm + 32 * i + c)) >> sh;
     if constexpr (!NN) {
 #pragma unroll
-      for (int t = 0; t < 4; ++t) sw[t] = ld4(sc + 1024 + 4 * (128 * wn + 32 * t + c)) >> sh;
+      for (int t = 0; t < NB; ++t) sw[t] = ld4(sc + 1024 + 4 * (32 * NB * wn + 32 * t + c)) >> sh;
     } else {
       sw[0] = ld4(sc + 1024 + 256 * wave + 4 * (step & 3)) >> (8 * (block & 3));
     }
@@ -366,13 +368,13 @@ __global__ __launch_bounds__(256, 1) void k_fp8_tile(Tile8Args a) {
   // and before half 1, when the next step's loads are in.  The loads go out evenly over the rest of the step: they are
   // 16 TB/s of the L2s' at full speed, and 1.5 to 2 at a time 8192^3 took 440 us, at 1 behind each instruction of half 1 404,
   // so 395.  The order is held: the compiler would issue all loads first.
-  constexpr int kMfma = 4 * MT, kPieces = 2 * (MT + 4), kReads = (kPieces + kMfma / 2 - 1) / (kMfma / 2);
+  constexpr int kMfma = NB * MT, kPieces = 2 * (MT + NB), kReads = (kPieces + kMfma / 2 - 1) / (kMfma / 2);
   constexpr int kFirst = 3 * kLoads / 8;  // of a step's loads: behind the second half of half 0's instructions
-  f32x16 acc[MT][4];
+  f32x16 acc[MT][NB];
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
-    for (int t = 0; t < 4; ++t) acc[i][t] = f32x16{};
+    for (int t = 0; t < NB; ++t) acc[i][t] = f32x16{};
   issue_scales(first >> 2, 0);
 #pragma unroll
   for (int d = 0; d < kDeep; ++d) {
@@ -391,14 +393,14 @@ __global__ __launch_bounds__(256, 1) void k_fp8_tile(Tile8Args a) {
   int buf = 0, slot = 0;  // of the step, of its scales
   for (int part = 0, step = first; part < 2; ++part) {
     const int end = part ? last : max(first, last - kDeep);
-    const uint64_t ix = part ? 0 : 128, iw = part ? 0 : NN ? 128 * (uint64_t)a.w.ldc : 128;
+    const uint64_t ix = part ? 0 : 128, jw = part ? 0 : NN ? 128 * (uint64_t)a.w.ldc : 128;
     if (part) point(last - 1);
     for (; step < end; ++step) {
       const int next = buf + 1 == kDeep ? 0 : buf + 1;
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int m = 0; m < kMfma; ++m) {
-        const int i = m >> 2, t = m & 3, late = m - kMfma / 2;
+        const int i = m / NB, t = m % NB, late = m - kMfma / 2;
         acc[i][t] = mfma8_32(fw[0][t], fx[0][i], acc[i][t], sw[NN ? 0 : t], sx[i]);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -416,7 +418,7 @@ __global__ __launch_bounds__(256, 1) void k_fp8_tile(Tile8Args a) {
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int m = 0; m < kMfma; ++m) {
-        const int i = m >> 2, t = m & 3;
+        const int i = m / NB, t = m % NB;
         acc[i][t] = mfma8_32(fw[1][t], fx[1][i], acc[i][t], sw[NN ? 0 : t], sx[i]);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -427,7 +429,7 @@ __global__ __launch_bounds__(256, 1) void k_fp8_tile(Tile8Args a) {
           if (p < kPieces) read_piece(0, next, p);
         __builtin_amdgcn_sched_barrier(0);
       }
-      to.x += ix, to.w += iw, to.row += (uint32_t)ix;
+      to.x += ix, to.w += jw, to.row += (uint32_t)ix;
       slot ^= (step & 3) == 3 ? 1 : 0;
       read_scales(step + 1, slot);  // (of no use behind the last step)
       buf = next;
@@ -445,8 +447,8 @@ __global__ __launch_bounds__(256, 1) void k_fp8_tile(Tile8Args a) {
   for (int i = 0; i < MT; ++i) {
     const int64_t m = (int64_t)m0 + 32 * MT * wm + 32 * i + lane / 8;
 #pragma unroll
-    for (int t0 = 0; t0 < 4; t0 += kTs) {
-      const int64_t n = (int64_t)n0 + 128 * wn + 32 * t0 + kWide * (lane % 8);
+    for (int t0 = 0; t0 < NB; t0 += kTs) {
+      const int64_t n = (int64_t)n0 + 32 * NB * wn + 32 * t0 + kWide * (lane % 8);
       const int valid = (int)min((int64_t)kWide, a.cols - n);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -495,7 +497,7 @@ __global__ __launch_bounds__(256) void k_fp8_join(const float* part, int splits,
 }
 
 struct Plan8 {
-  int mt;  // 64 mt rows a workgroup; 0: the few-row kernel
+  int mt, nb;  // 64 mt rows by 64 nb columns a workgroup; 0: the few-row kernel
   int64_t tiles_m, tiles_n;
   int splits, steps;
 };
@@ -504,27 +506,33 @@ struct Plan8 {
 // [14336, 4096] 19.3 against 13.9 and 20.0 in tiles, but by [4096, 14336] 26.7 against 20.5).
 static bool few_rows(int64_t rows, int64_t cols, int steps) { return rows <= 16 || (rows <= 32 && (steps <= 64 || cols > 8192)); }
 
-// The tile's height and how often the contraction is split over workgroups: one workgroup runs on a CU at a time, so a
-// grid takes rounds of its steps; every split writes and re-reads fp32 parts.  Times in us, as measured (a step of
-// each height; a workgroup's start and end; the join's launch; its bytes at 4 TB/s).  A round that does not fill
-// the card runs at higher clocks: half full, one of high tiles takes 0.8 of a full one; low ones wait for memory.
+// The tile and how often the contraction is split over workgroups: one workgroup runs on a CU at a time, so a grid takes
+// rounds of its steps, and every split writes and re-reads fp32 parts.  Times in us, fitted to 129 measured products (a step of
+// each tile; a workgroup's start and end; the share of a full round that a nearly empty one takes: it runs at higher clocks;
+// the join's launch, and its time for each sum); the plan taken is within 5 % of the best measured one in 119 of them.
+// 128 x 128 tiles are for what does not fill the card with larger ones: 94 x 884 x 10112 8.8 us against 10.4 of 64 x 256,
+// 171 x 10112 x 3183 17.7 against 21.1; they read their operands from the L2 more often, 8192^3 takes 540 us.
 static Plan8 plan8(const lrq_fp8* a, const lrq_fp8* b, bool nn) {
-  constexpr double kStep[4] = {0.72, 0.86, 1.19, 1.44}, kEmpty[4] = {1., 0.9, 0.6, 0.6}, kFixed[4] = {1.5, 5.5, 5.0, 6.0}, kJoin = 4.0, kPerByte = 2.0 / 4.0e6;
-  constexpr double kOnce = 0.86;  // of the lowest, where one row of tiles reads all of W from memory
+  struct Kind {
+    int mt, nb;
+    double step, fixed, empty;
+  };
+  constexpr Kind kKinds[] = {{1, 4, 0.53, 4., 0.7}, {2, 2, 0.47, 4., 0.7}, {2, 4, 0.75, 7., 0.65}, {3, 4, 1.06, 9., 0.6}, {4, 4, 1.37, 9., 0.65}};
+  constexpr double kJoin = 3.5, kPerByte = 1.4e-6;
   constexpr int kCus = 256;  // a fixed count, so that the workspace and the order of the sums depend on the shape alone
-  const int64_t rows = a->rows, cols = nn ? b->cols : b->rows, tiles_n = (cols + 255) / 256;
+  const int64_t rows = a->rows, cols = nn ? b->cols : b->rows;
   const int steps = (int)((a->cols + 127) / 128);
-  if (!nn && few_rows(rows, cols, steps)) return Plan8{0, 0, 0, 1, steps};
+  if (!nn && few_rows(rows, cols, steps)) return Plan8{0, 0, 0, 0, 1, steps};
   Plan8 best{};
   double least = 0.;
-  for (int mt = 1; mt <= 4; ++mt) {
-    Plan8 p{mt, (rows + 64 * mt - 1) / (64 * mt), tiles_n, 1, steps};
+  for (const Kind& k : kKinds) {
+    if (k.mt > 1 && 64 * (k.mt - 1) >= rows) continue;  // part of the tile without a row
+    Plan8 p{k.mt, k.nb, (rows + 64 * k.mt - 1) / (64 * k.mt), (cols + 64 * k.nb - 1) / (64 * k.nb), 1, steps};
     for (; p.splits <= 16 && p.splits <= std::max(1, steps / 4); ++p.splits) {
-      const int64_t wgs = p.tiles_m * tiles_n * p.splits, over = wgs % kCus;
-      const double rounds = (double)(wgs / kCus) + (over == 0 ? 0. : kEmpty[mt - 1] + (1. - kEmpty[mt - 1]) * (double)over / kCus);
-      const double step = p.tiles_m == 1 && mt == 1 ? kOnce : kStep[mt - 1];
-      const double cost = rounds * ((steps + p.splits - 1) / p.splits * step + kFixed[mt - 1]) +
-                          (p.splits > 1 ? kJoin + kPerByte * 4. * p.splits * rows * cols : 0.);
+      const int64_t wgs = p.tiles_m * p.tiles_n * p.splits, over = wgs % kCus;
+      const double rounds = (double)(wgs / kCus) + (over == 0 ? 0. : k.empty + (1. - k.empty) * (double)over / kCus);
+      const double cost = rounds * ((steps + p.splits - 1) / p.splits * k.step + k.fixed) +
+                          (p.splits > 1 ? kJoin + kPerByte * p.splits * rows * cols : 0.);
       if (best.mt == 0 || cost < least) best = p, least = cost;
     }
   }
@@ -603,21 +611,22 @@ static int fp8_product(const lrq_fp8* ta, const lrq_fp8* tb, bool nn, void* out,
   const Tile8Args a{operand(x), operand(w), need ? workspace : out, need ? ldp : ldo, cols, need ? (int)kF32 : odt, (int)p.tiles_m,
                     (int)p.tiles_n, p.splits, p.steps};
   using std::integral_constant;
-  const auto with = [&](auto mt) {
+  const auto with = [&](auto mt, auto nb) {
     const auto go = [&](auto kern) {
-      constexpr int kLds = Tile8Lds<mt()>::kLoop;
+      constexpr int kLds = Tile8Lds<mt(), nb()>::kLoop;
       const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
       if (e != hipSuccess) return (int)e;
       return launch(kern, dim3((unsigned)wgs), dim3(256), (size_t)kLds, s, a);
     };
-    const auto typed = [&](auto ot) { return nn ? go(k_fp8_tile<true, mt(), ot()>) : go(k_fp8_tile<false, mt(), ot()>); };
+    const auto typed = [&](auto ot) { return nn ? go(k_fp8_tile<true, mt(), nb(), ot()>) : go(k_fp8_tile<false, mt(), nb(), ot()>); };
     if (a.odt == kBf16) return typed(integral_constant<int, kBf16>{});
     return a.odt == kF16 ? typed(integral_constant<int, kF16>{}) : typed(integral_constant<int, kF32>{});
   };
-  if (p.mt == 4) LRQ_TRY(with(integral_constant<int, 4>{}));
-  else if (p.mt == 3) LRQ_TRY(with(integral_constant<int, 3>{}));
-  else if (p.mt == 2) LRQ_TRY(with(integral_constant<int, 2>{}));
-  else LRQ_TRY(with(integral_constant<int, 1>{}));
+  if (p.mt == 4) LRQ_TRY(with(integral_constant<int, 4>{}, integral_constant<int, 4>{}));
+  else if (p.mt == 3) LRQ_TRY(with(integral_constant<int, 3>{}, integral_constant<int, 4>{}));
+  else if (p.mt == 2 && p.nb == 4) LRQ_TRY(with(integral_constant<int, 2>{}, integral_constant<int, 4>{}));
+  else if (p.mt == 2) LRQ_TRY(with(integral_constant<int, 2>{}, integral_constant<int, 2>{}));
+  else LRQ_TRY(with(integral_constant<int, 1>{}, integral_constant<int, 4>{}));
   if (need == 0) return LRQ_OK;
   const dim3 grid((unsigned)std::min<int64_t>((rows * (ldp / 4) + 255) / 256, (int64_t)cu_count() * 32));
   return launch(k_fp8_join, grid, dim3(256), 0, s, (const float*)workspace, p.splits, rows, cols, ldp, out, ldo, odt);
