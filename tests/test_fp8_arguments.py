@@ -2,6 +2,7 @@
 any HIP call, the Python layer raises ValueError."""
 
 import ctypes
+import importlib
 
 import pytest
 import torch
@@ -181,6 +182,27 @@ def test_python_refusals(pkg):
         pkg.FP8Tensor(q.codes, q.scales, (256, 256), 64).descriptor()
     with pytest.raises(ValueError, match="at least one element"):
         pkg.FP8Tensor(q.codes, q.scales, (256, 0)).descriptor()
+
+
+def test_autograd_refusals(pkg):
+    """A weight whose gradient would be refused in the backward pass is refused in the call."""
+    AG = importlib.import_module("triton-kernel-test_amd.autograd")
+    x, a = torch.zeros(4, 256, dtype=torch.bfloat16), torch.zeros(256, 16, dtype=torch.bfloat16)
+    rows = pkg.FP8Tensor(torch.zeros(256, 256, dtype=torch.uint8), torch.zeros(256, 4, dtype=torch.uint8), (256, 256), 1)
+    for f in (lambda: AG.fp8_linear(x, rows), lambda: AG.rms_norm_linear(x, None, rows),
+              lambda: AG.rms_norm_linear(x, None, [rows, rows], residual=x),
+              lambda: AG.lora_linear_compressed(x, rows, a, a.mT.contiguous())):
+        with pytest.raises(ValueError, match="128 x 128"):
+            f()
+    for f in (lambda: AG.fp8_linear(rows, x), lambda: AG.fp8_linear(x[0, 0], x)):
+        with pytest.raises(ValueError, match="at least one dimension"):
+            f()
+    for w in ([], [x], x, (rows, None)):
+        with pytest.raises(ValueError, match="must be FP8Tensors"):
+            AG.rms_norm_linear(x, None, w)
+    for w in (None, x[0]):
+        with pytest.raises(ValueError, match="FP8Tensor or a dense matrix"):
+            AG.fp8_linear(x, w)
 
 
 def test_tensor_attributes(pkg):

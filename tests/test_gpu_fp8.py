@@ -381,3 +381,25 @@ def test_lora_on_an_8_bit_base(pkg, AG):
     g = dy @ b.detach().mT
     assert torch.equal(x.grad, torch.addmm(pkg.fp8_linear_backward(dy, q), g, a.detach().mT))
     assert a.grad.shape == a.shape and torch.isfinite(a.grad).all() and b.grad.shape == b.shape
+
+
+def test_no_tokens_no_outputs_one_row(pkg, AG):
+    """Autograd calls without tokens, by a weight without rows, and on a vector."""
+    w = _x(200, 300, BF, 1, 0.02).requires_grad_()
+    none = _x(4, 300, BF)[:0].requires_grad_()
+    y = AG.fp8_linear(none, w)
+    y.sum().backward()
+    assert y.shape == (0, 200) and none.grad.shape == (0, 300) and w.grad.eq(0).all()
+    x, empty = _x(4, 300, BF).requires_grad_(), _x(2, 300, BF)[:0].requires_grad_()
+    y = AG.fp8_linear(x, empty)
+    y.sum().backward()
+    assert y.shape == (4, 0) and x.grad.eq(0).all() and empty.grad.shape == (0, 300)
+    v = _x(1, 300, BF)[0].requires_grad_()
+    w.grad = None
+    y = AG.fp8_linear(v, w)
+    dy = _x(1, 200, BF, 5)
+    y.backward(dy[0])
+    q = pkg.fp8_quantize(w.detach(), 128)
+    assert torch.equal(y, pkg.fp8_linear(v.detach()[None], q)[0])
+    assert torch.equal(v.grad, pkg.fp8_linear_backward(dy, q)[0])
+    assert torch.equal(w.grad, pkg.fp8_weight_gradient(dy, v.detach()[None]))

@@ -266,3 +266,43 @@ def test_norm_and_products_together(pkg, AG, rows):
     a, b = AG.rms_norm_linear(x3, w.detach(), ws[:2])
     b.sum().backward()
     assert torch.isfinite(x3.grad).all()
+
+
+def test_no_rows(pkg, AG):
+    none, w = _r(4, 512, BF)[:0].requires_grad_(), _w(512, BF).requires_grad_()
+    q = pkg.fp8_quantize(_r(256, 512, BF, 1, 0.05), 128)
+    y, h = AG.rms_norm_linear(none, w, q, residual=none.detach())
+    (y.sum() + h.sum()).backward()
+    assert y.shape == (0, 256) and none.grad.shape == (0, 512) and w.grad.eq(0).all()
+
+
+def test_captured_step(pkg, AG):
+    """A layer's forward and backward pass in one graph, with a trained and a frozen product: every replay gives the eager
+    results of its inputs, with eager work between."""
+    frozen = pkg.fp8_quantize(_r(512, 512, BF, 1, 0.05), 128)
+    wn, wt = _w(512, BF).requires_grad_(), _r(384, 512, BF, 2, 0.05).requires_grad_()
+    x, res, dy = _r(300, 512, BF), _r(300, 512, BF, 1), _r(300, 384, BF, 4)
+
+    def step(x, res, dy):
+        x, res = x.detach().requires_grad_(), res.detach().requires_grad_()
+        y, h = AG.rms_norm_linear(x, wn, frozen, residual=res)
+        z = AG.fp8_linear(y, wt)
+        gx, gr, gn, gt = torch.autograd.grad([z, h], [x, res, wn, wt], [dy, h.detach()])
+        return z.detach(), gx, gr, gn, gt
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(x, res, dy)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(x, res, dy)
+    for seed in range(4):
+        x.copy_(_r(300, 512, BF, 10 + seed))
+        dy.copy_(_r(300, 384, BF, 20 + seed))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out]
+        for a, b in zip(got, step(x, res, dy)):
+            assert torch.equal(a, b)

@@ -73,8 +73,8 @@ class LoRALinearCompressed(torch.autograd.Function):
 
     Gradients: dx, dA, dB of compute_lora_gradient on the decoded x; W gets none.  ``fused``
     reads the codes directly for dA and x A (no decoded x), see the module docstring.  W may be an
-    ``MXFP4Tensor`` or ``FP8Tensor`` [out, in].  With ``dropout_p`` the LoRA branch reads dropout(x): y = x W^T + (dropout(x) A) B, its
-    mask drawn again from ``seed`` in the backward pass, where x is decoded for it."""
+    ``MXFP4Tensor`` or ``FP8Tensor`` [out, in].  With ``dropout_p`` the LoRA branch reads dropout(x):
+    y = x W^T + (dropout(x) A) B, its mask drawn again from ``seed`` in the backward pass, where x is decoded for it."""
 
     @staticmethod
     def forward(ctx, x, w, a, b, basis: Optional[LowRankBasis], bits: int, group: int, fused: bool = True,
@@ -141,7 +141,9 @@ def _codes_gemm_ok(c: CompressedActivation, a: torch.Tensor, dy2: torch.Tensor) 
 def lora_linear_compressed(x, w, a, b, basis: Optional[LowRankBasis] = None, bits: int = 4, group: int = 64,
                            fused: bool = True, dropout_p: float = 0.0, seed=None):
     """The LoRA layer that saves x compressed (``LoRALinearCompressed``).  w: dense [out, in], an
-    ``MXFP4Tensor`` or an ``FP8Tensor``; ``dropout_p`` > 0 needs a ``seed`` (``norm.dropout``'s), a new one for every step and layer."""
+    ``MXFP4Tensor`` or an ``FP8Tensor`` of block 128; ``dropout_p`` > 0 needs a ``seed`` (``norm.dropout``'s), a new one for
+    every step and layer."""
+    _frozen(w)
     return LoRALinearCompressed.apply(x, w, a, b, basis, bits, group, fused, dropout_p, seed)
 
 
@@ -242,6 +244,12 @@ def dropout_add_layer_norm(x: torch.Tensor, residual: Optional[torch.Tensor], we
     """(y, h) of h = residual + dropout(x), y = layer_norm(h), in one kernel each way; h is the residual stream that
     the next block adds to."""
     return _DropoutAddLayerNorm.apply(x, residual, weight, bias, p, seed, eps)
+
+
+def _frozen(w):
+    """A weight whose backward pass would be refused is refused before the forward one."""
+    if isinstance(w, _f8.FP8Tensor) and (len(w.shape) != 2 or w.block != 128):
+        raise ValueError(f"the gradient needs a weight with a scale for 128 x 128 of a matrix's elements, got {w}")
 
 
 def _weight(w):
@@ -369,7 +377,7 @@ class _FP8LinearTrained(torch.autograd.Function):
         if ctx.needs_input_grad[0]:
             dx = _f8.fp8_linear_backward(dy, _f8.FP8Tensor(codes, scales, ctx.shape, 128), ctx.dtype)
         if ctx.needs_input_grad[1]:
-            if ctx.tokens:
+            if ctx.tokens and dy.numel():
                 dw = _f8.fp8_gemm(_f8.fp8_quantize(dy, transpose=True),
                                   _f8.FP8Tensor(xc, xs, (ctx.shape[1], ctx.tokens), 1), ctx.w_dtype)
             else:
@@ -381,8 +389,11 @@ def fp8_linear(x: torch.Tensor, w, out_dtype: Optional[torch.dtype] = None) -> t
     """x w^T in 8 bits (``fp8.fp8_linear``), of x's type unless ``out_dtype`` says otherwise.  w: an ``FP8Tensor`` of block
     128 (frozen: a gradient for x alone) or a dense [out, in] weight, which is quantised in each call and gets its
     gradient; all products of the backward pass are in 8 bits too."""
+    if not isinstance(x, torch.Tensor) or x.dim() < 1:
+        raise ValueError("x must be a tensor of at least one dimension")
     out_dtype = x.dtype if out_dtype is None else out_dtype
     if isinstance(w, _f8.FP8Tensor):
+        _frozen(w)
         return _FP8Linear.apply(x, w, out_dtype)
     if not isinstance(w, torch.Tensor) or w.dim() != 2:
         raise ValueError("the weight must be an FP8Tensor or a dense matrix")
@@ -432,6 +443,8 @@ def rms_norm_linear(x: torch.Tensor, norm_weight: Optional[torch.Tensor], weight
     ws = (weights,) if single else tuple(weights)
     if not ws or not all(isinstance(w, _f8.FP8Tensor) for w in ws):
         raise ValueError("weights must be FP8Tensors")
+    for w in ws:
+        _frozen(w)
     out = _RmsNormLinear.apply(x, residual, norm_weight, eps, ws)
     return out[0] if single and residual is None else out
 
