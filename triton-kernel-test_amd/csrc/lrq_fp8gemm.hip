@@ -507,18 +507,21 @@ struct Plan8 {
 static bool few_rows(int64_t rows, int64_t cols, int steps) { return rows <= 16 || (rows <= 32 && (steps <= 64 || cols > 8192)); }
 
 // The tile and how often the contraction is split over workgroups: one workgroup runs on a CU at a time, so a grid takes
-// rounds of its steps, and every split writes and re-reads fp32 parts.  Times in us, fitted to 129 measured products (a step of
-// each tile; a workgroup's start and end; the share of a full round that a nearly empty one takes: it runs at higher clocks;
-// the join's launch, and its time for each sum); the plan taken is within 5 % of the best measured one in 119 of them.
-// 128 x 128 tiles are for what does not fill the card with larger ones: 94 x 884 x 10112 8.8 us against 10.4 of 64 x 256,
-// 171 x 10112 x 3183 17.7 against 21.1; they read their operands from the L2 more often, 8192^3 takes 540 us.
+// rounds of its longest split's steps, and every split writes and re-reads fp32 parts.  Times in us, fitted to 281 products
+// measured with every tile and split, half of them by weights that came from memory: a step of each tile; a workgroup's start
+// and end; the share of a full round that a nearly empty one takes, which runs at higher clocks; what a step waits longer for
+// W where few rows of tiles share it; the join's launch, and its time for each element of a part.  The plan taken is within 5 % of
+// the best one in 257 of them (1.3 % longer on average).  128 x 128 tiles are for what does not fill the card with larger ones:
+// 94 x 884 x 10112 8.8 us against 10.4 of 64 x 256, 171 x 10112 x 3183 17.7 against 21.1; they read their operands from the L2
+// more often, 8192^3 takes 540 us.
 static Plan8 plan8(const lrq_fp8* a, const lrq_fp8* b, bool nn) {
   struct Kind {
     int mt, nb;
     double step, fixed, empty;
   };
-  constexpr Kind kKinds[] = {{1, 4, 0.53, 4., 0.7}, {2, 2, 0.47, 4., 0.7}, {2, 4, 0.75, 7., 0.65}, {3, 4, 1.06, 9., 0.6}, {4, 4, 1.37, 9., 0.65}};
-  constexpr double kJoin = 3.5, kPerByte = 1.4e-6;
+  constexpr Kind kKinds[] = {{1, 4, 0.61, 3.9, 0.63}, {2, 2, 0.53, 3.1, 0.7}, {2, 4, 0.76, 7.3, 0.57}, {3, 4, 1.13, 7.9, 0.6},
+                             {4, 4, 1.44, 10.6, 0.5}};
+  constexpr double kAlone = 0.12, kJoin = 3.2, kPart = 1.1e-6;
   constexpr int kCus = 256;  // a fixed count, so that the workspace and the order of the sums depend on the shape alone
   const int64_t rows = a->rows, cols = nn ? b->cols : b->rows;
   const int steps = (int)((a->cols + 127) / 128);
@@ -531,8 +534,9 @@ static Plan8 plan8(const lrq_fp8* a, const lrq_fp8* b, bool nn) {
     for (; p.splits <= 16 && p.splits <= std::max(1, steps / 4); ++p.splits) {
       const int64_t wgs = p.tiles_m * p.tiles_n * p.splits, over = wgs % kCus;
       const double rounds = (double)(wgs / kCus) + (over == 0 ? 0. : k.empty + (1. - k.empty) * (double)over / kCus);
-      const double cost = rounds * ((steps + p.splits - 1) / p.splits * k.step + k.fixed) +
-                          (p.splits > 1 ? kJoin + kPerByte * p.splits * rows * cols : 0.);
+      const int run = std::min(steps, 4 * (((steps + 3) / 4 + p.splits - 1) / p.splits));
+      const double cost = rounds * (run * (k.step + kAlone * k.nb / p.tiles_m) + k.fixed) +
+                          (p.splits > 1 ? kJoin + kPart * p.splits * rows * cols : 0.);
       if (best.mt == 0 || cost < least) best = p, least = cost;
     }
   }
