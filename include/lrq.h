@@ -461,7 +461,7 @@ typedef struct lrq_fp8 {
  * to the even one.  A block with an infinity or a NaN becomes NaN (scale 255, codes 0). */
 int lrq_fp8_quantize(const void* x, int64_t ldx, int32_t dtype, const lrq_fp8* t, int32_t transpose, void* stream);
 
-/* out[rows, cols] = the values of t, rounded to dtype (exact in bf16 and fp32 down to their smallest normal numbers). */
+/* out[rows, cols] = the values of t, rounded to dtype (exact in fp32, and in bf16 but for its subnormal numbers). */
 int lrq_fp8_dequantize(const lrq_fp8* t, void* out, int64_t ldo, int32_t dtype, void* stream);
 
 /* out[a.rows, b.rows] = a b^T, both e4m3 with the same cols (any blocks); fp32 accumulation, out of out_dtype.  The
@@ -487,7 +487,7 @@ int lrq_fp8_linear(const void* x, int64_t ldx, int32_t dtype, int64_t rows, cons
 /* y = h * rstd * w per row of n columns, rstd = 1 / sqrt(mean(h^2) + eps) (fp32 [rows], kept for the backward pass).
  * h == NULL: the rows are x's (residual NULL).  Otherwise h = residual + x (residual may be NULL), rounded to dtype, is
  * written and normalised as stored.  w (of w_dtype) may be NULL: 1.  Exactly one of y (of dtype) and q is given: q, of block 1
- * and [rows, n], takes y quantised as by lrq_fp8_quantize, from its fp32 values. */
+ * and [rows, n], takes y quantised as by lrq_fp8_quantize, from its fp32 values.  h may be x or residual. */
 int lrq_rms_norm_fwd(const void* x, int64_t ldx, const void* residual, int64_t ld_residual, int32_t dtype, const void* w,
                      int32_t w_dtype, int64_t rows, int64_t n, float eps, void* h, int64_t ldh, void* y, int64_t ldy,
                      const lrq_fp8* q, float* rstd, void* stream);
@@ -495,7 +495,7 @@ int lrq_rms_norm_fwd(const void* x, int64_t ldx, const void* residual, int64_t l
 /* Gradients of lrq_rms_norm_fwd from dy and, if not NULL, dh (the gradient of h from its other uses): dx = dh + (gradient
  * through the norm), for x and the residual alike.  h: the rows that were normalised.  dw (w_dtype) may be NULL; otherwise
  * it is summed over the rows in a fixed order through `workspace` (4-byte aligned, lrq_rms_norm_bwd_workspace(rows, n)
- * bytes); rows == 0 writes zeros to it. */
+ * bytes); rows == 0 writes zeros to it.  dx may be dy or dh. */
 int lrq_rms_norm_bwd(const void* dy, int64_t lddy, const void* dh, int64_t lddh, const void* h, int64_t ldh, int32_t dtype,
                      const void* w, int32_t w_dtype, const float* rstd, int64_t rows, int64_t n, void* dx, int64_t lddx,
                      void* dw, void* workspace, int64_t workspace_bytes, void* stream);

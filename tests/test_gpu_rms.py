@@ -306,3 +306,28 @@ def test_captured_step(pkg, AG):
         got = [t.clone() for t in out]
         for a, b in zip(got, step(x, res, dy)):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("n", [100, 512, 5003, 9000, 20000])
+def test_outputs_over_inputs(pkg, n, dtype):
+    """Through the C ABI h may take the place of x or the residual, and dx that of dy or dh."""
+    L = importlib.import_module("triton-kernel-test_amd._lib")
+    rows, dt = 70, {BF: L.LRQ_BF16, F32: L.LRQ_F32}[dtype]
+    x, res, w, dh, dy = _r(rows, n, dtype), _r(rows, n, dtype, 1), _w(n, BF), _r(rows, n, dtype, 2), _r(rows, n, dtype, 3)
+    y, h, rstd = pkg.add_rms_norm_forward(x, res, w, EPS)
+    dx, dw = pkg.rms_norm_backward(dy, h, w, rstd, dh)
+    stream = torch.cuda.current_stream().cuda_stream
+    for over in range(2):
+        a, b, y2, r2 = x.clone(), res.clone(), torch.empty_like(x), torch.empty_like(rstd)
+        h2 = (a, b)[over]
+        L.call("lrq_rms_norm_fwd", a.data_ptr(), n, b.data_ptr(), n, dt, w.data_ptr(), L.LRQ_BF16, rows, n, EPS, h2.data_ptr(),
+               n, y2.data_ptr(), n, None, r2.data_ptr(), stream)
+        assert torch.equal(h2, h) and torch.equal(y2, y) and torch.equal(r2, rstd)
+        a, b, dw2 = dy.clone(), dh.clone(), torch.empty_like(dw)
+        size = L.call_raw("lrq_rms_norm_bwd_workspace", rows, n)
+        ws = torch.empty(size // 4, device="cuda")
+        dx2 = (a, b)[over]
+        L.call("lrq_rms_norm_bwd", a.data_ptr(), n, b.data_ptr(), n, h.data_ptr(), n, dt, w.data_ptr(), L.LRQ_BF16,
+               rstd.data_ptr(), rows, n, dx2.data_ptr(), n, dw2.data_ptr(), ws.data_ptr(), size, stream)
+        assert torch.equal(dx2, dx) and torch.equal(dw2, dw)

@@ -1,4 +1,5 @@
-// e4m3 quantise and dequantise (format: lrq_fp8.h).
+// e4m3 quantise and dequantise (format: lrq_fp8.h).  All are one pass and bound by memory: bf16 [14336, 4096] (176 MB read and
+// written) 28.6 us by rows, 27.6 by squares, 29.3 transposed, 27.8 back, 6.0 to 6.4 TB/s; [512, 4096] 3.4 to 4.4, about a launch.
 #include "lrq_fp8.h"
 
 namespace lrq {
@@ -57,8 +58,8 @@ __global__ __launch_bounds__(256) void k_fp8_square(const char* x, int64_t ldx, 
 
 // Blocks of 128 columns of the transpose's rows: 128 rows by 64 columns of x a workgroup.  Thread (g, c) holds columns 8 c ..
 // + 7 of rows 4 g .. + 3: four codes of a column are a dword of the output row, which passes through LDS to leave in
-// 16-byte pieces.  LDS row r (a column of x) keeps its dword d in slot d ^ 4 (r / 8): eight lanes of a write, one chunk
-// each, fall in different banks.
+// 16-byte pieces (a plain store would write 4 bytes of a row at a time).  LDS row r (a column of x) keeps its dword d in slot
+// d ^ 4 (r / 8): eight lanes of a write, one chunk each, fall in different banks.
 template <int DT>
 __global__ __launch_bounds__(256) void k_fp8_transpose(const char* x, int64_t ldx, Fp8 q) {
   constexpr int ES = Elem<DT>::kBytes;

@@ -192,7 +192,7 @@ def fp8_quantize(x: torch.Tensor, block: int = 1, transpose: bool = False) -> FP
 
 
 def fp8_dequantize(q: FP8Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """The values of q (exact in bf16 and fp32)."""
+    """The values of q, rounded to dtype (exact in fp32, and in bf16 but for its subnormal numbers)."""
     t = q.descriptor()
     out = (q._codes if q._buf is None else q._buf).new_empty(q.shape, dtype=dtype)
     with _on(q.device):
