@@ -19,11 +19,11 @@ def _lds(dests, low, high, what):
     assert all(a[1] <= b[0] for a, b in zip(spans, spans[1:])), f"{what}: two loads write the same bytes"
 
 
-TILES = [(1, 4), (2, 2), (2, 4), (3, 4), (4, 4)]  # 64 mt rows by 64 nb columns
+TILES = [(1, 2), (1, 4), (2, 2), (2, 4), (3, 4), (4, 4)]  # 64 mt rows by 64 nb columns
 
 
 def _deep(mt, nb):
-    return (160 * 1024 - 4096) // (64 * (mt + nb) * 128)
+    return min(4, (160 * 1024 - 2 * 2048) // (64 * (mt + nb) * 128))
 
 
 def _runs(steps, splits):
@@ -92,18 +92,11 @@ def test_tile(m, n, k, mt, nb, nn):
                                 _inside((128 * step + row) * ldw + n0 + ow, 16, n * ldw, "W codes")
                         dest += [(kx + 1024 * v, 1024) for v in np.unique(klw * WAVE + i)]
                     _lds(dest, kx, stage, "W")
-                    # scales: group g in slot (g - first / 4) % 2; every step's are loaded ahead of it
+                    # scales: group g in slot (g - first / 4) % 2
                     part = np.minimum(WAVE, mt - 1)
                     wpart = WAVE if nn else np.minimum(WAVE, nb - 1)
                     dest = [(ring + 256 * v, 256) for v in np.unique(part)] + [(ring + 1024 + 256 * v, 256) for v in np.unique(wpart)]
                     _lds(dest, ring, ring + 2048, "scales")
-                    slot, held = 0, {0: first // 4}
-                    for step in range(first, last):
-                        assert held[slot] == step // 4
-                        if step % 4 == 0 and step + 4 < last:
-                            held[slot ^ 1] = step // 4 + 1
-                        if step % 4 == 3:
-                            slot ^= 1
                     for g in {first // 4, (last - 1) // 4}:
                         for shift in (0, 7):
                             tall = -(-m // (1 << shift))
@@ -118,6 +111,60 @@ def test_tile(m, n, k, mt, nb, nn):
                             block = np.minimum((n0 + 32 * nb * (WAVE & 1)) // 128, wsteps - 1)
                             row = np.minimum(4 * g + (LANE & 3), steps - 1)
                             _inside(row * ldsw + (block & ~3), 4, wrows * ldsw, "W scales")
+
+
+@pytest.mark.parametrize("mt,nb", TILES)
+@pytest.mark.parametrize("first,steps", [(0, n) for n in (1, 2, 3, 4, 5, 6, 7, 8, 9, 12, 13, 17, 32, 112)] + [(8, 40), (12, 37)])
+def test_order(first, steps, mt, nb):
+    """What is read from LDS has come, and nothing is written over that is still to be read: a wave's loads in their order (they
+    come in in that order), its waits, which leave the newest so many under way, and its reads of each step."""
+    deep, loads = _deep(mt, nb), 2 * (mt + nb)
+    early, last = 3 * loads // 8, steps
+    issued, place, come = [], {}, {}  # loads in order; what a place holds or will hold; which loads are in
+
+    def issue(key, where):
+        issued.append((key, where))
+        place[where] = key
+
+    def wait(newest):
+        for i, (key, where) in enumerate(issued[:len(issued) - newest] if newest else issued):
+            come[where] = key
+
+    def scales(group, slot):
+        for operand in range(2):
+            issue(("scales", group, operand), ("slot", slot, operand))
+
+    def step_in(step, buf):
+        return all(come.get(("buf", buf, i)) == ("step", step, i) == place[("buf", buf, i)] for i in range(loads))
+
+    def scales_in(step, slot):
+        want = [("scales", step // 4, o) for o in range(2)]
+        return all(come.get(("slot", slot, o)) == want[o] == place[("slot", slot, o)] for o in range(2))
+
+    scales(first // 4, 0)
+    for d in range(deep):
+        for i in range(loads):
+            issue(("step", min(first + d, last - 1), i), ("buf", d, i))
+    wait((deep - 1) * loads)
+    assert step_in(first, 0) and scales_in(first, 0)  # half 0's operands are read here
+    buf = slot = 0
+    for step in range(first, last):
+        ahead = min(step + deep, last - 1)
+        assert step_in(step, buf)  # half 1's operands
+        for i in range(early):
+            issue(("step", ahead, i), ("buf", buf, i))
+        wait((deep - 2) * loads + early)
+        following = (buf + 1) % deep
+        if step % 4 == 0 and step + 4 < last:
+            scales(step // 4 + 1, slot ^ 1)
+        for i in range(early, loads):
+            issue(("step", ahead, i), ("buf", buf, i))
+        if step + 1 < last:
+            assert step_in(step + 1, following)  # half 0 of the next step
+        slot ^= step % 4 == 3
+        if step + 1 < last:
+            assert scales_in(step + 1, slot)
+        buf = following
 
 
 def _loads_x(mt):

@@ -250,7 +250,9 @@ struct Tile8Args {
 template <int MT, int NB>
 struct Tile8Lds {
   static constexpr int kX = 64 * MT * 128, kW = 64 * NB * 128, kStage = kX + kW, kScales = 2048;
-  static constexpr int kDeep = (160 * 1024 - 2 * kScales) / kStage, kRing = kDeep * kStage, kLoop = kRing + 2 * kScales;
+  static constexpr int kMost = (160 * 1024 - 2 * kScales) / kStage;
+  static constexpr int kDeep = kMost < 4 ? kMost : 4;  // (64 x 128 tiles six deep: 2 to 15 % slower)
+  static constexpr int kRing = kDeep * kStage, kLoop = kRing + 2 * kScales;
   static constexpr int kOut = 4 * 32 * (128 + 16);  // of the output, in the ring's place
   static_assert(kLoop <= 160 * 1024 && kOut <= kLoop);
 };
@@ -381,6 +383,8 @@ __global__ __launch_bounds__(256, 1) void k_fp8_tile(Tile8Args a) {
   // so 395.  The order is held: the compiler would issue all loads first.
   constexpr int kMfma = NB * MT, kPieces = 2 * (MT + NB), kReads = (kPieces + kMfma / 2 - 1) / (kMfma / 2);
   constexpr int kFirst = 3 * kLoads / 8;  // of a step's loads: behind the second half of half 0's instructions
+  // four steps' scales are issued with half 1 of the first step of the four before, and waited for with its last step's loads
+  static_assert((kDeep - 2) * kLoads + kFirst <= 3 * kLoads);
   f32x16 acc[MT][NB];
 #pragma unroll
   for (int i = 0; i < MT; ++i)
@@ -518,21 +522,21 @@ struct Plan8 {
 static bool few_rows(int64_t rows, int64_t cols, int steps) { return rows <= 16 || (rows <= 32 && (steps <= 64 || cols > 8192)); }
 
 // The tile and how often the contraction is split over workgroups: one workgroup runs on a CU at a time, so a grid takes
-// rounds of its longest split's steps, and every split writes and re-reads fp32 parts.  Times in us, fitted to 281 products
-// measured with every tile and split, half of them by weights that came from memory: a step of each tile; a workgroup's start
-// and end; the share of a full round that a nearly empty one takes, which runs at higher clocks; what a step waits longer for
-// W where few rows of tiles share it; the join's launch, and its time for each element of a part.  The plan taken is within 5 % of
-// the best one in 257 of them (1.3 % longer on average).  128 x 128 tiles are for what does not fill the card with larger ones:
-// 94 x 884 x 10112 8.8 us against 10.4 of 64 x 256, 171 x 10112 x 3183 17.7 against 21.1; they read their operands from the L2
-// more often, 8192^3 takes 540 us.
+// rounds of its longest split's steps, and every split writes and re-reads fp32 parts.  Times in us, fitted to 314 products
+// measured with every tile and split by weights that came from memory: a step of each tile; a workgroup's start and
+// end; the share of a full round that a nearly empty one takes, which runs at higher clocks; what a step waits longer for W
+// where few rows of tiles share it; the join's launch, and its time for each element of a part.  The plan taken is within 5 % of the
+// best one in 295 of them (0.9 % longer on average).  Low tiles are for what does not fill the card with higher ones, by
+// [4096, 4096]: 64 rows 14.2 us against 16.2 of 64 x 256, 256 rows 16.9 against 20.7, 1024 rows 22.8 of 128 x 128 against
+// 30.9 of 128 x 256; they read their operands from the L2s more often, 8192^3 takes 540 us in tiles of 128 x 128.
 static Plan8 plan8(const lrq_fp8* a, const lrq_fp8* b, bool nn) {
   struct Kind {
     int mt, nb;
     double step, fixed, empty;
   };
-  constexpr Kind kKinds[] = {{1, 4, 0.61, 3.9, 0.63}, {2, 2, 0.53, 3.1, 0.7}, {2, 4, 0.76, 7.3, 0.57}, {3, 4, 1.13, 7.9, 0.6},
-                             {4, 4, 1.44, 10.6, 0.5}};
-  constexpr double kAlone = 0.12, kJoin = 3.2, kPart = 1.1e-6;
+  constexpr Kind kKinds[] = {{1, 2, 0.44, 1.9, 0.75}, {1, 4, 0.71, 3.5, 0.47}, {2, 2, 0.58, 3.4, 0.51},
+                             {2, 4, 0.88, 5.5, 0.54}, {3, 4, 1.15, 7.0, 0.57}, {4, 4, 1.33, 9.8, 0.53}};
+  constexpr double kAlone = 0.16, kJoin = 2.75, kPart = 1.04e-6;
   constexpr int kCus = 256;  // a fixed count, so that the workspace and the order of the sums depend on the shape alone
   const int64_t rows = a->rows, cols = nn ? b->cols : b->rows;
   const int steps = (int)((a->cols + 127) / 128);
@@ -542,7 +546,7 @@ static Plan8 plan8(const lrq_fp8* a, const lrq_fp8* b, bool nn) {
   for (const Kind& k : kKinds) {
     if (k.mt > 1 && 64 * (k.mt - 1) >= rows) continue;  // part of the tile without a row
     Plan8 p{k.mt, k.nb, (rows + 64 * k.mt - 1) / (64 * k.mt), (cols + 64 * k.nb - 1) / (64 * k.nb), 1, steps};
-    for (; p.splits <= 16 && p.splits <= std::max(1, steps / 4); ++p.splits) {
+    for (; p.splits <= 16 && p.splits <= std::max(1, steps / 6); ++p.splits) {
       const int64_t wgs = p.tiles_m * p.tiles_n * p.splits, over = wgs % kCus;
       const double rounds = (double)(wgs / kCus) + (over == 0 ? 0. : k.empty + (1. - k.empty) * (double)over / kCus);
       const int run = std::min(steps, 4 * (((steps + 3) / 4 + p.splits - 1) / p.splits));
@@ -646,7 +650,8 @@ static int fp8_product(const lrq_fp8* ta, const lrq_fp8* tb, bool nn, void* out,
   else if (p.mt == 3) LRQ_TRY(with(integral_constant<int, 3>{}, integral_constant<int, 4>{}));
   else if (p.mt == 2 && p.nb == 4) LRQ_TRY(with(integral_constant<int, 2>{}, integral_constant<int, 4>{}));
   else if (p.mt == 2) LRQ_TRY(with(integral_constant<int, 2>{}, integral_constant<int, 2>{}));
-  else LRQ_TRY(with(integral_constant<int, 1>{}, integral_constant<int, 4>{}));
+  else if (p.nb == 4) LRQ_TRY(with(integral_constant<int, 1>{}, integral_constant<int, 4>{}));
+  else LRQ_TRY(with(integral_constant<int, 1>{}, integral_constant<int, 2>{}));
   if (need == 0) return LRQ_OK;
   const dim3 grid((unsigned)std::min<int64_t>((rows * (ldp / 4) + 255) / 256, (int64_t)cu_count() * 32));
   return launch(k_fp8_join, grid, dim3(256), 0, s, (const float*)workspace, p.splits, rows, cols, ldp, out, ldo, odt);
