@@ -19,11 +19,15 @@ def _lds(dests, low, high, what):
     assert all(a[1] <= b[0] for a, b in zip(spans, spans[1:])), f"{what}: two loads write the same bytes"
 
 
-TILES = [(1, 2), (1, 4), (2, 2), (2, 4), (3, 4), (4, 4)]  # 64 mt rows by 64 nb columns
+TILES = [(1, 1), (1, 2), (1, 4), (2, 2), (2, 4), (3, 4), (4, 4)]  # 64 mt rows by 64 nb columns
 
 
 def _deep(mt, nb):
     return min(4, (160 * 1024 - 2 * 2048) // (64 * (mt + nb) * 128))
+
+
+def _turn(r, nb):
+    return (r ^ (r >> 2 & 1)) & 3 if nb == 1 else r & 7
 
 
 def _runs(steps, splits):
@@ -56,7 +60,7 @@ def test_tile(m, n, k, mt, nb, nn):
     ldx, ldw, ldsx, ldsw = 128 * steps, 128 * wsteps, -(-steps // 4) * 4, -(-wsteps // 4) * 4
     kx, stage, ring = _lds_sizes(mt, nb)
     klx, klw = 2 * mt, 2 * nb
-    lanes, even = 4 * nb, 1 if nb == 2 else 2
+    lanes, even = 4 * nb, 1 if nb <= 2 else 2
     each = 64 // lanes
     wrows = -(-n // 128)
     for splits in {min(wanted, max(1, steps // 4)) for wanted in (1, 2, 3, 16)}:  # none without a step
@@ -85,8 +89,9 @@ def test_tile(m, n, k, mt, nb, nn):
                                 _inside(n0 * ldw + 128 * step + ow, 16, n * ldw, "W codes")
                         else:
                             r = 32 * WAVE + each * i + LANE // lanes
-                            ow = np.minimum(16 * ((LANE % lanes) ^ (r & 7)), min(64 * nb, 128 * wsteps - n0) - 16)
-                            assert (((32 * WAVE + each * (i % even) + LANE // lanes) & 7) == (r & 7)).all()  # offset i % even serves
+                            ow = np.minimum(16 * ((LANE % lanes) ^ _turn(r, nb)), min(64 * nb, 128 * wsteps - n0) - 16)
+                            # offset i % even serves
+                            assert (_turn(32 * WAVE + each * (i % even) + LANE // lanes, nb) == _turn(r, nb)).all()
                             for step in (first, last - 1):
                                 row = np.minimum(r, n - 1 - 128 * step)
                                 _inside((128 * step + row) * ldw + n0 + ow, 16, n * ldw, "W codes")
@@ -197,7 +202,7 @@ def test_reads_of_rows(mt):
                 assert all(len(set(banks[16 * g:16 * g + 16])) == 16 for g in range(4))
 
 
-@pytest.mark.parametrize("nb", [2, 4])
+@pytest.mark.parametrize("nb", [1, 2, 4])
 def test_reads_of_columns(nb):
     """NN: the transposing read of lane (c, h), half Q, piece q, gives bytes of column 32 t + c in rows 64 Q + 32 h + 16 q ..
     + 15, in the order in which X's operand has them."""
@@ -207,7 +212,7 @@ def test_reads_of_columns(nb):
         for i in range(2 * nb):
             r = 32 * wave + 64 // lanes * i + LANE // lanes
             for b in range(16):
-                image[1024 * (2 * nb * wave + i) + 16 * LANE + b] = np.stack([r, 16 * ((LANE % lanes) ^ (r & 7)) + b], 1)
+                image[1024 * (2 * nb * wave + i) + 16 * LANE + b] = np.stack([r, 16 * ((LANE % lanes) ^ _turn(r, nb)) + b], 1)
     assert (image >= 0).all()
     for wn in range(2):
         for t in range(nb):
@@ -215,7 +220,7 @@ def test_reads_of_columns(nb):
                 for q in range(2):
                     r = 64 * half + 32 * (LANE >> 5) + 16 * q + (LANE >> 1 & 7)
                     piece = 2 * nb * wn + 2 * t + (LANE >> 4 & 1)
-                    p = 64 * nb * r + 16 * (piece ^ (r & 7)) + 8 * (LANE & 1)
+                    p = 64 * nb * r + 16 * (piece ^ _turn(r, nb)) + 8 * (LANE & 1)
                     for second in range(2):
                         at = p + 8 * 64 * nb * second
                         for lane in range(64):

@@ -136,10 +136,11 @@ def test_gemm_nn(pkg, m, k, n, ba):
         assert_within(pkg.fp8_linear_backward(a, b, dtype), ref, bound, f"{m}x{n}x{k} {dtype}")
 
 
-# depth by columns: what each tile is chosen for (64 x 128 split and not, 64 x 256, 128 x 128 and split, 128 x 256, 192 x 256,
-# 256 x 256)
-@pytest.mark.parametrize("m,depth,cols", [(90, 4000, 256), (129, 1100, 2100), (50, 256, 40001), (400, 300, 5100), (500, 5000, 1300),
-                                          (700, 256, 6001), (1500, 300, 11000), (2000, 300, 8100)])
+# depth by columns: what each tile is chosen for, 64 x 64 (split, and not), 64 x 128, 64 x 256, 128 x 128, 128 x 256, 192 x 256,
+# 256 x 256
+@pytest.mark.parametrize("m,depth,cols", [(60, 2500, 700), (129, 1100, 2100), (60, 7000, 4100), (90, 5000, 2501), (130, 300, 6001),
+                                          (50, 256, 40001), (400, 300, 5100), (90, 7000, 4100), (700, 256, 6001),
+                                          (1500, 300, 11000), (2000, 300, 8100)])
 @pytest.mark.parametrize("nn", [False, True])
 def test_every_tile(pkg, m, depth, cols, nn):
     a = pkg.fp8_quantize(_x(m, depth, BF))

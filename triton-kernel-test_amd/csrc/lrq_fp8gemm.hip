@@ -245,8 +245,8 @@ struct Tile8Args {
 // which the last is half empty, 197.
 //
 // LDS: X and (NN false) W have rows of 128 bytes, row r's 16-byte piece p in slot p ^ (r / 2 % 8): 16 lanes of a read cover
-// all banks.  NN: 128 rows of W of 64 NB bytes, piece p of row r in slot p ^ (r % 8); the transposing read gives a lane its
-// column of 8 rows.
+// all banks.  NN: 128 rows of W of 64 NB bytes, piece p of row r in slot p ^ (r % 8) (NB 1, four pieces: p ^ r % 4 ^ r / 4 %
+// 2); the transposing read gives a lane its column of 8 rows.
 template <int MT, int NB>
 struct Tile8Lds {
   static constexpr int kX = 64 * MT * 128, kW = 64 * NB * 128, kStage = kX + kW, kScales = 2048;
@@ -281,7 +281,8 @@ __global__ __launch_bounds__(256, 1) void k_fp8_tile(Tile8Args a) {
   // ---- loads of 1 KB: 8 rows of 128 bytes (NN W: 16 / NB rows of 64 NB), at 32-bit offsets from a tile's first row
   const uint32_t sm0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)sm;
   // NN: row rw + kRows i of a step; its piece depends on the row's last three bits, so on i % 2 at most
-  constexpr int kLanes = 4 * NB, kRows = 64 / kLanes, kEven = kRows == 8 ? 1 : 2;
+  constexpr int kLanes = 4 * NB, kRows = 64 / kLanes, kEven = kRows >= 8 ? 1 : 2;
+  const auto turn = [](int r) { return NB == 1 ? (r ^ (r >> 2 & 1)) & 3 : r & 7; };
   const int rw = 32 * wave + lane / kLanes;
   struct {
     const uint8_t *x, *w;
@@ -309,7 +310,7 @@ __global__ __launch_bounds__(256, 1) void k_fp8_tile(Tile8Args a) {
   } else {
     const uint32_t mw = min(64u * NB, 128u * (uint32_t)a.w.steps - n0) - 16;
 #pragma unroll
-    for (int i = 0; i < kEven; ++i) ow[i] = min((uint32_t)(16 * ((lane % kLanes) ^ ((rw + kRows * i) & 7))), mw);
+    for (int i = 0; i < kEven; ++i) ow[i] = min((uint32_t)(16 * ((lane % kLanes) ^ turn(rw + kRows * i))), mw);
   }
   // load i of the step
   const auto issue = [&](int buf, int i) {
@@ -354,7 +355,7 @@ __global__ __launch_bounds__(256, 1) void k_fp8_tile(Tile8Args a) {
     } else {
       const int r = 64 * half + 32 * h + 16 * q + (lane >> 1 & 7), piece = 2 * NB * wn + 2 * t + (lane >> 4 & 1);
       typedef int i32x2 __attribute__((ext_vector_type(2)));
-      const auto p = (__attribute__((address_space(3))) i32x2*)(st + 64 * NB * r + 16 * (piece ^ (r & 7)) + 8 * (lane & 1));
+      const auto p = (__attribute__((address_space(3))) i32x2*)(st + 64 * NB * r + 16 * (piece ^ turn(r)) + 8 * (lane & 1));
       const i32x2 lo = __builtin_amdgcn_ds_read_tr8_b64_v2i32(p), hi = __builtin_amdgcn_ds_read_tr8_b64_v2i32(p + 64 * NB);
       fw[half][t].v[q] = u32x4{(uint32_t)lo[0], (uint32_t)lo[1], (uint32_t)hi[0], (uint32_t)hi[1]};
     }
@@ -381,7 +382,7 @@ __global__ __launch_bounds__(256, 1) void k_fp8_tile(Tile8Args a) {
   // and before half 1, when the next step's loads are in.  The loads go out evenly over the rest of the step: they are
   // 16 TB/s of the L2s' at full speed, and 1.5 to 2 at a time 8192^3 took 440 us, at 1 behind each instruction of half 1 404,
   // so 395.  The order is held: the compiler would issue all loads first.
-  constexpr int kMfma = NB * MT, kPieces = 2 * (MT + NB), kReads = (kPieces + kMfma / 2 - 1) / (kMfma / 2);
+  constexpr int kMfma = NB * MT, kHalf = (kMfma + 1) / 2, kPieces = 2 * (MT + NB), kReads = (kPieces + kHalf - 1) / kHalf;
   constexpr int kFirst = 3 * kLoads / 8;  // of a step's loads: behind the second half of half 0's instructions
   // four steps' scales are issued with half 1 of the first step of the four before, and waited for with its last step's loads
   static_assert((kDeep - 2) * kLoads + kFirst <= 3 * kLoads);
@@ -424,7 +425,7 @@ __global__ __launch_bounds__(256, 1) void k_fp8_tile(Tile8Args a) {
         if (late == 0) lds_meet();
 #pragma unroll
         for (int l = 0; l < kFirst; ++l)
-          if (l * (kMfma / 2) / kFirst == late) issue(buf, l);
+          if (l * kHalf / kFirst == late) issue(buf, l);
         __builtin_amdgcn_sched_barrier(0);
       }
       __builtin_amdgcn_s_waitcnt(vmcnt_imm((kDeep - 2) * kLoads + kFirst));
@@ -455,7 +456,7 @@ __global__ __launch_bounds__(256, 1) void k_fp8_tile(Tile8Args a) {
 
   // Out through LDS, 32 rows by 128 bytes of the wave's columns at a time: a lane has four neighbouring columns of one row,
   // and leaves with 16 bytes beside its neighbours'.
-  constexpr int ES = Elem<OT>::kBytes, kPitch = 128 + 16, kWide = 16 / ES, kCols = 128 / ES, kTs = kCols / 32;
+  constexpr int ES = Elem<OT>::kBytes, kPitch = 128 + 16, kWide = 16 / ES, kTs = NB * ES < 4 ? NB : 4 / ES;
   char* mine = sm + wave * 32 * kPitch;
   char* out = (char*)a.out + (a.splits > 1 ? (int64_t)z * a.x.rows * a.ldo * 4 : 0);
 #pragma unroll
@@ -464,7 +465,7 @@ __global__ __launch_bounds__(256, 1) void k_fp8_tile(Tile8Args a) {
 #pragma unroll
     for (int t0 = 0; t0 < NB; t0 += kTs) {
       const int64_t n = (int64_t)n0 + 32 * NB * wn + 32 * t0 + kWide * (lane % 8);
-      const int valid = (int)min((int64_t)kWide, a.cols - n);
+      const int valid = kWide * (lane % 8) < 32 * kTs ? (int)min((int64_t)kWide, a.cols - n) : 0;
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int t = t0; t < t0 + kTs; ++t) {
@@ -522,21 +523,23 @@ struct Plan8 {
 static bool few_rows(int64_t rows, int64_t cols, int steps) { return rows <= 16 || (rows <= 32 && (steps <= 64 || cols > 8192)); }
 
 // The tile and how often the contraction is split over workgroups: one workgroup runs on a CU at a time, so a grid takes
-// rounds of its longest split's steps, and every split writes and re-reads fp32 parts.  Times in us, fitted to 314 products
+// rounds of its longest split's steps, and every split writes and re-reads fp32 parts.  Times in us, fitted to 326 products
 // measured with every tile and split by weights that came from memory: a step of each tile; a workgroup's start and
 // end; the share of a full round that a nearly empty one takes, which runs at higher clocks; what a step waits longer for W
-// where few rows of tiles share it; the join's launch, and its time for each element of a part.  The plan taken is within 5 % of the
-// best one in 295 of them (0.9 % longer on average).  Low tiles are for what does not fill the card with higher ones, by
-// [4096, 4096]: 64 rows 14.2 us against 16.2 of 64 x 256, 256 rows 16.9 against 20.7, 1024 rows 22.8 of 128 x 128 against
-// 30.9 of 128 x 256; they read their operands from the L2s more often, 8192^3 takes 540 us in tiles of 128 x 128.
+// where few rows of tiles share it; the join's launch, and its time for each element of a part.  The plan taken is within 5 %
+// of the best one in 302 of them (1 % longer on average).  Small tiles are for what does not fill the card with larger ones: 64
+// rows by [4096, 4096] 12.5 us in tiles of 64 x 64, 14.1 of 64 x 128 and 16.2 of 64 x 256, 256 rows 14.7, 16.9 and 20.7 (19.2 of
+// 128 x 128), 1024 rows 22.8 of 128 x 128 against 30.9 of 128 x 256; they read their operands from the L2s more often, 8192^3
+// takes 540 us in tiles of 128 x 128.
 static Plan8 plan8(const lrq_fp8* a, const lrq_fp8* b, bool nn) {
   struct Kind {
     int mt, nb;
     double step, fixed, empty;
   };
-  constexpr Kind kKinds[] = {{1, 2, 0.44, 1.9, 0.75}, {1, 4, 0.71, 3.5, 0.47}, {2, 2, 0.58, 3.4, 0.51},
-                             {2, 4, 0.88, 5.5, 0.54}, {3, 4, 1.15, 7.0, 0.57}, {4, 4, 1.33, 9.8, 0.53}};
-  constexpr double kAlone = 0.16, kJoin = 2.75, kPart = 1.04e-6;
+  constexpr Kind kKinds[] = {{1, 1, 0.26, 0.9, 0.76}, {1, 2, 0.47, 2.0, 0.58}, {1, 4, 0.71, 3.4, 0.45}, {2, 2, 0.56, 3.1, 0.61},
+                             {2, 4, 0.90, 4.8, 0.56}, {3, 4, 1.18, 7.3, 0.52}, {4, 4, 1.36, 10.5, 0.46}};
+  constexpr double kHalves = 0.07;  // longer is a step of dy w by 64 columns, which reads half cache lines of W
+  constexpr double kAlone = 0.19, kJoin = 3.1, kPart = 0.9e-6;
   constexpr int kCus = 256;  // a fixed count, so that the workspace and the order of the sums depend on the shape alone
   const int64_t rows = a->rows, cols = nn ? b->cols : b->rows;
   const int steps = (int)((a->cols + 127) / 128);
@@ -550,7 +553,8 @@ static Plan8 plan8(const lrq_fp8* a, const lrq_fp8* b, bool nn) {
       const int64_t wgs = p.tiles_m * p.tiles_n * p.splits, over = wgs % kCus;
       const double rounds = (double)(wgs / kCus) + (over == 0 ? 0. : k.empty + (1. - k.empty) * (double)over / kCus);
       const int run = std::min(steps, 4 * (((steps + 3) / 4 + p.splits - 1) / p.splits));
-      const double cost = rounds * (run * (k.step + kAlone * k.nb / p.tiles_m) + k.fixed) +
+      const double step = k.step + kAlone * k.nb / p.tiles_m + (nn && k.nb == 1 ? kHalves : 0.);
+      const double cost = rounds * (run * step + k.fixed) +
                           (p.splits > 1 ? kJoin + kPart * p.splits * rows * cols : 0.);
       if (best.mt == 0 || cost < least) best = p, least = cost;
     }
@@ -651,6 +655,7 @@ static int fp8_product(const lrq_fp8* ta, const lrq_fp8* tb, bool nn, void* out,
   else if (p.mt == 2 && p.nb == 4) LRQ_TRY(with(integral_constant<int, 2>{}, integral_constant<int, 4>{}));
   else if (p.mt == 2) LRQ_TRY(with(integral_constant<int, 2>{}, integral_constant<int, 2>{}));
   else if (p.nb == 4) LRQ_TRY(with(integral_constant<int, 1>{}, integral_constant<int, 4>{}));
+  else if (p.nb == 1) LRQ_TRY(with(integral_constant<int, 1>{}, integral_constant<int, 1>{}));
   else LRQ_TRY(with(integral_constant<int, 1>{}, integral_constant<int, 2>{}));
   if (need == 0) return LRQ_OK;
   const dim3 grid((unsigned)std::min<int64_t>((rows * (ldp / 4) + 255) / 256, (int64_t)cu_count() * 32));
