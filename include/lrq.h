@@ -478,6 +478,14 @@ int lrq_fp8_gemm_nn(const lrq_fp8* a, const lrq_fp8* b, void* out, int64_t ldo, 
 /* Workspace bytes (>= 0) of lrq_fp8_gemm (nn == 0) or lrq_fp8_gemm_nn, or a negative LRQ_ERR_*.  Host only. */
 int64_t lrq_fp8_gemm_workspace(const lrq_fp8* a, const lrq_fp8* b, int32_t nn);
 
+/* lrq_fp8_quantize of x (blocks of 1 x 128) and lrq_fp8_gemm (nn == 0, x[rows, w.cols]) or lrq_fp8_gemm_nn (x[rows, w.rows]) of
+ * that by w, in one call.  `workspace` (16-byte aligned, lrq_fp8_quantize_gemm_workspace bytes) holds the quantised x too. */
+int lrq_fp8_quantize_gemm(const void* x, int64_t ldx, int32_t dtype, int64_t rows, const lrq_fp8* w, int32_t nn, void* out,
+                          int64_t ldo, int32_t out_dtype, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Workspace bytes (>= 0) of lrq_fp8_quantize_gemm, or a negative LRQ_ERR_*.  Host only. */
+int64_t lrq_fp8_quantize_gemm_workspace(int64_t rows, const lrq_fp8* w, int32_t nn);
+
 /* lrq_fp8_gemm with a = x[rows, w.cols] of bf16 or fp16 quantised on the way (blocks of 1 x 128), for at most
  * LRQ_FP8_LINEAR_ROWS rows; w.cols a multiple of 8. */
 #define LRQ_FP8_LINEAR_ROWS 4

@@ -112,6 +112,36 @@ def test_workspace(L):
     assert L.call_raw("lrq_fp8_gemm_workspace", b(big), b(big), 0) == 0
 
 
+@pytest.mark.parametrize("nn", [0, 1])
+def test_quantize_gemm(L, nn):
+    b = ctypes.byref
+    w = _t(L, rows=384, block=128)
+    depth, cols = (384, 256) if nn else (256, 384)
+    n = L.call_raw("lrq_fp8_quantize_gemm_workspace", 20, b(w), nn)
+    assert n >= 20 * (depth + 4)
+
+    def go(**kw):
+        a = dict(x=P, ldx=depth, dt=0, rows=20, w=b(w), nn=nn, out=Q, ldo=cols, odt=0, ws=R_, n=n)
+        a.update(kw)
+        return L.call_raw("lrq_fp8_quantize_gemm", *a.values(), None)
+    for kw, code in ((dict(x=None), "NULL"), (dict(out=None), "NULL"), (dict(ws=None), "NULL"), (dict(w=None), "NULL"),
+                     (dict(ldx=depth - 1), "SHAPE"), (dict(ldo=cols - 1), "SHAPE"), (dict(rows=-1), "SHAPE"),
+                     (dict(rows=1 << 31), "SHAPE"), (dict(dt=3), "UNSUPPORTED"), (dict(odt=3), "UNSUPPORTED"),
+                     (dict(x=ctypes.c_void_p(0x10001)), "ALIGN"), (dict(ws=ctypes.c_void_p(0x20008)), "ALIGN"),
+                     (dict(n=n - 1), "WORKSPACE"), (dict(w=b(_t(L, rows=384, block=128, ld_codes=1 << 24))), "SHAPE")):
+        assert go(**kw) == getattr(L, "LRQ_ERR_" + code), kw
+    assert go(rows=0, ws=None) == 0
+    assert L.call_raw("lrq_fp8_quantize_gemm_workspace", 0, b(w), nn) == 0
+    rows = b(_t(L, rows=384))
+    assert L.call_raw("lrq_fp8_quantize_gemm_workspace", 4, rows, 1) == L.LRQ_ERR_UNSUPPORTED
+    none = b(_t(L, rows=0, block=128))
+    assert L.call_raw("lrq_fp8_quantize_gemm_workspace", 4, none, 1) == L.LRQ_ERR_SHAPE
+    assert L.call_raw("lrq_fp8_quantize_gemm_workspace", 4, none, 0) == 4 * (256 + 4)
+    deep = _t(L, rows=64, cols=16384, ld_codes=16384, ld_scales=128, block=128)
+    parts = L.call_raw("lrq_fp8_gemm_workspace", b(_t(L, rows=100, cols=16384, ld_codes=16384, ld_scales=128)), b(deep), 0)
+    assert L.call_raw("lrq_fp8_quantize_gemm_workspace", 100, b(deep), 0) == parts + 100 * (16384 + 128) > 100 * (16384 + 128)
+
+
 def _fwd(L, **kw):
     a = dict(x=P, ldx=8, res=None, ldr=0, dt=0, w=Q, wdt=0, rows=4, n=8, eps=1e-6, h=None, ldh=0, y=R_, ldy=8, q=None, rstd=T_)
     a.update(kw)

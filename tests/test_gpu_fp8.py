@@ -322,6 +322,20 @@ def test_offsets_past_32_bits(pkg):
     assert torch.equal(big.codes[-300:].view(torch.uint8), q.codes.view(torch.uint8))
 
 
+@pytest.mark.parametrize("dtype", [BF, F16, F32], ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("m,n,k", [(5, 300, 1001), (40, 200, 4000), (300, 700, 520), (37, 4096, 512)])
+def test_one_call_is_two(pkg, m, n, k, dtype):
+    """Rows quantised and multiplied in one call, either way, their rows apart too: the bits of two calls."""
+    w = pkg.fp8_quantize(_x(n, k, F32, 1, 0.02), 128)
+    for f, cols in ((pkg.fp8_linear, k), (pkg.fp8_linear_backward, n)):
+        x = _x(m, cols, dtype, 2)
+        want = f(pkg.fp8_quantize(x), w, F32)
+        apart = torch.full((m, cols + 5), float("nan"), dtype=dtype, device="cuda")
+        apart[:, 3:3 + cols] = x
+        assert torch.equal(f(x, w, F32), want) and torch.equal(f(apart[:, 3:3 + cols], w, F32), want)
+        assert torch.equal(f(x[:, None], w, F32)[:, 0], want)
+
+
 # ---------------------------------------------------------------- autograd
 @pytest.fixture(scope="module")
 def AG(pkg):
