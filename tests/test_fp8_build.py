@@ -41,7 +41,7 @@ def test_no_kernel_spills(tmp_path):
             name = re.search(r"\.symbol:\s+'?(\S+?)\.kd", kernel).group(1)
             if re.search(r"k_(rms|fp8)_", name):
                 seen[name] = (get("vgpr_spill_count"), get("sgpr_spill_count"), get("private_segment_fixed_size"))
-    for stem, least in (("k_rms_fwd", 54), ("k_rms_bwd", 26), ("k_fp8_tile", 24), ("k_fp8_token", 12), ("k_fp8_rows", 3)):
+    for stem, least in (("k_rms_fwd", 54), ("k_rms_bwd", 26), ("k_fp8_tile", 42), ("k_fp8_token", 11), ("k_fp8_rows", 3)):
         assert sum(stem in n for n in seen) >= least, (stem, sum(stem in n for n in seen))
     bad = {n: v for n, v in seen.items() if v != (0, 0, 0)}
     assert not bad, bad

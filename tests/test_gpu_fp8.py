@@ -140,7 +140,7 @@ def test_gemm_nn(pkg, m, k, n, ba):
 # 256 x 256
 @pytest.mark.parametrize("m,depth,cols", [(60, 2500, 700), (129, 1100, 2100), (60, 7000, 4100), (90, 5000, 2501), (130, 300, 6001),
                                           (50, 256, 40001), (400, 300, 5100), (90, 7000, 4100), (700, 256, 6001),
-                                          (1500, 300, 11000), (2000, 300, 8100)])
+                                          (1500, 300, 11000), (2000, 300, 8100), (20, 5300, 700), (30, 256, 9000)])
 @pytest.mark.parametrize("nn", [False, True])
 def test_every_tile(pkg, m, depth, cols, nn):
     a = pkg.fp8_quantize(_x(m, depth, BF))

@@ -79,8 +79,8 @@ typedef uint32_t u32_byte __attribute__((aligned(1)));
 
 // Up to 16 TM rows of X by `own` rows of W (16 TN at most) a workgroup; its waves take runs of the K steps, D of them with all
 // loads in flight at once, and join in LDS.  Bound by W's bytes, which are read once, past the caches: one row by
-// [14336, 4096] from memory 13.6 to 15.8 us (4.3 to 3.7 TB/s), by [4096, 4096] 5.2 to 6.8, by [5120, 5120] 8.9 to 10.5; 32
-// rows by the first 19 to 20.  W is the instruction's first operand, so that a lane ends with four neighbouring outputs of one
+// [14336, 4096] from memory 13.6 to 15.8 us (4.3 to 3.7 TB/s), by [4096, 4096] 5.2 to 6.8, by [5120, 5120] 8.9 to 10.5;
+// 32 rows by the second 9.7.  W is the instruction's first operand, so that a lane ends with four neighbouring outputs of one
 // row of X.  Lane (j, g) holds pieces g and g + 4 of row j's 128 bytes (any order of K serves that both operands share): each
 // load of W takes 64 neighbouring bytes of 16 rows.
 //
@@ -519,19 +519,20 @@ struct Plan8 {
   int splits, steps;
 };
 
-// Rows that the few-row kernel takes: 16, and up to 32 except by few long rows of W (32 rows by [4096, 4096] 9.7 us and by
-// [14336, 4096] 19.3 against 13.9 and 20.0 in tiles, but by [4096, 14336] 26.7 against 20.5).
-static bool few_rows(int64_t rows, int64_t cols, int steps) { return rows <= 16 || (rows <= 32 && (steps <= 64 || cols > 8192)); }
+// Rows that the few-row kernel takes: 16, and up to 32 by a W that is neither tall nor wide, of which no workgroup has much
+// to read while it reads X again (from memory, 32 rows by [4096, 4096] 9.9 us against 11.8 in tiles, by [5120, 5120] 14.2 and
+// 14.3, but by [4096, 8192] 17.0 and 14.2, by [14336, 4096] 20.1 and 17.5; 16 rows by that 17.3 and 17.4).
+static bool few_rows(int64_t rows, int64_t cols, int steps) { return rows <= 16 || (rows <= 32 && steps <= 40 && cols <= 8192); }
 
 // The tile and how often the contraction is split over workgroups: one workgroup runs on a CU at a time, so a grid takes
 // rounds of its longest split's steps, and every split writes and re-reads fp32 parts.  Times in us, fitted to 380 products
 // measured with every tile and split by weights that came from memory: a step of each tile; a workgroup's start and
 // end; the share of a full round that a nearly empty one takes, which runs at higher clocks; what a step waits longer for W
-// where few rows of tiles share it; the join's launch, and its time for each element of a part, longer past what the L2s hold.  The
-// plan taken is within 5 % of the best one in 347 of them (1.1 % longer on average).  Small tiles are for what does not fill the card with larger ones: 64
-// rows by [4096, 4096] 12.5 us in tiles of 64 x 64, 14.1 of 64 x 128 and 16.2 of 64 x 256, 256 rows 14.7, 16.9 and 20.7 (19.2 of
-// 128 x 128), 1024 rows 22.8 of 128 x 128 against 30.9 of 128 x 256; they read their operands from the L2s more often, 8192^3
-// takes 540 us in tiles of 128 x 128.
+// where few rows of tiles share it; the join's launch, and its time for each element of a part, longer past what the L2s
+// hold.  The plan taken is within 5 % of the best one in 347 of them (1.1 % longer on average).  Small tiles are for what does
+// not fill the card with larger ones: 64 rows by [4096, 4096] 12.5 us in tiles of 64 x 64, 14.1 of 64 x 128 and 16.2 of 64 x
+// 256, 256 rows 14.7, 16.9 and 20.7 (19.2 of 128 x 128), 1024 rows 22.8 of 128 x 128 against 30.9 of 128 x 256; they read
+// their operands from the L2s more often, 8192^3 takes 540 us in tiles of 128 x 128.
 static Plan8 plan8(const lrq_fp8* a, const lrq_fp8* b, bool nn) {
   struct Kind {
     int mt, nb;
@@ -605,10 +606,9 @@ static int token(TokenArgs a, hipStream_t s) {
     if (n <= 4096) LRQ_GO(1, 16, 4, 256);
     if (n <= 8192) LRQ_GO(2, 16, 4, 256);
     LRQ_GO(2, 8, 4, 512 * ((n + 16383) / 16384));
-  } else {  // X is read again by every workgroup, at twice the bytes: more rows of W to each
+  } else {  // (8192 columns at most: few_rows)
     if (n <= 4096) LRQ_GO(1, 16, 2, 256);
-    if (n <= 8192) LRQ_GO(2, 16, 2, 256);
-    LRQ_GO(4, 8, 1, 256 * ((n + 16383) / 16384));
+    LRQ_GO(2, 16, 2, 256);
   }
 #undef LRQ_GO
 }
