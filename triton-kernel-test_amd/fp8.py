@@ -207,6 +207,11 @@ def _out_dtype(dtype: torch.dtype) -> int:
     return d
 
 
+def _out(x: torch.Tensor, rows: int, cols: int, dtype: torch.dtype) -> torch.Tensor:
+    """x's leading shape and cols, to be written (sizes one by one: 0.5 us less than a tuple of them)."""
+    return x.new_empty(rows, cols, dtype=dtype) if x.dim() == 2 else x.new_empty(x.shape[:-1] + (cols,), dtype=dtype)
+
+
 def _matrix(w: FP8Tensor, device: torch.device) -> LrqFp8:
     if not isinstance(w, FP8Tensor) or len(w.shape) != 2:
         raise ValueError("the weight must be an FP8Tensor of two dimensions")
@@ -219,7 +224,10 @@ def _product(name: str, a: FP8Tensor, tb: LrqFp8, cols: int, out_dtype, nn: int)
     dt = _out_dtype(out_dtype)
     ta = a.descriptor()
     rows, any_ = ta.rows, a._codes if a._buf is None else a._buf
-    out = any_.new_empty((rows, cols) if len(a.shape) == 2 else a.shape[:-1] + (cols,), dtype=out_dtype)
+    if len(a.shape) == 2:
+        out = any_.new_empty(rows, cols, dtype=out_dtype)
+    else:
+        out = any_.new_empty(a.shape[:-1] + (cols,), dtype=out_dtype)
     device, pa, pb, ws, n = out.device, ctypes.byref(ta), ctypes.byref(tb), None, 0
     if nn or rows > 16:  # (fewer rows split nothing over workgroups)
         n = call_raw("lrq_fp8_gemm_workspace", pa, pb, nn)
@@ -232,14 +240,14 @@ def _product(name: str, a: FP8Tensor, tb: LrqFp8, cols: int, out_dtype, nn: int)
 
 
 def _quantize_product(x: torch.Tensor, name: str, tb: LrqFp8, cols: int, out_dtype, nn: int) -> torch.Tensor:
-    """x quantised and multiplied in one call: of 37 rows 14.8 us of the host, in two 19.1."""
+    """x quantised and multiplied in one call: of 37 rows 14.3 us of the host, in two 18.6."""
     dt, odt = _dtype(x, name), _out_dtype(out_dtype)
     x2, rows, _, ldx = _rows(x, name)
     pb = ctypes.byref(tb)
     n = call_raw("lrq_fp8_quantize_gemm_workspace", rows, pb, nn)
     if n < 0:
         check(n, "lrq_fp8_quantize_gemm_workspace")
-    out = x.new_empty((rows, cols) if x.dim() == 2 else x.shape[:-1] + (cols,), dtype=out_dtype)
+    out = _out(x, rows, cols, out_dtype)
     ws = x.new_empty(n, dtype=torch.uint8)
     with _on(x.device):
         call("lrq_fp8_quantize_gemm", x2.data_ptr(), ldx, dt, rows, pb, nn, out.data_ptr(), cols, odt, ws.data_ptr(), n,
@@ -269,7 +277,7 @@ def fp8_linear(x: Union[torch.Tensor, FP8Tensor], w: FP8Tensor, out_dtype: torch
         return _quantize_product(x, "x", t, t.rows, out_dtype, 0)
     odt = _out_dtype(out_dtype)
     x2, rows, _, ldx = _rows(x, "x")
-    out = x.new_empty(x.shape[:-1] + (t.rows,), dtype=out_dtype)
+    out = _out(x, rows, t.rows, out_dtype)
     with _on(x.device):
         call("lrq_fp8_linear", _p(x2), ldx, dt, rows, ctypes.byref(t), _p(out), t.rows, odt, _stream(x.device))
     return out

@@ -39,7 +39,7 @@ def _forward(x, residual, weight, eps, fp8: bool, add: bool):
     else:
         y = _new(x)
         py, pq = y.data_ptr(), None
-    rstd = x.new_empty((rows,) if x.dim() == 2 else x.shape[:-1], dtype=torch.float32)
+    rstd = x.new_empty(rows if x.dim() == 2 else x.shape[:-1], dtype=torch.float32)  # (an int is 0.8 us less than a shape)
     with _on(device):
         call("lrq_rms_norm_fwd", x2.data_ptr(), ldx, _p(r2), ldr, dt, _p(w), wdt, rows, n, eps, _p(h), n, py, n, pq,
              rstd.data_ptr(), _stream(device))
