@@ -331,3 +331,34 @@ def test_outputs_over_inputs(pkg, n, dtype):
         L.call("lrq_rms_norm_bwd", a.data_ptr(), n, b.data_ptr(), n, h.data_ptr(), n, dt, w.data_ptr(), L.LRQ_BF16,
                rstd.data_ptr(), rows, n, dx2.data_ptr(), n, dw2.data_ptr(), ws.data_ptr(), size, stream)
         assert torch.equal(dx2, dx) and torch.equal(dw2, dw)
+
+
+def test_under_compressed_saved_tensors(pkg, AG):
+    """A norm's rows are kept compressed and decoded for its gradients; a trained product keeps its own 8 bits of x."""
+    def kept(t):
+        return pkg.decode(pkg.encode(t.detach(), None, bits=8, group_size=64))
+
+    x, w, dy = _r(64, 512, BF).requires_grad_(), _w(512, BF).requires_grad_(), _r(64, 512, BF, 2)
+    hooks = AG.compressed_saved_tensors(bits=8, group=64, min_numel=1)
+    with hooks:
+        y = AG.rms_norm(x * 1, w, EPS)
+    assert hooks.stats["compressed"] == 1
+    y.backward(dy)
+    _, rstd = pkg.rms_norm_forward(x.detach(), w.detach(), EPS)
+    for got, want in zip((x.grad, w.grad), pkg.rms_norm_backward(dy, kept(x), w.detach(), rstd)):
+        assert torch.equal(got, want)
+    q, wt = pkg.fp8_quantize(_r(256, 512, BF, 3, 0.05), 128), _r(128, 256, BF, 4, 0.05).requires_grad_()
+    x.grad = w.grad = None
+    hooks = AG.compressed_saved_tensors(bits=8, group=64, min_numel=1)
+    with hooks:
+        y, h = AG.rms_norm_linear(x, w, q, residual=x.detach(), eps=EPS)
+        z = AG.fp8_linear(y, wt)
+    assert hooks.stats["compressed"] == 1  # h
+    dz = _r(64, 128, BF, 5)
+    torch.autograd.backward([z, h], [dz, dy])
+    n8, hh, rstd = pkg.add_rms_norm_forward(x.detach(), x.detach(), w.detach(), EPS, fp8=True)
+    wq = pkg.fp8_quantize(wt.detach(), 128)
+    dn = pkg.fp8_linear_backward(pkg.fp8_linear_backward(dz, wq), q)
+    dx, dw = pkg.rms_norm_backward(dn, kept(hh), w.detach(), rstd, dy)
+    assert torch.equal(x.grad, dx) and torch.equal(w.grad, dw)
+    assert torch.equal(wt.grad, pkg.fp8_weight_gradient(dz, pkg.fp8_linear(n8, q)))
