@@ -461,6 +461,9 @@ typedef struct lrq_fp8 {
  * to the even one.  A block with an infinity or a NaN becomes NaN (scale 255, codes 0). */
 int lrq_fp8_quantize(const void* x, int64_t ldx, int32_t dtype, const lrq_fp8* t, int32_t transpose, void* stream);
 
+/* t = x[rows, cols] and tt = x^T [cols, rows], both of block 1, as two calls of lrq_fp8_quantize would make them. */
+int lrq_fp8_quantize_both(const void* x, int64_t ldx, int32_t dtype, const lrq_fp8* t, const lrq_fp8* tt, void* stream);
+
 /* out[rows, cols] = the values of t, rounded to dtype (exact in fp32, and in bf16 but for its subnormal numbers). */
 int lrq_fp8_dequantize(const lrq_fp8* t, void* out, int64_t ldo, int32_t dtype, void* stream);
 

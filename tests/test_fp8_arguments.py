@@ -112,6 +112,20 @@ def test_workspace(L):
     assert L.call_raw("lrq_fp8_gemm_workspace", b(big), b(big), 0) == 0
 
 
+@pytest.mark.parametrize("change,code", [
+    (dict(x=None), "NULL"), (dict(dt=3), "UNSUPPORTED"), (dict(ldx=255), "SHAPE"), (dict(x=ctypes.c_void_p(0x10001)), "ALIGN"),
+    (dict(t=dict(block=128)), "UNSUPPORTED"), (dict(tt=dict(block=128)), "UNSUPPORTED"), (dict(t=dict(rows=17)), "SHAPE"),
+    (dict(tt=dict(rows=255)), "SHAPE"), (dict(t=dict(codes=None)), "NULL"), (dict(tt=dict(scales=None)), "NULL"),
+    (dict(tt=dict(ld_codes=120)), "SHAPE"), (dict(t=dict(rows=0), tt=dict(cols=0)), "SHAPE"),
+])
+def test_quantize_both(L, change, code):
+    a = dict(x=P, ldx=256, dt=0, t={}, tt={})
+    a.update(change)
+    t, tt = _t(L, **a["t"]), _t(L, **{**dict(rows=256, cols=16), **a["tt"]})
+    got = L.call_raw("lrq_fp8_quantize_both", a["x"], a["ldx"], a["dt"], ctypes.byref(t), ctypes.byref(tt), None)
+    assert got == getattr(L, "LRQ_ERR_" + code)
+
+
 @pytest.mark.parametrize("nn", [0, 1])
 def test_quantize_gemm(L, nn):
     b = ctypes.byref
@@ -197,7 +211,7 @@ def test_rms_workspace(L):
 def test_python_refusals(pkg):
     x = torch.zeros(4, 256, dtype=torch.bfloat16)
     q = pkg.FP8Tensor(torch.zeros(256, 256, dtype=torch.uint8), torch.zeros(2, 4, dtype=torch.uint8), (256, 256), 128)
-    for f in (lambda: pkg.fp8_quantize(x), lambda: pkg.fp8_dequantize(q), lambda: pkg.fp8_linear(x, q),
+    for f in (lambda: pkg.fp8_quantize(x), lambda: pkg.fp8_quantize_both(x), lambda: pkg.fp8_dequantize(q), lambda: pkg.fp8_linear(x, q),
               lambda: pkg.fp8_linear_backward(x, q), lambda: pkg.fp8_weight_gradient(x, x), lambda: pkg.fp8_gemm(q, q),
               lambda: pkg.rms_norm_forward(x), lambda: pkg.add_rms_norm_forward(x, x),
               lambda: pkg.rms_norm_backward(x, x, None, torch.zeros(4)),

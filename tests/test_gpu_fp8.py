@@ -77,6 +77,25 @@ def test_quantize_edges(pkg, dtype):
     assert torch.equal(torch.isnan(d).cpu()[:, :128].any(1), lost[:, :128].any(1)) and not torch.isnan(d[:, 256:]).any()
 
 
+@pytest.mark.parametrize("dtype", [BF, F16, F32], ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("rows,n", [(1, 1), (1, 300), (7, 128), (128, 128), (129, 257), (130, 1000), (300, 127), (257, 5003)])
+def test_quantize_both(pkg, rows, n, dtype):
+    """The bits of two calls, also of rows apart and of blocks with zeros, NaN and infinity."""
+    x = _x(rows, n, dtype)
+    x[0, :min(n, 128)] = 0.0
+    x[rows - 1, n - 1] = float("nan")
+    if rows > 6 and n > 200:
+        x[6, 150] = float("inf")
+        x[:, 199] = 0.0
+    apart = torch.full((rows, n + 3), float("nan"), dtype=dtype, device="cuda")
+    apart[:, 1:1 + n] = x
+    wide = lambda q: q.scales[:, :-(-q.cols // 128)]
+    for t in (x, apart[:, 1:1 + n]):
+        for got, want in zip(pkg.fp8_quantize_both(t), (pkg.fp8_quantize(x), pkg.fp8_quantize(x, transpose=True))):
+            assert got.shape == want.shape and got.block == 1
+            assert torch.equal(got.codes.view(torch.uint8), want.codes.view(torch.uint8)) and torch.equal(wide(got), wide(want))
+
+
 def test_dequantize_every_code(pkg):
     """All 256 codes under small, middle and large scales, NaN scales among them, in blocks of both kinds."""
     codes = torch.arange(256, dtype=torch.uint8).repeat(6, 1).cuda()

@@ -148,6 +148,7 @@ SIGNATURES = {
     "lrq_fp8_gemm": (c_int32, [_E, _E, c_void_p, c_int64, c_int32, c_void_p, c_int64, c_void_p]),
     "lrq_fp8_gemm_nn": (c_int32, [_E, _E, c_void_p, c_int64, c_int32, c_void_p, c_int64, c_void_p]),
     "lrq_fp8_gemm_workspace": (c_int64, [_E, _E, c_int32]),
+    "lrq_fp8_quantize_both": (c_int32, [c_void_p, c_int64, c_int32, _E, _E, c_void_p]),
     "lrq_fp8_quantize_gemm": (c_int32, [c_void_p, c_int64, c_int32, c_int64, _E, c_int32, c_void_p, c_int64, c_int32, c_void_p,
                                         c_int64, c_void_p]),
     "lrq_fp8_quantize_gemm_workspace": (c_int64, [c_int64, _E, c_int32]),

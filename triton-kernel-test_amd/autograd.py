@@ -364,22 +364,23 @@ class _FP8LinearTrained(torch.autograd.Function):
         q = _f8.fp8_quantize(w, 128)
         ctx.shape, ctx.dtype, ctx.w_dtype = q.shape, x.dtype, w.dtype
         ctx.tokens = x.numel() // x.shape[-1] if x.shape[-1] else 0
-        xt = _f8.fp8_quantize(x, transpose=True) if ctx.needs_input_grad[1] and ctx.tokens else None
+        xq, xt = _f8.fp8_quantize_both(x) if ctx.needs_input_grad[1] and ctx.tokens else (x, None)
         ctx.save_for_backward(*((q.codes, q.scales) if ctx.needs_input_grad[0] else (None, None)),
                               *((xt.codes, xt.scales) if xt is not None else (None, None)))
-        return _f8.fp8_linear(x, q, out_dtype)
+        return _f8.fp8_linear(xq, q, out_dtype)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         codes, scales, xc, xs = ctx.saved_tensors
-        dx = dw = None
+        dx = dw = dyt = None
+        if ctx.needs_input_grad[1] and ctx.tokens and dy.numel():
+            dy, dyt = _f8.fp8_quantize_both(dy) if ctx.needs_input_grad[0] else (dy, _f8.fp8_quantize(dy, transpose=True))
         if ctx.needs_input_grad[0]:
             dx = _f8.fp8_linear_backward(dy, _f8.FP8Tensor(codes, scales, ctx.shape, 128), ctx.dtype)
         if ctx.needs_input_grad[1]:
-            if ctx.tokens and dy.numel():
-                dw = _f8.fp8_gemm(_f8.fp8_quantize(dy, transpose=True),
-                                  _f8.FP8Tensor(xc, xs, (ctx.shape[1], ctx.tokens), 1), ctx.w_dtype)
+            if dyt is not None:
+                dw = _f8.fp8_gemm(dyt, _f8.FP8Tensor(xc, xs, (ctx.shape[1], ctx.tokens), 1), ctx.w_dtype)
             else:
                 dw = torch.zeros(ctx.shape, dtype=ctx.w_dtype, device=dy.device)
         return dx, dw, None

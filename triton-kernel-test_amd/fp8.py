@@ -21,7 +21,7 @@ from ._lib import LrqFp8, call, call_raw, check
 from .api import _on, _p, _require_device, _stream
 from .norm import _DTYPE, _dtype, _rows
 
-__all__ = ["FP8Tensor", "fp8_from_parts", "fp8_quantize", "fp8_dequantize", "fp8_gemm", "fp8_linear",
+__all__ = ["FP8Tensor", "fp8_from_parts", "fp8_quantize", "fp8_quantize_both", "fp8_dequantize", "fp8_gemm", "fp8_linear",
            "fp8_linear_backward", "fp8_weight_gradient"]
 
 _BYTES = (torch.uint8, torch.float8_e4m3fn, torch.float8_e8m0fnu)
@@ -189,6 +189,21 @@ def fp8_quantize(x: torch.Tensor, block: int = 1, transpose: bool = False) -> FP
     with _on(x.device):
         call("lrq_fp8_quantize", _p(x2), ldx, dt, ctypes.byref(t), int(transpose), _stream(x.device))
     return q
+
+
+def fp8_quantize_both(x: torch.Tensor) -> tuple[FP8Tensor, FP8Tensor]:
+    """(``fp8_quantize(x)``, ``fp8_quantize(x, transpose=True)``) from one read of x: what a product and its weight's gradient
+    take."""
+    _require_device(x)
+    dt = _dtype(x, "x")
+    x2, rows, n, ldx = _rows(x, "x")
+    if rows == 0:
+        raise ValueError("the transpose of no rows has rows of no elements")
+    q, t = _empty(x, rows, n, x.shape, 1)
+    qt, tt = _empty(x, n, rows, (n, rows), 1)
+    with _on(x.device):
+        call("lrq_fp8_quantize_both", x2.data_ptr(), ldx, dt, ctypes.byref(t), ctypes.byref(tt), _stream(x.device))
+    return q, qt
 
 
 def fp8_dequantize(q: FP8Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
