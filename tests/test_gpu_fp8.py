@@ -438,3 +438,17 @@ def test_no_tokens_no_outputs_one_row(pkg, AG):
     assert torch.equal(y, pkg.fp8_linear(v.detach()[None], q)[0])
     assert torch.equal(v.grad, pkg.fp8_linear_backward(dy, q)[0])
     assert torch.equal(w.grad, pkg.fp8_weight_gradient(dy, v.detach()[None]))
+
+
+def test_trained_on_more_dimensions(pkg, AG):
+    """x [3, 5, K] and a gradient that is not contiguous: as on the rows flattened."""
+    x, w = _x(15, 300, BF), _x(200, 300, BF, 1, 0.02).requires_grad_()
+    dy = _x(200, 15, BF, 2).T
+    flat, deep = x.clone().requires_grad_(), x.reshape(3, 5, 300).clone().requires_grad_()
+    y = AG.fp8_linear(flat, w)
+    gx, gw = torch.autograd.grad(y, (flat, w), dy.contiguous())
+    y3 = AG.fp8_linear(deep, w)
+    gx3, gw3 = torch.autograd.grad(y3, (deep, w), dy.reshape(3, 5, 200))
+    assert torch.equal(y3.reshape(15, 200), y) and torch.equal(gx3.reshape(15, 300), gx) and torch.equal(gw3, gw)
+    assert torch.equal(torch.autograd.grad(AG.fp8_linear(flat, w), w, dy)[0], gw)
+    assert torch.equal(torch.autograd.grad(AG.fp8_linear(flat, w.detach()), flat, dy)[0], gx)
