@@ -54,14 +54,6 @@ __device__ __forceinline__ void ld_to_lds8(const uint8_t* base, uint32_t off, ui
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory");
 }
 
-// The largest of v over the lanes j, j + 16, j + 32, j + 48, in all of them.
-__device__ __forceinline__ uint32_t row_top(uint32_t v) {
-  const auto a = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-  v = max((uint32_t)a[0], (uint32_t)a[1]);
-  const auto b = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-  return max((uint32_t)b[0], (uint32_t)b[1]);
-}
-
 // ---------------------------------------------------------------- few rows
 struct TokenArgs {
   const char* x;  // fp8 codes, or 16-bit elements
