@@ -53,3 +53,27 @@ def test_every_tile_is_run(plans):
         got = plans([(m, cols, depth, nn) for m, depth, cols in _parameters(T.test_every_tile)])
         assert {p[:2] for p in got} - {(0, 0)} == TILES
         assert any(p[2] > 1 for p in got) and any(p[2] == 1 for p in got)
+
+
+def test_the_tiles_run_round(plans):
+    """``test_gpu_fp8_tiles``: each tile, whole and split, either way, takes more steps than its ring holds (4 at most), in one
+    piece also more than the two groups of four whose scales LDS holds; the last group is not whole."""
+    T = importlib.import_module("test_gpu_fp8_tiles")
+    assert {(t, s) for t, s, *_ in T.TILES} == {(t, s) for t in TILES for s in (False, True)}
+    for nn in (False, True):
+        for (tile, split, *_), (mt, nb, splits, steps) in zip(T.TILES, plans([(m, n, k, nn) for _, _, m, k, n in T.TILES])):
+            assert (mt, nb) == tile and (splits > 1) == split
+            groups = -(-steps // 4)
+            runs = [min(4 * (groups * (z + 1) // splits), steps) - 4 * (groups * z // splits) for z in range(splits)]
+            assert sum(runs) == steps and min(runs) > 4 and (split or steps > 8) and steps % 4 != 0, runs
+
+
+def test_the_few_row_kernel_is_run(plans):
+    """All its widths: tiles of rows, tiles of weight rows, waves."""
+    T = importlib.import_module("test_gpu_fp8_tiles")
+    assert all(p[0] == 0 for p in plans([(m, n, k, False) for m, k, n in T.FEW]))
+
+    def forms(shapes):
+        return {(1 if m <= 16 else 2, 1 if n <= 4096 else 2, 16 if n <= 8192 else 8) for m, _, n in shapes}
+    assert forms(T.FEW) == {(1, 1, 16), (1, 2, 16), (1, 2, 8), (2, 1, 16), (2, 2, 16)}
+    assert forms(T.FEW_16) == {(1, 1, 16), (1, 2, 16), (1, 2, 8)} and all(m <= 4 and k % 8 == 0 for m, k, _ in T.FEW_16)
