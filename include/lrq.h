@@ -469,7 +469,9 @@ int lrq_fp8_dequantize(const lrq_fp8* t, void* out, int64_t ldo, int32_t dtype, 
 
 /* out[a.rows, b.rows] = a b^T, both e4m3 with the same cols (any blocks); fp32 accumulation, out of out_dtype.  The
  * contraction may be split over workgroups: `workspace` (16-byte aligned, lrq_fp8_gemm_workspace(a, b, 0) bytes) takes
- * their fp32 sums, which are added in a fixed order. */
+ * their fp32 sums, which are added in a fixed order.  This and the products below add each eight neighbouring products along
+ * the contraction in a window: of the others what lies below 2^-13 of the largest one's power of two is dropped, so up to
+ * 7 * 2^-13 of that product, beside the roundings of fp32 additions. */
 int lrq_fp8_gemm(const lrq_fp8* a, const lrq_fp8* b, void* out, int64_t ldo, int32_t out_dtype, void* workspace,
                  int64_t workspace_bytes, void* stream);
 

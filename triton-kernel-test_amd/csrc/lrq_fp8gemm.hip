@@ -7,8 +7,10 @@
 //
 // A scale is constant over a K step of 128, a power of two, and the instructions multiply by it: no step's sums pass through
 // the vector unit.  The instructions add each eight neighbouring products in a fixed window: bits of a product below 2^-13 of
-// the largest one's power of two are lost (measured), the rest is fp32; the error of a long sum is about 1.5e-5 of the sum
-// of its magnitudes at most.
+// the largest one's power of two are lost (measured), so that each eight may lose 7 * 2^-13 of its largest product, in one
+// direction where all have one sign; the rest is fp32.  Measured on contractions of 4096 and 14336: normal operands are off by
+// 1.5e-5 of the outputs' size in the mean square and by 2e-6 of the sum of their magnitudes at most; positive ones by 4e-7 to
+// 5e-7 of it, as much as fp32 additions one after another.
 #include "lrq_fp8.h"
 #include "lrq_fp8plan.h"
 
