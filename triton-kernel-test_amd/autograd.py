@@ -398,6 +398,8 @@ def fp8_linear(x: torch.Tensor, w, out_dtype: Optional[torch.dtype] = None) -> t
         return _FP8Linear.apply(x, w, out_dtype)
     if not isinstance(w, torch.Tensor) or w.dim() != 2:
         raise ValueError("the weight must be an FP8Tensor or a dense matrix")
+    if not torch.is_grad_enabled():  # (a parameter asks for its gradient all the same, for which x is quantised along the tokens)
+        return _f8.fp8_linear(x, _f8.fp8_quantize(w, 128), out_dtype)
     return _FP8LinearTrained.apply(x, w, out_dtype)
 
 
